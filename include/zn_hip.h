@@ -65,6 +65,17 @@ typedef enum zn_act {
     ZN_ACT_TANH = 3     /* tanh(v)                                    */
 } zn_act;
 
+/* Gate activations of the gated Dense layer: the epilogue activations, then
+ * the two that only gate. */
+typedef enum zn_gate {
+    ZN_GATE_LINEAR = 0,
+    ZN_GATE_RELU = 1,
+    ZN_GATE_SIGMOID = 2, /* 1/(1+exp(-v)) */
+    ZN_GATE_TANH = 3,
+    ZN_GATE_SILU = 4,    /* v/(1+exp(-v)) */
+    ZN_GATE_GELU = 5     /* v/2 (1 + tanh(sqrt(2/pi) (v + 0.044715 v^3))) */
+} zn_gate;
+
 typedef struct zn_ctx zn_ctx;
 typedef struct zn_event zn_event;
 typedef struct zn_graph zn_graph;
@@ -394,6 +405,90 @@ int zn_hip_softmax_rows(zn_ctx *ctx, const float *in, float *out, int64_t rows, 
  * context's buffer cache. */
 int zn_hip_attention_forward(zn_ctx *ctx, const float *q, const float *k, const float *v, float *out, int64_t batch,
                              int64_t seq_len, int64_t d_k, float scale);
+
+/* --------------------------------- language-model blocks (device pointers) */
+/* No counterpart in the reference: the operators that a transformer block
+ * needs beside its Dense layers, forward and backward, in fp32.  Buffers of
+ * one call must not overlap unless it says so.  Like every device-pointer
+ * call they run on the context's stream, may be captured into a graph, and
+ * give the same bits each time. */
+
+/* Multi-head attention with shared key/value heads: query head h reads
+ * key/value head h / (q_heads / kv_heads).
+ *   S = scale Q.K^T over the visible pairs, lse = log sum exp S,
+ *   out = exp(S - lse).V
+ *  - Tensors are [batch, heads, positions, head_dim] at element strides
+ *    {q,kv,out}_stride_{b,h,s} for batch, head and position; dims are
+ *    contiguous.  The q strides also hold for grad_q, the kv strides for v,
+ *    grad_k and grad_v, the out strides for grad_out.  A position stride is at
+ *    least head_dim and at most 2^22; batch and head strides are >= 0, and > 0
+ *    for what a call writes (over extents above 1; rows that it writes must not
+ *    overlap).  head_dim is 1..128.
+ *  - q_lens and kv_lens: int32 device arrays of batch entries, the positions
+ *    of each sequence that hold tokens (clamped to 0..q_len and 0..kv_len);
+ *    null: all.  causal = 1: query i sees keys j <= i + kl - ql (ql, kl: the
+ *    sequence's lengths), so its last query sees every key.
+ *  - A masked pair takes no part, whatever its values are (infinities and NaN
+ *    too).  A query that sees no key has out = 0 and lse = -inf.  Rows of
+ *    padding (past a sequence's length) are written the same way: out 0, lse
+ *    -inf, gradients 0.
+ *  - lse: contiguous [batch, q_heads, q_len], natural logarithm; the backward
+ *    reads it.  The forward takes null where no backward follows. */
+int zn_hip_mha_forward(zn_ctx *ctx, const float *q, const float *k, const float *v, float *out, float *lse,
+                       int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t q_len, int64_t kv_len,
+                       int64_t head_dim, float scale, int causal, const void *q_lens, const void *kv_lens,
+                       int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_s, int64_t kv_stride_b,
+                       int64_t kv_stride_h, int64_t kv_stride_s, int64_t out_stride_b, int64_t out_stride_h,
+                       int64_t out_stride_s);
+/* Its backward, from the forward's out and lse and grad_out (laid out like
+ * out).  The probabilities are computed again, never stored:
+ *   P = exp(S - lse), grad_v = P^T.grad_out,
+ *   dS = P o (grad_out.v^T - rowsum(grad_out o out)),
+ *   grad_q = scale dS.k, grad_k = scale dS^T.q,
+ * the last two and grad_v summed over the query heads that share a head.  All
+ * three gradients are overwritten. */
+int zn_hip_mha_backward(zn_ctx *ctx, const float *q, const float *k, const float *v, const float *out,
+                        const float *lse, const float *grad_out, float *grad_q, float *grad_k, float *grad_v,
+                        int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t q_len, int64_t kv_len,
+                        int64_t head_dim, float scale, int causal, const void *q_lens, const void *kv_lens,
+                        int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_s, int64_t kv_stride_b,
+                        int64_t kv_stride_h, int64_t kv_stride_s, int64_t out_stride_b, int64_t out_stride_h,
+                        int64_t out_stride_s);
+
+/* Gated Dense layer: z = x.W + bias with W [in x 2 hidden] and bias [2
+ * hidden] (null: none), its first `hidden` columns the gate and the others
+ * the up projection; h = act(gate) * up [batch x hidden].  act is a zn_gate.
+ * z [batch x 2 hidden] is what the backward reads; null where none follows. */
+int zn_hip_gated_dense_forward(zn_ctx *ctx, int act, const float *x, const float *w, const float *bias, float *z,
+                               float *h, int64_t batch, int64_t in_size, int64_t hidden);
+/* Its backward, as zn_hip_dense_backward of the two projections:
+ *   grad_z = [grad_h * up * act'(gate) | grad_h * act(gate)],
+ *   grad_bias += column sums of grad_z (null: skipped),
+ *   grad_x = grad_z.W^T (null: skipped), grad_w = x^T.grad_z (overwritten).
+ * grad_z may be z itself. */
+int zn_hip_gated_dense_backward(zn_ctx *ctx, int act, const float *x, const float *w, const float *z,
+                                const float *grad_h, float *grad_z, float *grad_x, float *grad_w, float *grad_bias,
+                                int64_t batch, int64_t in_size, int64_t hidden);
+
+/* Distillation from a teacher's top logits.  Row r of logits (row stride ld
+ * >= vocab) are the student's; top_index (int32) and top_logits, both
+ * contiguous [rows x k], the teacher's k largest.  An entry whose index lies
+ * outside the vocabulary or whose logit is -inf is absent.  With T the
+ * temperature (> 0) and p = softmax(top_logits / T) over the present entries,
+ *   lse = log sum exp(logits / T),
+ *   loss = T^2 sum_i p_i (log p_i - (logits[top_index_i] / T - lse)).
+ * A row with no entry has loss and lse 0, and its logits are not read.  k is
+ * 0..1024; an index may stand twice, its entries then add up. */
+int zn_hip_distill_forward(zn_ctx *ctx, const float *logits, int64_t ld, const void *top_index,
+                           const float *top_logits, float *loss, float *lse, int64_t rows, int64_t vocab, int64_t k,
+                           float temperature);
+/* grad_logits (row stride grad_ld >= vocab; columns past vocab are left as
+ * they were) = grad_loss[r] T (softmax(logits / T) - sum_{top_index_i = v} p_i)
+ * from the forward's lse; zeros in a row with no entry.  grad_logits may be
+ * logits itself (with grad_ld = ld). */
+int zn_hip_distill_backward(zn_ctx *ctx, const float *logits, int64_t ld, const void *top_index,
+                            const float *top_logits, const float *lse, const float *grad_loss, float *grad_logits,
+                            int64_t grad_ld, int64_t rows, int64_t vocab, int64_t k, float temperature);
 
 /* ------------------------------- Backend drop-ins on host slices (sync) */
 /* Each takes the reference method's slices as (pointer, length) pairs and its

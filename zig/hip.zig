@@ -33,6 +33,7 @@ pub const ABI_VERSION: c_int = 1;
 
 pub const Layout = enum(c_int) { nn = 0, nt = 1, tn = 2 };
 pub const Act = enum(c_int) { linear = 0, relu = 1, sigmoid = 2, tanh = 3 };
+pub const Gate = enum(c_int) { linear = 0, relu = 1, sigmoid = 2, tanh = 3, silu = 4, gelu = 5 };
 
 // ---------------------------------------------------------------- context
 pub extern fn zn_hip_abi_version() c_int;
@@ -92,6 +93,14 @@ pub extern fn zn_hip_conv2d_backward_im2col(ctx: ?*Ctx, input: ?[*]const f32, we
 pub extern fn zn_hip_conv2d_backward_direct(ctx: ?*Ctx, input: ?[*]const f32, weights: ?[*]const f32, grad_output: ?[*]const f32, grad_input: ?[*]f32, grad_weights: ?[*]f32, grad_bias: ?[*]f32, batch: i64, in_channels: i64, out_channels: i64, k_h: i64, k_w: i64, in_h: i64, in_w: i64, out_h: i64, out_w: i64, stride_h: i64, stride_w: i64, pad_h: i64, pad_w: i64) c_int;
 pub extern fn zn_hip_softmax_rows(ctx: ?*Ctx, in: ?[*]const f32, out: ?[*]f32, rows: i64, n: i64, scale: f32) c_int;
 pub extern fn zn_hip_attention_forward(ctx: ?*Ctx, q: ?[*]const f32, k: ?[*]const f32, v: ?[*]const f32, out: ?[*]f32, batch: i64, seq_len: i64, d_k: i64, scale: f32) c_int;
+
+// ---------------------------- language-model blocks (device pointers)
+pub extern fn zn_hip_mha_forward(ctx: ?*Ctx, q: ?[*]const f32, k: ?[*]const f32, v: ?[*]const f32, out: ?[*]f32, lse: ?[*]f32, batch: i64, q_heads: i64, kv_heads: i64, q_len: i64, kv_len: i64, head_dim: i64, scale: f32, causal: c_int, q_lens: ?*const anyopaque, kv_lens: ?*const anyopaque, q_stride_b: i64, q_stride_h: i64, q_stride_s: i64, kv_stride_b: i64, kv_stride_h: i64, kv_stride_s: i64, out_stride_b: i64, out_stride_h: i64, out_stride_s: i64) c_int;
+pub extern fn zn_hip_mha_backward(ctx: ?*Ctx, q: ?[*]const f32, k: ?[*]const f32, v: ?[*]const f32, out: ?[*]const f32, lse: ?[*]const f32, grad_out: ?[*]const f32, grad_q: ?[*]f32, grad_k: ?[*]f32, grad_v: ?[*]f32, batch: i64, q_heads: i64, kv_heads: i64, q_len: i64, kv_len: i64, head_dim: i64, scale: f32, causal: c_int, q_lens: ?*const anyopaque, kv_lens: ?*const anyopaque, q_stride_b: i64, q_stride_h: i64, q_stride_s: i64, kv_stride_b: i64, kv_stride_h: i64, kv_stride_s: i64, out_stride_b: i64, out_stride_h: i64, out_stride_s: i64) c_int;
+pub extern fn zn_hip_gated_dense_forward(ctx: ?*Ctx, act: c_int, x: ?[*]const f32, w: ?[*]const f32, bias: ?[*]const f32, z: ?[*]f32, h: ?[*]f32, batch: i64, in_size: i64, hidden: i64) c_int;
+pub extern fn zn_hip_gated_dense_backward(ctx: ?*Ctx, act: c_int, x: ?[*]const f32, w: ?[*]const f32, z: ?[*]const f32, grad_h: ?[*]const f32, grad_z: ?[*]f32, grad_x: ?[*]f32, grad_w: ?[*]f32, grad_bias: ?[*]f32, batch: i64, in_size: i64, hidden: i64) c_int;
+pub extern fn zn_hip_distill_forward(ctx: ?*Ctx, logits: ?[*]const f32, ld: i64, top_index: ?*const anyopaque, top_logits: ?[*]const f32, loss: ?[*]f32, lse: ?[*]f32, rows: i64, vocab: i64, k: i64, temperature: f32) c_int;
+pub extern fn zn_hip_distill_backward(ctx: ?*Ctx, logits: ?[*]const f32, ld: i64, top_index: ?*const anyopaque, top_logits: ?[*]const f32, lse: ?[*]const f32, grad_loss: ?[*]const f32, grad_logits: ?[*]f32, grad_ld: i64, rows: i64, vocab: i64, k: i64, temperature: f32) c_int;
 
 // ------------------------------------ Backend drop-ins on host slices
 pub extern fn zn_hip_mat_mul(ctx: ?*Ctx, a: ?[*]const f32, a_len: usize, b: ?[*]const f32, b_len: usize, c: ?[*]f32, c_len: usize, m: usize, n: usize, k: usize, accumulate: c_int) c_int;

@@ -30,6 +30,7 @@ TILES = {"auto": -1, "256x128": 0, "128x128": 1, "128x64": 2, "64x64": 3, "32x32
          "256x256": 7, "256x256s": 8, "256x128s": 9, "128x128s": 10, "128x64s": 11, "128x128sc": 12,
          "conv128x128s": 13, "conv64x128s": 14}
 ACT_LINEAR, ACT_RELU, ACT_SIGMOID, ACT_TANH = 0, 1, 2, 3
+GATES = {"linear": 0, "relu": 1, "sigmoid": 2, "tanh": 3, "silu": 4, "gelu": 5}
 
 
 class ZnError(RuntimeError):
@@ -158,6 +159,12 @@ SIGNATURES = {
     "zn_hip_conv2d_backward_direct": (I, [P] + [P] * 6 + [I64] * 13),
     "zn_hip_softmax_rows": (I, [P, P, P, I64, I64, F]),
     "zn_hip_attention_forward": (I, [P, P, P, P, P, I64, I64, I64, F]),
+    "zn_hip_mha_forward": (I, [P] * 6 + [I64] * 6 + [F, I, P, P] + [I64] * 9),
+    "zn_hip_mha_backward": (I, [P] * 10 + [I64] * 6 + [F, I, P, P] + [I64] * 9),
+    "zn_hip_gated_dense_forward": (I, [P, I] + [P] * 5 + [I64] * 3),
+    "zn_hip_gated_dense_backward": (I, [P, I] + [P] * 8 + [I64] * 3),
+    "zn_hip_distill_forward": (I, [P, P, I64, P, P, P, P, I64, I64, I64, F]),
+    "zn_hip_distill_backward": (I, [P, P, I64, P, P, P, P, P, I64, I64, I64, I64, F]),
     "zn_hip_conv2d_forward_host": (I, [P, P, S, P, S, P, S, P, S] + [S] * 11),
     "zn_hip_conv2d_backward_host": (I, [P, P, S, P, S, P, S, P, S, P, S, P, S] + [S] * 12),
     "zn_hip_attention_forward_host": (I, [P, P, S, P, S, P, S, P, S, P, S, S, S, F]),

@@ -37,6 +37,17 @@ def act_id(act) -> int:
                                    f"{act!r} is not on the GEMM path (linear, relu, sigmoid, tanh)") from None
 
 
+def gate_id(act) -> int:
+    """Map a gate activation's name to its C-ABI id (zn_gate)."""
+    if isinstance(act, int):
+        return act
+    try:
+        return _lib.GATES[str(act)]
+    except KeyError:
+        raise InvalidArgumentError(_lib.ZN_ERR_INVALID_ARG, "gate",
+                                   f"{act!r} is not a gate ({', '.join(_lib.GATES)})") from None
+
+
 def layout_id(layout) -> int:
     if isinstance(layout, int):
         return layout
@@ -351,6 +362,58 @@ class Context:
         check(_lib.load().zn_hip_attention_forward(self.handle, _dptr(q), _dptr(k), _dptr(v), _dptr(out), batch,
                                                    seq_len, d_k, float(scale)), "zn_hip_attention_forward")
 
+    # --- language-model blocks on device pointers
+    def mha_forward(self, q, k, v, out, lse, batch, q_heads, kv_heads, q_len, kv_len, head_dim, scale, causal=False,
+                    q_lens=None, kv_lens=None, q_strides=None, kv_strides=None, out_strides=None) -> None:
+        """Multi-head attention with shared key/value heads, causal and length masks.  Tensors are
+        [batch, heads, positions, head_dim] at (batch, head, position) element strides (None: contiguous);
+        lse ([batch, q_heads, q_len]) is what the backward reads and may be None; q_lens and kv_lens are
+        int32 device arrays of the sequences' lengths."""
+        check(_lib.load().zn_hip_mha_forward(
+            self.handle, _dptr(q), _dptr(k), _dptr(v), _dptr(out), _dptr(lse), batch, q_heads, kv_heads, q_len, kv_len,
+            head_dim, float(scale), int(causal), _dptr(q_lens), _dptr(kv_lens),
+            *_mha_strides(q_heads, kv_heads, q_len, kv_len, head_dim, q_strides, kv_strides, out_strides)),
+            "zn_hip_mha_forward")
+
+    def mha_backward(self, q, k, v, out, lse, grad_out, grad_q, grad_k, grad_v, batch, q_heads, kv_heads, q_len, kv_len,
+                     head_dim, scale, causal=False, q_lens=None, kv_lens=None, q_strides=None, kv_strides=None,
+                     out_strides=None) -> None:
+        """The gradients of mha_forward from its out and lse; grad_q is laid out like q, grad_k and grad_v like
+        k, grad_out like out.  The probabilities are computed again."""
+        check(_lib.load().zn_hip_mha_backward(
+            self.handle, _dptr(q), _dptr(k), _dptr(v), _dptr(out), _dptr(lse), _dptr(grad_out), _dptr(grad_q),
+            _dptr(grad_k), _dptr(grad_v), batch, q_heads, kv_heads, q_len, kv_len, head_dim, float(scale), int(causal),
+            _dptr(q_lens), _dptr(kv_lens),
+            *_mha_strides(q_heads, kv_heads, q_len, kv_len, head_dim, q_strides, kv_strides, out_strides)),
+            "zn_hip_mha_backward")
+
+    def gated_dense_forward(self, act, x, w, bias, z, h, batch, in_size, hidden) -> None:
+        """h = act(gate) * up with [gate | up] = x.W + bias, W [in_size x 2 hidden] (bias may be None); z
+        ([batch x 2 hidden], the projections) is what the backward reads and may be None."""
+        check(_lib.load().zn_hip_gated_dense_forward(self.handle, gate_id(act), _dptr(x), _dptr(w), _dptr(bias), _dptr(z),
+                                                     _dptr(h), batch, in_size, hidden), "zn_hip_gated_dense_forward")
+
+    def gated_dense_backward(self, act, x, w, z, grad_h, grad_z, grad_x, grad_w, grad_bias, batch, in_size,
+                             hidden) -> None:
+        """The gradients of gated_dense_forward; grad_bias accumulates, grad_bias and grad_x may be None."""
+        check(_lib.load().zn_hip_gated_dense_backward(
+            self.handle, gate_id(act), _dptr(x), _dptr(w), _dptr(z), _dptr(grad_h), _dptr(grad_z), _dptr(grad_x),
+            _dptr(grad_w), _dptr(grad_bias), batch, in_size, hidden), "zn_hip_gated_dense_backward")
+
+    def distill_forward(self, logits, ld, top_index, top_logits, loss, lse, rows, vocab, k, temperature=1.0) -> None:
+        """Per row, the divergence of the teacher's top logits ([rows x k] int32 indices and float32 logits) from
+        the student's distribution over the vocabulary, and the log-sum-exp that the backward reads."""
+        check(_lib.load().zn_hip_distill_forward(self.handle, _dptr(logits), ld, _dptr(top_index), _dptr(top_logits),
+                                                 _dptr(loss), _dptr(lse), rows, vocab, k, float(temperature)),
+              "zn_hip_distill_forward")
+
+    def distill_backward(self, logits, ld, top_index, top_logits, lse, grad_loss, grad_logits, grad_ld, rows, vocab, k,
+                         temperature=1.0) -> None:
+        """The gradient of distill_forward's losses, weighted by grad_loss ([rows]); grad_logits may be logits."""
+        check(_lib.load().zn_hip_distill_backward(
+            self.handle, _dptr(logits), ld, _dptr(top_index), _dptr(top_logits), _dptr(lse), _dptr(grad_loss),
+            _dptr(grad_logits), grad_ld, rows, vocab, k, float(temperature)), "zn_hip_distill_backward")
+
     def close(self) -> None:
         if self.handle:
             for g in list(self._graphs):  # zn_hip_destroy releases them
@@ -369,6 +432,13 @@ class Context:
             self.close()
         except Exception:
             pass
+
+
+def _mha_strides(q_heads, kv_heads, q_len, kv_len, head_dim, q, kv, out):
+    """The nine element strides of an mha call, contiguous [batch, heads, positions, dims] where not given."""
+    q_own = (q_heads * q_len * head_dim, q_len * head_dim, head_dim)
+    kv_own = (kv_heads * kv_len * head_dim, kv_len * head_dim, head_dim)
+    return (*(q_own if q is None else q), *(kv_own if kv is None else kv), *(q_own if out is None else out))
 
 
 def _dptr(x) -> Optional[int]:

@@ -601,3 +601,6 @@ extern "C" __global__ __launch_bounds__(256) void zn_attention_combine(ZnAttnArg
     for (int i = 0; i < 2; ++i)
         if (lane + 64 * i < p.d_k) row[lane + 64 * i] = o[i] / sum;
 }
+
+// The masked, grouped form for training (zn_mha_*).
+#include "mha_f32.h"

@@ -8,6 +8,7 @@
 
 #include "../zn_kernel_args.h"
 #include "zn_activation.h"
+#include "zn_gate.h"
 
 typedef float zn_f32x4 __attribute__((ext_vector_type(4)));
 
@@ -549,5 +550,175 @@ extern "C" __global__ __launch_bounds__(64) void zn_hold_stream(ZnEltArgs p) {
     for (int64_t i = 0; i < p.n; ++i) {
         __builtin_amdgcn_s_sleep(8);
         if (__builtin_amdgcn_s_memrealtime() - start >= ticks) break;
+    }
+}
+
+// ------------------------------------------------- gated Dense, elementwise
+// h = act(gate) * up from z = [gate | up] [rows x 2n].
+extern "C" __global__ __launch_bounds__(256) void zn_gate_forward(ZnGateArgs p) {
+    const int64_t total = p.rows * p.n;
+    for (int64_t i = gtid(); i < total; i += gstride()) {
+        const int64_t r = i / p.n, c = i - r * p.n;
+        const float *z = p.z + r * 2 * p.n + c;
+        p.h[i] = zn_gate(z[0], p.act) * z[p.n];
+    }
+}
+
+// grad_z = [grad_h * up * act'(gate) | grad_h * act(gate)].
+extern "C" __global__ __launch_bounds__(256) void zn_gate_backward(ZnGateArgs p) {
+    const int64_t total = p.rows * p.n;
+    for (int64_t i = gtid(); i < total; i += gstride()) {
+        const int64_t r = i / p.n, c = i - r * p.n;
+        const int64_t at = r * 2 * p.n + c;
+        float y, d;
+        zn_gate_slope(p.z[at], p.act, y, d);
+        const float g = p.grad_h[i];
+        p.grad_z[at] = g * p.z[at + p.n] * d;
+        p.grad_z[at + p.n] = g * y;
+    }
+}
+
+// --------------------------------------------- distillation from top logits
+// Per token: p = softmax(top / T) over the teacher's present entries, lse =
+// log sum exp(logits / T) over the vocabulary,
+//   loss = T^2 sum_i p_i (log p_i - logits[index_i] / T + lse),
+//   grad = grad_loss T (softmax(logits / T) - sum_{index_i = v} p_i).
+// An entry is absent when its index lies outside the vocabulary or its logit
+// is -inf; a row without entries has loss, lse and gradient 0 and its logits
+// are not read.  Sums are fp32 in a fixed order.
+namespace {
+
+constexpr int kDistillMaxK = 1024, kDistillThreads = 256;
+constexpr int kDistillPer = kDistillMaxK / kDistillThreads;
+
+// x / T to the last bit or so (inv = 1 / T, rounded): the rounding of inv times |x / T| would reach every probability.
+__device__ __forceinline__ float over_t(float x, const ZnDistillArgs &p) {
+    const float q = x * p.inv_temperature;
+    const float r = __builtin_fmaf(-q, p.temperature, x);
+    return __builtin_fabsf(q) < INFINITY ? __builtin_fmaf(r, p.inv_temperature, q) : q;
+}
+__device__ __forceinline__ float exp_nat(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f); }
+
+// The teacher's row: this thread's entries (tid + 256 q), with index -1 where absent, their probability and its logarithm.
+struct DistillTeacher {
+    int at[kDistillPer];
+    float prob[kDistillPer], logp[kDistillPer];
+    bool any;
+    __device__ __forceinline__ DistillTeacher(const ZnDistillArgs &p, int64_t row, float *red) {
+        float mx = -INFINITY;
+        bool some = false;
+#pragma unroll
+        for (int q = 0; q < kDistillPer; ++q) {
+            const int i = threadIdx.x + q * kDistillThreads;
+            at[q] = -1;
+            logp[q] = -INFINITY;
+            if (i < p.k) {
+                const int v = p.index[row * p.k + i];
+                const float t = p.top[row * p.k + i];
+                if (v >= 0 && v < p.vocab && t != -INFINITY) {
+                    at[q] = v;
+                    logp[q] = over_t(t, p);
+                    some = true;
+                }
+            }
+            mx = fmaxf(mx, logp[q]);
+        }
+        any = __syncthreads_or(some);
+        mx = block_reduce<true>(mx, red);
+        float sum = 0.0f;
+#pragma unroll
+        for (int q = 0; q < kDistillPer; ++q) {
+            prob[q] = at[q] >= 0 ? expf(logp[q] - mx) : 0.0f;
+            sum += prob[q];
+        }
+        sum = block_reduce<false>(sum, red);
+        const float log_sum = logf(sum);
+#pragma unroll
+        for (int q = 0; q < kDistillPer; ++q) {
+            prob[q] = prob[q] / sum;
+            logp[q] = (logp[q] - mx) - log_sum;
+        }
+    }
+};
+
+}  // namespace
+
+extern "C" __global__ __launch_bounds__(256) void zn_distill_forward(ZnDistillArgs p) {
+    __shared__ float red[kSoftmaxThreads / 64];
+    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+        const DistillTeacher t(p, row, red);
+        if (!t.any) {
+            if (threadIdx.x == 0) {
+                p.loss[row] = 0.0f;
+                p.lse[row] = 0.0f;
+            }
+            continue;
+        }
+        const float *src = p.logits + row * p.ld;
+        float m = -INFINITY, l = 0.0f;
+        for (int i = threadIdx.x; i < p.vocab; i += kDistillThreads) {
+            const float s = over_t(src[i], p);
+            const float mn = fmaxf(m, s), ref = mn == -INFINITY ? 0.0f : mn;
+            l = l * exp_nat(m - ref) + exp_nat(s - ref);
+            m = mn;
+        }
+        const float mx = block_reduce<true>(m, red), ref = mx == -INFINITY ? 0.0f : mx;
+        const float sum = block_reduce<false>(l * exp_nat(m - ref), red);
+        const float lse = mx + logf(sum);
+        float term = 0.0f;
+#pragma unroll
+        for (int q = 0; q < kDistillPer; ++q)
+            if (t.at[q] >= 0 && t.prob[q] != 0.0f)
+                term += t.prob[q] * (t.logp[q] - (over_t(src[t.at[q]], p) - lse));
+        term = block_reduce<false>(term, red);
+        if (threadIdx.x == 0) {
+            p.loss[row] = p.temperature * p.temperature * term;
+            p.lse[row] = lse;
+        }
+    }
+}
+
+extern "C" __global__ __launch_bounds__(256) void zn_distill_backward(ZnDistillArgs p) {
+    __shared__ float red[kSoftmaxThreads / 64];
+    __shared__ int idx[kDistillMaxK];
+    __shared__ float prob[kDistillMaxK];
+    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+        const DistillTeacher t(p, row, red);
+        const float *src = p.logits + row * p.ld;
+        float *dst = p.grad + row * p.grad_ld;
+        if (!t.any) {
+            for (int i = threadIdx.x; i < p.vocab; i += kDistillThreads) dst[i] = 0.0f;
+            continue;
+        }
+        const float lse = p.lse[row], g = p.grad_loss[row] * p.temperature;
+        float own[kDistillPer];  // read before the row is written, which may be the logits' own
+#pragma unroll
+        for (int q = 0; q < kDistillPer; ++q) {
+            const int i = threadIdx.x + q * kDistillThreads;
+            own[q] = t.at[q] >= 0 ? exp_nat(over_t(src[t.at[q]], p) - lse) : 0.0f;
+            if (i < p.k) {
+                idx[i] = t.at[q];
+                prob[i] = t.prob[q];
+            }
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < p.vocab; i += kDistillThreads)
+            dst[i] = g * exp_nat(over_t(src[i], p) - lse);
+        __syncthreads();
+        // the first entry of each index subtracts all of that index's, in order
+#pragma unroll
+        for (int q = 0; q < kDistillPer; ++q) {
+            const int i = threadIdx.x + q * kDistillThreads;
+            if (i >= p.k || t.at[q] < 0) continue;
+            float sum = 0.0f;
+            bool first = true;
+            for (int j = 0; j < p.k; ++j)
+                if (idx[j] == t.at[q]) {
+                    first &= j >= i;
+                    sum += prob[j];
+                }
+            if (first) dst[t.at[q]] = g * (own[q] - sum);
+        }
+        __syncthreads();  // idx and prob are the next row's from here on
     }
 }

@@ -1,0 +1,242 @@
+// Language-model blocks of the C ABI (include/zn_hip.h): grouped attention,
+// the gated Dense layer and distillation, forward and backward.  Included by
+// zn_hip.cpp, whose helpers it uses.
+#ifndef ZN_BLOCK_OPS_H
+#define ZN_BLOCK_OPS_H
+
+#include <cmath>
+
+// ------------------------------------------------------- grouped attention
+namespace {
+
+constexpr int64_t kMhaMaxDim = 128;
+constexpr int64_t kMhaMaxRow = (int64_t)1 << 22;  // position stride: a block of 64 rows stays inside 32-bit offsets
+
+// Element strides that a call only reads, or (written) also writes.
+bool mha_strides_ok(int64_t sb, int64_t sh, int64_t ss, int64_t batch, int64_t heads, int64_t rows, int64_t dim,
+                    bool written) {
+    if (ss < dim || ss > kMhaMaxRow || sb < 0 || sh < 0) return false;
+    return !written || rows == 0 || ((sb > 0 || batch <= 1) && (sh > 0 || heads <= 1));
+}
+
+// The checks and the argument block that both directions share.  *work: there is something to do.
+int mha_args(zn_ctx *ctx, ZnMhaArgs &a, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t q_len, int64_t kv_len,
+             int64_t head_dim, float scale, int causal, const void *q_lens, const void *kv_lens, const int64_t (&qs)[3],
+             const int64_t (&ks)[3], const int64_t (&os)[3], bool backward, bool *work) {
+    *work = false;
+    if (!ctx || batch < 0 || q_heads < 0 || kv_heads < 0 || q_len < 0 || kv_len < 0 || head_dim < 1 ||
+        head_dim > kMhaMaxDim || !std::isfinite(scale) || causal < 0 || causal > 1)
+        return ZN_ERR_INVALID_ARG;
+    if (kv_heads == 0 ? q_heads != 0 : q_heads % kv_heads != 0) return ZN_ERR_INVALID_ARG;
+    if (!mha_strides_ok(qs[0], qs[1], qs[2], batch, q_heads, q_len, head_dim, backward) ||
+        !mha_strides_ok(ks[0], ks[1], ks[2], batch, kv_heads, kv_len, head_dim, backward) ||
+        !mha_strides_ok(os[0], os[1], os[2], batch, q_heads, q_len, head_dim, !backward))
+        return ZN_ERR_INVALID_ARG;
+    constexpr int64_t kMax = INT_MAX / 2;
+    if (batch > kMax || q_heads > kMax || q_len > kMax || kv_len > kMax || batch * q_heads > kMax || batch * kv_heads > kMax)
+        return ZN_ERR_OVERFLOW;
+    std::memset(&a, 0, sizeof(a));
+    std::memcpy(a.qs, qs, sizeof(a.qs));
+    std::memcpy(a.ks, ks, sizeof(a.ks));
+    std::memcpy(a.os, os, sizeof(a.os));
+    a.q_lens = static_cast<const int32_t *>(q_lens);
+    a.kv_lens = static_cast<const int32_t *>(kv_lens);
+    a.batch = (int32_t)batch;
+    a.q_heads = (int32_t)q_heads;
+    a.kv_heads = (int32_t)kv_heads;
+    a.group = kv_heads ? (int32_t)(q_heads / kv_heads) : 0;
+    a.q_len = (int32_t)q_len;
+    a.kv_len = (int32_t)kv_len;
+    a.dim = (int32_t)head_dim;
+    a.causal = causal;
+    a.scale = scale;
+    a.scale_log2 = scale * 1.44269504088896340736f;
+    *work = batch > 0 && kv_heads > 0;
+    return ZN_OK;
+}
+
+int mha_rows(zn_ctx *ctx, MhaKernel kernel, int64_t heads, int64_t rows, ZnMhaArgs &a) {
+    return launch(ctx, ctx->mha[kernel], (unsigned)heads, (unsigned)std::min<int64_t>(cdiv(rows, 4), 65535), 256, &a);
+}
+
+}  // namespace
+
+int zn_hip_mha_forward(zn_ctx *ctx, const float *q, const float *k, const float *v, float *out, float *lse,
+                       int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t q_len, int64_t kv_len,
+                       int64_t head_dim, float scale, int causal, const void *q_lens, const void *kv_lens,
+                       int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_s, int64_t kv_stride_b,
+                       int64_t kv_stride_h, int64_t kv_stride_s, int64_t out_stride_b, int64_t out_stride_h,
+                       int64_t out_stride_s) {
+    ZnMhaArgs a;
+    bool work = false;
+    int rc = mha_args(ctx, a, batch, q_heads, kv_heads, q_len, kv_len, head_dim, scale, causal, q_lens, kv_lens,
+                      {q_stride_b, q_stride_h, q_stride_s}, {kv_stride_b, kv_stride_h, kv_stride_s},
+                      {out_stride_b, out_stride_h, out_stride_s}, false, &work);
+    if (rc || !work || q_len == 0) return rc;
+    if (!q || !out || (kv_len > 0 && (!k || !v))) return ZN_ERR_INVALID_ARG;
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.out = out;
+    a.lse = lse;
+    if ((rc = select_device(ctx))) return rc;
+    return mha_rows(ctx, kMhaForwardRows, batch * q_heads, q_len, a);
+}
+
+int zn_hip_mha_backward(zn_ctx *ctx, const float *q, const float *k, const float *v, const float *out,
+                        const float *lse, const float *grad_out, float *grad_q, float *grad_k, float *grad_v,
+                        int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t q_len, int64_t kv_len,
+                        int64_t head_dim, float scale, int causal, const void *q_lens, const void *kv_lens,
+                        int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_s, int64_t kv_stride_b,
+                        int64_t kv_stride_h, int64_t kv_stride_s, int64_t out_stride_b, int64_t out_stride_h,
+                        int64_t out_stride_s) {
+    ZnMhaArgs a;
+    bool work = false;
+    int rc = mha_args(ctx, a, batch, q_heads, kv_heads, q_len, kv_len, head_dim, scale, causal, q_lens, kv_lens,
+                      {q_stride_b, q_stride_h, q_stride_s}, {kv_stride_b, kv_stride_h, kv_stride_s},
+                      {out_stride_b, out_stride_h, out_stride_s}, true, &work);
+    if (rc || !work || (q_len == 0 && kv_len == 0)) return rc;
+    if (q_len > 0 && (!q || !out || !lse || !grad_out || !grad_q)) return ZN_ERR_INVALID_ARG;
+    if (kv_len > 0 && (!k || !v || !grad_k || !grad_v)) return ZN_ERR_INVALID_ARG;
+    if ((rc = select_device(ctx))) return rc;
+    Lease delta(ctx);
+    if (q_len > 0 && (rc = delta.get((size_t)(batch * q_heads) * (size_t)q_len))) return rc;
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.out = const_cast<float *>(out);
+    a.lse = const_cast<float *>(lse);
+    a.grad_out = grad_out;
+    a.grad_q = grad_q;
+    a.grad_k = grad_k;
+    a.grad_v = grad_v;
+    a.delta = delta.ptr;
+    if (q_len > 0 && (rc = mha_rows(ctx, kMhaGradQRows, batch * q_heads, q_len, a))) return rc;
+    if (kv_len > 0 && (rc = mha_rows(ctx, kMhaGradKvRows, batch * kv_heads, kv_len, a))) return rc;
+    return ZN_OK;
+}
+
+// ----------------------------------------------------------- gated Dense
+static bool gated_extents_ok(int64_t batch, int64_t in_size, int64_t hidden) {
+    return batch <= INT_MAX && in_size <= INT_MAX && hidden <= INT_MAX / 2;
+}
+
+int zn_hip_gated_dense_forward(zn_ctx *ctx, int act, const float *x, const float *w, const float *bias, float *z,
+                               float *h, int64_t batch, int64_t in_size, int64_t hidden) {
+    if (!ctx || act < ZN_GATE_LINEAR || act > ZN_GATE_GELU || batch < 0 || in_size < 0 || hidden < 0)
+        return ZN_ERR_INVALID_ARG;
+    if (!gated_extents_ok(batch, in_size, hidden)) return ZN_ERR_OVERFLOW;
+    if (batch == 0 || hidden == 0) return ZN_OK;
+    if (!h || (in_size > 0 && (!x || !w))) return ZN_ERR_INVALID_ARG;
+    int rc = select_device(ctx);
+    if (rc) return rc;
+    Lease own(ctx);
+    if (!z) {
+        if ((rc = own.get((size_t)batch * 2 * (size_t)hidden))) return rc;
+        z = own.ptr;
+    }
+    if ((rc = gemm_launch(ctx, ZN_LAYOUT_NN, batch, 2 * hidden, in_size, x, in_size, 0, w, 2 * hidden, 0, z, 2 * hidden, 0, 1,
+                          0, bias, ZN_ACT_LINEAR)))
+        return rc;
+    ZnGateArgs g;
+    std::memset(&g, 0, sizeof(g));
+    g.z = z;
+    g.h = h;
+    g.rows = batch;
+    g.n = hidden;
+    g.act = act;
+    return elt_launch(ctx, kGateForward, batch * hidden, g);
+}
+
+int zn_hip_gated_dense_backward(zn_ctx *ctx, int act, const float *x, const float *w, const float *z,
+                                const float *grad_h, float *grad_z, float *grad_x, float *grad_w, float *grad_bias,
+                                int64_t batch, int64_t in_size, int64_t hidden) {
+    if (!ctx || act < ZN_GATE_LINEAR || act > ZN_GATE_GELU || batch < 0 || in_size < 0 || hidden < 0)
+        return ZN_ERR_INVALID_ARG;
+    if (!gated_extents_ok(batch, in_size, hidden)) return ZN_ERR_OVERFLOW;
+    const int64_t n = 2 * hidden;
+    if (batch > 0 && hidden > 0 && (!z || !grad_h || !grad_z)) return ZN_ERR_INVALID_ARG;
+    if (in_size > 0 && hidden > 0 && (!grad_w || (batch > 0 && (!x || !w)))) return ZN_ERR_INVALID_ARG;
+    int rc = select_device(ctx);
+    if (rc) return rc;
+    if (hidden == 0) return grad_x && batch > 0 && in_size > 0 ? zn_hip_fill_f32(ctx, grad_x, 0.0f, batch * in_size) : ZN_OK;
+    if (batch == 0) return in_size > 0 ? zn_hip_fill_f32(ctx, grad_w, 0.0f, in_size * n) : ZN_OK;
+    ZnGateArgs g;
+    std::memset(&g, 0, sizeof(g));
+    g.z = z;
+    g.grad_h = grad_h;
+    g.grad_z = grad_z;
+    g.rows = batch;
+    g.n = hidden;
+    g.act = act;
+    if ((rc = elt_launch(ctx, kGateBackward, batch * hidden, g))) return rc;
+    if (grad_bias)
+        return dense_backward_impl(ctx, ZN_ACT_LINEAR, x, w, nullptr, nullptr, grad_z, grad_x, grad_w, grad_bias, batch,
+                                   in_size, n, true, ZN_ACT_LINEAR, nullptr, nullptr);
+    if (in_size == 0) return ZN_OK;
+    if (grad_x && (rc = gemm_launch(ctx, ZN_LAYOUT_NT, batch, in_size, n, grad_z, n, 0, w, n, 0, grad_x, in_size, 0, 1, 0,
+                                    nullptr, ZN_ACT_LINEAR)))
+        return rc;
+    return gemm_launch(ctx, ZN_LAYOUT_TN, in_size, n, batch, x, in_size, 0, grad_z, n, 0, grad_w, n, 0, 1, 0, nullptr,
+                       ZN_ACT_LINEAR);
+}
+
+// ---------------------------------------------------------- distillation
+namespace {
+
+constexpr int64_t kDistillMaxK = 1024;
+
+int distill_args(zn_ctx *ctx, ZnDistillArgs &a, const float *logits, int64_t ld, const void *index, const float *top,
+                 int64_t rows, int64_t vocab, int64_t k, float temperature) {
+    if (!ctx || rows < 0 || vocab < 0 || k < 0 || k > kDistillMaxK || ld < vocab || !(temperature > 0.0f) ||
+        !std::isfinite(temperature) || !std::isfinite(1.0f / temperature))
+        return ZN_ERR_INVALID_ARG;
+    if (vocab > INT_MAX / 2) return ZN_ERR_OVERFLOW;
+    std::memset(&a, 0, sizeof(a));
+    if (rows == 0) return ZN_OK;
+    if (vocab > 0 && k > 0 && (!logits || !index || !top)) return ZN_ERR_INVALID_ARG;
+    a.logits = logits;
+    a.index = static_cast<const int32_t *>(index);
+    a.top = top;
+    a.ld = ld;
+    a.rows = rows;
+    a.vocab = (int32_t)vocab;
+    a.k = vocab > 0 ? (int32_t)k : 0;
+    a.temperature = temperature;
+    a.inv_temperature = 1.0f / temperature;
+    return ZN_OK;
+}
+
+}  // namespace
+
+int zn_hip_distill_forward(zn_ctx *ctx, const float *logits, int64_t ld, const void *top_index,
+                           const float *top_logits, float *loss, float *lse, int64_t rows, int64_t vocab, int64_t k,
+                           float temperature) {
+    ZnDistillArgs a;
+    int rc = distill_args(ctx, a, logits, ld, top_index, top_logits, rows, vocab, k, temperature);
+    if (rc || rows == 0) return rc;
+    if (!loss || !lse) return ZN_ERR_INVALID_ARG;
+    a.loss = loss;
+    a.lse = lse;
+    if ((rc = select_device(ctx))) return rc;
+    return launch(ctx, ctx->elt[kDistillForward], (unsigned)std::min<int64_t>(rows, 8 * cus_now(ctx)), 1, 256, &a);
+}
+
+int zn_hip_distill_backward(zn_ctx *ctx, const float *logits, int64_t ld, const void *top_index,
+                            const float *top_logits, const float *lse, const float *grad_loss, float *grad_logits,
+                            int64_t grad_ld, int64_t rows, int64_t vocab, int64_t k, float temperature) {
+    ZnDistillArgs a;
+    int rc = distill_args(ctx, a, logits, ld, top_index, top_logits, rows, vocab, k, temperature);
+    if (rc) return rc;
+    if (grad_ld < vocab) return ZN_ERR_INVALID_ARG;
+    if (rows == 0 || vocab == 0) return ZN_OK;
+    if (!grad_logits || (k > 0 && (!lse || !grad_loss))) return ZN_ERR_INVALID_ARG;
+    a.lse = const_cast<float *>(lse);
+    a.grad_loss = grad_loss;
+    a.grad = grad_logits;
+    a.grad_ld = grad_ld;
+    if ((rc = select_device(ctx))) return rc;
+    return launch(ctx, ctx->elt[kDistillBackward], (unsigned)std::min<int64_t>(rows, 8 * cus_now(ctx)), 1, 256, &a);
+}
+
+#endif

@@ -74,13 +74,16 @@ constexpr TileShape kTiles[kNumTiles] = {{256, 128, 16, 512, "x", true, true, tr
                                          {64, 128, 32, 256, "ch", false, false, false}};
 constexpr const char *kLayoutName[3] = {"nn", "nt", "tn"};
 
-enum EltKernel { kFill, kCopy, kAddBias, kActFwd, kActBwd, kAccBias, kIm2col, kSoftmax, kCol2im, kRowSum, kDenseGrad, kRegroup, kPack, kToNhwc, kHold, kCol2imPx, kReduceSlices, kNumElt };
+enum EltKernel { kFill, kCopy, kAddBias, kActFwd, kActBwd, kAccBias, kIm2col, kSoftmax, kCol2im, kRowSum, kDenseGrad, kRegroup, kPack, kToNhwc, kHold, kCol2imPx, kReduceSlices,
+                 kGateForward, kGateBackward, kDistillForward, kDistillBackward, kNumElt };
 constexpr const char *kEltName[kNumElt] = {"zn_fill_f32",        "zn_copy_f32", "zn_add_bias",
                                            "zn_activation_forward", "zn_activation_backward",
                                            "zn_accumulate_bias", "zn_im2col",   "zn_softmax_rows",
                                            "zn_col2im",          "zn_row_sum",  "zn_dense_grad_prologue",
                                            "zn_weight_regroup", "zn_pack_rows", "zn_nchw_to_nhwc",
-                                           "zn_hold_stream",     "zn_col2im_px", "zn_reduce_slices"};
+                                           "zn_hold_stream",     "zn_col2im_px", "zn_reduce_slices",
+                                           "zn_gate_forward",    "zn_gate_backward", "zn_distill_forward",
+                                           "zn_distill_backward"};
 
 constexpr const char *kGemmObject = "zn_gemm_gfx950.hsaco";
 constexpr const char *kConvObject = "zn_conv_gfx950.hsaco";
@@ -94,6 +97,10 @@ constexpr int kAttnQueries = 128;  // queries per workgroup (4 waves x 32)
 constexpr int kAttnSplitDims[4] = {32, 64, 96, 128};
 constexpr unsigned kAttnSplitThreads[4] = {256, 512, 512, 512};
 constexpr int kAttnSplitQueries[4] = {128, 256, 128, 128};
+
+// Grouped attention (kernels/mha_f32.h), in the attention code object.
+enum MhaKernel { kMhaForwardRows, kMhaGradQRows, kMhaGradKvRows, kNumMha };
+constexpr const char *kMhaName[kNumMha] = {"zn_mha_forward_rows", "zn_mha_grad_q_rows", "zn_mha_grad_kv_rows"};
 
 struct ScratchDevice;
 
@@ -176,6 +183,7 @@ struct zn_ctx {
     hipFunction_t attn[2][2] = {};             // fused attention [head dim 32/64][16-byte I/O]
     hipFunction_t attn_split[4] = {};          // the split form [head dim 32/64/96/128]
     hipFunction_t attn_combine = nullptr;      // merges its key ranges
+    hipFunction_t mha[kNumMha] = {};           // grouped attention
     hipFunction_t gemm[3][kNumTiles][3] = {};  // [layout][tile][staging: 4-byte, 16-byte, 16-byte unaligned (r only)]
     int gemm_threads[3][kNumTiles][3] = {};    // their workgroup sizes (the kernels' launch bounds)
     hipFunction_t conv[kNumTiles][2][2] = {};  // implicit-GEMM convolution [tile][16-byte W rows][4-pixel gather]
@@ -1990,6 +1998,8 @@ int zn_hip_create(int device, const char *code_object_dir, zn_ctx **out) {
     }
     if (hipModuleGetFunction(&ctx->attn_combine, ctx->attn_module, "zn_attention_combine") != hipSuccess)
         return bail(ZN_ERR_SYMBOL);
+    for (int i = 0; i < kNumMha; ++i)
+        if (hipModuleGetFunction(&ctx->mha[i], ctx->attn_module, kMhaName[i]) != hipSuccess) return bail(ZN_ERR_SYMBOL);
     void *counters = nullptr;
     if ((e = hipMalloc(&counters, kCounterSlots * kCounterStride * sizeof(int32_t))) != hipSuccess) {
         (void)hipGetLastError();
@@ -3301,6 +3311,9 @@ int zn_hip_attention_forward(zn_ctx *ctx, const float *q, const float *k, const 
     return gemm_launch(ctx, ZN_LAYOUT_NN, seq_len, d_k, seq_len, scores.ptr, seq_len, ss, v, d_k, sd, out, d_k, sd,
                        batch, 0, nullptr, ZN_ACT_LINEAR);
 }
+
+// ------------------------------------------------ language-model blocks
+#include "zn_block_ops.h"
 
 // ------------------------------------------------ host-slice drop-ins
 int zn_hip_mat_mul(zn_ctx *ctx, const float *a, size_t a_len, const float *b, size_t b_len, float *c, size_t c_len,

@@ -244,4 +244,46 @@ struct ZnRegroupArgs {
     int32_t out_channels, channels, taps_per_channel;
 };
 
+// Multi-head attention with shared key/value heads (kernels/mha_f32.h): query
+// head h of sequence b reads key/value head h / group.  Tensors are [batch,
+// heads, positions, dim] with element strides {batch, head, position} and
+// contiguous dims: qs for q and grad_q, ks for k, v, grad_k and grad_v, os
+// for out and grad_out; lse and delta are contiguous [batch, q_heads, q_len].
+struct ZnMhaArgs {
+    const float *q, *k, *v;
+    float *out, *lse;             // read by the backward
+    const float *grad_out;
+    float *grad_q, *grad_k, *grad_v;
+    float *delta;                 // sum over dims of grad_out * out, written and read by the backward
+    const int32_t *q_lens, *kv_lens;  // per sequence, or null: all of q_len, kv_len
+    int64_t qs[3], ks[3], os[3];
+    int32_t batch, q_heads, kv_heads, group, q_len, kv_len, dim, causal;
+    float scale, scale_log2;      // scale_log2 = scale * log2(e)
+};
+
+// Gated Dense layer, elementwise: z = [gate | up] [rows x 2n].  Forward:
+// h = act(gate) * up.  Backward: grad_z = [grad_h * up * act'(gate) | grad_h * act(gate)].
+struct ZnGateArgs {
+    const float *z;
+    const float *grad_h;  // backward
+    float *h;             // forward
+    float *grad_z;        // backward
+    int64_t rows, n;
+    int32_t act;
+};
+
+// Distillation from a teacher's top logits (zn_distill_*): one row of
+// `logits` (row stride ld) per token, k teacher entries a row.
+struct ZnDistillArgs {
+    const float *logits;
+    const int32_t *index;
+    const float *top;
+    float *loss, *lse;
+    const float *grad_loss;
+    float *grad;
+    int64_t ld, grad_ld, rows;
+    int32_t vocab, k;
+    float temperature, inv_temperature;
+};
+
 #endif
