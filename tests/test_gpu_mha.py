@@ -327,6 +327,14 @@ def test_far_rows(ctx):
     check(got, ref.out, ref.out_bound, "out")
 
 
+def test_keys_without_queries_have_no_gradient(ctx):
+    t = ctx.to_device(np.ones(2 * 3 * 5 * 8, np.float32))
+    for hq, sq in ((0, 4), (2, 0)):
+        gk, gv = (ctx.alloc(2 * 2 * 5 * 8).fill(7.0) for _ in range(2))
+        ctx.mha_backward(t, t, t, t, t, t, t, gk, gv, 2, hq, 2, sq, 5, 8, 1.0)
+        assert (gk.download() == 0).all() and (gv.download() == 0).all()
+
+
 def test_bad_calls_leave_an_error(ctx):
     from zigneuron_amd import InvalidArgumentError
     t = ctx.alloc(4096)

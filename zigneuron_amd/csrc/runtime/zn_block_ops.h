@@ -35,6 +35,8 @@ int mha_args(zn_ctx *ctx, ZnMhaArgs &a, int64_t batch, int64_t q_heads, int64_t 
     constexpr int64_t kMax = INT_MAX / 2;
     if (batch > kMax || q_heads > kMax || q_len > kMax || kv_len > kMax || batch * q_heads > kMax || batch * kv_heads > kMax)
         return ZN_ERR_OVERFLOW;
+    constexpr int64_t kMaxRows = (int64_t)65535 * kMhaTile;  // the grid's second extent
+    if (kv_len > kMaxRows || (kv_heads && q_heads / kv_heads * q_len > kMaxRows)) return ZN_ERR_OVERFLOW;
     std::memset(&a, 0, sizeof(a));
     std::memcpy(a.qs, qs, sizeof(a.qs));
     std::memcpy(a.ks, ks, sizeof(a.ks));
@@ -55,8 +57,10 @@ int mha_args(zn_ctx *ctx, ZnMhaArgs &a, int64_t batch, int64_t q_heads, int64_t 
     return ZN_OK;
 }
 
-int mha_rows(zn_ctx *ctx, MhaKernel kernel, int64_t heads, int64_t rows, ZnMhaArgs &a) {
-    return launch(ctx, ctx->mha[kernel], (unsigned)heads, (unsigned)std::min<int64_t>(cdiv(rows, 4), 65535), 256, &a);
+// One launch over tiles of `rows` query rows or keys.
+int mha_launch(zn_ctx *ctx, MhaKernel kernel, int64_t rows, ZnMhaArgs &a) {
+    const int dim = (a.dim - 1) / 32;
+    return launch(ctx, ctx->mha[kernel][dim], (unsigned)(a.batch * a.kv_heads), (unsigned)cdiv(rows, kMhaTile), kMhaThreads[dim], &a);
 }
 
 }  // namespace
@@ -72,7 +76,7 @@ int zn_hip_mha_forward(zn_ctx *ctx, const float *q, const float *k, const float 
     int rc = mha_args(ctx, a, batch, q_heads, kv_heads, q_len, kv_len, head_dim, scale, causal, q_lens, kv_lens,
                       {q_stride_b, q_stride_h, q_stride_s}, {kv_stride_b, kv_stride_h, kv_stride_s},
                       {out_stride_b, out_stride_h, out_stride_s}, false, &work);
-    if (rc || !work || q_len == 0) return rc;
+    if (rc || !work || q_heads == 0 || q_len == 0) return rc;
     if (!q || !out || (kv_len > 0 && (!k || !v))) return ZN_ERR_INVALID_ARG;
     a.q = q;
     a.k = k;
@@ -80,7 +84,7 @@ int zn_hip_mha_forward(zn_ctx *ctx, const float *q, const float *k, const float 
     a.out = out;
     a.lse = lse;
     if ((rc = select_device(ctx))) return rc;
-    return mha_rows(ctx, kMhaForwardRows, batch * q_heads, q_len, a);
+    return mha_launch(ctx, kMhaForward, a.group * q_len, a);
 }
 
 int zn_hip_mha_backward(zn_ctx *ctx, const float *q, const float *k, const float *v, const float *out,
@@ -96,11 +100,12 @@ int zn_hip_mha_backward(zn_ctx *ctx, const float *q, const float *k, const float
                       {q_stride_b, q_stride_h, q_stride_s}, {kv_stride_b, kv_stride_h, kv_stride_s},
                       {out_stride_b, out_stride_h, out_stride_s}, true, &work);
     if (rc || !work || (q_len == 0 && kv_len == 0)) return rc;
-    if (q_len > 0 && (!q || !out || !lse || !grad_out || !grad_q)) return ZN_ERR_INVALID_ARG;
+    const bool queries = q_heads > 0 && q_len > 0;
+    if (queries && (!q || !out || !lse || !grad_out || !grad_q)) return ZN_ERR_INVALID_ARG;
     if (kv_len > 0 && (!k || !v || !grad_k || !grad_v)) return ZN_ERR_INVALID_ARG;
     if ((rc = select_device(ctx))) return rc;
     Lease delta(ctx);
-    if (q_len > 0 && (rc = delta.get((size_t)(batch * q_heads) * (size_t)q_len))) return rc;
+    if (queries && (rc = delta.get((size_t)(batch * q_heads) * (size_t)q_len))) return rc;
     a.q = q;
     a.k = k;
     a.v = v;
@@ -111,9 +116,8 @@ int zn_hip_mha_backward(zn_ctx *ctx, const float *q, const float *k, const float
     a.grad_k = grad_k;
     a.grad_v = grad_v;
     a.delta = delta.ptr;
-    if (q_len > 0 && (rc = mha_rows(ctx, kMhaGradQRows, batch * q_heads, q_len, a))) return rc;
-    if (kv_len > 0 && (rc = mha_rows(ctx, kMhaGradKvRows, batch * kv_heads, kv_len, a))) return rc;
-    return ZN_OK;
+    if (queries && (rc = mha_launch(ctx, kMhaGradQ, a.group * q_len, a))) return rc;
+    return kv_len > 0 ? mha_launch(ctx, kMhaGradKv, kv_len, a) : ZN_OK;
 }
 
 // ----------------------------------------------------------- gated Dense

@@ -98,9 +98,11 @@ constexpr int kAttnSplitDims[4] = {32, 64, 96, 128};
 constexpr unsigned kAttnSplitThreads[4] = {256, 512, 512, 512};
 constexpr int kAttnSplitQueries[4] = {128, 256, 128, 128};
 
-// Grouped attention (kernels/mha_f32.h), in the attention code object.
-enum MhaKernel { kMhaForwardRows, kMhaGradQRows, kMhaGradKvRows, kNumMha };
-constexpr const char *kMhaName[kNumMha] = {"zn_mha_forward_rows", "zn_mha_grad_q_rows", "zn_mha_grad_kv_rows"};
+// Grouped attention (kernels/mha_f32.h), in the attention code object: zn_mha_<what>_<padded head dim>.
+enum MhaKernel { kMhaForward, kMhaGradQ, kMhaGradKv, kNumMha };
+constexpr const char *kMhaName[kNumMha] = {"zn_mha_forward", "zn_mha_grad_q", "zn_mha_grad_kv"};
+constexpr unsigned kMhaThreads[4] = {256, 256, 512, 512};
+constexpr int kMhaTile = 128;  // query rows or keys of a workgroup
 
 struct ScratchDevice;
 
@@ -183,7 +185,7 @@ struct zn_ctx {
     hipFunction_t attn[2][2] = {};             // fused attention [head dim 32/64][16-byte I/O]
     hipFunction_t attn_split[4] = {};          // the split form [head dim 32/64/96/128]
     hipFunction_t attn_combine = nullptr;      // merges its key ranges
-    hipFunction_t mha[kNumMha] = {};           // grouped attention
+    hipFunction_t mha[kNumMha][4] = {};        // grouped attention [head dim 32/64/96/128]
     hipFunction_t gemm[3][kNumTiles][3] = {};  // [layout][tile][staging: 4-byte, 16-byte, 16-byte unaligned (r only)]
     int gemm_threads[3][kNumTiles][3] = {};    // their workgroup sizes (the kernels' launch bounds)
     hipFunction_t conv[kNumTiles][2][2] = {};  // implicit-GEMM convolution [tile][16-byte W rows][4-pixel gather]
@@ -1999,7 +2001,11 @@ int zn_hip_create(int device, const char *code_object_dir, zn_ctx **out) {
     if (hipModuleGetFunction(&ctx->attn_combine, ctx->attn_module, "zn_attention_combine") != hipSuccess)
         return bail(ZN_ERR_SYMBOL);
     for (int i = 0; i < kNumMha; ++i)
-        if (hipModuleGetFunction(&ctx->mha[i], ctx->attn_module, kMhaName[i]) != hipSuccess) return bail(ZN_ERR_SYMBOL);
+        for (int d = 0; d < 4; ++d) {
+            char name[64];
+            std::snprintf(name, sizeof(name), "%s_%d", kMhaName[i], 32 * (d + 1));
+            if (hipModuleGetFunction(&ctx->mha[i][d], ctx->attn_module, name) != hipSuccess) return bail(ZN_ERR_SYMBOL);
+        }
     void *counters = nullptr;
     if ((e = hipMalloc(&counters, kCounterSlots * kCounterStride * sizeof(int32_t))) != hipSuccess) {
         (void)hipGetLastError();
