@@ -27,6 +27,8 @@
 #include "zn_mfma_stage.h"
 #include "zn_split.h"
 
+#include <type_traits>
+
 namespace {
 
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -101,30 +103,31 @@ __device__ __forceinline__ void mha_row_forward(const ZnMhaArgs &p, int b, int h
     if (p.lse && lane == 0) p.lse[((int64_t)b * p.q_heads + h) * p.q_len + i] = mha_lse(s.m, s.l);
 }
 
-// grad_q of a row; writes delta too.
+// Where a query's lse (log2 domain) and delta lie.
+__device__ __forceinline__ const float *mha_side(const ZnMhaArgs &p, int b, int h, int i) {
+    return p.side + (((int64_t)b * p.q_heads + h) * p.q_blocks + i / 32) * 64 + i % 32;
+}
+
 __device__ __forceinline__ void mha_row_grad_q(const ZnMhaArgs &p, int b, int h, int i, int lane) {
     const MhaSeq seq(p, b);
-    const int64_t at = ((int64_t)b * p.q_heads + h) * p.q_len + i;
     int n = seq.seen(i);
-    const float lse = n ? p.lse[at] : -INFINITY;
-    if (lse == -INFINITY) n = 0;
+    const float *side = mha_side(p, b, h, i);
+    const float lse2 = n ? side[0] : INFINITY, delta = n ? side[32] : 0.0f;
+    if (lse2 == INFINITY) n = 0;
     const float *k = p.k + b * p.ks[0] + (h / p.group) * p.ks[1], *v = p.v + b * p.ks[0] + (h / p.group) * p.ks[1];
-    const int64_t oat = b * p.os[0] + h * p.os[1] + i * p.os[2], qat = b * p.qs[0] + h * p.qs[1] + i * p.qs[2];
+    const int64_t qat = b * p.qs[0] + h * p.qs[1] + i * p.qs[2];
     MhaRow q(p.q + qat, n ? p.dim : 0, lane);
-    const MhaRow g(p.grad_out + oat, n ? p.dim : 0, lane), o(p.out + oat, n ? p.dim : 0, lane);
-    const float delta = g.dot(o);
+    const MhaRow g(p.grad_out + b * p.os[0] + h * p.os[1] + i * p.os[2], n ? p.dim : 0, lane);
     q.a *= p.scale_log2;
     q.b *= p.scale_log2;
     float ga = 0.0f, gb = 0.0f;
     for (int j = 0; j < n; ++j) {
         const MhaRow kr(k + j * p.ks[2], p.dim, lane), vr(v + j * p.ks[2], p.dim, lane);
-        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(lse, -kLog2e, q.dot(kr)));
-        const float ds = e * (g.dot(vr) - delta);
+        const float ds = __builtin_amdgcn_exp2f(q.dot(kr) - lse2) * (g.dot(vr) - delta);
         ga += ds * kr.a;
         gb += ds * kr.b;
     }
     MhaRow::store(p.grad_q + qat, p.dim, lane, ga * p.scale, gb * p.scale);
-    if (lane == 0) p.delta[at] = delta;
 }
 
 // grad_k and grad_v of a row: the query heads of the group in order, their queries ascending.
@@ -136,14 +139,13 @@ __device__ __forceinline__ void mha_row_grad_kv(const ZnMhaArgs &p, int b, int k
     float ka = 0.0f, kb = 0.0f, va = 0.0f, vb = 0.0f;
     for (int h = kh * p.group; in && h < (kh + 1) * p.group; ++h)
         for (int i = seq.first(j); i < seq.ql; ++i) {
-            const int64_t at = ((int64_t)b * p.q_heads + h) * p.q_len + i;
-            const float lse = p.lse[at];
-            if (lse == -INFINITY) continue;
+            const float *side = mha_side(p, b, h, i);
+            if (side[0] == INFINITY) continue;
             const MhaRow q(p.q + b * p.qs[0] + h * p.qs[1] + i * p.qs[2], p.dim, lane);
             const MhaRow g(p.grad_out + b * p.os[0] + h * p.os[1] + i * p.os[2], p.dim, lane);
             const float s = wave_sum((q.a * p.scale_log2) * kr.a + (q.b * p.scale_log2) * kr.b);
-            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(lse, -kLog2e, s));
-            const float ds = e * (g.dot(vr) - p.delta[at]);
+            const float e = __builtin_amdgcn_exp2f(s - side[0]);
+            const float ds = e * (g.dot(vr) - side[32]);
             va += e * g.a;
             vb += e * g.b;
             ka += ds * q.a;
@@ -157,8 +159,8 @@ __device__ __forceinline__ void mha_row_grad_kv(const ZnMhaArgs &p, int b, int k
 // The same on the bf16 matrix cores, every operand value split into three bf16
 // parts (zn_split.h).  One side of the products stays in a wave's registers
 // (queries for O and dQ, keys for dK and dV); the other side's two tensors
-// (K and V, or Q and dO) come past in blocks of 32 rows, split by the thread
-// that loads them and staged in LDS, two stages.
+// (K and V, or Q and dO) come past in blocks of 32 rows, staged in LDS, two
+// stages.
 //
 // A staged tensor serves products over its dims and over its rows: rows lie
 // in slices of 32 dims, a row's 64 bytes as four 16-byte chunks, chunk c the
@@ -167,101 +169,144 @@ __device__ __forceinline__ void mha_row_grad_kv(const ZnMhaArgs &p, int b, int k
 // (ds_read_b64_tr_b16), whose 4 x 16 blocks are the halves of the chunks.  The
 // same chunk order over rows is that of the accumulators: the two 16-row
 // blocks of S that a lane holds are its fragment of the next product.
-template <int DP, int NT>
-struct MhaStage {
+//
+// The splitting is 6.5 vector instructions a value.  Where a tensor goes past
+// many tiles it is split once, by a kernel of its own, into an image of the
+// staged blocks (10 bytes of traffic a value), which the tiles then bring to LDS
+// by DMA (MhaImageStage).  Where it goes past few, the thread that loads a value
+// splits it (MhaRawStage).
+template <int DP>
+struct MhaBlock {
     static constexpr int BR = 32, SL = DP / 32, DB = DP / 16;
-    static constexpr int kPart = BR * DP * 2;  // bytes of one bf16 part of a tensor's block
-    static constexpr int kStage = 6 * kPart;
-    static constexpr int kUnits = BR * DP / 4;  // staging units of 8 values: the first tensor's, then the second's
-    static constexpr int UPT = (kUnits + NT - 1) / NT;
-    static_assert(kUnits / 2 % kWave == 0, "a wave's units are all of one tensor");
-
-    char *lds;
-    const float *base[2];
-    int64_t stride[2];
-    int dim, tid;
-    int frag, tr;      // this lane's place in a fragment over dims, over rows
-    uint32_t off[UPT];
-    int pos[UPT];
-    bool second[UPT];
-    float g[UPT][8];
+    static constexpr int kPart = BR * DP * 2;    // bytes of one bf16 part of a tensor's block
+    static constexpr int kImage = 3 * kPart;     // of a block
+    static constexpr int kStage = 2 * kImage;    // of two tensors' blocks
 
     __device__ static __forceinline__ int slot(int r, int c) { return r * 64 + ((c ^ (-(r >> 2) & 3)) << 4); }
+    // Where row r of a block has chunk lh of slice sl, part q.
+    __device__ static __forceinline__ int place(int r, int lh, int sl, int q) { return q * kPart + sl * (BR * 64) + slot(r, lh); }
+};
 
-    __device__ __forceinline__ MhaStage(char *lds, int tid, int dim, const float *x, int64_t sx, const float *y, int64_t sy)
-        : lds(lds), dim(dim), tid(tid) {
-        base[0] = x;
-        base[1] = y;
-        stride[0] = sx;
-        stride[1] = sy;
-        const int lane = tid & (kWave - 1), li = lane & 15, lh = lane >> 4;
-        frag = slot(li, lh);
-        tr = slot(4 * lh + li / 4, li % 4);
-#pragma unroll
-        for (int j = 0; j < UPT; ++j) {
-            const int u = j * NT + tid;
-            second[j] = __builtin_amdgcn_readfirstlane(u) >= kUnits / 2;
-            const int v = second[j] ? u - kUnits / 2 : u;
-            const int row = v / (DP / 8), dc = v % (DP / 8), d = 32 * (dc / 4) + 4 * (dc % 4);
-            off[j] = (uint32_t)(row * (int)(second[j] ? sy : sx) + d) * 4u;
-            pos[j] = (second[j] ? 3 * kPart : 0) + (dc / 4) * (BR * 64) + slot(row, dc % 4);
-            if (u >= kUnits) off[j] = kOutOfRange;
-        }
-    }
-    // Rows r0 .. r0 + 31 of the two tensors, zeros from row `end` on (and in every row where r0 >= end).
-    __device__ __forceinline__ void load(int r0, int end) {
-        const int n = min(BR, end - r0);
-        __amdgpu_buffer_rsrc_t r[2];
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-            r[t] = make_rsrc(base[t] + (n > 0 ? (int64_t)r0 * stride[t] : 0), n > 0 ? (uint32_t)((n - 1) * (int)stride[t] + dim) * 4u : 0u);
-#pragma unroll
-        for (int j = 0; j < UPT; ++j) {
-            if (j * NT + tid >= kUnits) continue;  // whole waves
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int d = (pos_dim(j) + 16 * h);
-                const uint32_t o = d < dim ? off[j] + 64u * h : kOutOfRange;
-                const zn_f32x4 v = __builtin_bit_cast(zn_f32x4, __builtin_amdgcn_raw_buffer_load_b128(second[j] ? r[1] : r[0], o, 0, 0));
-#pragma unroll
-                for (int e = 0; e < 4; ++e) g[j][4 * h + e] = v[e];
-            }
-        }
-    }
-    // the first dim of unit j's first four
-    __device__ __forceinline__ int pos_dim(int j) const {
-        const int u = j * NT + tid, v = second[j] ? u - kUnits / 2 : u, dc = v % (DP / 8);
-        return 32 * (dc / 4) + 4 * (dc % 4);
-    }
-    // Unit j's values, the first tensor's times `scale`, to stage st.
-    __device__ __forceinline__ void stage(int st, int j, float scale) {
-        if (j * NT + tid >= kUnits) return;
-        if (dim & 3) {  // the last four of a row end inside it
-            const int d = pos_dim(j);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) g[j][e] = d + (e < 4 ? e : 12 + e) < dim ? g[j][e] : 0.0f;
-        }
-        float x[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = second[j] ? g[j][e] : g[j][e] * scale;
-        zn_u32x4 w[3];
-        split8(x, w);
-#pragma unroll
-        for (int q = 0; q < 3; ++q) *reinterpret_cast<zn_u32x4 *>(lds + st * kStage + pos[j] + q * kPart) = w[q];
+// Fragments of a staged block.
+template <int DP>
+struct MhaFrags : MhaBlock<DP> {
+    typedef MhaBlock<DP> B;
+    const char *lds;
+    int frag, tr;  // this lane's place in a fragment over dims, over rows
+    __device__ __forceinline__ MhaFrags(const char *lds, int lane) : lds(lds) {
+        frag = B::slot(lane & 15, lane >> 4);
+        tr = B::slot(4 * (lane >> 4) + (lane & 15) / 4, lane % 4);
     }
     // Part q of tensor t: rows 16 rb + li, chunk lh of slice sl
     __device__ __forceinline__ zn_bf16x8 dims(int st, int t, int q, int sl, int rb) const {
-        return __builtin_bit_cast(
-            zn_bf16x8, *reinterpret_cast<const zn_u32x4 *>(lds + st * kStage + (3 * t + q) * kPart + sl * (BR * 64) + rb * (16 * 64) + frag));
+        return __builtin_bit_cast(zn_bf16x8, *reinterpret_cast<const zn_u32x4 *>(lds + st * B::kStage + t * B::kImage + q * B::kPart +
+                                                                                sl * (B::BR * 64) + rb * (16 * 64) + frag));
     }
     // ... dims 16 db + li, rows 4 lh .. 4 lh + 3 and 16 + 4 lh .. 16 + 4 lh + 3
     __device__ __forceinline__ zn_bf16x8 rows(int st, int t, int q, int db) const {
         typedef short s4 __attribute__((ext_vector_type(4)));
-        typedef short s8 __attribute__((ext_vector_type(8)));
         typedef __attribute__((address_space(3))) s4 ls4;
-        char *at = lds + st * kStage + (3 * t + q) * kPart + (db / 2) * (BR * 64) + 8 * (db & 1) + tr;
+        const char *at = lds + st * B::kStage + t * B::kImage + q * B::kPart + (db / 2) * (B::BR * 64) + 8 * (db & 1) + tr;
         const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ls4 *)at), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ls4 *)(at + 16 * 64));
         return __builtin_bit_cast(zn_bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+};
+
+// Blocks of two tensors from their images, NW waves.
+template <int DP, int NW>
+struct MhaImageStage {
+    typedef MhaBlock<DP> B;
+    static constexpr int kChunks = B::kImage / 1024;  // wave instructions a tensor
+    char *lds;
+    const char *src[2];  // the images of the current heads
+    int wave;
+    uint32_t lane16;
+    __device__ __forceinline__ MhaImageStage(char *lds, int tid, const char *x, const char *y) : lds(lds), src{x, y} {
+        wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+        lane16 = (tid & (kWave - 1)) * 16;
+    }
+    // buffer_load ... lds, as DmaStage issues it: 1 KB at LDS address `to` from byte `at` of r
+    __device__ static __forceinline__ void dma(__amdgpu_buffer_rsrc_t r, char *to, uint32_t lane16, uint32_t at) {
+        const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(zn_lds_void *)to);
+        asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" : : "s"(m0), "v"(lane16), "s"(r), "s"(at) : "memory");
+    }
+    __device__ __forceinline__ void fetch(int st, int blk) {
+        __amdgpu_buffer_rsrc_t r[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+            r[t] = make_rsrc(reinterpret_cast<const float *>(src[t] + (int64_t)blk * B::kImage), B::kImage);
+#pragma unroll
+        for (int i = 0; i < (2 * kChunks + NW - 1) / NW; ++i) {
+            const int c = i * NW + wave, t = c >= kChunks;
+            if (c < 2 * kChunks) dma(t ? r[1] : r[0], lds + st * B::kStage + c * 1024, lane16, (uint32_t)(c - t * kChunks) * 1024u);
+        }
+    }
+    __device__ __forceinline__ void arrive() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+    __device__ __forceinline__ void commit(int) {}
+};
+
+// Blocks of K and V from the tensors themselves.
+template <int DP, int NW>
+struct MhaRawStage {
+    typedef MhaBlock<DP> B;
+    static constexpr int NT = NW * kWave;
+    static constexpr int kUnits = B::BR * DP / 4;  // staging units of 8 values: the first tensor's, then the second's
+    static constexpr int UPT = (kUnits + NT - 1) / NT;
+    static_assert(kUnits / 2 % kWave == 0, "a wave's units are all of one tensor");
+
+    char *lds;
+    const float *src[2];
+    int64_t stride;
+    int dim, tid, end;  // rows from `end` on are zeros
+    float g[UPT][8];
+
+    __device__ __forceinline__ MhaRawStage(char *lds, int tid, const float *x, const float *y, int64_t stride, int dim, int end)
+        : lds(lds), src{x, y}, stride(stride), dim(dim), tid(tid), end(end) {}
+    // Unit j's tensor, row, slice and chunk.
+    __device__ __forceinline__ void unit(int j, bool &second, int &row, int &sl, int &c) const {
+        const int u = j * NT + tid;
+        second = __builtin_amdgcn_readfirstlane(u) >= kUnits / 2;
+        const int v = second ? u - kUnits / 2 : u, dc = v % (DP / 8);
+        row = v / (DP / 8);
+        sl = dc / 4;
+        c = dc % 4;
+    }
+    __device__ __forceinline__ void fetch(int, int blk) {
+        const int r0 = blk * B::BR, n = min(B::BR, end - r0);
+        const uint32_t bytes = n > 0 ? (uint32_t)((n - 1) * (int)stride + dim) * 4u : 0u;
+        __amdgpu_buffer_rsrc_t r[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) r[t] = make_rsrc(src[t] + (n > 0 ? (int64_t)r0 * stride : 0), bytes);
+#pragma unroll
+        for (int j = 0; j < UPT; ++j) {
+            if (j * NT + tid >= kUnits) continue;  // whole waves
+            bool second;
+            int row, sl, c;
+            unit(j, second, row, sl, c);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int d = 32 * sl + 4 * c + 16 * h;
+                const uint32_t o = d < dim ? (uint32_t)(row * (int)stride + d) * 4u : kOutOfRange;
+                const zn_f32x4 v = __builtin_bit_cast(zn_f32x4, __builtin_amdgcn_raw_buffer_load_b128(second ? r[1] : r[0], o, 0, 0));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) g[j][4 * h + e] = d + e < dim ? v[e] : 0.0f;
+            }
+        }
+    }
+    __device__ __forceinline__ void arrive() {}
+    __device__ __forceinline__ void commit(int st) {
+#pragma unroll
+        for (int j = 0; j < UPT; ++j) {
+            if (j * NT + tid >= kUnits) continue;
+            bool second;
+            int row, sl, c;
+            unit(j, second, row, sl, c);
+            zn_u32x4 w[3];
+            split8(g[j], w);
+#pragma unroll
+            for (int q = 0; q < 3; ++q)
+                *reinterpret_cast<zn_u32x4 *>(lds + st * B::kStage + (second ? B::kImage : 0) + B::place(row, c, sl, q)) = w[q];
+        }
     }
 };
 
@@ -328,11 +373,14 @@ struct MhaQuery {
     }
 };
 
-// O and lse (BACK false) or dQ and delta (BACK true) of NW x FQ x 16 query rows.
-template <int DP, int NW, int FQ, bool BACK>
+// O and lse (BACK false, K and V split here or before) or dQ (BACK true, everything split before) of NW x FQ x 16 query rows.
+template <int DP, int NW, int FQ, bool BACK, bool IMAGE>
 struct MhaQueryTile {
-    typedef MhaStage<DP, NW * kWave> Stage;
-    static constexpr int SL = Stage::SL, DB = Stage::DB;
+    typedef MhaFrags<DP> Frags;
+    typedef typename std::conditional<IMAGE, MhaImageStage<DP, NW>, MhaRawStage<DP, NW>>::type Stage;
+    static constexpr int SL = Frags::SL, DB = Frags::DB;
+    static constexpr int kBytes = 2 * Frags::kStage;
+    static_assert(IMAGE || !BACK, "the backward's tensors are all split before");
 
     __device__ static __forceinline__ void run(const ZnMhaArgs &p, char *lds) {
         const int tid = threadIdx.x, lane = tid & (kWave - 1);
@@ -340,10 +388,11 @@ struct MhaQueryTile {
         const int li = lane & 15, lh = lane >> 4;
         const int b = blockIdx.x / p.kv_heads, kh = blockIdx.x - b * p.kv_heads;
         const int rows = p.group * p.q_len;
-        // causal rows see more the later they come: the long tiles first
-        const int r0 = (int)(gridDim.y - 1 - blockIdx.y) * (NW * FQ * 16), w0 = r0 + wave * FQ * 16;
+        // causal rows see more the later they come: the last tiles of each head first
+        const int per = (int)gridDim.y / p.group, g0 = (int)blockIdx.y % p.group;
+        const int r0 = (g0 * per + per - 1 - (int)blockIdx.y / p.group) * (NW * FQ * 16), w0 = r0 + wave * FQ * 16;
+        if (r0 >= rows) return;
         const MhaSeq seq(p, b);
-        const float *k = p.k + b * p.ks[0] + kh * p.ks[1], *v = p.v + b * p.ks[0] + kh * p.ks[1];
 
         // keys that the tile's rows see: none past `last`; the wave's rows all see those before `all`
         int lim[FQ], all = INT_MAX, any = 0;
@@ -353,29 +402,27 @@ struct MhaQueryTile {
         for (int f = 0; f < FQ; ++f) {
             const MhaQuery r(p, kh, w0 + 16 * f + li);
             lim[f] = r.in ? seq.seen(r.i) : 0;
-            const float *q = p.q + b * p.qs[0] + r.h * p.qs[1] + r.i * p.qs[2];
             if constexpr (BACK) {
-                const int64_t at = ((int64_t)b * p.q_heads + r.h) * p.q_len + r.i;
-                const float lse = lim[f] ? p.lse[at] : -INFINITY;
-                if (lse == -INFINITY) lim[f] = 0;
-                lse2[f] = lse;
-                const int64_t oat = b * p.os[0] + r.h * p.os[1] + r.i * p.os[2];
-                const float *g = lim[f] ? p.grad_out + oat : nullptr, *o = lim[f] ? p.out + oat : nullptr;
-                mha_row_frags<SL>(g, p.dim, lh, 1.0f, gf[f]);
-                float sum = 0.0f;
+                const float *side = mha_side(p, b, r.h, r.i);
+                lse2[f] = lim[f] ? side[0] : INFINITY;
+                delta[f] = lim[f] ? side[32] : 0.0f;
+                const int64_t at = (((int64_t)b * p.q_heads + r.h) * p.q_blocks + r.i / 32) * Frags::kImage;
 #pragma unroll
-                for (int c = 0; c < 2 * SL; ++c)
+                for (int sl = 0; sl < SL; ++sl)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int d = 16 * c + 4 * lh + e;
-                        if (lim[f] && d < p.dim) sum = __builtin_fmaf(g[d], o[d], sum);
+                    for (int q = 0; q < 3; ++q) {
+                        const int64_t o = at + Frags::place(r.i % 32, lh, sl, q);
+                        zn_u32x4 x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
+                        if (lim[f]) {
+                            x = *reinterpret_cast<const zn_u32x4 *>(p.qi + o);
+                            y = *reinterpret_cast<const zn_u32x4 *>(p.gi + o);
+                        }
+                        qf[f][sl][q] = __builtin_bit_cast(zn_bf16x8, x);
+                        gf[f][sl][q] = __builtin_bit_cast(zn_bf16x8, y);
                     }
-                sum += __shfl_xor(sum, 16);
-                sum += __shfl_xor(sum, 32);
-                delta[f] = sum;
-                if (r.in && lh == 0) p.delta[at] = sum;
+            } else {
+                mha_row_frags<SL>(lim[f] ? p.q + b * p.qs[0] + r.h * p.qs[1] + r.i * p.qs[2] : nullptr, p.dim, lh, p.scale_log2, qf[f]);
             }
-            mha_row_frags<SL>(lim[f] ? q : nullptr, p.dim, lh, p.scale_log2, qf[f]);
             all = min(all, lim[f]);
             any = max(any, lim[f]);
         }
@@ -401,19 +448,29 @@ struct MhaQueryTile {
             for (int d = 0; d < DB; ++d) o[f][d] = zn_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
 
-        Stage sg(lds, tid, p.dim, k, p.ks[2], v, p.ks[2]);
+        const Frags fr(lds, lane);
         const int nblk = (last + 31) / 32;
-        sg.load(0, seq.kl);
-#pragma unroll
-        for (int j = 0; j < Stage::UPT; ++j) sg.stage(0, j, 1.0f);
-        for (int blk = 0; blk < nblk; ++blk) {
-            const int st = blk & 1, k0 = 32 * blk;
-            __syncthreads();  // block blk is in LDS; every wave is done with block blk - 1
-            sg.load(k0 + 32, blk + 1 < nblk ? seq.kl : 0);
-            if (k0 + 32 <= all) block<false>(sg, st, k0, lane, lim, qf, gf, lse2, delta, o, m, l);
-            else if (k0 < any) block<true>(sg, st, k0, lane, lim, qf, gf, lse2, delta, o, m, l);
-#pragma unroll
-            for (int j = 0; j < Stage::UPT; ++j) sg.stage(st ^ 1, j, 1.0f);
+        auto walk = [&](Stage sg) {
+            if (nblk > 0) {
+                sg.fetch(0, 0);
+                sg.commit(0);
+            }
+            for (int blk = 0; blk < nblk; ++blk) {
+                const int st = blk & 1, k0 = 32 * blk;
+                sg.arrive();
+                __syncthreads();  // block blk is in LDS; every wave is done with block blk - 1
+                if (blk + 1 < nblk) sg.fetch(st ^ 1, blk + 1);
+                if (k0 + 32 <= all) block<false>(fr, st, k0, lane, lim, qf, gf, lse2, delta, o, m, l);
+                else if (k0 < any) block<true>(fr, st, k0, lane, lim, qf, gf, lse2, delta, o, m, l);
+                if (blk + 1 < nblk) sg.commit(st ^ 1);
+            }
+        };
+        if constexpr (IMAGE) {
+            const int64_t at = ((int64_t)b * p.kv_heads + kh) * p.k_blocks * Frags::kImage;
+            walk(Stage(lds, tid, p.ki + at, p.vi + at));
+        } else {
+            const int64_t at = b * p.ks[0] + kh * p.ks[1];
+            walk(Stage(lds, tid, p.k + at, p.v + at, p.ks[2], p.dim, seq.kl));
         }
 
         bool bad = false;
@@ -460,7 +517,7 @@ struct MhaQueryTile {
 
     // One block of 32 keys: S^T = K (cQ)^T (and dP^T = V dO^T), then O^T += V^T P^T or dQ^T += K^T dS^T.
     template <bool MASK>
-    __device__ static __forceinline__ void block(const Stage &sg, int st, int k0, int lane, const int (&lim)[FQ],
+    __device__ static __forceinline__ void block(const Frags &sg, int st, int k0, int lane, const int (&lim)[FQ],
                                                  const zn_bf16x8 (&qf)[FQ][SL][3], const zn_bf16x8 (&gf)[BACK ? FQ : 1][SL][3],
                                                  const float (&lse2)[FQ], const float (&delta)[FQ], zn_f32x4 (&o)[FQ][DB],
                                                  float (&m)[FQ], float (&l)[FQ]) {
@@ -497,10 +554,9 @@ struct MhaQueryTile {
         for (int f = 0; f < FQ; ++f) {
             float x[8];
             if constexpr (BACK) {
-                const float ml = lse2[f] * -kLog2e;  // its rounding moves the whole row by less than its scores' own
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const float pe = __builtin_amdgcn_exp2f(__builtin_fmaf(s[f][e / 4][e % 4], kSplitUnscale, ml));
+                    const float pe = __builtin_amdgcn_exp2f(__builtin_fmaf(s[f][e / 4][e % 4], kSplitUnscale, -lse2[f]));
                     const float de = __builtin_fmaf(dp[f][e / 4][e % 4], kSplitUnscale, -delta[f]);
                     x[e] = pe * de;
                     if (MASK && k0 + 16 * (e / 4) + 4 * lh + e % 4 >= lim[f]) x[e] = 0.0f;
@@ -552,10 +608,10 @@ struct MhaQueryTile {
 // in LDS).  S = (cQ) K^T and dP = dO V^T, dV^T += dO^T P and dK^T += Q^T dS.
 template <int DP, int NW, int FK>
 struct MhaKeyTile {
-    typedef MhaStage<DP, NW * kWave> Stage;
-    static constexpr int SL = Stage::SL, DB = Stage::DB;
-    static constexpr int kRows = 2 * Stage::kStage;     // lse and delta of two stages' rows: [stage][lse, delta][32]
-    static constexpr int kBytes = kRows + 2 * 2 * 32 * 4;
+    typedef MhaFrags<DP> Frags;
+    static constexpr int SL = Frags::SL, DB = Frags::DB;
+    static constexpr int kSide = 2 * Frags::kStage;  // lse and delta of two stages' rows: [stage][lse, delta][32]
+    static constexpr int kBytes = kSide + 2 * 64 * 4;
 
     __device__ static __forceinline__ void run(const ZnMhaArgs &p, char *lds) {
         const int tid = threadIdx.x, lane = tid & (kWave - 1);
@@ -571,46 +627,55 @@ struct MhaKeyTile {
 #pragma unroll
         for (int f = 0; f < FK; ++f) {
             const int j = w0 + 16 * f + li;
-            mha_row_frags<SL>(j < seq.kl ? p.k + kat + j * p.ks[2] : nullptr, p.dim, lh, 1.0f, kf[f]);
-            mha_row_frags<SL>(j < seq.kl ? p.v + kat + j * p.ks[2] : nullptr, p.dim, lh, 1.0f, vf[f]);
+            const int64_t at = (((int64_t)b * p.kv_heads + kh) * p.k_blocks + j / 32) * Frags::kImage;
+#pragma unroll
+            for (int sl = 0; sl < SL; ++sl)
+#pragma unroll
+                for (int q = 0; q < 3; ++q) {
+                    const int64_t o = at + Frags::place(j % 32, lh, sl, q);
+                    zn_u32x4 x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
+                    if (j < seq.kl) {
+                        x = *reinterpret_cast<const zn_u32x4 *>(p.ki + o);
+                        y = *reinterpret_cast<const zn_u32x4 *>(p.vi + o);
+                    }
+                    kf[f][sl][q] = __builtin_bit_cast(zn_bf16x8, x);
+                    vf[f][sl][q] = __builtin_bit_cast(zn_bf16x8, y);
+                }
 #pragma unroll
             for (int d = 0; d < DB; ++d) dk[f][d] = dv[f][d] = zn_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
         // query blocks of a head that see any of the tile's keys
         const int b0 = j0 < seq.kl ? seq.first(j0) / 32 : 0, nb = j0 < seq.kl ? max(0, (seq.ql + 31) / 32 - b0) : 0;
         const int total = nb * p.group;
-        float *side = reinterpret_cast<float *>(lds + kRows);
-        float mine = 0.0f;
-        auto enter = [&](Stage &sg, int t) {  // block t's tensors and, in the first wave, its rows' lse and delta
-            const int g = nb ? t / nb : 0, h = kh * p.group + g, i0 = 32 * (b0 + t - g * nb);
-            const bool in = t < total;
-            sg.base[0] = p.q + b * p.qs[0] + (in ? h : 0) * p.qs[1];
-            sg.base[1] = p.grad_out + b * p.os[0] + (in ? h : 0) * p.os[1];
-            sg.load(i0, in ? seq.ql : 0);
-            if (wave == 0) {
-                const int i = i0 + (lane & 31);
-                mine = lane < 32 ? -INFINITY : 0.0f;
-                if (in && i < seq.ql) mine = (lane < 32 ? p.lse : p.delta)[((int64_t)b * p.q_heads + h) * p.q_len + i];
-                // exp2(s - inf) = 0: a row that sees nothing has no probabilities
-                if (lane < 32) mine = mine == -INFINITY ? INFINITY : mine * kLog2e;
+        const float *side = reinterpret_cast<const float *>(lds + kSide);
+        const int64_t head0 = ((int64_t)b * p.q_heads + kh * p.group) * p.q_blocks;  // the group's first query block
+        MhaImageStage<DP, NW> sg(lds, tid, nullptr, nullptr);
+        auto fetch = [&](int st, int g, int blk) {
+            const int64_t at = head0 + (int64_t)g * p.q_blocks;
+            sg.src[0] = p.qi + at * Frags::kImage;
+            sg.src[1] = p.gi + at * Frags::kImage;
+            sg.fetch(st, blk);
+            if (wave == NW - 1) {  // 256 bytes: a value to a lane
+                const __amdgpu_buffer_rsrc_t r = make_rsrc(p.side + (at + blk) * 64, 256);
+                const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(zn_lds_void *)(lds + kSide + st * 256));
+                asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, 0 offen lds" : : "s"(m0), "v"(sg.lane16 / 4), "s"(r) : "memory");
             }
         };
-        auto leave = [&](Stage &sg, int st) {
-#pragma unroll
-            for (int j = 0; j < Stage::UPT; ++j) sg.stage(st, j, p.scale_log2);
-            if (wave == 0) side[st * 64 + lane] = mine;
-        };
-        Stage sg(lds, tid, p.dim, p.q, p.qs[2], p.grad_out, p.os[2]);
-        enter(sg, 0);
-        leave(sg, 0);
+        const Frags fr(lds, lane);
+        int g = 0, blk = b0;
+        if (total > 0) fetch(0, g, blk);
         for (int t = 0; t < total; ++t) {
-            const int st = t & 1, i0 = 32 * (b0 + t % nb);
+            const int st = t & 1, i0 = 32 * blk;
+            sg.arrive();
             __syncthreads();
-            enter(sg, t + 1);
+            if (++blk == b0 + nb) {
+                blk = b0;
+                ++g;
+            }
+            if (t + 1 < total) fetch(st ^ 1, g, blk);
             const int hi = w0 + FK * 16;  // keys of this wave: [w0, hi)
-            if (i0 + seq.edge >= hi - 1 && hi <= seq.kl) block<false>(sg, st, side + st * 64, i0, w0, seq, lane, kf, vf, dk, dv);
-            else if (min(i0 + 31, seq.ql - 1) + seq.edge >= w0 && w0 < seq.kl) block<true>(sg, st, side + st * 64, i0, w0, seq, lane, kf, vf, dk, dv);
-            leave(sg, st ^ 1);
+            if (i0 + seq.edge >= hi - 1 && hi <= seq.kl) block<false>(fr, st, side + st * 64, i0, w0, seq, lane, kf, vf, dk, dv);
+            else if (min(i0 + 31, seq.ql - 1) + seq.edge >= w0 && w0 < seq.kl) block<true>(fr, st, side + st * 64, i0, w0, seq, lane, kf, vf, dk, dv);
         }
 
         bool bad = false;
@@ -641,7 +706,7 @@ struct MhaKeyTile {
     }
 
     template <bool MASK>
-    __device__ static __forceinline__ void block(const Stage &sg, int st, const float *side, int i0, int w0, const MhaSeq &seq,
+    __device__ static __forceinline__ void block(const Frags &sg, int st, const float *side, int i0, int w0, const MhaSeq &seq,
                                                  int lane, const zn_bf16x8 (&kf)[FK][SL][3], const zn_bf16x8 (&vf)[FK][SL][3],
                                                  zn_f32x4 (&dk)[FK][DB], zn_f32x4 (&dv)[FK][DB]) {
         const int li = lane & 15, lh = lane >> 4;
@@ -712,25 +777,79 @@ struct MhaKeyTile {
     }
 };
 
+// Tensors to their images: a workgroup to a block of 32 rows, a unit of 8
+// values to a thread and step.  Rows past a sequence's length are zeros, and on
+// the query side rows that see nothing (lse -inf); blocks past it are not read
+// and not written.  10 bytes of traffic a value, and out's 4 for delta.
+template <int DP>
+__device__ __forceinline__ void mha_split(const ZnMhaSplitArgs &a) {
+    typedef MhaBlock<DP> B;
+    int which = 0;
+#pragma unroll
+    for (int i = 1; i < 4; ++i)
+        if (i < a.ops && (int)blockIdx.x >= a.op[i].first) which = i;
+    const ZnMhaSplitOp &p = a.op[which];
+    const int wg = (int)blockIdx.x - p.first, blk = wg % p.blocks, bh = wg / p.blocks, b = bh / p.heads, h = bh - b * p.heads;
+    const int n = p.lens ? min(max(p.lens[b], 0), p.len) : p.len, r0 = 32 * blk;
+    if (r0 >= n) return;
+    const int64_t at = b * p.stride[0] + h * p.stride[1];
+    char *dst = p.dst + ((int64_t)bh * p.blocks + blk) * B::kImage;
+    for (int u = threadIdx.x; u < B::SL * 32 * 4; u += 256) {
+        const int sl = u / 128, row = u / 4 % 32, c = u % 4, i = r0 + row;
+        const bool in = i < n && !(p.lse && p.lse[(int64_t)bh * p.len + i] == -INFINITY);
+        const float *src = p.src + at + i * p.stride[2];
+        float x[8];
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            const int d = 32 * sl + 4 * c + 16 * g;
+            zn_f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (in && d + 4 <= a.dim) {
+                v = *reinterpret_cast<const zn_f32x4u *>(src + d);
+            } else if (in) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (d + e < a.dim) v[e] = src[d + e];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[4 * g + e] = v[e] * p.scale;
+        }
+        zn_u32x4 w[3];
+        split8(x, w);
+#pragma unroll
+        for (int q = 0; q < 3; ++q) *reinterpret_cast<zn_u32x4 *>(dst + B::place(row, c, sl, q)) = w[q];
+    }
+    if (p.side) {  // 8 threads to a row
+        const int row = threadIdx.x / 8, i = r0 + row;
+        const float lse = i < n ? p.lse[(int64_t)bh * p.len + i] : -INFINITY;
+        const float *g = p.src + at + i * p.stride[2], *o = p.out + at + i * p.stride[2];
+        float sum = 0.0f;
+        if (lse != -INFINITY)
+            for (int d = threadIdx.x % 8; d < a.dim; d += 8) sum = __builtin_fmaf(g[d], o[d], sum);
+#pragma unroll
+        for (int s = 1; s < 8; s <<= 1) sum += __shfl_xor(sum, s);
+        float *side = p.side + ((int64_t)bh * p.blocks + blk) * 64 + row;
+        if (threadIdx.x % 8 == 0) {
+            side[0] = lse == -INFINITY ? INFINITY : lse * kLog2e;
+            side[32] = sum;
+        }
+    }
+}
+
 }  // namespace
 
 // Grid: x = sequence and key/value head (its tiles share an XCD's L2), y = tiles.
-#define ZN_MHA_KERNELS(DP, NW, FQ, FK)                                                                       \
-    extern "C" __global__ __launch_bounds__(NW * 64, 2) void zn_mha_forward_##DP(ZnMhaArgs p) {              \
-        typedef MhaQueryTile<DP, NW, FQ, false> T;                                                           \
-        __shared__ __attribute__((aligned(1024))) char lds[2 * T::Stage::kStage];                            \
-        T::run(p, lds);                                                                                      \
-    }                                                                                                        \
-    extern "C" __global__ __launch_bounds__(NW * 64, 2) void zn_mha_grad_q_##DP(ZnMhaArgs p) {               \
-        typedef MhaQueryTile<DP, NW, FQ, true> T;                                                            \
-        __shared__ __attribute__((aligned(1024))) char lds[2 * T::Stage::kStage];                            \
-        T::run(p, lds);                                                                                      \
-    }                                                                                                        \
-    extern "C" __global__ __launch_bounds__(NW * 64, 2) void zn_mha_grad_kv_##DP(ZnMhaArgs p) {              \
-        typedef MhaKeyTile<DP, NW, FK> T;                                                                    \
-        __shared__ __attribute__((aligned(1024))) char lds[T::kBytes];                                       \
-        T::run(p, lds);                                                                                      \
+#define ZN_MHA_KERNEL(NAME, NW, ...)                                                  \
+    extern "C" __global__ __launch_bounds__(NW * 64, 2) void NAME(ZnMhaArgs p) {      \
+        typedef __VA_ARGS__ T;                                                        \
+        __shared__ __attribute__((aligned(1024))) char lds[T::kBytes];                \
+        T::run(p, lds);                                                               \
     }
+#define ZN_MHA_KERNELS(DP, NW, FQ, FK)                                                                          \
+    ZN_MHA_KERNEL(zn_mha_forward_##DP, NW, MhaQueryTile<DP, NW, FQ, false, true>)                               \
+    ZN_MHA_KERNEL(zn_mha_forward_raw_##DP, NW, MhaQueryTile<DP, NW, FQ, false, false>)                          \
+    ZN_MHA_KERNEL(zn_mha_grad_q_##DP, NW, MhaQueryTile<DP, NW, FQ, true, true>)                                 \
+    ZN_MHA_KERNEL(zn_mha_grad_kv_##DP, NW, MhaKeyTile<DP, NW, FK>)                                              \
+    extern "C" __global__ __launch_bounds__(256) void zn_mha_split_##DP(ZnMhaSplitArgs a) { mha_split<DP>(a); }
 ZN_MHA_KERNELS(32, 4, 2, 2)
 ZN_MHA_KERNELS(64, 4, 2, 2)
 ZN_MHA_KERNELS(96, 8, 1, 1)

@@ -16,7 +16,7 @@ constexpr int64_t kMhaMaxRow = (int64_t)1 << 22;  // position stride: a block of
 bool mha_strides_ok(int64_t sb, int64_t sh, int64_t ss, int64_t batch, int64_t heads, int64_t rows, int64_t dim,
                     bool written) {
     if (ss < dim || ss > kMhaMaxRow || sb < 0 || sh < 0) return false;
-    return !written || rows == 0 || ((sb > 0 || batch <= 1) && (sh > 0 || heads <= 1));
+    return !written || rows == 0 || heads == 0 || ((sb > 0 || batch <= 1) && (sh > 0 || heads <= 1));
 }
 
 // The checks and the argument block that both directions share.  *work: there is something to do.
@@ -57,11 +57,43 @@ int mha_args(zn_ctx *ctx, ZnMhaArgs &a, int64_t batch, int64_t q_heads, int64_t 
     return ZN_OK;
 }
 
-// One launch over tiles of `rows` query rows or keys.
-int mha_launch(zn_ctx *ctx, MhaKernel kernel, int64_t rows, ZnMhaArgs &a) {
+// One launch over tiles of query rows or keys.
+int mha_tiles(zn_ctx *ctx, MhaKernel kernel, ZnMhaArgs &a) {
     const int dim = (a.dim - 1) / 32;
-    return launch(ctx, ctx->mha[kernel][dim], (unsigned)(a.batch * a.kv_heads), (unsigned)cdiv(rows, kMhaTile), kMhaThreads[dim], &a);
+    // query rows: the same number of tiles for each head of the group, whose last ones start first
+    const int64_t y = kernel == kMhaGradKv ? cdiv(a.kv_len, kMhaTile) : a.group * cdiv(cdiv((int64_t)a.group * a.q_len, kMhaTile), a.group);
+    return launch(ctx, ctx->mha[kernel][dim], (unsigned)(a.batch * a.kv_heads), (unsigned)y, kMhaThreads[dim], &a);
 }
+
+// The images that a call's tiles read (kernels/mha_f32.h), in one leased buffer.
+struct MhaImages {
+    Lease lease;
+    ZnMhaSplitArgs s;
+    int64_t bytes = 0, groups = 0;
+    explicit MhaImages(zn_ctx *ctx) : lease(ctx) { std::memset(&s, 0, sizeof(s)); }
+    // A tensor's image: its offset in the buffer.
+    int64_t add(const ZnMhaArgs &a, const float *src, const int64_t (&stride)[3], const int32_t *lens, int heads, int len, float scale) {
+        ZnMhaSplitOp &op = s.op[s.ops++];
+        op.src = src;
+        std::memcpy(op.stride, stride, sizeof(op.stride));
+        op.lens = lens;
+        op.heads = heads;
+        op.len = len;
+        op.blocks = (int32_t)cdiv(len, 32);
+        op.scale = scale;
+        op.first = (int32_t)groups;
+        groups += (int64_t)a.batch * heads * op.blocks;
+        const int64_t at = bytes;
+        bytes += (int64_t)a.batch * heads * op.blocks * (192 * 32) * cdiv(a.dim, 32);
+        return at;
+    }
+    int get(int64_t more) { return lease.get((size_t)((bytes + more) / 4)); }
+    char *at(int64_t offset) const { return reinterpret_cast<char *>(lease.ptr) + offset; }
+    int run(zn_ctx *ctx, const ZnMhaArgs &a) {
+        s.dim = a.dim;
+        return groups ? launch(ctx, ctx->mha[kMhaSplit][(a.dim - 1) / 32], (unsigned)groups, 1, 256, &s) : ZN_OK;
+    }
+};
 
 }  // namespace
 
@@ -78,13 +110,23 @@ int zn_hip_mha_forward(zn_ctx *ctx, const float *q, const float *k, const float 
                       {out_stride_b, out_stride_h, out_stride_s}, false, &work);
     if (rc || !work || q_heads == 0 || q_len == 0) return rc;
     if (!q || !out || (kv_len > 0 && (!k || !v))) return ZN_ERR_INVALID_ARG;
+    if ((rc = select_device(ctx))) return rc;
     a.q = q;
     a.k = k;
     a.v = v;
     a.out = out;
     a.lse = lse;
-    if ((rc = select_device(ctx))) return rc;
-    return mha_launch(ctx, kMhaForward, a.group * q_len, a);
+    // Each tile splits what it reads: past a few tiles, once for all of them is cheaper.
+    if (a.group * q_len <= 4 * kMhaTile) return mha_tiles(ctx, kMhaForwardRaw, a);
+    MhaImages im(ctx);
+    const int64_t ki = im.add(a, k, a.ks, a.kv_lens, a.kv_heads, a.kv_len, 1.0f), vi = im.add(a, v, a.ks, a.kv_lens, a.kv_heads, a.kv_len, 1.0f);
+    if (im.groups > INT_MAX / 2) return ZN_ERR_OVERFLOW;
+    if ((rc = im.get(0))) return rc;
+    a.k_blocks = im.s.op[0].blocks;
+    a.ki = im.s.op[0].dst = im.at(ki);
+    a.vi = im.s.op[1].dst = im.at(vi);
+    if ((rc = im.run(ctx, a))) return rc;
+    return mha_tiles(ctx, kMhaForward, a);
 }
 
 int zn_hip_mha_backward(zn_ctx *ctx, const float *q, const float *k, const float *v, const float *out,
@@ -104,20 +146,32 @@ int zn_hip_mha_backward(zn_ctx *ctx, const float *q, const float *k, const float
     if (queries && (!q || !out || !lse || !grad_out || !grad_q)) return ZN_ERR_INVALID_ARG;
     if (kv_len > 0 && (!k || !v || !grad_k || !grad_v)) return ZN_ERR_INVALID_ARG;
     if ((rc = select_device(ctx))) return rc;
-    Lease delta(ctx);
-    if (queries && (rc = delta.get((size_t)(batch * q_heads) * (size_t)q_len))) return rc;
     a.q = q;
     a.k = k;
     a.v = v;
-    a.out = const_cast<float *>(out);
-    a.lse = const_cast<float *>(lse);
     a.grad_out = grad_out;
     a.grad_q = grad_q;
     a.grad_k = grad_k;
     a.grad_v = grad_v;
-    a.delta = delta.ptr;
-    if (queries && (rc = mha_launch(ctx, kMhaGradQ, a.group * q_len, a))) return rc;
-    return kv_len > 0 ? mha_launch(ctx, kMhaGradKv, kv_len, a) : ZN_OK;
+    MhaImages im(ctx);
+    const int64_t qi = im.add(a, q, a.qs, a.q_lens, a.q_heads, a.q_len, a.scale_log2);
+    const int64_t gi = im.add(a, grad_out, a.os, a.q_lens, a.q_heads, a.q_len, 1.0f);
+    const int64_t ki = im.add(a, k, a.ks, a.kv_lens, a.kv_heads, a.kv_len, 1.0f);
+    const int64_t vi = im.add(a, v, a.ks, a.kv_lens, a.kv_heads, a.kv_len, 1.0f);
+    if (im.groups > INT_MAX / 2) return ZN_ERR_OVERFLOW;
+    a.q_blocks = im.s.op[0].blocks;
+    a.k_blocks = im.s.op[2].blocks;
+    if ((rc = im.get((int64_t)a.batch * a.q_heads * a.q_blocks * 256))) return rc;
+    a.qi = im.s.op[0].dst = im.at(qi);
+    a.gi = im.s.op[1].dst = im.at(gi);
+    a.ki = im.s.op[2].dst = im.at(ki);
+    a.vi = im.s.op[3].dst = im.at(vi);
+    im.s.op[0].lse = im.s.op[1].lse = lse;
+    im.s.op[1].out = out;
+    a.side = im.s.op[1].side = reinterpret_cast<float *>(im.at(im.bytes));
+    if ((rc = im.run(ctx, a))) return rc;
+    if (queries && (rc = mha_tiles(ctx, kMhaGradQ, a))) return rc;
+    return kv_len > 0 ? mha_tiles(ctx, kMhaGradKv, a) : ZN_OK;
 }
 
 // ----------------------------------------------------------- gated Dense

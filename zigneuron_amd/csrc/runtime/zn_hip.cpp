@@ -99,8 +99,9 @@ constexpr unsigned kAttnSplitThreads[4] = {256, 512, 512, 512};
 constexpr int kAttnSplitQueries[4] = {128, 256, 128, 128};
 
 // Grouped attention (kernels/mha_f32.h), in the attention code object: zn_mha_<what>_<padded head dim>.
-enum MhaKernel { kMhaForward, kMhaGradQ, kMhaGradKv, kNumMha };
-constexpr const char *kMhaName[kNumMha] = {"zn_mha_forward", "zn_mha_grad_q", "zn_mha_grad_kv"};
+enum MhaKernel { kMhaForward, kMhaForwardRaw, kMhaGradQ, kMhaGradKv, kMhaSplit, kNumMha };
+constexpr const char *kMhaName[kNumMha] = {"zn_mha_forward", "zn_mha_forward_raw", "zn_mha_grad_q", "zn_mha_grad_kv",
+                                           "zn_mha_split"};
 constexpr unsigned kMhaThreads[4] = {256, 256, 512, 512};
 constexpr int kMhaTile = 128;  // query rows or keys of a workgroup
 

@@ -248,17 +248,40 @@ struct ZnRegroupArgs {
 // head h of sequence b reads key/value head h / group.  Tensors are [batch,
 // heads, positions, dim] with element strides {batch, head, position} and
 // contiguous dims: qs for q and grad_q, ks for k, v, grad_k and grad_v, os
-// for out and grad_out; lse and delta are contiguous [batch, q_heads, q_len].
+// for out and grad_out; lse is contiguous [batch, q_heads, q_len].
 struct ZnMhaArgs {
     const float *q, *k, *v;
     float *out, *lse;             // read by the backward
     const float *grad_out;
     float *grad_q, *grad_k, *grad_v;
-    float *delta;                 // sum over dims of grad_out * out, written and read by the backward
     const int32_t *q_lens, *kv_lens;  // per sequence, or null: all of q_len, kv_len
     int64_t qs[3], ks[3], os[3];
     int32_t batch, q_heads, kv_heads, group, q_len, kv_len, dim, causal;
     float scale, scale_log2;      // scale_log2 = scale * log2(e)
+    // Split images (zn_mha_split_*): per head, blocks of 32 rows as the tiles
+    // stage them; qi (times scale_log2) and gi have q_blocks blocks a head, ki
+    // and vi k_blocks.  side: per query block 32 values lse * log2(e) (+inf
+    // where a row sees nothing), then 32 of delta, the sum of grad_out * out.
+    const char *qi, *gi, *ki, *vi;
+    const float *side;
+    int32_t q_blocks, k_blocks;
+};
+
+// One tensor to its image: workgroups [first, first + batch * heads * blocks).
+struct ZnMhaSplitOp {
+    const float *src;
+    char *dst;
+    int64_t stride[3];
+    const int32_t *lens;          // valid rows of each sequence, or null: all of len
+    const float *lse;             // query side: a row with lse -inf is zeros (contiguous [batch, heads, len])
+    const float *out;             // grad_out: the forward's out (same strides), for delta
+    float *side;                  // grad_out: lse and delta per block
+    float scale;
+    int32_t heads, len, blocks, first;
+};
+struct ZnMhaSplitArgs {
+    ZnMhaSplitOp op[4];
+    int32_t ops, dim;
 };
 
 // Gated Dense layer, elementwise: z = [gate | up] [rows x 2n].  Forward:
