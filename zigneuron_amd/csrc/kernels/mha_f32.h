@@ -192,21 +192,26 @@ template <int DP>
 struct MhaFrags : MhaBlock<DP> {
     typedef MhaBlock<DP> B;
     const char *lds;
-    int frag, tr;  // this lane's place in a fragment over dims, over rows
+    int frag, tr[2];  // this lane's place in a fragment over dims, over rows (even and odd blocks of dims)
     __device__ __forceinline__ MhaFrags(const char *lds, int lane) : lds(lds) {
         frag = B::slot(lane & 15, lane >> 4);
-        tr = B::slot(4 * (lane >> 4) + (lane & 15) / 4, lane % 4);
+        tr[0] = B::slot(4 * (lane >> 4) + (lane & 15) / 4, lane % 4 / 2) + lane % 2 * 8;
+        tr[1] = tr[0] ^ 32;
     }
+    // The first of the 4 dims of block db that a lane of quarter lh has in an accumulator whose rows are dims.
+    __device__ static __forceinline__ int dim_of(int db, int lh) { return 32 * (db / 2) + 8 * (db & 1) + 4 * (lh / 2) + 16 * (lh & 1); }
     // Part q of tensor t: rows 16 rb + li, chunk lh of slice sl
     __device__ __forceinline__ zn_bf16x8 dims(int st, int t, int q, int sl, int rb) const {
         return __builtin_bit_cast(zn_bf16x8, *reinterpret_cast<const zn_u32x4 *>(lds + st * B::kStage + t * B::kImage + q * B::kPart +
                                                                                 sl * (B::BR * 64) + rb * (16 * 64) + frag));
     }
-    // ... dims 16 db + li, rows 4 lh .. 4 lh + 3 and 16 + 4 lh .. 16 + 4 lh + 3
+    // ... 16 dims of block db (chunks 0 and 1 of its slice, or 2 and 3), rows 4 lh .. 4 lh + 3 and 16 + 4 lh .. 16 + 4 lh + 3.
+    // Whole chunks: the 4 rows of a 16-lane group leave the other half of the banks to the next group's (rotated) chunks; the
+    // first or second halves of all four chunks met in half of the banks (a third of the LDS cycles were conflicts).
     __device__ __forceinline__ zn_bf16x8 rows(int st, int t, int q, int db) const {
         typedef short s4 __attribute__((ext_vector_type(4)));
         typedef __attribute__((address_space(3))) s4 ls4;
-        const char *at = lds + st * B::kStage + t * B::kImage + q * B::kPart + (db / 2) * (B::BR * 64) + 8 * (db & 1) + tr;
+        const char *at = lds + st * B::kStage + t * B::kImage + q * B::kPart + (db / 2) * (B::BR * 64) + tr[db & 1];
         const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ls4 *)at), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ls4 *)(at + 16 * 64));
         return __builtin_bit_cast(zn_bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
     }
@@ -510,7 +515,7 @@ struct MhaQueryTile {
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
                 const zn_f32x4 x = BACK ? o[f][d] * p.scale : o[f][d] / div;
-                mha_store4(row, 16 * d + 4 * lh, p.dim, x);
+                mha_store4(row, Frags::dim_of(d, lh), p.dim, x);
             }
         }
     }
@@ -590,15 +595,19 @@ struct MhaQueryTile {
             for (int q = 0; q < 3; ++q) pf[f][q] = __builtin_bit_cast(zn_bf16x8, w[q]);
         }
 #pragma unroll
-        for (int d = 0; d < DB; ++d) {
-            zn_bf16x8 a[3];
+        for (int d = 0; d < DB; d += 2) {
+            zn_bf16x8 a[2][3];
 #pragma unroll
-            for (int q = 0; q < 3; ++q) a[q] = sg.rows(st, BACK ? 0 : 1, q, d);
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int q = 0; q < 3; ++q) a[c][q] = sg.rows(st, BACK ? 0 : 1, q, d + c);
 #pragma unroll
             for (int pr = 0; pr < 6; ++pr)
 #pragma unroll
-                for (int f = 0; f < FQ; ++f)
-                    o[f][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[kMhaPA[pr]], pf[f][kMhaPB[pr]], o[f][d], 0, 0, 0);
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int f = 0; f < FQ; ++f)
+                        o[f][d + c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[c][kMhaPA[pr]], pf[f][kMhaPB[pr]], o[f][d + c], 0, 0, 0);
         }
     }
 };
@@ -699,8 +708,8 @@ struct MhaKeyTile {
             if (j >= p.kv_len) continue;
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
-                mha_store4(p.grad_k + kat + j * p.ks[2], 16 * d + 4 * lh, p.dim, dk[f][d]);
-                mha_store4(p.grad_v + kat + j * p.ks[2], 16 * d + 4 * lh, p.dim, dv[f][d]);
+                mha_store4(p.grad_k + kat + j * p.ks[2], Frags::dim_of(d, lh), p.dim, dk[f][d]);
+                mha_store4(p.grad_v + kat + j * p.ks[2], Frags::dim_of(d, lh), p.dim, dv[f][d]);
             }
         }
     }
@@ -762,17 +771,21 @@ struct MhaKeyTile {
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int d = 0; d < DB; ++d) {
-                zn_bf16x8 a[3];
+            for (int d = 0; d < DB; d += 2) {
+                zn_bf16x8 a[2][3];
 #pragma unroll
-                for (int q = 0; q < 3; ++q) a[q] = sg.rows(st, 1 - t, q, d);
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int q = 0; q < 3; ++q) a[c][q] = sg.rows(st, 1 - t, q, d + c);
 #pragma unroll
                 for (int pr = 0; pr < 6; ++pr)
 #pragma unroll
-                    for (int f = 0; f < FK; ++f) {
-                        zn_f32x4 &x = t ? dk[f][d] : dv[f][d];
-                        x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[kMhaPA[pr]], t ? df[f][kMhaPB[pr]] : pf[f][kMhaPB[pr]], x, 0, 0, 0);
-                    }
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int f = 0; f < FK; ++f) {
+                            zn_f32x4 &x = t ? dk[f][d + c] : dv[f][d + c];
+                            x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[c][kMhaPA[pr]], t ? df[f][kMhaPB[pr]] : pf[f][kMhaPB[pr]], x, 0, 0, 0);
+                        }
             }
     }
 };
