@@ -187,6 +187,9 @@ struct MhaBlock {
     __device__ static __forceinline__ int place(int r, int lh, int sl, int q) { return q * kPart + sl * (BR * 64) + slot(r, lh); }
 };
 
+// Six fragments: over dims rows 0 .. 15 and 16 .. 31, over rows two blocks of 16 dims, three parts each.
+typedef zn_bf16x8 MhaSix[2][3];
+
 // Fragments of a staged block.
 template <int DP>
 struct MhaFrags : MhaBlock<DP> {
@@ -205,6 +208,16 @@ struct MhaFrags : MhaBlock<DP> {
         return __builtin_bit_cast(zn_bf16x8, *reinterpret_cast<const zn_u32x4 *>(lds + st * B::kStage + t * B::kImage + q * B::kPart +
                                                                                 sl * (B::BR * 64) + rb * (16 * 64) + frag));
     }
+    __device__ __forceinline__ void dims(int st, int t, int sl, MhaSix &a) const {
+#pragma unroll
+        for (int q = 2; q >= 0; --q)  // in the order of their use
+#pragma unroll
+            for (int rb = 0; rb < 2; ++rb) a[rb][q] = dims(st, t, q, sl, rb);
+    }
+    __device__ __forceinline__ void dims(int st, int t, int sl, int q, MhaSix &a) const {
+#pragma unroll
+        for (int rb = 0; rb < 2; ++rb) a[rb][q] = dims(st, t, q, sl, rb);
+    }
     // ... 16 dims of block db (chunks 0 and 1 of its slice, or 2 and 3), rows 4 lh .. 4 lh + 3 and 16 + 4 lh .. 16 + 4 lh + 3.
     // Whole chunks: the 4 rows of a 16-lane group leave the other half of the banks to the next group's (rotated) chunks; the
     // first or second halves of all four chunks met in half of the banks (a third of the LDS cycles were conflicts).
@@ -214,6 +227,16 @@ struct MhaFrags : MhaBlock<DP> {
         const char *at = lds + st * B::kStage + t * B::kImage + q * B::kPart + (db / 2) * (B::BR * 64) + tr[db & 1];
         const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ls4 *)at), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ls4 *)(at + 16 * 64));
         return __builtin_bit_cast(zn_bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+    __device__ __forceinline__ void rows(int st, int t, int db, MhaSix &a) const {
+#pragma unroll
+        for (int q = 2; q >= 0; --q)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) a[c][q] = rows(st, t, q, db + c);
+    }
+    __device__ __forceinline__ void rows(int st, int t, int db, int q, MhaSix &a) const {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) a[c][q] = rows(st, t, q, db + c);
     }
 };
 
@@ -246,7 +269,13 @@ struct MhaImageStage {
             if (c < 2 * kChunks) dma(t ? r[1] : r[0], lds + st * B::kStage + c * 1024, lane16, (uint32_t)(c - t * kChunks) * 1024u);
         }
     }
-    __device__ __forceinline__ void arrive() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+    // Wait for the blocks on their way: vmcnt(0) as a builtin, which the compiler counts.  Its own loads before the loop are then
+    // known to be done; with the wait in inline assembly it waits for them again inside the loop, and so for the blocks just asked for.
+    __device__ __forceinline__ void arrive() {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0x0f70);
+        asm volatile("" ::: "memory");
+    }
     __device__ __forceinline__ void commit(int) {}
 };
 
@@ -314,6 +343,62 @@ struct MhaRawStage {
         }
     }
 };
+
+// The instruction order of a group's M products, the R fragment reads of the
+// next group spread between them: left alone the compiler reads a fragment
+// right before its use and waits out the whole latency (128 dims, dQ: 1.03e9
+// CU cycles, so 0.91e9).
+template <int M, int R>
+__device__ __forceinline__ void mha_order() {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x8, M / R, 0);  // MFMA
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);    // LDS read
+    }
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// The same with one set of fragments: a part's last product frees its
+// registers for the next group's (load(part)), requested 6 F to 10 F products
+// before their use.  x(c, f) += a[c] . b(f) for c < 2, f < F.  READS: LDS reads
+// of a part.  For the key tiles, which two sets make spill (and a reload from
+// scratch waits for the blocks on their way too).
+template <int F, int READS, typename Acc, typename Operand, typename Load>
+__device__ __forceinline__ void mha_group(MhaSix &a, Acc x, Operand b, Load load) {
+    auto products = [&](auto count) {  // part 3 - count of a with parts count - 1 .. 0 of b
+        constexpr int N = decltype(count)::value, P = 3 - N;
+#pragma unroll
+        for (int q = N - 1; q >= 0; --q)
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int f = 0; f < F; ++f)
+                    x(c, f) = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[c][P], b(f)[q], x(c, f), 0, 0, 0);
+        load(P);
+        __builtin_amdgcn_sched_group_barrier(0x8, 2 * F * N, 0);                         // MFMA
+        if constexpr (READS > 0) __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);  // LDS read
+    };
+    products(std::integral_constant<int, 1>());
+    products(std::integral_constant<int, 2>());
+    products(std::integral_constant<int, 3>());
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// Probabilities (or dS) times kSplitScale, which their exponent has, to the parts of a fragment.
+constexpr float kSplitLog2 = 24.0f;  // log2 of kSplitScale
+__device__ __forceinline__ void mha_split8(const float (&x)[8], zn_bf16x8 (&f)[3]) {
+    zn_u32x4 w[3];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        uint32_t hi, mid, lo;
+        split_scaled(x[2 * e], x[2 * e + 1], hi, mid, lo);
+        w[0][e] = hi;
+        w[1][e] = mid;
+        w[2][e] = lo;
+    }
+#pragma unroll
+    for (int q = 0; q < 3; ++q) f[q] = __builtin_bit_cast(zn_bf16x8, w[q]);
+}
 
 // The six products of two split operands, largest last.
 constexpr int kMhaPA[6] = {2, 1, 0, 1, 0, 0}, kMhaPB[6] = {0, 1, 2, 0, 1, 0};
@@ -465,8 +550,7 @@ struct MhaQueryTile {
                 sg.arrive();
                 __syncthreads();  // block blk is in LDS; every wave is done with block blk - 1
                 if (blk + 1 < nblk) sg.fetch(st ^ 1, blk + 1);
-                if (k0 + 32 <= all) block<false>(fr, st, k0, lane, lim, qf, gf, lse2, delta, o, m, l);
-                else if (k0 < any) block<true>(fr, st, k0, lane, lim, qf, gf, lse2, delta, o, m, l);
+                if (k0 < any) block(fr, st, k0 + 32 > all, k0, lane, lim, qf, gf, lse2, delta, o, m, l);
                 if (blk + 1 < nblk) sg.commit(st ^ 1);
             }
         };
@@ -505,7 +589,7 @@ struct MhaQueryTile {
             float sum = 0.0f;
             if constexpr (!BACK) {
                 sum = l[f] + __shfl_xor(l[f], 16);
-                sum += __shfl_xor(sum, 32);
+                sum = (sum + __shfl_xor(sum, 32)) * (1.0f / kSplitScale);  // the probabilities' factor
             }
             if (!r.in) continue;
             float *row = BACK ? p.grad_q + b * p.qs[0] + r.h * p.qs[1] + r.i * p.qs[2]
@@ -521,8 +605,8 @@ struct MhaQueryTile {
     }
 
     // One block of 32 keys: S^T = K (cQ)^T (and dP^T = V dO^T), then O^T += V^T P^T or dQ^T += K^T dS^T.
-    template <bool MASK>
-    __device__ static __forceinline__ void block(const Frags &sg, int st, int k0, int lane, const int (&lim)[FQ],
+    // `mask` (of the whole wave): some of its pairs are masked.  One code for both, as MhaKeyTile's.
+    __device__ static __forceinline__ void block(const Frags &sg, int st, bool mask, int k0, int lane, const int (&lim)[FQ],
                                                  const zn_bf16x8 (&qf)[FQ][SL][3], const zn_bf16x8 (&gf)[BACK ? FQ : 1][SL][3],
                                                  const float (&lse2)[FQ], const float (&delta)[FQ], zn_f32x4 (&o)[FQ][DB],
                                                  float (&m)[FQ], float (&l)[FQ]) {
@@ -535,25 +619,34 @@ struct MhaQueryTile {
                 s[f][rb] = zn_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
                 if constexpr (BACK) dp[f][rb] = zn_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
             }
+        MhaSix a[2];
+        constexpr int ND = (BACK ? 2 : 1) * SL, NR = DB / 2;  // groups of products over dims, over rows
+        sg.dims(st, 0, 0, a[0]);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int t = 0; t < (BACK ? 2 : 1); ++t)
+        for (int i = 0; i < ND; ++i) {
+            const int t = i / SL, sl = i % SL;
+            if (i + 1 < ND) sg.dims(st, (i + 1) / SL, (i + 1) % SL, a[(i + 1) & 1]);
+            else sg.rows(st, BACK ? 0 : 1, 0, a[(i + 1) & 1]);
 #pragma unroll
-            for (int sl = 0; sl < SL; ++sl) {
-                zn_bf16x8 a[2][3];
+            for (int pr = 0; pr < 6; ++pr)
 #pragma unroll
                 for (int rb = 0; rb < 2; ++rb)
 #pragma unroll
-                    for (int q = 0; q < 3; ++q) a[rb][q] = sg.dims(st, t, q, sl, rb);
+                    for (int f = 0; f < FQ; ++f) {
+                        zn_f32x4 &x = t ? dp[BACK ? f : 0][rb] : s[f][rb];
+                        x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i & 1][rb][kMhaPA[pr]], t ? gf[BACK ? f : 0][sl][kMhaPB[pr]] : qf[f][sl][kMhaPB[pr]], x, 0, 0, 0);
+                    }
+            if (i + 1 < ND) mha_order<12 * FQ, 6>();
+            else mha_order<12 * FQ, 12>();
+        }
+        if (mask) {
 #pragma unroll
-                for (int pr = 0; pr < 6; ++pr)
+            for (int f = 0; f < FQ; ++f)
 #pragma unroll
-                    for (int rb = 0; rb < 2; ++rb)
-#pragma unroll
-                        for (int f = 0; f < FQ; ++f) {
-                            if (t == 0) s[f][rb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[rb][kMhaPA[pr]], qf[f][sl][kMhaPB[pr]], s[f][rb], 0, 0, 0);
-                            else dp[BACK ? f : 0][rb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[rb][kMhaPA[pr]], gf[BACK ? f : 0][sl][kMhaPB[pr]], dp[BACK ? f : 0][rb], 0, 0, 0);
-                        }
-            }
+                for (int e = 0; e < 8; ++e)
+                    if (k0 + 16 * (e / 4) + 4 * lh + e % 4 >= lim[f]) s[f][e / 4][e % 4] = -INFINITY;
+        }
         zn_bf16x8 pf[FQ][3];
 #pragma unroll
         for (int f = 0; f < FQ; ++f) {
@@ -561,25 +654,23 @@ struct MhaQueryTile {
             if constexpr (BACK) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const float pe = __builtin_amdgcn_exp2f(__builtin_fmaf(s[f][e / 4][e % 4], kSplitUnscale, -lse2[f]));
+                    const float pe = __builtin_amdgcn_exp2f(__builtin_fmaf(s[f][e / 4][e % 4], kSplitUnscale, kSplitLog2 - lse2[f]));
                     const float de = __builtin_fmaf(dp[f][e / 4][e % 4], kSplitUnscale, -delta[f]);
                     x[e] = pe * de;
-                    if (MASK && k0 + 16 * (e / 4) + 4 * lh + e % 4 >= lim[f]) x[e] = 0.0f;
                 }
             } else {
                 float mb = -INFINITY;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    if (MASK && k0 + 16 * (e / 4) + 4 * lh + e % 4 >= lim[f]) s[f][e / 4][e % 4] = -INFINITY;
                     mb = fmaxf(mb, s[f][e / 4][e % 4]);
                 }
                 const float mn = fmaxf(m[f], max_over_rows(mb) * kSplitUnscale);
-                const float ref = MASK && mn == -INFINITY ? 0.0f : mn;
-                const float alpha = __builtin_amdgcn_exp2f(m[f] - ref);
+                const float ref = mn == -INFINITY ? 0.0f : mn;  // nothing seen so far
+                const float alpha = __builtin_amdgcn_exp2f(m[f] - ref), up = kSplitLog2 - ref;
                 float rs = 0.0f;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[f][e / 4][e % 4], kSplitUnscale, -ref));
+                    x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[f][e / 4][e % 4], kSplitUnscale, up));
                     rs += x[e];
                 }
                 l[f] = l[f] * alpha + rs;
@@ -589,25 +680,20 @@ struct MhaQueryTile {
                     for (int d = 0; d < DB; ++d) o[f][d] *= alpha;
                 }
             }
-            zn_u32x4 w[3];
-            split8(x, w);
-#pragma unroll
-            for (int q = 0; q < 3; ++q) pf[f][q] = __builtin_bit_cast(zn_bf16x8, w[q]);
+            mha_split8(x, pf[f]);
         }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int d = 0; d < DB; d += 2) {
-            zn_bf16x8 a[2][3];
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-                for (int q = 0; q < 3; ++q) a[c][q] = sg.rows(st, BACK ? 0 : 1, q, d + c);
+        for (int i = 0; i < NR; ++i) {
+            if (i + 1 < NR) sg.rows(st, BACK ? 0 : 1, 2 * (i + 1), a[(ND + i + 1) & 1]);
 #pragma unroll
             for (int pr = 0; pr < 6; ++pr)
 #pragma unroll
                 for (int c = 0; c < 2; ++c)
 #pragma unroll
                     for (int f = 0; f < FQ; ++f)
-                        o[f][d + c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[c][kMhaPA[pr]], pf[f][kMhaPB[pr]], o[f][d + c], 0, 0, 0);
+                        o[f][2 * i + c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[(ND + i) & 1][c][kMhaPA[pr]], pf[f][kMhaPB[pr]], o[f][2 * i + c], 0, 0, 0);
+            mha_order<12 * FQ, 12>();
         }
     }
 };
@@ -683,8 +769,8 @@ struct MhaKeyTile {
             }
             if (t + 1 < total) fetch(st ^ 1, g, blk);
             const int hi = w0 + FK * 16;  // keys of this wave: [w0, hi)
-            if (i0 + seq.edge >= hi - 1 && hi <= seq.kl) block<false>(fr, st, side + st * 64, i0, w0, seq, lane, kf, vf, dk, dv);
-            else if (min(i0 + 31, seq.ql - 1) + seq.edge >= w0 && w0 < seq.kl) block<true>(fr, st, side + st * 64, i0, w0, seq, lane, kf, vf, dk, dv);
+            if (min(i0 + 31, seq.ql - 1) + seq.edge >= w0 && w0 < seq.kl)
+                block(fr, st, i0 + seq.edge < hi - 1 || hi > seq.kl, side + st * 64, i0, w0, seq, lane, kf, vf, dk, dv);
         }
 
         bool bad = false;
@@ -714,79 +800,95 @@ struct MhaKeyTile {
         }
     }
 
-    template <bool MASK>
-    __device__ static __forceinline__ void block(const Frags &sg, int st, const float *side, int i0, int w0, const MhaSeq &seq,
+    // One block of 32 queries.  `mask` (of the whole wave): some of its pairs are masked.  One code for both: with a copy for
+    // each, the sums lie in other registers at the end of the copies, and moving them together spills.
+    __device__ static __forceinline__ void block(const Frags &sg, int st, bool mask, const float *side, int i0, int w0, const MhaSeq &seq,
                                                  int lane, const zn_bf16x8 (&kf)[FK][SL][3], const zn_bf16x8 (&vf)[FK][SL][3],
                                                  zn_f32x4 (&dk)[FK][DB], zn_f32x4 (&dv)[FK][DB]) {
         const int li = lane & 15, lh = lane >> 4;
+        constexpr int NR = DB / 2;
         zn_f32x4 s[FK][2], dp[FK][2];
+        MhaSix a;
+#pragma unroll
+        for (int q = 2; q >= 0; --q) sg.dims(st, 0, 0, q, a);
 #pragma unroll
         for (int f = 0; f < FK; ++f)
 #pragma unroll
             for (int rb = 0; rb < 2; ++rb) s[f][rb] = dp[f][rb] = zn_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        __builtin_amdgcn_sched_barrier(0);
+        // S
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int i = 0; i < SL; ++i)
+            mha_group<FK, 2>(a, [&](int rb, int f) -> zn_f32x4 & { return s[f][rb]; }, [&](int f) -> const zn_bf16x8(&)[3] { return kf[f][i]; },
+                             [&](int q) { sg.dims(st, i + 1 < SL ? 0 : 1, i + 1 < SL ? i + 1 : 0, q, a); });
+        // P times 2^24, in the place of S
+        {
+            zn_f32x4 ml[2];
 #pragma unroll
-            for (int sl = 0; sl < SL; ++sl) {
-                zn_bf16x8 a[2][3];
+            for (int rb = 0; rb < 2; ++rb) ml[rb] = kSplitLog2 - *reinterpret_cast<const zn_f32x4 *>(side + 16 * rb + 4 * lh);
 #pragma unroll
-                for (int rb = 0; rb < 2; ++rb)
+            for (int f = 0; f < FK; ++f)
 #pragma unroll
-                    for (int q = 0; q < 3; ++q) a[rb][q] = sg.dims(st, t, q, sl, rb);
-#pragma unroll
-                for (int pr = 0; pr < 6; ++pr)
-#pragma unroll
-                    for (int rb = 0; rb < 2; ++rb)
-#pragma unroll
-                        for (int f = 0; f < FK; ++f) {
-                            if (t == 0) s[f][rb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[rb][kMhaPA[pr]], kf[f][sl][kMhaPB[pr]], s[f][rb], 0, 0, 0);
-                            else dp[f][rb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[rb][kMhaPA[pr]], vf[f][sl][kMhaPB[pr]], dp[f][rb], 0, 0, 0);
-                        }
-            }
-        zn_f32x4 ml[2], dl[2];
-#pragma unroll
-        for (int rb = 0; rb < 2; ++rb) {
-            ml[rb] = *reinterpret_cast<const zn_f32x4 *>(side + 16 * rb + 4 * lh);
-            dl[rb] = *reinterpret_cast<const zn_f32x4 *>(side + 32 + 16 * rb + 4 * lh);
+                for (int e = 0; e < 8; ++e)
+                    s[f][e / 4][e % 4] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[f][e / 4][e % 4], kSplitUnscale, ml[e / 4][e % 4]));
         }
-        zn_bf16x8 pf[FK][3], df[FK][3];
+        if (mask) {
+#pragma unroll
+            for (int f = 0; f < FK; ++f) {
+                const int j = w0 + 16 * f + li;
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (j >= seq.kl || j > i0 + 16 * (e / 4) + 4 * lh + e % 4 + seq.edge) s[f][e / 4][e % 4] = 0.0f;
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        // dP
+#pragma unroll
+        for (int i = 0; i < SL; ++i) {
+            auto acc = [&](int rb, int f) -> zn_f32x4 & { return dp[f][rb]; };
+            auto operand = [&](int f) -> const zn_bf16x8(&)[3] { return vf[f][i]; };
+            if (i + 1 < SL) mha_group<FK, 2>(a, acc, operand, [&](int q) { sg.dims(st, 1, i + 1, q, a); });
+            else mha_group<FK, 4>(a, acc, operand, [&](int q) { sg.rows(st, 1, 0, q, a); });
+        }
+        // dS times 2^24, in the place of P, and P's parts; dS's take their registers once dV is done
+        zn_bf16x8 pf[FK][3];
+        {
+            zn_f32x4 dl[2];
+#pragma unroll
+            for (int rb = 0; rb < 2; ++rb) dl[rb] = *reinterpret_cast<const zn_f32x4 *>(side + 32 + 16 * rb + 4 * lh);
+#pragma unroll
+            for (int f = 0; f < FK; ++f) {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    x[e] = s[f][e / 4][e % 4];
+                    s[f][e / 4][e % 4] = x[e] * __builtin_fmaf(dp[f][e / 4][e % 4], kSplitUnscale, -dl[e / 4][e % 4]);
+                }
+                mha_split8(x, pf[f]);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        // dV^T += dO^T P
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+            mha_group<FK, 4>(a, [&](int c, int f) -> zn_f32x4 & { return dv[f][2 * i + c]; }, [&](int f) -> const zn_bf16x8(&)[3] { return pf[f]; },
+                             [&](int q) { sg.rows(st, i + 1 < NR ? 1 : 0, i + 1 < NR ? 2 * (i + 1) : 0, q, a); });
+        // dK^T += Q^T dS
 #pragma unroll
         for (int f = 0; f < FK; ++f) {
-            const int j = w0 + 16 * f + li;
-            float x[8], y[8];
+            float y[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[f][e / 4][e % 4], kSplitUnscale, -ml[e / 4][e % 4]));
-                y[e] = x[e] * __builtin_fmaf(dp[f][e / 4][e % 4], kSplitUnscale, -dl[e / 4][e % 4]);
-                if (MASK && (j >= seq.kl || j > i0 + 16 * (e / 4) + 4 * lh + e % 4 + seq.edge)) x[e] = y[e] = 0.0f;
-            }
-            zn_u32x4 w[3];
-            split8(x, w);
-#pragma unroll
-            for (int q = 0; q < 3; ++q) pf[f][q] = __builtin_bit_cast(zn_bf16x8, w[q]);
-            split8(y, w);
-#pragma unroll
-            for (int q = 0; q < 3; ++q) df[f][q] = __builtin_bit_cast(zn_bf16x8, w[q]);
+            for (int e = 0; e < 8; ++e) y[e] = s[f][e / 4][e % 4];
+            mha_split8(y, pf[f]);
         }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int d = 0; d < DB; d += 2) {
-                zn_bf16x8 a[2][3];
-#pragma unroll
-                for (int c = 0; c < 2; ++c)
-#pragma unroll
-                    for (int q = 0; q < 3; ++q) a[c][q] = sg.rows(st, 1 - t, q, d + c);
-#pragma unroll
-                for (int pr = 0; pr < 6; ++pr)
-#pragma unroll
-                    for (int c = 0; c < 2; ++c)
-#pragma unroll
-                        for (int f = 0; f < FK; ++f) {
-                            zn_f32x4 &x = t ? dk[f][d + c] : dv[f][d + c];
-                            x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[c][kMhaPA[pr]], t ? df[f][kMhaPB[pr]] : pf[f][kMhaPB[pr]], x, 0, 0, 0);
-                        }
-            }
+        for (int i = 0; i < NR; ++i) {
+            auto acc = [&](int c, int f) -> zn_f32x4 & { return dk[f][2 * i + c]; };
+            auto operand = [&](int f) -> const zn_bf16x8(&)[3] { return pf[f]; };
+            if (i + 1 < NR) mha_group<FK, 4>(a, acc, operand, [&](int q) { sg.rows(st, 0, 2 * (i + 1), q, a); });
+            else mha_group<FK, 0>(a, acc, operand, [](int) {});
+        }
     }
 };
 

@@ -33,10 +33,9 @@ typedef float zn_f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 constexpr float kSplitScale = 16777216.0f;
 constexpr float kSplitUnscale = 1.0f / (16777216.0f * 16777216.0f);
 
-// Two fp32 values to the three bf16 parts of each, packed (low half: x0).
-__device__ __forceinline__ void split_pair(float x0, float x1, uint32_t &hi, uint32_t &mid, uint32_t &lo) {
+// Two fp32 values, times kSplitScale already, to the three bf16 parts of each, packed (low half: t0).
+__device__ __forceinline__ void split_scaled(float t0, float t1, uint32_t &hi, uint32_t &mid, uint32_t &lo) {
     typedef float f2 __attribute__((ext_vector_type(2)));
-    const float t0 = x0 * kSplitScale, t1 = x1 * kSplitScale;
     const zn_bf16x2 h = __builtin_convertvector((f2{t0, t1}), zn_bf16x2);
     const uint32_t hb = __builtin_bit_cast(uint32_t, h);
     const float r0 = t0 - __builtin_bit_cast(float, hb << 16), r1 = t1 - __builtin_bit_cast(float, hb & 0xffff0000u);
@@ -47,6 +46,11 @@ __device__ __forceinline__ void split_pair(float x0, float x1, uint32_t &hi, uin
     hi = __builtin_bit_cast(uint32_t, h);
     mid = __builtin_bit_cast(uint32_t, m);
     lo = __builtin_bit_cast(uint32_t, l);
+}
+
+// Two fp32 values to the three bf16 parts of each.
+__device__ __forceinline__ void split_pair(float x0, float x1, uint32_t &hi, uint32_t &mid, uint32_t &lo) {
+    split_scaled(x0 * kSplitScale, x1 * kSplitScale, hi, mid, lo);
 }
 
 // Eight values to the fragments of their three parts.
