@@ -110,6 +110,9 @@ SHAPES = [
     (2, 4, 2, 31, 31, 32), (1, 3, 1, 32, 33, 31), (1, 2, 2, 33, 65, 64), (2, 6, 2, 64, 64, 40), (1, 4, 4, 65, 63, 65),
     (1, 2, 1, 127, 129, 96), (1, 2, 2, 128, 128, 128), (1, 7, 1, 100, 100, 76), (1, 1, 1, 257, 300, 127),
     (2, 2, 1, 300, 257, 80), (1, 8, 2, 1, 513, 64), (3, 2, 1, 17, 700, 128), (1, 1, 1, 640, 640, 64), (16, 4, 4, 64, 64, 64),
+    # few rows of a long cache, long walks of few tiles, tiles that read split images
+    (1, 1, 1, 1, 5000, 96), (2, 8, 1, 2, 2049, 128), (1, 5, 1, 3, 999, 50), (1, 1, 1, 2000, 40, 32), (1, 1, 1, 40, 2000, 96),
+    (1, 3, 1, 1000, 1000, 128),
 ]
 
 
@@ -176,12 +179,13 @@ def test_queries_that_see_nothing(ctx, sq, sk):
     both(ctx, q, k, v, g, 0.1, True, what="empty rows")
 
 
+@pytest.mark.parametrize("s,bad", [(150, 101), (700, 555)])
 @pytest.mark.parametrize("dim", [64, 128])
-def test_masked_values_reach_nothing(ctx, dim):
+def test_masked_values_reach_nothing(ctx, dim, s, bad):
     """A causal mask beside NaN, infinities and the lowest value: only queries that see them may have them."""
-    b, hq, hk, s = 1, 2, 1, 150
+    b, hq, hk = 1, 2, 1
     q, k, v, g = make(13, b, hq, hk, s, s, dim)
-    bad = 101  # queries from here on see a NaN key, so they and the gradients that they feed are NaN
+    # queries from `bad` on see a NaN key, so they and the gradients that they feed are NaN
     k2, v2 = k.copy(), v.copy()
     k2[:, :, bad:], v2[:, :, bad:] = np.nan, np.inf
     v2[:, :, bad + 1:] = np.finfo(np.float32).min
@@ -196,6 +200,21 @@ def test_masked_values_reach_nothing(ctx, dim):
     gq, gk, gv = run_backward(ctx, q, k2, v2, out, lse, g, 0.1, True)
     check(gq[:, :, :bad], grads[0], bounds[0], "grad_q")
     assert np.isnan(gq[:, :, bad:]).all() and np.isnan(gk).all() and np.isnan(gv).all()
+
+
+@pytest.mark.parametrize("dim", [24, 64, 96, 128])
+def test_a_few_rows_beside_a_masked_nan(ctx, dim):
+    """Four new tokens against a long cache whose last keys only the last of them see."""
+    shape = (2, 4, 2, 4, 1500, dim)
+    q, k, v, _ = make(43, *shape)
+    ref = Mha(q, k, v, 0.1, True)
+    v[:, :, -2:] = np.nan  # the last two queries'
+    k[:, :, -1:] = np.inf
+    announce(f"mha few rows beside NaN, dim {dim}")
+    out, lse = run_forward(ctx, q, k, v, 0.1, True)
+    check(out[:, :, :2], ref.out[:, :, :2], ref.out_bound[:, :, :2], "out")
+    check(lse[:, :, :2], ref.lse[:, :, :2], ref.lse_bound[:, :, :2], "lse")
+    assert np.isnan(out[:, :, 2:]).all()
 
 
 @pytest.mark.parametrize("dim", [16, 64, 128])

@@ -95,12 +95,35 @@ struct MhaRowState {
 
 __device__ __forceinline__ float mha_lse(float m, float l) { return l == 0.0f ? -INFINITY : (m + __log2f(l)) * kLn2; }
 
-__device__ __forceinline__ void mha_row_forward(const ZnMhaArgs &p, int b, int h, int i, int lane) {
+// Where sums go: to the tensor's row, or to this split's part of it.
+__device__ __forceinline__ float *mha_part(const ZnMhaArgs &p, int64_t row) { return p.part + (row * p.splits + blockIdx.z) * p.part_ld; }
+__device__ __forceinline__ int64_t mha_query_row(const ZnMhaArgs &p, int b, int h, int i) { return ((int64_t)b * p.q_heads + h) * p.q_len + i; }
+// ... key rows behind all query rows, dK's then dV's
+__device__ __forceinline__ int64_t mha_key_row(const ZnMhaArgs &p, int b, int kh, int j, bool v) {
+    return (int64_t)p.batch * p.q_heads * p.q_len + (((int64_t)(v ? p.batch : 0) + b) * p.kv_heads + kh) * p.kv_len + j;
+}
+
+// O and lse of a row from its sums, or its part: dims lane and lane + 64.
+__device__ __forceinline__ void mha_row_finish(const ZnMhaArgs &p, int b, int h, int i, int lane, float m, float l, float oa, float ob) {
+    if (p.splits > 1) {
+        float *part = mha_part(p, mha_query_row(p, b, h, i));
+        MhaRow::store(part, p.dim, lane, oa, ob);
+        if (lane == 0) {
+            part[p.part_ld - 4] = m;
+            part[p.part_ld - 3] = l;
+        }
+        return;
+    }
+    const float r = l == 0.0f ? 1.0f : l;
+    MhaRow::store(p.out + b * p.os[0] + h * p.os[1] + i * p.os[2], p.dim, lane, oa / r, ob / r);
+    if (p.lse && lane == 0) p.lse[mha_query_row(p, b, h, i)] = mha_lse(m, l);
+}
+
+// A row's walk over keys [from, to), those of them that it sees.
+__device__ __forceinline__ void mha_row_forward(const ZnMhaArgs &p, int b, int h, int i, int from, int to, int lane) {
     MhaRowState s;
-    s.walk(p, b, h, i, 0, MhaSeq(p, b).seen(i), lane);
-    const float r = s.l == 0.0f ? 1.0f : s.l;
-    MhaRow::store(p.out + b * p.os[0] + h * p.os[1] + i * p.os[2], p.dim, lane, s.oa / r, s.ob / r);
-    if (p.lse && lane == 0) p.lse[((int64_t)b * p.q_heads + h) * p.q_len + i] = mha_lse(s.m, s.l);
+    s.walk(p, b, h, i, from, min(to, MhaSeq(p, b).seen(i)), lane);
+    mha_row_finish(p, b, h, i, lane, s.m, s.l, s.oa, s.ob);
 }
 
 // Where a query's lse (log2 domain) and delta lie.
@@ -108,51 +131,57 @@ __device__ __forceinline__ const float *mha_side(const ZnMhaArgs &p, int b, int 
     return p.side + (((int64_t)b * p.q_heads + h) * p.q_blocks + i / 32) * 64 + i % 32;
 }
 
-__device__ __forceinline__ void mha_row_grad_q(const ZnMhaArgs &p, int b, int h, int i, int lane) {
+// grad_q of a row over keys [from, to).
+__device__ __forceinline__ void mha_row_grad_q(const ZnMhaArgs &p, int b, int h, int i, int from, int to, int lane) {
     const MhaSeq seq(p, b);
-    int n = seq.seen(i);
+    int n = min(to, seq.seen(i));
     const float *side = mha_side(p, b, h, i);
-    const float lse2 = n ? side[0] : INFINITY, delta = n ? side[32] : 0.0f;
-    if (lse2 == INFINITY) n = 0;
+    const float lse2 = from < n ? side[0] : INFINITY, delta = from < n ? side[32] : 0.0f;
+    if (lse2 == INFINITY) n = from;
     const float *k = p.k + b * p.ks[0] + (h / p.group) * p.ks[1], *v = p.v + b * p.ks[0] + (h / p.group) * p.ks[1];
     const int64_t qat = b * p.qs[0] + h * p.qs[1] + i * p.qs[2];
-    MhaRow q(p.q + qat, n ? p.dim : 0, lane);
-    const MhaRow g(p.grad_out + b * p.os[0] + h * p.os[1] + i * p.os[2], n ? p.dim : 0, lane);
+    MhaRow q(p.q + qat, from < n ? p.dim : 0, lane);
+    const MhaRow g(p.grad_out + b * p.os[0] + h * p.os[1] + i * p.os[2], from < n ? p.dim : 0, lane);
     q.a *= p.scale_log2;
     q.b *= p.scale_log2;
     float ga = 0.0f, gb = 0.0f;
-    for (int j = 0; j < n; ++j) {
+    for (int j = from; j < n; ++j) {
         const MhaRow kr(k + j * p.ks[2], p.dim, lane), vr(v + j * p.ks[2], p.dim, lane);
         const float ds = __builtin_amdgcn_exp2f(q.dot(kr) - lse2) * (g.dot(vr) - delta);
         ga += ds * kr.a;
         gb += ds * kr.b;
     }
-    MhaRow::store(p.grad_q + qat, p.dim, lane, ga * p.scale, gb * p.scale);
+    if (p.splits > 1) MhaRow::store(mha_part(p, mha_query_row(p, b, h, i)), p.dim, lane, ga, gb);
+    else MhaRow::store(p.grad_q + qat, p.dim, lane, ga * p.scale, gb * p.scale);
 }
 
-// grad_k and grad_v of a row: the query heads of the group in order, their queries ascending.
-__device__ __forceinline__ void mha_row_grad_kv(const ZnMhaArgs &p, int b, int kh, int j, int lane) {
+// grad_k and grad_v of a row over the query blocks [from, to) of its tile's walk: nb blocks from b0 of each query head of the
+// group, the heads in order, the queries ascending.
+__device__ __forceinline__ void mha_row_grad_kv(const ZnMhaArgs &p, int b, int kh, int j, int b0, int nb, int from, int to, int lane) {
     const MhaSeq seq(p, b);
     const bool in = j < seq.kl;
     const int64_t kat = b * p.ks[0] + kh * p.ks[1] + j * p.ks[2];
     const MhaRow kr(p.k + kat, in ? p.dim : 0, lane), vr(p.v + kat, in ? p.dim : 0, lane);
     float ka = 0.0f, kb = 0.0f, va = 0.0f, vb = 0.0f;
-    for (int h = kh * p.group; in && h < (kh + 1) * p.group; ++h)
-        for (int i = seq.first(j); i < seq.ql; ++i) {
+    for (int t = from; in && t < to; ++t) {
+        const int g = t / nb, h = kh * p.group + g, i0 = 32 * (b0 + t - g * nb);
+        for (int i = max(i0, seq.first(j)); i < min(i0 + 32, seq.ql); ++i) {
             const float *side = mha_side(p, b, h, i);
             if (side[0] == INFINITY) continue;
             const MhaRow q(p.q + b * p.qs[0] + h * p.qs[1] + i * p.qs[2], p.dim, lane);
-            const MhaRow g(p.grad_out + b * p.os[0] + h * p.os[1] + i * p.os[2], p.dim, lane);
+            const MhaRow d(p.grad_out + b * p.os[0] + h * p.os[1] + i * p.os[2], p.dim, lane);
             const float s = wave_sum((q.a * p.scale_log2) * kr.a + (q.b * p.scale_log2) * kr.b);
             const float e = __builtin_amdgcn_exp2f(s - side[0]);
-            const float ds = e * (g.dot(vr) - side[32]);
-            va += e * g.a;
-            vb += e * g.b;
+            const float ds = e * (d.dot(vr) - side[32]);
+            va += e * d.a;
+            vb += e * d.b;
             ka += ds * q.a;
             kb += ds * q.b;
         }
-    MhaRow::store(p.grad_k + kat, p.dim, lane, ka * p.scale, kb * p.scale);
-    MhaRow::store(p.grad_v + kat, p.dim, lane, va, vb);
+    }
+    const bool part = p.splits > 1;
+    MhaRow::store(part ? mha_part(p, mha_key_row(p, b, kh, j, false)) : p.grad_k + kat, p.dim, lane, ka * p.scale, kb * p.scale);
+    MhaRow::store(part ? mha_part(p, mha_key_row(p, b, kh, j, true)) : p.grad_v + kat, p.dim, lane, va, vb);
 }
 
 // ------------------------------------------------------------------- tiles
@@ -240,6 +269,13 @@ struct MhaFrags : MhaBlock<DP> {
     }
 };
 
+// A pointer that is the same in the whole wave, in scalar registers, where inline assembly takes its descriptor from.
+__device__ __forceinline__ const float *mha_uniform(const void *p) {
+    const uint64_t x = reinterpret_cast<uint64_t>(p);
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x), hi = __builtin_amdgcn_readfirstlane((uint32_t)(x >> 32));
+    return reinterpret_cast<const float *>((uint64_t)hi << 32 | lo);
+}
+
 // Blocks of two tensors from their images, NW waves.
 template <int DP, int NW>
 struct MhaImageStage {
@@ -262,7 +298,7 @@ struct MhaImageStage {
         __amdgpu_buffer_rsrc_t r[2];
 #pragma unroll
         for (int t = 0; t < 2; ++t)
-            r[t] = make_rsrc(reinterpret_cast<const float *>(src[t] + (int64_t)blk * B::kImage), B::kImage);
+            r[t] = make_rsrc(mha_uniform(src[t] + (int64_t)blk * B::kImage), B::kImage);
 #pragma unroll
         for (int i = 0; i < (2 * kChunks + NW - 1) / NW; ++i) {
             const int c = i * NW + wave, t = c >= kChunks;
@@ -472,15 +508,14 @@ struct MhaQueryTile {
     static constexpr int kBytes = 2 * Frags::kStage;
     static_assert(IMAGE || !BACK, "the backward's tensors are all split before");
 
-    __device__ static __forceinline__ void run(const ZnMhaArgs &p, char *lds) {
+    // Tile y: causal rows see more the later they come, so the last tiles of each head come first.
+    __device__ static __forceinline__ void run(const ZnMhaArgs &p, int y, char *lds) {
         const int tid = threadIdx.x, lane = tid & (kWave - 1);
         const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
         const int li = lane & 15, lh = lane >> 4;
         const int b = blockIdx.x / p.kv_heads, kh = blockIdx.x - b * p.kv_heads;
-        const int rows = p.group * p.q_len;
-        // causal rows see more the later they come: the last tiles of each head first
-        const int per = (int)gridDim.y / p.group, g0 = (int)blockIdx.y % p.group;
-        const int r0 = (g0 * per + per - 1 - (int)blockIdx.y / p.group) * (NW * FQ * 16), w0 = r0 + wave * FQ * 16;
+        const int rows = p.group * p.q_len, per = p.query_tiles / p.group;
+        const int r0 = (y % p.group * per + per - 1 - y / p.group) * (NW * FQ * 16), w0 = r0 + wave * FQ * 16;
         if (r0 >= rows) return;
         const MhaSeq seq(p, b);
 
@@ -539,14 +574,16 @@ struct MhaQueryTile {
         }
 
         const Frags fr(lds, lane);
-        const int nblk = (last + 31) / 32;
+        // this split's share of the blocks
+        const int all_blocks = (last + 31) / 32, share = (all_blocks + p.splits - 1) / p.splits;
+        const int blk0 = __builtin_amdgcn_readfirstlane(min((int)blockIdx.z * share, all_blocks)), nblk = __builtin_amdgcn_readfirstlane(min(blk0 + share, all_blocks));
         auto walk = [&](Stage sg) {
-            if (nblk > 0) {
-                sg.fetch(0, 0);
+            if (blk0 < nblk) {
+                sg.fetch(0, blk0);
                 sg.commit(0);
             }
-            for (int blk = 0; blk < nblk; ++blk) {
-                const int st = blk & 1, k0 = 32 * blk;
+            for (int blk = blk0; blk < nblk; ++blk) {
+                const int st = (blk - blk0) & 1, k0 = 32 * blk;
                 sg.arrive();
                 __syncthreads();  // block blk is in LDS; every wave is done with block blk - 1
                 if (blk + 1 < nblk) sg.fetch(st ^ 1, blk + 1);
@@ -578,8 +615,8 @@ struct MhaQueryTile {
             for (int x = 0; x < 16 * FQ; ++x) {
                 const MhaQuery r(p, kh, w0 + x);
                 if (!r.in) break;
-                if constexpr (BACK) mha_row_grad_q(p, b, r.h, r.i, lane);
-                else mha_row_forward(p, b, r.h, r.i, lane);
+                if constexpr (BACK) mha_row_grad_q(p, b, r.h, r.i, 32 * blk0, 32 * nblk, lane);
+                else mha_row_forward(p, b, r.h, r.i, 32 * blk0, 32 * nblk, lane);
             }
             return;
         }
@@ -592,9 +629,19 @@ struct MhaQueryTile {
                 sum = (sum + __shfl_xor(sum, 32)) * (1.0f / kSplitScale);  // the probabilities' factor
             }
             if (!r.in) continue;
+            if (p.splits > 1) {
+                float *part = mha_part(p, mha_query_row(p, b, r.h, r.i));
+#pragma unroll
+                for (int d = 0; d < DB; ++d) mha_store4(part, Frags::dim_of(d, lh), p.dim, o[f][d]);
+                if (!BACK && lh == 0) {
+                    part[p.part_ld - 4] = m[f];
+                    part[p.part_ld - 3] = sum;
+                }
+                continue;
+            }
             float *row = BACK ? p.grad_q + b * p.qs[0] + r.h * p.qs[1] + r.i * p.qs[2]
                               : p.out + b * p.os[0] + r.h * p.os[1] + r.i * p.os[2];
-            if (!BACK && p.lse && lh == 0) p.lse[((int64_t)b * p.q_heads + r.h) * p.q_len + r.i] = mha_lse(m[f], sum);
+            if (!BACK && p.lse && lh == 0) p.lse[mha_query_row(p, b, r.h, r.i)] = mha_lse(m[f], sum);
             const float div = BACK ? 1.0f : (sum == 0.0f ? 1.0f : sum);
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
@@ -708,12 +755,12 @@ struct MhaKeyTile {
     static constexpr int kSide = 2 * Frags::kStage;  // lse and delta of two stages' rows: [stage][lse, delta][32]
     static constexpr int kBytes = kSide + 2 * 64 * 4;
 
-    __device__ static __forceinline__ void run(const ZnMhaArgs &p, char *lds) {
+    __device__ static __forceinline__ void run(const ZnMhaArgs &p, int y, char *lds) {
         const int tid = threadIdx.x, lane = tid & (kWave - 1);
         const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
         const int li = lane & 15, lh = lane >> 4;
         const int b = blockIdx.x / p.kv_heads, kh = blockIdx.x - b * p.kv_heads;
-        const int j0 = (int)blockIdx.y * (NW * FK * 16), w0 = j0 + wave * FK * 16;
+        const int j0 = y * (NW * FK * 16), w0 = j0 + wave * FK * 16;
         const MhaSeq seq(p, b);
         const int64_t kat = b * p.ks[0] + kh * p.ks[1];
 
@@ -741,7 +788,10 @@ struct MhaKeyTile {
         }
         // query blocks of a head that see any of the tile's keys
         const int b0 = j0 < seq.kl ? seq.first(j0) / 32 : 0, nb = j0 < seq.kl ? max(0, (seq.ql + 31) / 32 - b0) : 0;
-        const int total = nb * p.group;
+        // this split's share of the blocks of all the group's heads
+        const int share = (nb * p.group + p.splits - 1) / p.splits;
+        const int from = __builtin_amdgcn_readfirstlane(min((int)blockIdx.z * share, nb * p.group));
+        const int total = __builtin_amdgcn_readfirstlane(min(from + share, nb * p.group));
         const float *side = reinterpret_cast<const float *>(lds + kSide);
         const int64_t head0 = ((int64_t)b * p.q_heads + kh * p.group) * p.q_blocks;  // the group's first query block
         MhaImageStage<DP, NW> sg(lds, tid, nullptr, nullptr);
@@ -751,16 +801,16 @@ struct MhaKeyTile {
             sg.src[1] = p.gi + at * Frags::kImage;
             sg.fetch(st, blk);
             if (wave == NW - 1) {  // 256 bytes: a value to a lane
-                const __amdgpu_buffer_rsrc_t r = make_rsrc(p.side + (at + blk) * 64, 256);
+                const __amdgpu_buffer_rsrc_t r = make_rsrc(mha_uniform(p.side + (at + blk) * 64), 256);
                 const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(zn_lds_void *)(lds + kSide + st * 256));
                 asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, 0 offen lds" : : "s"(m0), "v"(sg.lane16 / 4), "s"(r) : "memory");
             }
         };
         const Frags fr(lds, lane);
-        int g = 0, blk = b0;
-        if (total > 0) fetch(0, g, blk);
-        for (int t = 0; t < total; ++t) {
-            const int st = t & 1, i0 = 32 * blk;
+        int g = __builtin_amdgcn_readfirstlane(nb ? from / nb : 0), blk = __builtin_amdgcn_readfirstlane(b0 + from - g * nb);
+        if (from < total) fetch(0, g, blk);
+        for (int t = from; t < total; ++t) {
+            const int st = (t - from) & 1, i0 = 32 * blk;
             sg.arrive();
             __syncthreads();
             if (++blk == b0 + nb) {
@@ -785,17 +835,20 @@ struct MhaKeyTile {
                     dv[f][d][r] *= kSplitUnscale;
                 }
         if (__builtin_amdgcn_ballot_w64(bad)) {
-            for (int j = w0; j < min(w0 + FK * 16, p.kv_len); ++j) mha_row_grad_kv(p, b, kh, j, lane);
+            for (int j = w0; j < min(w0 + FK * 16, p.kv_len); ++j) mha_row_grad_kv(p, b, kh, j, b0, nb, from, total, lane);
             return;
         }
 #pragma unroll
         for (int f = 0; f < FK; ++f) {
             const int j = w0 + 16 * f + li;
             if (j >= p.kv_len) continue;
+            const bool part = p.splits > 1;
+            float *rk = part ? mha_part(p, mha_key_row(p, b, kh, j, false)) : p.grad_k + kat + j * p.ks[2];
+            float *rv = part ? mha_part(p, mha_key_row(p, b, kh, j, true)) : p.grad_v + kat + j * p.ks[2];
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
-                mha_store4(p.grad_k + kat + j * p.ks[2], Frags::dim_of(d, lh), p.dim, dk[f][d]);
-                mha_store4(p.grad_v + kat + j * p.ks[2], Frags::dim_of(d, lh), p.dim, dv[f][d]);
+                mha_store4(rk, Frags::dim_of(d, lh), p.dim, dk[f][d]);
+                mha_store4(rv, Frags::dim_of(d, lh), p.dim, dv[f][d]);
             }
         }
     }
@@ -892,6 +945,176 @@ struct MhaKeyTile {
     }
 };
 
+// O and lse of at most 16 query rows of a key/value head: a few new tokens
+// against a long cache, bound by reading K and V once.  The fp32 matrix cores
+// keep up with that (16 rows, most of them padding, take 4 x 16 of their products
+// for 16 keys of 64 dims: 18 TB/s of K and V), so nothing is split and nothing passes
+// through LDS: each of the NW waves of each workgroup and split walks its own
+// keys, 16 at a time, loaded one step ahead straight into the fragments (K:
+// lane li a key, 4 dims of each 16 per quarter; V: lane li DB neighbouring
+// dims of one key per quarter).  The waves' sums are joined in LDS.
+template <int DP, int NW>
+struct MhaFew {
+    static constexpr int G = DP / 16;  // groups of 16 dims; also the 16-dim blocks of O^T, block c the dims G li + c
+    static constexpr int kLd = DP + 4;
+    static constexpr int kBytes = NW * 16 * kLd * 4;
+    struct Keys {
+        float k[G][4], v[4][G];
+    };
+
+    __device__ static __forceinline__ void load4(__amdgpu_buffer_rsrc_t r, uint32_t row, int d, int dim, float (&x)[4]) {
+        const uint32_t off = d < dim ? row + (uint32_t)d * 4u : kOutOfRange;
+        const zn_f32x4 v = __builtin_bit_cast(zn_f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = d + e < dim ? v[e] : 0.0f;
+    }
+
+    __device__ static __forceinline__ void run(const ZnMhaArgs &p, char *lds) {
+        const int tid = threadIdx.x, lane = tid & (kWave - 1);
+        const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+        const int li = lane & 15, lh = lane >> 4;
+        const int b = blockIdx.x / p.kv_heads, kh = blockIdx.x - b * p.kv_heads;
+        const MhaSeq seq(p, b);
+        const MhaQuery r(p, kh, li);
+        const int lim = r.in ? seq.seen(r.i) : 0;
+        int any = lim;
+#pragma unroll
+        for (int s = 1; s < 16; s <<= 1) any = max(any, __shfl_xor(any, s));
+        any = __builtin_amdgcn_readfirstlane(any);
+        float q[G][4];
+        const float *row = p.q + b * p.qs[0] + r.h * p.qs[1] + r.i * p.qs[2];
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int d = 16 * g + 4 * lh + e;
+                q[g][e] = lim && d < p.dim ? row[d] * p.scale_log2 : 0.0f;
+            }
+        // the wave's share of the keys that any row sees, whole steps of 16
+        const int steps = (any + 15) / 16, walks = p.splits * NW, share = (steps + walks - 1) / walks;
+        const int s0 = min(((int)blockIdx.z * NW + wave) * share, steps), s1 = min(s0 + share, steps);
+        const int64_t at = b * p.ks[0] + kh * p.ks[1];
+        const int stride = (int)p.ks[2];
+        auto load = [&](int s, Keys &x) {
+            const int k0 = 16 * s, n = min(16, any - k0);  // s < s1: at least one
+            const uint32_t bytes = (uint32_t)((n - 1) * stride + p.dim) * 4u;
+            const __amdgpu_buffer_rsrc_t rk = make_rsrc(p.k + at + (int64_t)k0 * p.ks[2], bytes);
+            const __amdgpu_buffer_rsrc_t rv = make_rsrc(p.v + at + (int64_t)k0 * p.ks[2], bytes);
+#pragma unroll
+            for (int g = 0; g < G; ++g) load4(rk, (uint32_t)(li * stride) * 4u, 16 * g + 4 * lh, p.dim, x.k[g]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t off = (uint32_t)((4 * lh + e) * stride) * 4u;
+#pragma unroll
+                for (int c = 0; c + 4 <= G; c += 4) {
+                    float y[4];
+                    load4(rv, off, G * li + c, p.dim, y);
+#pragma unroll
+                    for (int z = 0; z < 4; ++z) x.v[e][c + z] = y[z];
+                }
+#pragma unroll
+                for (int c = G / 4 * 4; c < G; ++c) {
+                    const int d = G * li + c;
+                    x.v[e][c] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rv, d < p.dim ? off + (uint32_t)d * 4u : kOutOfRange, 0, 0));
+                }
+            }
+        };
+        zn_f32x4 o[G];
+#pragma unroll
+        for (int c = 0; c < G; ++c) o[c] = zn_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        float m = -INFINITY, l = 0.0f;
+        Keys x[2];
+        auto step = [&](int s, const Keys &y) {
+            zn_f32x4 t[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) t[e & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(y.k[g][e], q[g][e], t[e & 1], 0, 0, 0);
+            t[0] += t[1];
+            float mb = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (16 * s + 4 * lh + e >= lim) t[0][e] = -INFINITY;
+                mb = fmaxf(mb, t[0][e]);
+            }
+            const float mn = fmaxf(m, max_over_rows(mb)), ref = mn == -INFINITY ? 0.0f : mn;
+            const float alpha = __builtin_amdgcn_exp2f(m - ref);
+            float rs = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                t[0][e] = __builtin_amdgcn_exp2f(t[0][e] - ref);
+                rs += t[0][e];
+            }
+            l = l * alpha + rs;
+            m = mn;
+#pragma unroll
+            for (int c = 0; c < G; ++c) o[c] *= alpha;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)  // key 16 s + 4 lh + e
+#pragma unroll
+                for (int c = 0; c < G; ++c) o[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(y.v[e][c], t[0][e], o[c], 0, 0, 0);
+        };
+        if (s0 < s1) load(s0, x[0]);
+        for (int s = s0; s < s1; s += 2) {
+            if (s + 1 < s1) load(s + 1, x[1]);
+            step(s, x[0]);
+            if (s + 1 < s1) {
+                if (s + 2 < s1) load(s + 2, x[0]);
+                step(s + 1, x[1]);
+            }
+        }
+        l += __shfl_xor(l, 16);
+        l += __shfl_xor(l, 32);
+        // a value that is not finite in a pair masked for some rows only: the rows one by one
+        bool bad = !(l < INFINITY);
+#pragma unroll
+        for (int c = 0; c < G; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) bad |= !(__builtin_fabsf(o[c][e]) < INFINITY);
+        float *mine = reinterpret_cast<float *>(lds) + wave * 16 * kLd;  // [row][dims, maximum, sum]
+        if (__builtin_amdgcn_ballot_w64(bad)) {
+            for (int y = 0; y < 16; ++y) {
+                const MhaQuery w(p, kh, y);
+                MhaRowState t;
+                if (w.in) t.walk(p, b, w.h, w.i, 16 * s0, min(16 * s1, seq.seen(w.i)), lane);
+                MhaRow::store(mine + y * kLd, p.dim, lane, t.oa, t.ob);
+                if (lane == 0) {
+                    mine[y * kLd + DP] = t.m;
+                    mine[y * kLd + DP + 1] = t.l;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int c = 0; c < G; ++c) mine[li * kLd + G * (4 * lh + e) + c] = o[c][e];
+            if (lh == 0) {
+                mine[li * kLd + DP] = m;
+                mine[li * kLd + DP + 1] = l;
+            }
+        }
+        __syncthreads();
+        const float *sums = reinterpret_cast<const float *>(lds);
+        for (int y = wave; y < 16; y += NW) {  // a wave to a row, the waves' sums in order
+            const MhaQuery w(p, kh, y);
+            if (!w.in) break;
+            float mx = -INFINITY, sl = 0.0f, oa = 0.0f, ob = 0.0f;
+#pragma unroll
+            for (int z = 0; z < NW; ++z) mx = fmaxf(mx, sums[(z * 16 + y) * kLd + DP]);
+            const float ref = mx == -INFINITY ? 0.0f : mx;
+#pragma unroll
+            for (int z = 0; z < NW; ++z) {
+                const float *t = sums + (z * 16 + y) * kLd;
+                const float f = __builtin_amdgcn_exp2f(t[DP] - ref);
+                sl += f * t[DP + 1];
+                if (lane < p.dim) oa += f * t[lane];
+                if (lane + 64 < p.dim) ob += f * t[lane + 64];
+            }
+            mha_row_finish(p, b, w.h, w.i, lane, mx, sl, oa, ob);
+        }
+    }
+};
+
 // Tensors to their images: a workgroup to a block of 32 rows, a unit of 8
 // values to a thread and step.  Rows past a sequence's length are zeros, and on
 // the query side rows that see nothing (lse -inf); blocks past it are not read
@@ -952,22 +1175,74 @@ __device__ __forceinline__ void mha_split(const ZnMhaSplitArgs &a) {
 
 }  // namespace
 
-// Grid: x = sequence and key/value head (its tiles share an XCD's L2), y = tiles.
-#define ZN_MHA_KERNEL(NAME, NW, ...)                                                  \
-    extern "C" __global__ __launch_bounds__(NW * 64, 2) void NAME(ZnMhaArgs p) {      \
-        typedef __VA_ARGS__ T;                                                        \
-        __shared__ __attribute__((aligned(1024))) char lds[T::kBytes];                \
-        T::run(p, lds);                                                               \
+// Rows of partial sums: the splits in order, a wave to a row, lane l its dims l
+// and l + 64, eight splits' loads in flight.
+extern "C" __global__ __launch_bounds__(256) void zn_mha_join(ZnMhaJoinArgs a) {
+    const ZnMhaJoinOp &p = a.op[blockIdx.y];
+    const int lane = threadIdx.x & (kWave - 1);
+    const int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
+    if (row >= p.rows) return;
+    const float *src = p.part + row * a.splits * a.part_ld;
+    float mx = -INFINITY;
+    if (a.forward) {
+        for (int z = lane; z < a.splits; z += kWave) mx = fmaxf(mx, src[(int64_t)z * a.part_ld + a.part_ld - 4]);
+#pragma unroll
+        for (int s = 32; s > 0; s >>= 1) mx = fmaxf(mx, __shfl_xor(mx, s));
     }
-#define ZN_MHA_KERNELS(DP, NW, FQ, FK)                                                                          \
-    ZN_MHA_KERNEL(zn_mha_forward_##DP, NW, MhaQueryTile<DP, NW, FQ, false, true>)                               \
-    ZN_MHA_KERNEL(zn_mha_forward_raw_##DP, NW, MhaQueryTile<DP, NW, FQ, false, false>)                          \
-    ZN_MHA_KERNEL(zn_mha_grad_q_##DP, NW, MhaQueryTile<DP, NW, FQ, true, true>)                                 \
-    ZN_MHA_KERNEL(zn_mha_grad_kv_##DP, NW, MhaKeyTile<DP, NW, FK>)                                              \
+    const float ref = mx == -INFINITY ? 0.0f : mx;
+    float sl = 0.0f, oa = 0.0f, ob = 0.0f;
+    for (int z0 = 0; z0 < a.splits; z0 += 8) {
+        float x[8], y[8], m[8], l[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const bool in = z0 + u < a.splits;
+            const float *t = src + (int64_t)(in ? z0 + u : 0) * a.part_ld;
+            x[u] = in && lane < a.dim ? t[lane] : 0.0f;
+            y[u] = in && lane + 64 < a.dim ? t[lane + 64] : 0.0f;
+            m[u] = in && a.forward ? t[a.part_ld - 4] : -INFINITY;
+            l[u] = in && a.forward ? t[a.part_ld - 3] : 0.0f;
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const float f = a.forward ? __builtin_amdgcn_exp2f(m[u] - ref) : 1.0f;
+            sl += f * l[u];
+            oa += f * x[u];
+            ob += f * y[u];
+        }
+    }
+    const int64_t bh = row / p.len;
+    float *dst = p.dst + bh / p.heads * p.stride[0] + bh % p.heads * p.stride[1] + row % p.len * p.stride[2];
+    if (a.forward) {
+        const float r = sl == 0.0f ? 1.0f : sl;
+        MhaRow::store(dst, a.dim, lane, oa / r, ob / r);
+        if (a.lse && lane == 0) a.lse[row] = mha_lse(mx, sl);
+    } else {
+        MhaRow::store(dst, a.dim, lane, oa * p.factor, ob * p.factor);
+    }
+}
+
+// Grid: x = sequence and key/value head (its tiles share an XCD's L2), y = tiles, z = splits.
+#define ZN_MHA_KERNEL(NAME, NW, BYTES, ...)                                           \
+    extern "C" __global__ __launch_bounds__(NW * 64, 2) void NAME(ZnMhaArgs p) {      \
+        __shared__ __attribute__((aligned(1024))) char lds[BYTES];                    \
+        __VA_ARGS__;                                                                  \
+    }
+#define ZN_MHA_KERNELS(DP, NW, F)                                                                               \
+    typedef MhaQueryTile<DP, NW, F, false, true> MhaForward##DP;                                                \
+    typedef MhaQueryTile<DP, NW, F, false, false> MhaForwardRaw##DP;                                            \
+    typedef MhaQueryTile<DP, NW, F, true, true> MhaGradQ##DP;                                                   \
+    typedef MhaKeyTile<DP, NW, F> MhaGradKv##DP;                                                                \
+    typedef MhaFew<DP, 4> MhaFew##DP;                                                                           \
+    ZN_MHA_KERNEL(zn_mha_few_##DP, 4, MhaFew##DP::kBytes, MhaFew##DP::run(p, lds))                              \
+    ZN_MHA_KERNEL(zn_mha_forward_##DP, NW, MhaForward##DP::kBytes, MhaForward##DP::run(p, blockIdx.y, lds))      \
+    ZN_MHA_KERNEL(zn_mha_forward_raw_##DP, NW, MhaForwardRaw##DP::kBytes, MhaForwardRaw##DP::run(p, blockIdx.y, lds)) \
+    ZN_MHA_KERNEL(zn_mha_grad_##DP, NW, MhaGradKv##DP::kBytes,                                                  \
+                  if ((int)blockIdx.y < p.key_tiles) MhaGradKv##DP::run(p, blockIdx.y, lds);                    \
+                  else MhaGradQ##DP::run(p, blockIdx.y - p.key_tiles, lds))                                     \
     extern "C" __global__ __launch_bounds__(256) void zn_mha_split_##DP(ZnMhaSplitArgs a) { mha_split<DP>(a); }
-ZN_MHA_KERNELS(32, 4, 2, 2)
-ZN_MHA_KERNELS(64, 4, 2, 2)
-ZN_MHA_KERNELS(96, 8, 1, 1)
-ZN_MHA_KERNELS(128, 8, 1, 1)
+ZN_MHA_KERNELS(32, 4, 2)
+ZN_MHA_KERNELS(64, 4, 2)
+ZN_MHA_KERNELS(96, 8, 1)
+ZN_MHA_KERNELS(128, 8, 1)
 
 #endif

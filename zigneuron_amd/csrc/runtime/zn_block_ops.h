@@ -36,7 +36,7 @@ int mha_args(zn_ctx *ctx, ZnMhaArgs &a, int64_t batch, int64_t q_heads, int64_t 
     if (batch > kMax || q_heads > kMax || q_len > kMax || kv_len > kMax || batch * q_heads > kMax || batch * kv_heads > kMax)
         return ZN_ERR_OVERFLOW;
     constexpr int64_t kMaxRows = (int64_t)65535 * kMhaTile;  // the grid's second extent
-    if (kv_len > kMaxRows || (kv_heads && q_heads / kv_heads * q_len > kMaxRows)) return ZN_ERR_OVERFLOW;
+    if (kv_len + (kv_heads ? q_heads / kv_heads * (q_len + kMhaTile) : 0) > kMaxRows) return ZN_ERR_OVERFLOW;
     std::memset(&a, 0, sizeof(a));
     std::memcpy(a.qs, qs, sizeof(a.qs));
     std::memcpy(a.ks, ks, sizeof(a.ks));
@@ -57,12 +57,39 @@ int mha_args(zn_ctx *ctx, ZnMhaArgs &a, int64_t batch, int64_t q_heads, int64_t 
     return ZN_OK;
 }
 
-// One launch over tiles of query rows or keys.
-int mha_tiles(zn_ctx *ctx, MhaKernel kernel, ZnMhaArgs &a) {
+// Query tiles of a key/value head: the same number for each query head of its group.
+int64_t mha_query_tiles(const ZnMhaArgs &a) { return a.group * cdiv(cdiv((int64_t)a.group * a.q_len, kMhaTile), std::max(a.group, 1)); }
+
+// Parts that tiles' walks of `blocks` blocks are cut into: as many as leave no
+// CU idle, up to 32, with at least 4 blocks each.
+int mha_splits(const zn_ctx *ctx, const ZnMhaArgs &a, int64_t tiles, int64_t blocks) {
+    const int64_t slots = cus_now(ctx) * (a.dim <= 64 ? 2 : 1);  // workgroups at once
+    return (int)std::max<int64_t>(1, std::min<int64_t>({32, slots / std::max<int64_t>(1, tiles), blocks / 4}));
+}
+
+int mha_tiles(zn_ctx *ctx, MhaKernel kernel, ZnMhaArgs &a, int64_t y) {
     const int dim = (a.dim - 1) / 32;
-    // query rows: the same number of tiles for each head of the group, whose last ones start first
-    const int64_t y = kernel == kMhaGradKv ? cdiv(a.kv_len, kMhaTile) : a.group * cdiv(cdiv((int64_t)a.group * a.q_len, kMhaTile), a.group);
-    return launch(ctx, ctx->mha[kernel][dim], (unsigned)(a.batch * a.kv_heads), (unsigned)y, kMhaThreads[dim], &a);
+    return launch(ctx, ctx->mha[kernel][dim], (unsigned)(a.batch * a.kv_heads), (unsigned)y, kernel == kMhaFew ? 256 : kMhaThreads[dim], &a,
+                  (unsigned)a.splits);
+}
+
+int mha_join(zn_ctx *ctx, const ZnMhaArgs &a, ZnMhaJoinArgs &j, int ops) {
+    j.splits = a.splits;
+    j.part_ld = a.part_ld;
+    j.dim = a.dim;
+    int64_t rows = 0;
+    for (int i = 0; i < ops; ++i) rows = std::max(rows, j.op[i].rows);
+    return launch(ctx, ctx->mha_join, (unsigned)cdiv(rows, 4), (unsigned)ops, 256, &j);
+}
+
+void mha_join_op(ZnMhaJoinOp &op, const float *part, float *dst, const int64_t (&stride)[3], int64_t batch, int32_t heads, int32_t len, float factor) {
+    op.part = part;
+    op.dst = dst;
+    std::memcpy(op.stride, stride, sizeof(op.stride));
+    op.rows = batch * heads * len;
+    op.heads = heads;
+    op.len = len;
+    op.factor = factor;
 }
 
 // The images that a call's tiles read (kernels/mha_f32.h), in one leased buffer.
@@ -116,17 +143,36 @@ int zn_hip_mha_forward(zn_ctx *ctx, const float *q, const float *k, const float 
     a.v = v;
     a.out = out;
     a.lse = lse;
-    // Each tile splits what it reads: past a few tiles, once for all of them is cheaper.
-    if (a.group * q_len <= 4 * kMhaTile) return mha_tiles(ctx, kMhaForwardRaw, a);
+    // At most 16 rows of a head read K and V as they are.  Each tile splits what it reads: past a few tiles, once for all of
+    // them is cheaper.
+    const int64_t rows = (int64_t)a.group * q_len, heads = (int64_t)a.batch * a.kv_heads;
+    const MhaKernel kernel = rows <= kMhaFewRows ? kMhaFew : rows <= 4 * kMhaTile ? kMhaForwardRaw : kMhaForward;
+    a.query_tiles = kernel == kMhaFew ? 1 : (int32_t)mha_query_tiles(a);
+    a.splits = kernel == kMhaFew ? (int32_t)std::max<int64_t>(1, std::min<int64_t>({64, 2 * cus_now(ctx) / heads, kv_len / 256}))
+                                 : mha_splits(ctx, a, heads * a.query_tiles, cdiv(kv_len, 32));
+    Lease part(ctx);
+    if (a.splits > 1) {
+        a.part_ld = (a.dim + 3) / 4 * 4 + 4;
+        if ((rc = part.get((size_t)(batch * q_heads * q_len) * a.splits * a.part_ld))) return rc;
+        a.part = part.ptr;
+    }
     MhaImages im(ctx);
-    const int64_t ki = im.add(a, k, a.ks, a.kv_lens, a.kv_heads, a.kv_len, 1.0f), vi = im.add(a, v, a.ks, a.kv_lens, a.kv_heads, a.kv_len, 1.0f);
-    if (im.groups > INT_MAX / 2) return ZN_ERR_OVERFLOW;
-    if ((rc = im.get(0))) return rc;
-    a.k_blocks = im.s.op[0].blocks;
-    a.ki = im.s.op[0].dst = im.at(ki);
-    a.vi = im.s.op[1].dst = im.at(vi);
-    if ((rc = im.run(ctx, a))) return rc;
-    return mha_tiles(ctx, kMhaForward, a);
+    if (kernel == kMhaForward && kv_len > 0) {
+        const int64_t ki = im.add(a, k, a.ks, a.kv_lens, a.kv_heads, a.kv_len, 1.0f), vi = im.add(a, v, a.ks, a.kv_lens, a.kv_heads, a.kv_len, 1.0f);
+        if (im.groups > INT_MAX / 2) return ZN_ERR_OVERFLOW;
+        if ((rc = im.get(0))) return rc;
+        a.k_blocks = im.s.op[0].blocks;
+        a.ki = im.s.op[0].dst = im.at(ki);
+        a.vi = im.s.op[1].dst = im.at(vi);
+        if ((rc = im.run(ctx, a))) return rc;
+    }
+    if ((rc = mha_tiles(ctx, kernel, a, a.query_tiles)) || a.splits == 1) return rc;
+    ZnMhaJoinArgs j;
+    std::memset(&j, 0, sizeof(j));
+    j.forward = 1;
+    j.lse = lse;
+    mha_join_op(j.op[0], a.part, out, a.os, a.batch, a.q_heads, a.q_len, 1.0f);
+    return mha_join(ctx, a, j, 1);
 }
 
 int zn_hip_mha_backward(zn_ctx *ctx, const float *q, const float *k, const float *v, const float *out,
@@ -170,8 +216,25 @@ int zn_hip_mha_backward(zn_ctx *ctx, const float *q, const float *k, const float
     im.s.op[1].out = out;
     a.side = im.s.op[1].side = reinterpret_cast<float *>(im.at(im.bytes));
     if ((rc = im.run(ctx, a))) return rc;
-    if (queries && (rc = mha_tiles(ctx, kMhaGradQ, a))) return rc;
-    return kv_len > 0 ? mha_tiles(ctx, kMhaGradKv, a) : ZN_OK;
+    a.key_tiles = (int32_t)cdiv(kv_len, kMhaTile);
+    a.query_tiles = queries ? (int32_t)mha_query_tiles(a) : 0;
+    const int64_t y = a.key_tiles + a.query_tiles;
+    a.splits = mha_splits(ctx, a, (int64_t)a.batch * a.kv_heads * y, std::max<int64_t>(a.k_blocks, (int64_t)a.group * a.q_blocks));
+    Lease part(ctx);
+    const int64_t q_rows = batch * q_heads * q_len, k_rows = batch * kv_heads * kv_len;
+    if (a.splits > 1) {
+        a.part_ld = (a.dim + 3) / 4 * 4;
+        if ((rc = part.get((size_t)(q_rows + 2 * k_rows) * a.splits * a.part_ld))) return rc;
+        a.part = part.ptr;
+    }
+    if ((rc = mha_tiles(ctx, kMhaGrad, a, y)) || a.splits == 1) return rc;
+    ZnMhaJoinArgs j;
+    std::memset(&j, 0, sizeof(j));
+    const int64_t per = (int64_t)a.splits * a.part_ld;
+    mha_join_op(j.op[0], a.part, grad_q, a.qs, a.batch, queries ? a.q_heads : 0, a.q_len, a.scale);
+    mha_join_op(j.op[1], a.part + q_rows * per, grad_k, a.ks, a.batch, a.kv_heads, a.kv_len, 1.0f);
+    mha_join_op(j.op[2], a.part + (q_rows + k_rows) * per, grad_v, a.ks, a.batch, a.kv_heads, a.kv_len, 1.0f);
+    return mha_join(ctx, a, j, 3);
 }
 
 // ----------------------------------------------------------- gated Dense

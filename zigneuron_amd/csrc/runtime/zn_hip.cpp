@@ -99,11 +99,11 @@ constexpr unsigned kAttnSplitThreads[4] = {256, 512, 512, 512};
 constexpr int kAttnSplitQueries[4] = {128, 256, 128, 128};
 
 // Grouped attention (kernels/mha_f32.h), in the attention code object: zn_mha_<what>_<padded head dim>.
-enum MhaKernel { kMhaForward, kMhaForwardRaw, kMhaGradQ, kMhaGradKv, kMhaSplit, kNumMha };
-constexpr const char *kMhaName[kNumMha] = {"zn_mha_forward", "zn_mha_forward_raw", "zn_mha_grad_q", "zn_mha_grad_kv",
-                                           "zn_mha_split"};
+enum MhaKernel { kMhaFew, kMhaForward, kMhaForwardRaw, kMhaGrad, kMhaSplit, kNumMha };
+constexpr const char *kMhaName[kNumMha] = {"zn_mha_few", "zn_mha_forward", "zn_mha_forward_raw", "zn_mha_grad", "zn_mha_split"};
 constexpr unsigned kMhaThreads[4] = {256, 256, 512, 512};
 constexpr int kMhaTile = 128;  // query rows or keys of a workgroup
+constexpr int kMhaFewRows = 16;  // query rows of zn_mha_few
 
 struct ScratchDevice;
 
@@ -187,6 +187,7 @@ struct zn_ctx {
     hipFunction_t attn_split[4] = {};          // the split form [head dim 32/64/96/128]
     hipFunction_t attn_combine = nullptr;      // merges its key ranges
     hipFunction_t mha[kNumMha][4] = {};        // grouped attention [head dim 32/64/96/128]
+    hipFunction_t mha_join = nullptr;          // adds up its splits
     hipFunction_t gemm[3][kNumTiles][3] = {};  // [layout][tile][staging: 4-byte, 16-byte, 16-byte unaligned (r only)]
     int gemm_threads[3][kNumTiles][3] = {};    // their workgroup sizes (the kernels' launch bounds)
     hipFunction_t conv[kNumTiles][2][2] = {};  // implicit-GEMM convolution [tile][16-byte W rows][4-pixel gather]
@@ -2007,6 +2008,7 @@ int zn_hip_create(int device, const char *code_object_dir, zn_ctx **out) {
             std::snprintf(name, sizeof(name), "%s_%d", kMhaName[i], 32 * (d + 1));
             if (hipModuleGetFunction(&ctx->mha[i][d], ctx->attn_module, name) != hipSuccess) return bail(ZN_ERR_SYMBOL);
         }
+    if (hipModuleGetFunction(&ctx->mha_join, ctx->attn_module, "zn_mha_join") != hipSuccess) return bail(ZN_ERR_SYMBOL);
     void *counters = nullptr;
     if ((e = hipMalloc(&counters, kCounterSlots * kCounterStride * sizeof(int32_t))) != hipSuccess) {
         (void)hipGetLastError();
