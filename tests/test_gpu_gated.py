@@ -89,7 +89,8 @@ def test_gates(ctx, act, bias):
 
 SIZES = [(1, 1, 1), (1, 64, 64), (1, 1023, 515), (2, 17, 3), (3, 300, 1001), (4, 1024, 4096), (5, 4, 128), (8, 515, 64),
          (9, 96, 130), (16, 1024, 512), (17, 33, 65), (31, 1000, 63), (64, 64, 64), (65, 65, 65), (100, 7, 200), (128, 512, 256),
-         (129, 100, 127), (255, 300, 129), (300, 1001, 333), (1000, 64, 1000), (2048, 256, 512)]
+         (129, 100, 127), (255, 300, 129), (300, 1001, 333), (1000, 64, 1000), (2048, 256, 512),
+         (1, 4100, 400), (16, 2049, 1000), (7, 3001, 515), (2048, 1024, 1024), (1025, 130, 1030), (333, 257, 4099)]
 
 
 @pytest.mark.parametrize("size", SIZES)

@@ -554,29 +554,69 @@ extern "C" __global__ __launch_bounds__(64) void zn_hold_stream(ZnEltArgs p) {
 }
 
 // ------------------------------------------------- gated Dense, elementwise
-// h = act(gate) * up from z = [gate | up] [rows x 2n].
+// h = act(gate) * up from z = [gate | up] [rows x 2n].  blockIdx.x: 256 units, blockIdx.y: rows.
 extern "C" __global__ __launch_bounds__(256) void zn_gate_forward(ZnGateArgs p) {
-    const int64_t total = p.rows * p.n;
-    for (int64_t i = gtid(); i < total; i += gstride()) {
-        const int64_t r = i / p.n, c = i - r * p.n;
+    const int64_t c = gtid();
+    if (c >= p.n) return;
+    for (int64_t r = blockIdx.y; r < p.rows; r += gridDim.y) {
         const float *z = p.z + r * 2 * p.n + c;
-        p.h[i] = zn_gate(z[0], p.act) * z[p.n];
+        p.h[r * p.n + c] = zn_gate(z[0], p.act) * z[p.n];
     }
 }
 
-// grad_z = [grad_h * up * act'(gate) | grad_h * act(gate)].
-extern "C" __global__ __launch_bounds__(256) void zn_gate_backward(ZnGateArgs p) {
-    const int64_t total = p.rows * p.n;
-    for (int64_t i = gtid(); i < total; i += gstride()) {
-        const int64_t r = i / p.n, c = i - r * p.n;
-        const int64_t at = r * 2 * p.n + c;
-        float y, d;
-        zn_gate_slope(p.z[at], p.act, y, d);
-        const float g = p.grad_h[i];
-        p.grad_z[at] = g * p.z[at + p.n] * d;
-        p.grad_z[at + p.n] = g * y;
+// grad_z = [grad_h * up * act'(gate) | grad_h * act(gate)] and, where asked
+// for, its column sums per split of rows (grad_z may be z).  blockIdx.x: 256
+// units (_v: whole float4s, 4 units to a thread and 4 rows at once; one and one
+// otherwise), blockIdx.y: a split of rows, in ascending order.
+template <int W>
+__device__ __forceinline__ void gate_backward(const ZnGateArgs &p) {
+    typedef float vec __attribute__((ext_vector_type(W)));
+    constexpr int kRows = W;  // rows at once: 256 / W threads span the 256 units
+    const int lane = threadIdx.x % (256 / W), sub = threadIdx.x / (256 / W);
+    const int64_t c = (int64_t)blockIdx.x * 256 + lane * W;
+    const int64_t r0 = (int64_t)blockIdx.y * p.rows_per_split, r1 = min(p.rows, r0 + p.rows_per_split);
+    float sg[W], su[W];
+#pragma unroll
+    for (int e = 0; e < W; ++e) sg[e] = su[e] = 0.0f;
+    if (c < p.n)
+        for (int64_t r = r0 + sub; r < r1; r += kRows) {
+            const int64_t at = r * 2 * p.n + c;
+            const vec g = *reinterpret_cast<const vec *>(p.z + at), u = *reinterpret_cast<const vec *>(p.z + at + p.n);
+            const vec h = *reinterpret_cast<const vec *>(p.grad_h + r * p.n + c);
+            vec dg, du;
+#pragma unroll
+            for (int e = 0; e < W; ++e) {
+                float y, d;
+                zn_gate_slope(g[e], p.act, y, d);
+                dg[e] = h[e] * u[e] * d;
+                du[e] = h[e] * y;
+                sg[e] += dg[e];
+                su[e] += du[e];
+            }
+            *reinterpret_cast<vec *>(p.grad_z + at) = dg;
+            *reinterpret_cast<vec *>(p.grad_z + at + p.n) = du;
+        }
+    if (!p.partial) return;
+    __shared__ float part[2][kRows][256];
+#pragma unroll
+    for (int e = 0; e < W; ++e) {
+        part[0][sub][lane * W + e] = sg[e];
+        part[1][sub][lane * W + e] = su[e];
+    }
+    __syncthreads();
+    const int64_t col = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (col >= p.n) return;
+    float *dst = p.partial + (int64_t)blockIdx.y * 2 * p.n + col;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        float t = 0.0f;
+#pragma unroll
+        for (int s = 0; s < kRows; ++s) t += part[q][s][threadIdx.x];
+        dst[q * p.n] = t;
     }
 }
+extern "C" __global__ __launch_bounds__(256) void zn_gate_backward(ZnGateArgs p) { gate_backward<1>(p); }
+extern "C" __global__ __launch_bounds__(256) void zn_gate_backward_v(ZnGateArgs p) { gate_backward<4>(p); }
 
 // --------------------------------------------- distillation from top logits
 // Per token: p = softmax(top / T) over the teacher's present entries, lse =

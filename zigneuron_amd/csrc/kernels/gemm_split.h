@@ -9,7 +9,10 @@
 #include "../zn_kernel_args.h"
 
 #include "gemm_core.h"
+#include "zn_gate.h"
 #include "zn_split.h"
+
+#include <type_traits>
 
 namespace {
 
@@ -49,8 +52,15 @@ namespace {
 //    matrix cores (plain), about five times slower.  Its finite values then
 //    have that arithmetic's bits; taking only the others from there changes
 //    how the main loop is scheduled (NN and NT on 128x128 2 to 3% slower).
-template <int NW, int FM, int BN, bool AK, bool BKC, bool FLUSH, int GC, int AB, int NV, int G = kGNone, bool GU = false>
+//  * GATED: the two projections of a gated Dense layer (X-contiguous B of 2
+//    hidden columns, p.n of them): half of the tile's columns are the gate's
+//    and the other half the up projection's of the same units, so that a lane
+//    holds both sums of a unit and the store applies the gate.
+template <int NW, int FM, int BN, bool AK, bool BKC, bool FLUSH, int GC, int AB, int NV, int G = kGNone, bool GU = false,
+          bool GATED = false>
 struct SplitTile {
+    typedef typename std::conditional<GATED, ZnGatedArgs, ZnGemmArgs>::type Args;
+    static_assert(!GATED || (AK && !BKC && G == kGNone), "the gated product is a plain NN one");
     static constexpr int NT = NW * kWave;
     static constexpr int BM = 16 * FM * NW, BK = 32;
     static constexpr int FN = BN / 16, NG = FN / GC;  // column blocks, in groups of GC
@@ -87,13 +97,24 @@ struct SplitTile {
         }
     }
 
-    __device__ static __forceinline__ void run(const ZnGemmArgs &p, char *lds) {
+    // Column of B behind column x of the tile at n0, and whether it is one of the problem's.
+    __device__ static __forceinline__ int column(const Args &p, int n0, int x, bool &in) {
+        if constexpr (GATED) {
+            const int unit = n0 + x % (BN / 2);
+            in = unit < p.n / 2;
+            return x < BN / 2 ? unit : p.n / 2 + unit;
+        }
+        in = n0 + x < p.n;
+        return n0 + x;
+    }
+
+    __device__ static __forceinline__ void run(const Args &p, char *lds) {
         const int tid = threadIdx.x, lane = tid & (kWave - 1);
         const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
         const int li = lane & 15, lh = lane >> 4;
         int tm, tn, slice;
         tile_coords(p, tm, tn, slice);
-        const int m0 = tm * BM + wave * 16 * FM, n0 = tn * BN;
+        const int m0 = tm * BM + wave * 16 * FM, n0 = tn * (GATED ? BN / 2 : BN);
         const int64_t bz = blockIdx.y;
         const int kbeg = slice * p.k_chunk;
         const int kend = min(p.k, kbeg + p.k_chunk);
@@ -123,9 +144,10 @@ struct SplitTile {
         for (int j = 0; j < UB; ++j) {
             const int u = j * NT + tid;
             const int row = BKC ? u / 4 : u % BN, c = BKC ? u % 4 : u / BN;
-            const int x = n0 + row;
+            bool in;
+            const int x = column(p, n0, row, in);
             kq[j] = BKC ? 4 * c : __builtin_amdgcn_readfirstlane(4 * c);
-            offb[j] = x < p.n ? (uint32_t)(BKC ? x * ldb + kbeg + 4 * c : x) * 4u : kOutOfRange;
+            offb[j] = in ? (uint32_t)(BKC ? x * ldb + kbeg + 4 * c : x) * 4u : kOutOfRange;
             lpos[j] = slot(row, c);
             if constexpr (GATHER_K) {
                 const int oh = zn_udiv(x, cg.ow_mul, cg.ow_shift), ow = x - oh * cg.out_w;
@@ -398,12 +420,13 @@ struct SplitTile {
                 }
             }
         if (__builtin_amdgcn_ballot_w64(bad)) plain(p, ra, rb, acc, m0, n0, kbeg, kend, lane);
-        store(p, acc, bz, m0, n0, lane, slice);
+        if constexpr (GATED) store_gated(p, acc, m0, n0, lane);
+        else store(p, acc, bz, m0, n0, lane, slice);
     }
 
     // The wave's sums on the fp32 matrix cores: a value that is not finite, or so large that its scaled split or sums
     // overflow, makes the split sums infinite or NaN.
-    __device__ static __forceinline__ void plain(const ZnGemmArgs &p, __amdgpu_buffer_rsrc_t ra, __amdgpu_buffer_rsrc_t rb,
+    __device__ static __forceinline__ void plain(const Args &p, __amdgpu_buffer_rsrc_t ra, __amdgpu_buffer_rsrc_t rb,
                                                  zn_f32x4 (&acc)[FM][FN], int mw, int nw, int kbeg, int kend, int lane) {
         const int li = lane & 15, lh = lane >> 4;
         const int lda = (int)p.lda, ldb = (int)p.ldb;
@@ -422,8 +445,9 @@ struct SplitTile {
             }
 #pragma unroll
             for (int f = 0; f < FN; ++f) {
-                const int x = nw + 16 * f + li;
-                const bool in = x < p.n && kk < kend;
+                bool in;
+                const int x = column(p, nw, 16 * f + li, in);
+                in = in && kk < kend;
                 uint32_t off;
                 if constexpr (G == kGNone) {
                     off = in ? (uint32_t)(BKC ? x * ldb + kk : kk * ldb + x) * 4u : kOutOfRange;
@@ -494,6 +518,35 @@ struct SplitTile {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) v[r] = zn_activate(v[r], ACT);
                 store4(crow, nw + 16 * fn + 4 * lh, p.n, v);
+            }
+        }
+    }
+    // h = act(gate) * up and, where z is kept, the projections themselves; the bias of all columns is requested first.
+    __device__ static __forceinline__ void store_gated(const ZnGatedArgs &p, const zn_f32x4 (&acc)[FM][FN], int mw, int nw, int lane) {
+        const int li = lane & 15, lh = lane >> 4, hidden = p.n / 2;
+        zn_f32x4 bias[FN];
+#pragma unroll
+        for (int fn = 0; fn < FN; ++fn) {
+            bias[fn] = zn_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (p.bias) bias[fn] = load4(p.bias + (fn < FN / 2 ? 0 : hidden), nw + 16 * (fn % (FN / 2)) + 4 * lh, hidden);
+        }
+#pragma unroll
+        for (int fm = 0; fm < FM; ++fm) {
+            const int row = mw + 16 * fm + li;
+            if (row >= p.m) continue;
+#pragma unroll
+            for (int fn = 0; fn < FN / 2; ++fn) {
+                const int col = nw + 16 * fn + 4 * lh;
+                const zn_f32x4 g = acc[fm][fn] + bias[fn], u = acc[fm][fn + FN / 2] + bias[fn + FN / 2];
+                zn_f32x4 h;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) h[r] = zn_gate(g[r], p.act) * u[r];
+                if (p.z) {
+                    float *zrow = p.z + (int64_t)row * p.n;
+                    store4(zrow, col, hidden, g);
+                    store4(zrow + hidden, col, hidden, u);
+                }
+                store4(p.c + (int64_t)row * p.ldc, col, hidden, h);
             }
         }
     }

@@ -11,6 +11,7 @@
 // buffer loads, out-of-range lanes read zero, no branches), and the work
 // derived from the top layer (its K <= 16 products) runs on the matrix cores.
 #include "gemm_core.h"
+#include "gemm_split.h"
 
 namespace {
 
@@ -715,3 +716,116 @@ ZN_PAIR_BWD_KERNELS(0)
 ZN_PAIR_BWD_KERNELS(1)
 ZN_PAIR_BWD_KERNELS(2)
 ZN_PAIR_BWD_KERNELS(3)
+
+// ------------------------------------------------------------- gated Dense
+// zn_gated_<tile>: both projections of a gated Dense layer, the gate and the
+// product in one launch, on the tiles of operands split into bf16 parts
+// (SplitTile, GATED): what the projections alone cost, without z going through
+// memory and back (4096 x 1024 x 2 x 4096: 325 us as a product and a pass).
+#define ZN_GATED_TILE(TILE, NW, FM, BN, FLUSH, GC, AB, NV, MINB)                                                \
+    extern "C" __global__ __launch_bounds__(NW * 64, MINB) void zn_gated_##TILE(ZnGatedArgs p) {                \
+        typedef SplitTile<NW, FM, BN, true, false, FLUSH, GC, AB, NV, kGNone, false, true> T;                   \
+        __shared__ __attribute__((aligned(1024))) char lds[2 * T::kStage];                                      \
+        T::run(p, lds);                                                                                         \
+    }
+ZN_GATED_TILE(sw, 8, 2, 256, false, 1, 1, 5, 2)
+ZN_GATED_TILE(sx, 8, 2, 128, true, 1, 2, 3, 2)
+ZN_GATED_TILE(sr, 8, 1, 128, true, 1, 2, 3, 4)
+ZN_GATED_TILE(sn, 4, 2, 64, true, 2, 2, 3, 2)
+
+namespace {
+// Bias, z and h of one unit of row m from its two sums.
+__device__ __forceinline__ void gated_finish(const ZnGatedArgs &p, int m, int unit, float g, float v) {
+    const int hidden = p.n / 2;
+    if (p.bias) {
+        g += p.bias[unit];
+        v += p.bias[hidden + unit];
+    }
+    if (p.z) {
+        p.z[(int64_t)m * p.n + unit] = g;
+        p.z[(int64_t)m * p.n + hidden + unit] = v;
+    }
+    p.c[(int64_t)m * p.ldc + unit] = zn_gate(g, p.act) * v;
+}
+}  // namespace
+
+// The same for at most 16 rows, bound by reading W once: 32 units to a
+// workgroup, whose 16 waves share its part of K (blockIdx.z of p.splits: narrow
+// layers give every CU one) in steps of 16 and add their sums in LDS, in wave
+// order.  On the fp32 matrix cores, x as the operand of 16 columns: a lane loads
+// 4 neighbouring columns of a row of W (lanes 0 - 7 the gate's, 8 - 15 the up
+// projection's: 128 bytes of each a row), which are its rows of four products;
+// four steps' loads are in flight.  16 rows cost 32 clocks a kilobyte of W, 18
+// TB/s on the chip.  MI355X, 4 x 1024 x 2 x 4096: 9.4 us (W at 5.1 TB/s alone
+// 6.6); 1 x 4096 x 2 x 8192 56 us (53).
+extern "C" __global__ __launch_bounds__(1024, 1) void zn_gated_few(ZnGatedArgs p) {
+    constexpr int NW = 16, kAhead = 4, kLd = 65;
+    __shared__ float sums[NW][16][kLd];  // [wave][row][32 gate, 32 up]
+    const int tid = threadIdx.x, lane = tid & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const int li = lane & 15, lh = lane >> 4, hidden = p.n / 2, n0 = blockIdx.x * 32;
+    const uint32_t row = (uint32_t)p.n * 4u;
+    const __amdgpu_buffer_rsrc_t rw = make_rsrc(p.b, (uint32_t)p.k * row);
+    const __amdgpu_buffer_rsrc_t rx = make_rsrc(p.a, (uint32_t)p.m * (uint32_t)p.k * 4u);
+    const uint32_t col = (uint32_t)((li < 8 ? 0 : hidden) + n0 + 4 * (li & 7)) * 4u;
+    const int steps = (p.k + 15) / 16, walks = NW * p.splits, share = (steps + walks - 1) / walks;
+    const int s0 = min(((int)blockIdx.z * NW + wave) * share, steps), s1 = min(s0 + share, steps);
+    zn_f32x4 acc[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) acc[c] = zn_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s = s0; s < s1; s += kAhead) {
+        zn_f32x4 w[kAhead][4], x[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int k = 16 * (s + u) + 4 * lh;  // k .. k + 3: those past the end read zeros, as do all of a step past the wave's
+            const bool in = s + u < s1;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+                w[u][t] = __builtin_bit_cast(zn_f32x4, __builtin_amdgcn_raw_buffer_load_b128(rw, in && k + t < p.k ? (uint32_t)(k + t) * row + col : kOutOfRange, 0, 0));
+            x[u] = __builtin_bit_cast(zn_f32x4, __builtin_amdgcn_raw_buffer_load_b128(rx, in && li < p.m ? (uint32_t)(li * p.k + k) * 4u : kOutOfRange, 0, 0));
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const float xt = 16 * (s + u) + 4 * lh + t < p.k ? x[u][t] : 0.0f;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[u][t][c], xt, acc[c], 0, 0, 0);
+            }
+    }
+    // row 4 lh + r of block c: column 4 (4 lh + r) + c of the 32 gate and 32 up columns; column li: row li of x
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sums[wave][li][4 * (4 * lh + r) + c] = acc[c][r];
+    __syncthreads();
+    if (tid >= 512) return;
+    const int m = tid / 32, u = tid % 32, unit = n0 + u;
+    if (m >= p.m || unit >= hidden) return;
+    float g = 0.0f, v = 0.0f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+        g += sums[w][m][u];
+        v += sums[w][m][32 + u];
+    }
+    if (p.splits > 1) {
+        float *dst = p.ws + ((int64_t)blockIdx.z * p.m + m) * p.n + unit;
+        dst[0] = g;
+        dst[hidden] = v;
+        return;
+    }
+    gated_finish(p, m, unit, g, v);
+}
+
+// The parts of K in order.
+extern "C" __global__ __launch_bounds__(256) void zn_gated_few_join(ZnGatedArgs p) {
+    const int hidden = p.n / 2, unit = blockIdx.x * 256 + threadIdx.x, m = blockIdx.y;
+    if (unit >= hidden) return;
+    float g = 0.0f, v = 0.0f;
+    for (int z = 0; z < p.splits; ++z) {
+        const float *src = p.ws + ((int64_t)z * p.m + m) * p.n + unit;
+        g += src[0];
+        v += src[hidden];
+    }
+    gated_finish(p, m, unit, g, v);
+}

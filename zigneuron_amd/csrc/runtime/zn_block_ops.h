@@ -242,6 +242,30 @@ static bool gated_extents_ok(int64_t batch, int64_t in_size, int64_t hidden) {
     return batch <= INT_MAX && in_size <= INT_MAX && hidden <= INT_MAX / 2;
 }
 
+// One problem's operands stay below 2 GiB, as every GEMM's.
+constexpr int64_t kGatedLimit = (int64_t)INT_MAX / 4;
+
+// At most 16 rows: from this many weights on the kernel that reads them once
+// (MI355X, us with it and as a product and a pass: 4 x 1024 x 8192 9.4 and 14.6,
+// 1 x 4096 x 16384 56 and 81; 4 x 512 x 1024 7.3 and 5.7, 8 x 1024 x 2048 8.2 and 7.7;
+// in parts of K, of at least 1024 each: 5 x 4096 x 8192 41 us whole, 32 in two).
+constexpr int64_t kFewWeights = (int64_t)3 << 20;
+
+// Whether the two projections, n columns together, run as one launch with the
+// gate: by the estimates of the unsplit split tiles, and of the product on its
+// own (K slices where they pay, or the fp32 kernels at the 75 TFLOP/s that they
+// reach on such sizes) with a pass over z at 4 TB/s behind it.  MI355X, us in one
+// launch and in two: 777 x 1023 x 2002 39 and 53, 4096 x 64 x 2048 19 and 42,
+// 2048 x 256 x 1024 16 and 20, 4096 x 1024 x 8192 332 and 348; 1024 x 512 x
+// 1024 21 and 18, 512 x 2048 x 4096 (K slices) 75 and 65, 256 x 1024 x 2048
+// 34 and 27, 64 x 256 x 512 13 and 5.
+static bool gated_pays(const zn_ctx *ctx, int64_t m, int64_t n, int64_t k) {
+    const double one = estimate_split(ctx, m, n, k, 1, 0).us;
+    double two = 2e-6 * (double)m * n * k / 75.0;
+    if (split_pays(ctx, ZN_LAYOUT_NN, m, n, k, 1)) two = std::min(two, estimate_split(ctx, m, n, k, 1, (int64_t)kScratchBytes).us);
+    return one < two + 2.0 + 6.0 * (double)m * n / 4e6;
+}
+
 int zn_hip_gated_dense_forward(zn_ctx *ctx, int act, const float *x, const float *w, const float *bias, float *z,
                                float *h, int64_t batch, int64_t in_size, int64_t hidden) {
     if (!ctx || act < ZN_GATE_LINEAR || act > ZN_GATE_GELU || batch < 0 || in_size < 0 || hidden < 0)
@@ -251,13 +275,51 @@ int zn_hip_gated_dense_forward(zn_ctx *ctx, int act, const float *x, const float
     if (!h || (in_size > 0 && (!x || !w))) return ZN_ERR_INVALID_ARG;
     int rc = select_device(ctx);
     if (rc) return rc;
+    const int64_t n = 2 * hidden;
+    ZnGatedArgs p;
+    std::memset(&p, 0, sizeof(p));
+    p.a = x;
+    p.b = w;
+    p.c = h;
+    p.z = z;
+    p.bias = bias;
+    p.lda = in_size;
+    p.ldb = n;
+    p.ldc = hidden;
+    p.m = (int32_t)batch;
+    p.n = (int32_t)n;
+    p.k = (int32_t)in_size;
+    p.act = act;
+    p.group_m = 1;
+    p.splits = 1;
+    p.batch = 1;
+    p.k_chunk = (int32_t)in_size;
+    const bool fits = in_size > 0 && batch <= kGatedLimit / std::max<int64_t>(in_size, 1) && in_size <= kGatedLimit / n;
+    if (fits && batch <= 16 && in_size * n >= kFewWeights) {
+        const int64_t wgs = cdiv(hidden, 32);
+        p.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>(cus_now(ctx) / wgs, in_size / 512));
+        Lease part(ctx);
+        if (p.splits > 1) {
+            if ((rc = part.get((size_t)(p.splits * batch * n)))) return rc;
+            p.ws = part.ptr;
+        }
+        if ((rc = launch(ctx, ctx->gated_few, (unsigned)wgs, 1, 1024, &p, (unsigned)p.splits)) || p.splits == 1) return rc;
+        return launch(ctx, ctx->gated_few_join, (unsigned)cdiv(hidden, 256), (unsigned)batch, 256, &p);
+    }
+    if (fits && gated_pays(ctx, batch, n, in_size)) {
+        const Tile tile = estimate_split(ctx, batch, n, in_size, 1, 0).tile;
+        p.tiles_m = (int32_t)cdiv(batch, kTiles[tile].bm);
+        p.tiles_n = (int32_t)cdiv(hidden, kTiles[tile].bn / 2);
+        const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
+        p.xcd_remap = (tile == kTileSR || tile == kTileSN) && tiles % 8 == 0;  // as the plain product's
+        return launch(ctx, ctx->gated[tile - kTileSW], (unsigned)tiles, 1, (unsigned)kTiles[tile].threads, &p);
+    }
     Lease own(ctx);
     if (!z) {
-        if ((rc = own.get((size_t)batch * 2 * (size_t)hidden))) return rc;
+        if ((rc = own.get((size_t)batch * (size_t)n))) return rc;
         z = own.ptr;
     }
-    if ((rc = gemm_launch(ctx, ZN_LAYOUT_NN, batch, 2 * hidden, in_size, x, in_size, 0, w, 2 * hidden, 0, z, 2 * hidden, 0, 1,
-                          0, bias, ZN_ACT_LINEAR)))
+    if ((rc = gemm_launch(ctx, ZN_LAYOUT_NN, batch, n, in_size, x, in_size, 0, w, n, 0, z, n, 0, 1, 0, bias, ZN_ACT_LINEAR)))
         return rc;
     ZnGateArgs g;
     std::memset(&g, 0, sizeof(g));
@@ -266,7 +328,7 @@ int zn_hip_gated_dense_forward(zn_ctx *ctx, int act, const float *x, const float
     g.rows = batch;
     g.n = hidden;
     g.act = act;
-    return elt_launch(ctx, kGateForward, batch * hidden, g);
+    return launch(ctx, ctx->elt[kGateForward], (unsigned)cdiv(hidden, 256), (unsigned)std::min<int64_t>(batch, 65535), 256, &g);
 }
 
 int zn_hip_gated_dense_backward(zn_ctx *ctx, int act, const float *x, const float *w, const float *z,
@@ -290,11 +352,41 @@ int zn_hip_gated_dense_backward(zn_ctx *ctx, int act, const float *x, const floa
     g.rows = batch;
     g.n = hidden;
     g.act = act;
-    if ((rc = elt_launch(ctx, kGateBackward, batch * hidden, g))) return rc;
-    if (grad_bias)
-        return dense_backward_impl(ctx, ZN_ACT_LINEAR, x, w, nullptr, nullptr, grad_z, grad_x, grad_w, grad_bias, batch,
-                                   in_size, n, true, ZN_ACT_LINEAR, nullptr, nullptr);
-    if (in_size == 0) return ZN_OK;
+    // row splits for about 8 workgroups a CU, at least 16 rows each
+    const bool vec = hidden % 4 == 0 && aligned16(z) && aligned16(grad_h) && aligned16(grad_z);
+    const int64_t cus = cus_now(ctx), groups = cdiv(hidden, 256);
+    int64_t splits = std::max<int64_t>(1, std::min<int64_t>({cdiv(batch, 16), 8 * cus / groups, 65535}));
+    const int64_t per = cdiv(batch, splits);
+    splits = cdiv(batch, per);
+    g.rows_per_split = (int32_t)per;
+    Lease part(ctx);
+    ZnReduceArgs r;
+    std::memset(&r, 0, sizeof(r));
+    if (grad_bias) {
+        if ((rc = part.get((size_t)(splits * n)))) return rc;
+        g.partial = part.ptr;
+        r.ws = part.ptr;
+        r.c = grad_bias;
+        r.m = 1;
+        r.n = (int32_t)n;
+        r.ldc = n;
+        r.batch = 1;
+        r.splits = (int32_t)splits;
+        r.accumulate = 1;
+        r.act = ZN_ACT_LINEAR;
+        r.vec = n % 4 == 0 && aligned16(grad_bias) && aligned16(part.ptr) ? 1 : 0;
+    }
+    if ((rc = launch(ctx, ctx->elt[vec ? kGateBackwardV : kGateBackward], (unsigned)groups, (unsigned)splits, 256, &g))) return rc;
+    if (in_size == 0) return grad_bias ? launch_reduce(ctx, r) : ZN_OK;
+    int64_t wg_nt = 0, wg_tn = 0;
+    if (const int tile = grouped_tile(ctx, batch, in_size, n, grad_x != nullptr, &wg_nt, &wg_tn)) {
+        ZnColSumArgs none;
+        std::memset(&none, 0, sizeof(none));
+        const int64_t blocks = grad_bias ? std::max<int64_t>(1, std::min<int64_t>(cdiv(n / (r.vec ? 4 : 1), 256), 8 * cus)) : 0;
+        return dense_backward_grouped(ctx, x, w, grad_z, grad_x, grad_w, r, (int)blocks, none, batch, in_size, n, (int)wg_nt,
+                                      (int)wg_tn, tile, ZN_ACT_LINEAR, nullptr, nullptr);
+    }
+    if (grad_bias && (rc = launch_reduce(ctx, r))) return rc;
     if (grad_x && (rc = gemm_launch(ctx, ZN_LAYOUT_NT, batch, in_size, n, grad_z, n, 0, w, n, 0, grad_x, in_size, 0, 1, 0,
                                     nullptr, ZN_ACT_LINEAR)))
         return rc;

@@ -75,14 +75,15 @@ constexpr TileShape kTiles[kNumTiles] = {{256, 128, 16, 512, "x", true, true, tr
 constexpr const char *kLayoutName[3] = {"nn", "nt", "tn"};
 
 enum EltKernel { kFill, kCopy, kAddBias, kActFwd, kActBwd, kAccBias, kIm2col, kSoftmax, kCol2im, kRowSum, kDenseGrad, kRegroup, kPack, kToNhwc, kHold, kCol2imPx, kReduceSlices,
-                 kGateForward, kGateBackward, kDistillForward, kDistillBackward, kNumElt };
+                 kGateForward, kGateBackward, kGateBackwardV, kDistillForward, kDistillBackward, kNumElt };
 constexpr const char *kEltName[kNumElt] = {"zn_fill_f32",        "zn_copy_f32", "zn_add_bias",
                                            "zn_activation_forward", "zn_activation_backward",
                                            "zn_accumulate_bias", "zn_im2col",   "zn_softmax_rows",
                                            "zn_col2im",          "zn_row_sum",  "zn_dense_grad_prologue",
                                            "zn_weight_regroup", "zn_pack_rows", "zn_nchw_to_nhwc",
                                            "zn_hold_stream",     "zn_col2im_px", "zn_reduce_slices",
-                                           "zn_gate_forward",    "zn_gate_backward", "zn_distill_forward",
+                                           "zn_gate_forward",    "zn_gate_backward", "zn_gate_backward_v",
+                                           "zn_distill_forward",
                                            "zn_distill_backward"};
 
 constexpr const char *kGemmObject = "zn_gemm_gfx950.hsaco";
@@ -188,6 +189,8 @@ struct zn_ctx {
     hipFunction_t attn_combine = nullptr;      // merges its key ranges
     hipFunction_t mha[kNumMha][4] = {};        // grouped attention [head dim 32/64/96/128]
     hipFunction_t mha_join = nullptr;          // adds up its splits
+    hipFunction_t gated[4] = {};               // gated Dense forward [sw, sx, sr, sn]
+    hipFunction_t gated_few = nullptr, gated_few_join = nullptr;  // ... of at most 16 rows
     hipFunction_t gemm[3][kNumTiles][3] = {};  // [layout][tile][staging: 4-byte, 16-byte, 16-byte unaligned (r only)]
     int gemm_threads[3][kNumTiles][3] = {};    // their workgroup sizes (the kernels' launch bounds)
     hipFunction_t conv[kNumTiles][2][2] = {};  // implicit-GEMM convolution [tile][16-byte W rows][4-pixel gather]
@@ -1974,6 +1977,14 @@ int zn_hip_create(int device, const char *code_object_dir, zn_ctx **out) {
     if (hipModuleGetFunction(&ctx->pair_fwd[0], ctx->mlp_module, "zn_dense_pair_fwd") != hipSuccess ||
         hipModuleGetFunction(&ctx->pair_fwd[1], ctx->mlp_module, "zn_dense_pair_fwd_v") != hipSuccess)
         return bail(ZN_ERR_SYMBOL);
+    for (int t = 0; t < 4; ++t) {
+        char name[64];
+        std::snprintf(name, sizeof(name), "zn_gated_%s", kTiles[kTileSW + t].suffix);
+        if (hipModuleGetFunction(&ctx->gated[t], ctx->mlp_module, name) != hipSuccess) return bail(ZN_ERR_SYMBOL);
+    }
+    if (hipModuleGetFunction(&ctx->gated_few, ctx->mlp_module, "zn_gated_few") != hipSuccess ||
+        hipModuleGetFunction(&ctx->gated_few_join, ctx->mlp_module, "zn_gated_few_join") != hipSuccess)
+        return bail(ZN_ERR_SYMBOL);
     for (int v = 0; v < 2; ++v) {
         int threads = 0;
         if (hipFuncGetAttribute(&threads, HIP_FUNC_ATTRIBUTE_MAX_THREADS_PER_BLOCK, ctx->pair_fwd[v]) != hipSuccess ||
@@ -2649,6 +2660,24 @@ static int dense_backward_grouped(zn_ctx *ctx, const float *input, const float *
     return launch(ctx, f, (unsigned)(wg_nt + wg_tn + (cs.splits > 0 ? d.wg_colsum : bias_blocks)), 1, 256, &d);
 }
 
+// Small layers: grad_input, grad_weights and the bias gradient in one
+// launch (C2's layers: 5 launches -> 2, or 1 without a prologue).  Up
+// to 2 workgroups per CU of 32x32 tiles whose four waves split K (C2
+// step 44 -> 33 us), else up to 2 per CU of unsplit 64x64 tiles.  The tile's
+// side and its numbers of workgroups, or 0 for launches of their own.
+static int grouped_tile(const zn_ctx *ctx, int64_t batch, int64_t in_size, int64_t out_size, bool grad_input, int64_t *wg_nt,
+                        int64_t *wg_tn) {
+    const bool small = in_size > 0 && batch <= 2048 && out_size <= 2048 && ctx->forced_tile < 0 &&
+                       ctx->forced_splits == 0 && in_size <= INT_MAX / 4 / std::max<int64_t>(batch, out_size);
+    for (int t : {32, 64}) {
+        *wg_nt = grad_input ? cdiv(batch, t) * cdiv(in_size, t) : 0;
+        *wg_tn = cdiv(in_size, t) * cdiv(out_size, t);
+        if (t == 32 && ctx->forced_wave_split == 0) continue;
+        if (small && *wg_nt + *wg_tn <= 2 * cus_now(ctx)) return t;
+    }
+    return 0;
+}
+
 // Dense.backward (src/layer.zig:411-475) on device pointers:
 //   gaa = activationBackward(act, y, grad_output)  and  grad_bias += sum_rows gaa
 // in one pass (zn_dense_grad_prologue: per-split column sums, then the
@@ -2693,23 +2722,8 @@ static int dense_backward_impl(zn_ctx *ctx, int act, const float *input, const f
         // gaa without a prologue: a ready buffer, or grad_output of a linear layer
         const bool no_prologue = gaa_ready || act == ZN_ACT_LINEAR;
         const float *gaa = gaa_ready ? grad_after_act : (act == ZN_ACT_LINEAR ? grad_output : grad_after_act);
-        // Small layers: grad_input, grad_weights and the bias gradient in one
-        // launch (C2's layers: 5 launches -> 2, or 1 without a prologue).  Up
-        // to 2 workgroups per CU of 32x32 tiles whose four waves split K (C2
-        // step 44 -> 33 us), else up to 2 per CU of unsplit 64x64 tiles.
-        const bool small = in_size > 0 && batch <= 2048 && out_size <= 2048 && ctx->forced_tile < 0 &&
-                           ctx->forced_splits == 0 && in_size <= INT_MAX / 4 / std::max<int64_t>(batch, out_size);
-        int tile = 0;
         int64_t wg_nt = 0, wg_tn = 0;
-        for (int t : {32, 64}) {
-            wg_nt = grad_input ? cdiv(batch, t) * cdiv(in_size, t) : 0;
-            wg_tn = cdiv(in_size, t) * cdiv(out_size, t);
-            if (t == 32 && ctx->forced_wave_split == 0) continue;
-            if (small && wg_nt + wg_tn <= 2 * cus) {
-                tile = t;
-                break;
-            }
-        }
+        const int tile = grouped_tile(ctx, batch, in_size, out_size, grad_input != nullptr, &wg_nt, &wg_tn);
         ZnColSumArgs cs;
         std::memset(&cs, 0, sizeof(cs));
         if (tile && no_prologue && splits <= kMaxColSumSplits) {

@@ -307,6 +307,13 @@ struct ZnMhaSplitArgs {
     int32_t ops, dim;
 };
 
+// Gated Dense layer in one launch: h [m x n/2] (in c, row stride ldc) from the
+// two projections x . W, W [k x n] with the gate's n/2 columns first; z [m x n]
+// receives them where not null; act is a zn_gate.
+struct ZnGatedArgs : ZnGemmArgs {
+    float *z;
+};
+
 // Gated Dense layer, elementwise: z = [gate | up] [rows x 2n].  Forward:
 // h = act(gate) * up.  Backward: grad_z = [grad_h * up * act'(gate) | grad_h * act(gate)].
 struct ZnGateArgs {
@@ -314,8 +321,9 @@ struct ZnGateArgs {
     const float *grad_h;  // backward
     float *h;             // forward
     float *grad_z;        // backward
+    float *partial;       // backward, or null: column sums of grad_z per row split, [splits x 2n]
     int64_t rows, n;
-    int32_t act;
+    int32_t act, rows_per_split;  // blockIdx.y: the rows of a split
 };
 
 // Distillation from a teacher's top logits (zn_distill_*): one row of
