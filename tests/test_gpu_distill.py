@@ -26,21 +26,22 @@ def make(seed, rows, vocab, k):
     return logits, index, top, rng.random(rows).astype(np.float32)
 
 
-def run(ctx, logits, index, top, grad_loss, t, ld=None, alias=False):
+def run(ctx, logits, index, top, grad_loss, t, ld=None, alias=False, grad_ld=None):
     """(loss, lse, grad_logits); the columns past the vocabulary have to stay."""
     rows, vocab = logits.shape
     k = index.shape[1]
     ld = ld or vocab
+    gld = grad_ld or ld
     host = np.full((rows, ld), 5.0, np.float32)
     host[:, :vocab] = logits
     dl, dt = ctx.to_device(host), ctx.to_device(np.concatenate([top.ravel(), [0]]))
     di = ctx.to_device(np.concatenate([index.ravel(), [0]]).astype(np.int32).view(np.float32))
     dg = ctx.to_device(grad_loss)
     loss, lse = ctx.alloc(rows + 1).fill(9.0), ctx.alloc(rows + 1).fill(9.0)
-    grad = dl if alias else ctx.alloc(rows * ld).fill(5.0)
+    grad = dl if alias else ctx.alloc(rows * gld).fill(5.0)
     ctx.distill_forward(dl, ld, di, dt, loss, lse, rows, vocab, k, t)
-    ctx.distill_backward(dl, ld, di, dt, lse, dg, grad, ld, rows, vocab, k, t)
-    loss, lse, grad = loss.download(), lse.download(), grad.download(rows * ld).reshape(rows, ld)
+    ctx.distill_backward(dl, ld, di, dt, lse, dg, grad, gld, rows, vocab, k, t)
+    loss, lse, grad = loss.download(), lse.download(), grad.download(rows * gld).reshape(rows, gld)
     assert loss[rows] == 9.0 and lse[rows] == 9.0 and (grad[:, vocab:] == 5.0).all()
     return loss[:rows], lse[:rows], grad[:, :vocab]
 
@@ -68,6 +69,7 @@ def test_row_strides_and_in_place(ctx, vocab, ld):
     a = make(vocab, 6, vocab, 9)
     both(ctx, *a, 2.0, ld=ld)
     both(ctx, *a, 2.0, ld=ld, alias=True)
+    both(ctx, *a, 2.0, ld=ld, grad_ld=ld + 2)
 
 
 @pytest.mark.parametrize("vocab", [300, 40000])

@@ -637,7 +637,17 @@ __device__ __forceinline__ float over_t(float x, const ZnDistillArgs &p) {
     const float r = __builtin_fmaf(-q, p.temperature, x);
     return __builtin_fabsf(q) < INFINITY ? __builtin_fmaf(r, p.inv_temperature, q) : q;
 }
-__device__ __forceinline__ float exp_nat(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f); }
+
+// A row of floats from any 4-byte address: `head` values up to the first whole
+// 16 bytes, then float4s, then a tail.
+struct DistillSpan {
+    int head, n4, tail;
+    __device__ __forceinline__ DistillSpan(const float *at, int n) {
+        head = min(n, (int)(-(reinterpret_cast<uintptr_t>(at) >> 2) & 3));
+        n4 = (n - head) / 4;
+        tail = head + 4 * n4;
+    }
+};
 
 // The teacher's row: this thread's entries (tid + 256 q), with index -1 where absent, their probability and its logarithm.
 struct DistillTeacher {
@@ -683,81 +693,191 @@ struct DistillTeacher {
 
 }  // namespace
 
+namespace {
+
+// Running maximum m and sum l of exp((x - m) / T) over this thread's share of
+// src[0 .. n), 16 values at a time.  Differences before the factor: the large
+// terms' exponents are then small and so are their roundings.
+__device__ __forceinline__ void distill_scan(const float *src, int n, float scale, float &m, float &l) {
+    const DistillSpan span(src, n);
+    const zn_f32x4 *body = reinterpret_cast<const zn_f32x4 *>(src + span.head);
+    auto join = [&](auto &x, int count) {
+        float mx = m;
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (u < count) mx = fmaxf(fmaxf(fmaxf(mx, x[u][0]), fmaxf(x[u][1], x[u][2])), x[u][3]);
+        const float ref = mx == -INFINITY ? 0.0f : mx;
+        l *= __builtin_amdgcn_exp2f((m - ref) * scale);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (u < count) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) l += __builtin_amdgcn_exp2f((x[u][e] - ref) * scale);
+            }
+        m = mx;
+    };
+    zn_f32x4 x[4];
+    int i = threadIdx.x;
+    for (; i + 3 * kDistillThreads < span.n4; i += 4 * kDistillThreads) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) x[u] = body[i + u * kDistillThreads];
+        join(x, 4);
+    }
+    for (; i < span.n4; i += kDistillThreads) {
+        x[0] = body[i];
+        join(x, 1);
+    }
+    // at most 3 values before and 3 behind the float4s, a thread each
+    const int t = threadIdx.x, j = t < span.head ? t : span.tail + t - span.head;
+    if (j < n) {
+        x[0] = zn_f32x4{src[j], -INFINITY, -INFINITY, -INFINITY};
+        join(x, 1);
+    }
+}
+
+// The block's maximum and sum from its threads'.
+__device__ __forceinline__ void distill_reduce(float scale, float &m, float &l, float *red) {
+    const float mx = block_reduce<true>(m, red), ref = mx == -INFINITY ? 0.0f : mx;
+    l = block_reduce<false>(l * __builtin_amdgcn_exp2f((m - ref) * scale), red);
+    m = mx;
+}
+
+// lse and loss of a row from the maximum and sum over its whole vocabulary.
+__device__ __forceinline__ void distill_finish(const ZnDistillArgs &p, int64_t row, const DistillTeacher &t, float m, float l, float *red) {
+    const float *src = p.logits + row * p.ld;
+    const float lse = over_t(m, p) + logf(l);
+    float term = 0.0f;
+#pragma unroll
+    for (int q = 0; q < kDistillPer; ++q)
+        if (t.at[q] >= 0 && t.prob[q] != 0.0f) term += t.prob[q] * (t.logp[q] - (over_t(src[t.at[q]], p) - lse));
+    term = block_reduce<false>(term, red);
+    if (threadIdx.x == 0) {
+        p.loss[row] = p.temperature * p.temperature * term;
+        p.lse[row] = lse;
+    }
+}
+
+__device__ __forceinline__ void distill_nothing(const ZnDistillArgs &p, int64_t row) {
+    if (threadIdx.x == 0) {
+        p.loss[row] = 0.0f;
+        p.lse[row] = 0.0f;
+    }
+}
+
+}  // namespace
+
+// A workgroup to a row (MI355X, 4096 rows of 32000: see the backward) or, with
+// parts > 1, to a part of one (blockIdx.y) whose maximum and sum go to p.part for
+// zn_distill_join: few rows then still fill the chip.
 extern "C" __global__ __launch_bounds__(256) void zn_distill_forward(ZnDistillArgs p) {
     __shared__ float red[kSoftmaxThreads / 64];
     for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
         const DistillTeacher t(p, row, red);
         if (!t.any) {
-            if (threadIdx.x == 0) {
-                p.loss[row] = 0.0f;
-                p.lse[row] = 0.0f;
-            }
+            if (p.parts == 1) distill_nothing(p, row);
             continue;
         }
-        const float *src = p.logits + row * p.ld;
+        const int from = min((int)blockIdx.y * p.part_len, p.vocab), to = min(from + p.part_len, p.vocab);
         float m = -INFINITY, l = 0.0f;
-        for (int i = threadIdx.x; i < p.vocab; i += kDistillThreads) {
-            const float s = over_t(src[i], p);
-            const float mn = fmaxf(m, s), ref = mn == -INFINITY ? 0.0f : mn;
-            l = l * exp_nat(m - ref) + exp_nat(s - ref);
-            m = mn;
-        }
-        const float mx = block_reduce<true>(m, red), ref = mx == -INFINITY ? 0.0f : mx;
-        const float sum = block_reduce<false>(l * exp_nat(m - ref), red);
-        const float lse = mx + logf(sum);
-        float term = 0.0f;
-#pragma unroll
-        for (int q = 0; q < kDistillPer; ++q)
-            if (t.at[q] >= 0 && t.prob[q] != 0.0f)
-                term += t.prob[q] * (t.logp[q] - (over_t(src[t.at[q]], p) - lse));
-        term = block_reduce<false>(term, red);
-        if (threadIdx.x == 0) {
-            p.loss[row] = p.temperature * p.temperature * term;
-            p.lse[row] = lse;
+        distill_scan(p.logits + row * p.ld + from, to - from, p.scale_log2, m, l);
+        distill_reduce(p.scale_log2, m, l, red);
+        if (p.parts == 1) {
+            distill_finish(p, row, t, m, l, red);
+        } else if (threadIdx.x == 0) {
+            float *part = p.part + (row * p.parts + blockIdx.y) * 2;
+            part[0] = m;
+            part[1] = l;
         }
     }
 }
 
+// The parts of each row in order.
+extern "C" __global__ __launch_bounds__(256) void zn_distill_join(ZnDistillArgs p) {
+    __shared__ float red[kSoftmaxThreads / 64];
+    const int64_t row = blockIdx.x;
+    const DistillTeacher t(p, row, red);
+    if (!t.any) {
+        distill_nothing(p, row);
+        return;
+    }
+    float m = -INFINITY, l = 0.0f;
+    if ((int)threadIdx.x < p.parts) {  // at most a part to a thread
+        m = p.part[(row * p.parts + threadIdx.x) * 2];
+        l = p.part[(row * p.parts + threadIdx.x) * 2 + 1];
+    }
+    distill_reduce(p.scale_log2, m, l, red);
+    distill_finish(p, row, t, m, l, red);
+}
+
+// A workgroup to a row, or to a part of one (blockIdx.y), whose own entries it
+// then corrects.  Logits are read once and gradients written once.
 extern "C" __global__ __launch_bounds__(256) void zn_distill_backward(ZnDistillArgs p) {
     __shared__ float red[kSoftmaxThreads / 64];
     __shared__ int idx[kDistillMaxK];
     __shared__ float prob[kDistillMaxK];
     for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
         const DistillTeacher t(p, row, red);
-        const float *src = p.logits + row * p.ld;
-        float *dst = p.grad + row * p.grad_ld;
+        const int from = min((int)blockIdx.y * p.part_len, p.vocab), to = min(from + p.part_len, p.vocab), n = to - from;
+        const float *src = p.logits + row * p.ld + from;
+        float *dst = p.grad + row * p.grad_ld + from;
+        const DistillSpan span(dst, n);
+        const int tid = threadIdx.x, rest = tid < span.head ? tid : span.tail + tid - span.head;
+        zn_f32x4 *body = reinterpret_cast<zn_f32x4 *>(dst + span.head);
         if (!t.any) {
-            for (int i = threadIdx.x; i < p.vocab; i += kDistillThreads) dst[i] = 0.0f;
+            for (int i = tid; i < span.n4; i += kDistillThreads) body[i] = zn_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (rest < n) dst[rest] = 0.0f;
             continue;
         }
-        const float lse = p.lse[row], g = p.grad_loss[row] * p.temperature;
+        const float centre = p.lse[row] * p.temperature, g = p.grad_loss[row] * p.temperature, scale = p.scale_log2;
+        auto value = [&](float x) { return __builtin_amdgcn_exp2f((x - centre) * scale); };
         float own[kDistillPer];  // read before the row is written, which may be the logits' own
 #pragma unroll
         for (int q = 0; q < kDistillPer; ++q) {
-            const int i = threadIdx.x + q * kDistillThreads;
-            own[q] = t.at[q] >= 0 ? exp_nat(over_t(src[t.at[q]], p) - lse) : 0.0f;
+            const int i = tid + q * kDistillThreads;
+            const int v = t.at[q] >= from && t.at[q] < to ? t.at[q] - from : -1;
+            own[q] = v >= 0 ? value(src[v]) : 0.0f;
             if (i < p.k) {
-                idx[i] = t.at[q];
+                idx[i] = v;
                 prob[i] = t.prob[q];
             }
         }
         __syncthreads();
-        for (int i = threadIdx.x; i < p.vocab; i += kDistillThreads)
-            dst[i] = g * exp_nat(over_t(src[i], p) - lse);
+        // loads at the stores' places: whole 16 bytes of the gradients, 4-byte aligned ones of the logits
+        typedef float vec4u __attribute__((ext_vector_type(4), aligned(4)));
+        const vec4u *from4 = reinterpret_cast<const vec4u *>(src + span.head);
+        int i = tid;
+        for (; i + 3 * kDistillThreads < span.n4; i += 4 * kDistillThreads) {
+            zn_f32x4 x[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) x[u] = from4[i + u * kDistillThreads];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[u][e] = g * value(x[u][e]);
+                body[i + u * kDistillThreads] = x[u];
+            }
+        }
+        for (; i < span.n4; i += kDistillThreads) {
+            zn_f32x4 x = from4[i];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = g * value(x[e]);
+            body[i] = x;
+        }
+        if (rest < n) dst[rest] = g * value(src[rest]);
         __syncthreads();
         // the first entry of each index subtracts all of that index's, in order
 #pragma unroll
         for (int q = 0; q < kDistillPer; ++q) {
-            const int i = threadIdx.x + q * kDistillThreads;
-            if (i >= p.k || t.at[q] < 0) continue;
+            const int i = tid + q * kDistillThreads;
+            if (i >= p.k || idx[i] < 0) continue;
             float sum = 0.0f;
             bool first = true;
             for (int j = 0; j < p.k; ++j)
-                if (idx[j] == t.at[q]) {
+                if (idx[j] == idx[i]) {
                     first &= j >= i;
                     sum += prob[j];
                 }
-            if (first) dst[t.at[q]] = g * (own[q] - sum);
+            if (first) dst[idx[i]] = g * (own[q] - sum);
         }
         __syncthreads();  // idx and prob are the next row's from here on
     }

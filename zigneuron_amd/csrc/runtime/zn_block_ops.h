@@ -297,7 +297,7 @@ int zn_hip_gated_dense_forward(zn_ctx *ctx, int act, const float *x, const float
     const bool fits = in_size > 0 && batch <= kGatedLimit / std::max<int64_t>(in_size, 1) && in_size <= kGatedLimit / n;
     if (fits && batch <= 16 && in_size * n >= kFewWeights) {
         const int64_t wgs = cdiv(hidden, 32);
-        p.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>(cus_now(ctx) / wgs, in_size / 512));
+        p.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>(cus_now(ctx) / wgs, in_size / 1024));
         Lease part(ctx);
         if (p.splits > 1) {
             if ((rc = part.get((size_t)(p.splits * batch * n)))) return rc;
@@ -402,7 +402,7 @@ constexpr int64_t kDistillMaxK = 1024;
 int distill_args(zn_ctx *ctx, ZnDistillArgs &a, const float *logits, int64_t ld, const void *index, const float *top,
                  int64_t rows, int64_t vocab, int64_t k, float temperature) {
     if (!ctx || rows < 0 || vocab < 0 || k < 0 || k > kDistillMaxK || ld < vocab || !(temperature > 0.0f) ||
-        !std::isfinite(temperature) || !std::isfinite(1.0f / temperature))
+        !std::isfinite(temperature) || !std::isfinite(1.5f / temperature))
         return ZN_ERR_INVALID_ARG;
     if (vocab > INT_MAX / 2) return ZN_ERR_OVERFLOW;
     std::memset(&a, 0, sizeof(a));
@@ -417,8 +417,16 @@ int distill_args(zn_ctx *ctx, ZnDistillArgs &a, const float *logits, int64_t ld,
     a.k = vocab > 0 ? (int32_t)k : 0;
     a.temperature = temperature;
     a.inv_temperature = 1.0f / temperature;
+    a.scale_log2 = 1.44269504088896340736f / temperature;
+    // fewer rows than fill the chip twice over: parts of them, of at least 4096 values
+    const int64_t parts = std::max<int64_t>(1, std::min<int64_t>({2 * cus_now(ctx) / rows, vocab / 4096, 64}));
+    a.part_len = (int32_t)(cdiv(cdiv(vocab, parts), 4) * 4);
+    a.parts = vocab > 0 ? (int32_t)cdiv(vocab, a.part_len) : 1;
     return ZN_OK;
 }
+
+// Workgroups that rows go over in turn.
+unsigned distill_rows(const zn_ctx *ctx, int64_t rows) { return (unsigned)std::min<int64_t>(rows, 16 * cus_now(ctx)); }
 
 }  // namespace
 
@@ -432,7 +440,13 @@ int zn_hip_distill_forward(zn_ctx *ctx, const float *logits, int64_t ld, const v
     a.loss = loss;
     a.lse = lse;
     if ((rc = select_device(ctx))) return rc;
-    return launch(ctx, ctx->elt[kDistillForward], (unsigned)std::min<int64_t>(rows, 8 * cus_now(ctx)), 1, 256, &a);
+    Lease part(ctx);
+    if (a.parts > 1) {
+        if ((rc = part.get((size_t)(rows * a.parts) * 2))) return rc;
+        a.part = part.ptr;
+    }
+    if ((rc = launch(ctx, ctx->elt[kDistillForward], distill_rows(ctx, rows), (unsigned)a.parts, 256, &a)) || a.parts == 1) return rc;
+    return launch(ctx, ctx->elt[kDistillJoin], (unsigned)rows, 1, 256, &a);
 }
 
 int zn_hip_distill_backward(zn_ctx *ctx, const float *logits, int64_t ld, const void *top_index,
@@ -449,7 +463,7 @@ int zn_hip_distill_backward(zn_ctx *ctx, const float *logits, int64_t ld, const 
     a.grad = grad_logits;
     a.grad_ld = grad_ld;
     if ((rc = select_device(ctx))) return rc;
-    return launch(ctx, ctx->elt[kDistillBackward], (unsigned)std::min<int64_t>(rows, 8 * cus_now(ctx)), 1, 256, &a);
+    return launch(ctx, ctx->elt[kDistillBackward], distill_rows(ctx, rows), (unsigned)a.parts, 256, &a);
 }
 
 #endif

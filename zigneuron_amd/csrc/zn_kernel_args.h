@@ -337,7 +337,11 @@ struct ZnDistillArgs {
     float *grad;
     int64_t ld, grad_ld, rows;
     int32_t vocab, k;
-    float temperature, inv_temperature;
+    float temperature, inv_temperature, scale_log2;  // scale_log2 = log2(e) / temperature
+    // parts of a row's vocabulary, part_len long (a multiple of 4); part: the
+    // forward's maximum and sum of each, [rows][parts][2]
+    int32_t parts, part_len;
+    float *part;
 };
 
 #endif
