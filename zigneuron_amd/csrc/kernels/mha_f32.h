@@ -282,10 +282,10 @@ struct MhaImageStage {
     typedef MhaBlock<DP> B;
     static constexpr int kChunks = B::kImage / 1024;  // wave instructions a tensor
     char *lds;
-    const char *src[2];  // the images of the current heads
+    const char *x, *y;  // the images of the current heads
     int wave;
     uint32_t lane16;
-    __device__ __forceinline__ MhaImageStage(char *lds, int tid, const char *x, const char *y) : lds(lds), src{x, y} {
+    __device__ __forceinline__ MhaImageStage(char *lds, int tid, const char *x, const char *y) : lds(lds), x(x), y(y) {
         wave = __builtin_amdgcn_readfirstlane(tid / kWave);
         lane16 = (tid & (kWave - 1)) * 16;
     }
@@ -295,14 +295,14 @@ struct MhaImageStage {
         asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" : : "s"(m0), "v"(lane16), "s"(r), "s"(at) : "memory");
     }
     __device__ __forceinline__ void fetch(int st, int blk) {
-        __amdgpu_buffer_rsrc_t r[2];
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-            r[t] = make_rsrc(mha_uniform(src[t] + (int64_t)blk * B::kImage), B::kImage);
+        const __amdgpu_buffer_rsrc_t rx = make_rsrc(mha_uniform(x + (int64_t)blk * B::kImage), B::kImage);
+        const __amdgpu_buffer_rsrc_t ry = make_rsrc(mha_uniform(y + (int64_t)blk * B::kImage), B::kImage);
 #pragma unroll
         for (int i = 0; i < (2 * kChunks + NW - 1) / NW; ++i) {
-            const int c = i * NW + wave, t = c >= kChunks;
-            if (c < 2 * kChunks) dma(t ? r[1] : r[0], lds + st * B::kStage + c * 1024, lane16, (uint32_t)(c - t * kChunks) * 1024u);
+            const int c = i * NW + wave;
+            char *to = lds + st * B::kStage + c * 1024;
+            if (c < kChunks) dma(rx, to, lane16, (uint32_t)c * 1024u);
+            else if (c < 2 * kChunks) dma(ry, to, lane16, (uint32_t)(c - kChunks) * 1024u);
         }
     }
     // Wait for the blocks on their way: vmcnt(0) as a builtin, which the compiler counts.  Its own loads before the loop are then
@@ -397,10 +397,13 @@ __device__ __forceinline__ void mha_order() {
 // The same with one set of fragments: a part's last product frees its
 // registers for the next group's (load(part)), requested 6 F to 10 F products
 // before their use.  x(c, f) += a[c] . b(f) for c < 2, f < F.  READS: LDS reads
-// of a part.  For the key tiles, which two sets make spill (and a reload from
+// of a part.  FLUSH: the six products are summed from zero and then added, one
+// rounding of a long sum per block instead of six (4 heads of 4096 x 128 on a
+// key/value head, against 64 bits: dK 1.9e-6 -> 8e-7).  For the key tiles, which two sets make spill (and a reload from
 // scratch waits for the blocks on their way too).
-template <int F, int READS, typename Acc, typename Operand, typename Load>
+template <int F, int READS, bool FLUSH, typename Acc, typename Operand, typename Load>
 __device__ __forceinline__ void mha_group(MhaSix &a, Acc x, Operand b, Load load) {
+    zn_f32x4 t[2][F];
     auto products = [&](auto count) {  // part 3 - count of a with parts count - 1 .. 0 of b
         constexpr int N = decltype(count)::value, P = 3 - N;
 #pragma unroll
@@ -408,8 +411,10 @@ __device__ __forceinline__ void mha_group(MhaSix &a, Acc x, Operand b, Load load
 #pragma unroll
             for (int c = 0; c < 2; ++c)
 #pragma unroll
-                for (int f = 0; f < F; ++f)
-                    x(c, f) = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[c][P], b(f)[q], x(c, f), 0, 0, 0);
+                for (int f = 0; f < F; ++f) {
+                    zn_f32x4 &y = FLUSH ? t[c][f] : x(c, f);
+                    y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[c][P], b(f)[q], FLUSH && N == 1 ? zn_f32x4{0.0f, 0.0f, 0.0f, 0.0f} : y, 0, 0, 0);
+                }
         load(P);
         __builtin_amdgcn_sched_group_barrier(0x8, 2 * F * N, 0);                         // MFMA
         if constexpr (READS > 0) __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);  // LDS read
@@ -417,6 +422,12 @@ __device__ __forceinline__ void mha_group(MhaSix &a, Acc x, Operand b, Load load
     products(std::integral_constant<int, 1>());
     products(std::integral_constant<int, 2>());
     products(std::integral_constant<int, 3>());
+    if constexpr (FLUSH) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int f = 0; f < F; ++f) x(c, f) += t[c][f];
+    }
     __builtin_amdgcn_sched_barrier(0);
 }
 
@@ -762,6 +773,8 @@ struct MhaKeyTile {
         const int b = blockIdx.x / p.kv_heads, kh = blockIdx.x - b * p.kv_heads;
         const int j0 = y * (NW * FK * 16), w0 = j0 + wave * FK * 16;
         const MhaSeq seq(p, b);
+        const int ql = __builtin_amdgcn_readfirstlane(seq.ql), kl = __builtin_amdgcn_readfirstlane(seq.kl);
+        const int edge = __builtin_amdgcn_readfirstlane(seq.edge);
         const int64_t kat = b * p.ks[0] + kh * p.ks[1];
 
         zn_bf16x8 kf[FK][SL][3], vf[FK][SL][3];
@@ -776,7 +789,7 @@ struct MhaKeyTile {
                 for (int q = 0; q < 3; ++q) {
                     const int64_t o = at + Frags::place(j % 32, lh, sl, q);
                     zn_u32x4 x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
-                    if (j < seq.kl) {
+                    if (j < kl) {
                         x = *reinterpret_cast<const zn_u32x4 *>(p.ki + o);
                         y = *reinterpret_cast<const zn_u32x4 *>(p.vi + o);
                     }
@@ -787,21 +800,24 @@ struct MhaKeyTile {
             for (int d = 0; d < DB; ++d) dk[f][d] = dv[f][d] = zn_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
         // query blocks of a head that see any of the tile's keys
-        const int b0 = j0 < seq.kl ? seq.first(j0) / 32 : 0, nb = j0 < seq.kl ? max(0, (seq.ql + 31) / 32 - b0) : 0;
+        const int b0 = j0 < kl ? max(0, j0 - edge) / 32 : 0, nb = j0 < kl ? max(0, (ql + 31) / 32 - b0) : 0;
         // this split's share of the blocks of all the group's heads
         const int share = (nb * p.group + p.splits - 1) / p.splits;
         const int from = __builtin_amdgcn_readfirstlane(min((int)blockIdx.z * share, nb * p.group));
         const int total = __builtin_amdgcn_readfirstlane(min(from + share, nb * p.group));
         const float *side = reinterpret_cast<const float *>(lds + kSide);
         const int64_t head0 = ((int64_t)b * p.q_heads + kh * p.group) * p.q_blocks;  // the group's first query block
-        MhaImageStage<DP, NW> sg(lds, tid, nullptr, nullptr);
+        const char *const qi = p.qi + head0 * Frags::kImage, *const gi = p.gi + head0 * Frags::kImage;
+        const float *const sides = p.side + head0 * 64;
+        const int q_blocks = p.q_blocks;
+        MhaImageStage<DP, NW> sg(lds, tid, qi, gi);
         auto fetch = [&](int st, int g, int blk) {
-            const int64_t at = head0 + (int64_t)g * p.q_blocks;
-            sg.src[0] = p.qi + at * Frags::kImage;
-            sg.src[1] = p.gi + at * Frags::kImage;
+            const int64_t at = (int64_t)g * q_blocks;
+            sg.x = qi + at * Frags::kImage;
+            sg.y = gi + at * Frags::kImage;
             sg.fetch(st, blk);
             if (wave == NW - 1) {  // 256 bytes: a value to a lane
-                const __amdgpu_buffer_rsrc_t r = make_rsrc(mha_uniform(p.side + (at + blk) * 64), 256);
+                const __amdgpu_buffer_rsrc_t r = make_rsrc(mha_uniform(sides + (at + blk) * 64), 256);
                 const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(zn_lds_void *)(lds + kSide + st * 256));
                 asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, 0 offen lds" : : "s"(m0), "v"(sg.lane16 / 4), "s"(r) : "memory");
             }
@@ -819,8 +835,8 @@ struct MhaKeyTile {
             }
             if (t + 1 < total) fetch(st ^ 1, g, blk);
             const int hi = w0 + FK * 16;  // keys of this wave: [w0, hi)
-            if (min(i0 + 31, seq.ql - 1) + seq.edge >= w0 && w0 < seq.kl)
-                block(fr, st, i0 + seq.edge < hi - 1 || hi > seq.kl, side + st * 64, i0, w0, seq, lane, kf, vf, dk, dv);
+            if (min(i0 + 31, ql - 1) + edge >= w0 && w0 < kl)
+                block(fr, st, i0 + edge < hi - 1 || hi > kl, side + st * 64, i0, w0, kl, edge, lane, kf, vf, dk, dv);
         }
 
         bool bad = false;
@@ -855,7 +871,7 @@ struct MhaKeyTile {
 
     // One block of 32 queries.  `mask` (of the whole wave): some of its pairs are masked.  One code for both: with a copy for
     // each, the sums lie in other registers at the end of the copies, and moving them together spills.
-    __device__ static __forceinline__ void block(const Frags &sg, int st, bool mask, const float *side, int i0, int w0, const MhaSeq &seq,
+    __device__ static __forceinline__ void block(const Frags &sg, int st, bool mask, const float *side, int i0, int w0, int kl, int edge,
                                                  int lane, const zn_bf16x8 (&kf)[FK][SL][3], const zn_bf16x8 (&vf)[FK][SL][3],
                                                  zn_f32x4 (&dk)[FK][DB], zn_f32x4 (&dv)[FK][DB]) {
         const int li = lane & 15, lh = lane >> 4;
@@ -872,7 +888,7 @@ struct MhaKeyTile {
         // S
 #pragma unroll
         for (int i = 0; i < SL; ++i)
-            mha_group<FK, 2>(a, [&](int rb, int f) -> zn_f32x4 & { return s[f][rb]; }, [&](int f) -> const zn_bf16x8(&)[3] { return kf[f][i]; },
+            mha_group<FK, 2, false>(a, [&](int rb, int f) -> zn_f32x4 & { return s[f][rb]; }, [&](int f) -> const zn_bf16x8(&)[3] { return kf[f][i]; },
                              [&](int q) { sg.dims(st, i + 1 < SL ? 0 : 1, i + 1 < SL ? i + 1 : 0, q, a); });
         // P times 2^24, in the place of S
         {
@@ -891,7 +907,7 @@ struct MhaKeyTile {
                 const int j = w0 + 16 * f + li;
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    if (j >= seq.kl || j > i0 + 16 * (e / 4) + 4 * lh + e % 4 + seq.edge) s[f][e / 4][e % 4] = 0.0f;
+                    if (j >= kl || j > i0 + 16 * (e / 4) + 4 * lh + e % 4 + edge) s[f][e / 4][e % 4] = 0.0f;
             }
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -900,8 +916,8 @@ struct MhaKeyTile {
         for (int i = 0; i < SL; ++i) {
             auto acc = [&](int rb, int f) -> zn_f32x4 & { return dp[f][rb]; };
             auto operand = [&](int f) -> const zn_bf16x8(&)[3] { return vf[f][i]; };
-            if (i + 1 < SL) mha_group<FK, 2>(a, acc, operand, [&](int q) { sg.dims(st, 1, i + 1, q, a); });
-            else mha_group<FK, 4>(a, acc, operand, [&](int q) { sg.rows(st, 1, 0, q, a); });
+            if (i + 1 < SL) mha_group<FK, 2, false>(a, acc, operand, [&](int q) { sg.dims(st, 1, i + 1, q, a); });
+            else mha_group<FK, 4, false>(a, acc, operand, [&](int q) { sg.rows(st, 1, 0, q, a); });
         }
         // dS times 2^24, in the place of P, and P's parts; dS's take their registers once dV is done
         zn_bf16x8 pf[FK][3];
@@ -924,7 +940,7 @@ struct MhaKeyTile {
         // dV^T += dO^T P
 #pragma unroll
         for (int i = 0; i < NR; ++i)
-            mha_group<FK, 4>(a, [&](int c, int f) -> zn_f32x4 & { return dv[f][2 * i + c]; }, [&](int f) -> const zn_bf16x8(&)[3] { return pf[f]; },
+            mha_group<FK, 4, true>(a, [&](int c, int f) -> zn_f32x4 & { return dv[f][2 * i + c]; }, [&](int f) -> const zn_bf16x8(&)[3] { return pf[f]; },
                              [&](int q) { sg.rows(st, i + 1 < NR ? 1 : 0, i + 1 < NR ? 2 * (i + 1) : 0, q, a); });
         // dK^T += Q^T dS
 #pragma unroll
@@ -939,8 +955,8 @@ struct MhaKeyTile {
         for (int i = 0; i < NR; ++i) {
             auto acc = [&](int c, int f) -> zn_f32x4 & { return dk[f][2 * i + c]; };
             auto operand = [&](int f) -> const zn_bf16x8(&)[3] { return pf[f]; };
-            if (i + 1 < NR) mha_group<FK, 4>(a, acc, operand, [&](int q) { sg.rows(st, 0, 2 * (i + 1), q, a); });
-            else mha_group<FK, 0>(a, acc, operand, [](int) {});
+            if (i + 1 < NR) mha_group<FK, 4, true>(a, acc, operand, [&](int q) { sg.rows(st, 0, 2 * (i + 1), q, a); });
+            else mha_group<FK, 0, true>(a, acc, operand, [](int) {});
         }
     }
 };
