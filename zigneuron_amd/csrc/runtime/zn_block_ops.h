@@ -60,11 +60,26 @@ int mha_args(zn_ctx *ctx, ZnMhaArgs &a, int64_t batch, int64_t q_heads, int64_t 
 // Query tiles of a key/value head: the same number for each query head of its group.
 int64_t mha_query_tiles(const ZnMhaArgs &a) { return a.group * cdiv(cdiv((int64_t)a.group * a.q_len, kMhaTile), std::max(a.group, 1)); }
 
-// Parts that tiles' walks of `blocks` blocks are cut into: as many as leave no
-// CU idle, up to 32, with at least 4 blocks each.
-int mha_splits(const zn_ctx *ctx, const ZnMhaArgs &a, int64_t tiles, int64_t blocks) {
+// Parts that tiles' walks of `blocks` blocks are cut into, at most as many as
+// fill the chip once and 64: the time of a part's blocks (forward 0.8 us and 0.012
+// a dim each, backward 1.7 times that) against the join, 4 us and `rows` rows of
+// each part written and read at 2 TB/s.  MI355X, us whole and in parts: 1 x
+// 4096 x 128 forward 232 and (9) 57, its backward 479 and (4) 160; 4 x 256 x 64
+// 23 and (8) 12; but 64 x 256 x 64 (128 tiles of 8 blocks) 24 and (2) 29.
+int mha_splits(const zn_ctx *ctx, const ZnMhaArgs &a, int64_t tiles, int64_t blocks, int64_t rows, bool backward) {
     const int64_t slots = cus_now(ctx) * (a.dim <= 64 ? 2 : 1);  // workgroups at once
-    return (int)std::max<int64_t>(1, std::min<int64_t>({32, slots / std::max<int64_t>(1, tiles), blocks / 4}));
+    const int64_t most = std::min<int64_t>({64, slots / std::max<int64_t>(1, tiles), blocks});
+    const double block_us = (0.8 + 0.012 * a.dim) * (backward ? 1.7 : 1.0);
+    int best = 1;
+    double best_us = block_us * (double)blocks;
+    for (int64_t s = 2; s <= most; ++s) {
+        const double us = block_us * (double)cdiv(blocks, s) + 4.0 + 8.0 * (double)(rows * s) * a.dim / 2e6;
+        if (us < best_us) {
+            best = (int)s;
+            best_us = us;
+        }
+    }
+    return best;
 }
 
 int mha_tiles(zn_ctx *ctx, MhaKernel kernel, ZnMhaArgs &a, int64_t y) {
@@ -146,10 +161,10 @@ int zn_hip_mha_forward(zn_ctx *ctx, const float *q, const float *k, const float 
     // At most 16 rows of a head read K and V as they are.  Each tile splits what it reads: past a few tiles, once for all of
     // them is cheaper.
     const int64_t rows = (int64_t)a.group * q_len, heads = (int64_t)a.batch * a.kv_heads;
-    const MhaKernel kernel = rows <= kMhaFewRows ? kMhaFew : rows <= 4 * kMhaTile ? kMhaForwardRaw : kMhaForward;
+    const MhaKernel kernel = rows <= kMhaFewRows ? kMhaFew : rows < 3 * kMhaTile ? kMhaForwardRaw : kMhaForward;
     a.query_tiles = kernel == kMhaFew ? 1 : (int32_t)mha_query_tiles(a);
     a.splits = kernel == kMhaFew ? (int32_t)std::max<int64_t>(1, std::min<int64_t>({64, 2 * cus_now(ctx) / heads, kv_len / 256}))
-                                 : mha_splits(ctx, a, heads * a.query_tiles, cdiv(kv_len, 32));
+                                 : mha_splits(ctx, a, heads * a.query_tiles, cdiv(kv_len, 32), batch * q_heads * q_len, false);
     Lease part(ctx);
     if (a.splits > 1) {
         a.part_ld = (a.dim + 3) / 4 * 4 + 4;
@@ -219,9 +234,10 @@ int zn_hip_mha_backward(zn_ctx *ctx, const float *q, const float *k, const float
     a.key_tiles = (int32_t)cdiv(kv_len, kMhaTile);
     a.query_tiles = queries ? (int32_t)mha_query_tiles(a) : 0;
     const int64_t y = a.key_tiles + a.query_tiles;
-    a.splits = mha_splits(ctx, a, (int64_t)a.batch * a.kv_heads * y, std::max<int64_t>(a.k_blocks, (int64_t)a.group * a.q_blocks));
-    Lease part(ctx);
     const int64_t q_rows = batch * q_heads * q_len, k_rows = batch * kv_heads * kv_len;
+    a.splits = mha_splits(ctx, a, (int64_t)a.batch * a.kv_heads * y, std::max<int64_t>(a.k_blocks, (int64_t)a.group * a.q_blocks),
+                          q_rows + 2 * k_rows, true);
+    Lease part(ctx);
     if (a.splits > 1) {
         a.part_ld = (a.dim + 3) / 4 * 4;
         if ((rc = part.get((size_t)(q_rows + 2 * k_rows) * a.splits * a.part_ld))) return rc;
