@@ -411,7 +411,9 @@ int zn_hip_attention_forward(zn_ctx *ctx, const float *q, const float *k, const 
  * needs beside its Dense layers, forward and backward, in fp32.  Buffers of
  * one call must not overlap unless it says so.  Like every device-pointer
  * call they run on the context's stream, may be captured into a graph, and
- * give the same bits each time. */
+ * give the same bits each time.  Sizes past a launch's or a 32-bit offset's
+ * range are ZN_ERR_OVERFLOW.  Workspaces (split tensors: 6 bytes a value of
+ * what the attention reads; partial sums) come from the context's buffer cache. */
 
 /* Multi-head attention with shared key/value heads: query head h reads
  * key/value head h / (q_heads / kv_heads).

@@ -51,7 +51,7 @@ def test_mha(lib, blank, back):
                 {"scale": float("inf")}, {"scale": float("nan")}, {"causal": 2}, {"causal": -1}, {"qs": 15}, {"ks": 15}, {"os": 15},
                 {"qs": (1 << 22) + 1}, {"ks": (1 << 22) + 1}, {"os": (1 << 22) + 1}, {"qb": -1}, {"kh": -1}, {"ob": -1}):
         assert mha(lib, blank, back, **bad) == INVALID, bad
-    for big in ({"batch": BIG}, {"q_len": BIG}, {"kv_len": BIG}, {"q_heads": BIG}, {"batch": 1 << 29, "q_heads": 8}):
+    for big in ({"batch": BIG}, {"q_len": BIG}, {"kv_len": BIG}, {"q_heads": BIG}, {"batch": 1 << 29, "q_heads": 8}, {"batch": 1 << 23}):
         assert mha(lib, blank, back, **big) == OVERFLOW, big
     for nothing in ({"batch": 0}, {"q_heads": 0, "kv_heads": 0}, {"q_len": 0, "kv_len": 0}):
         assert mha(lib, blank, back, **nothing) == 0, nothing
@@ -77,7 +77,7 @@ def test_gated(lib, blank):
         assert call() not in (0, INVALID, OVERFLOW)
         for bad in ({"act": -1}, {"act": 6}, {"batch": -1}, {"n_in": -1}, {"hidden": -1}, *({n: None} for n in needed)):
             assert call(**bad) == INVALID, bad
-        for big in ({"batch": BIG}, {"n_in": BIG}, {"hidden": BIG}):
+        for big in ({"batch": BIG}, {"n_in": BIG}, {"hidden": BIG}, {"batch": 1 << 16, "n_in": 1 << 14}, {"n_in": 1 << 15, "hidden": 1 << 14}):
             assert call(**big) == OVERFLOW, big
     assert f(batch=0) == 0 and f(hidden=0) == 0
 

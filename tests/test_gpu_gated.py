@@ -180,6 +180,26 @@ def test_the_same_bits_each_time_and_in_a_graph(ctx):
     graph.close()
 
 
+@pytest.mark.parametrize("size", [(5, 2000, 900), (200, 300, 260), (2048, 256, 512)])
+def test_forced_launch_choices_hold_for_the_projections(ctx, size):
+    """A forced tile or split is the projections' too: the result is the same layer's, within its bound."""
+    x, w, b, _, _ = make(12, *size)
+    z, ez, h, eh = forward_ref("gelu", x, w, b)
+    try:
+        for force in (lambda: ctx.set_gemm_tile("64x64"), lambda: ctx.set_gemm_splits(2), lambda: ctx.set_gemm_wave_split(4)):
+            force()
+            gz, gh = run_forward(ctx, "gelu", x, w, b)
+            check(gz, z, ez, "z")
+            check(gh, h, eh, "h")
+            ctx.set_gemm_tile("auto")
+            ctx.set_gemm_splits(0)
+            ctx.set_gemm_wave_split(-1)
+    finally:
+        ctx.set_gemm_tile("auto")
+        ctx.set_gemm_splits(0)
+        ctx.set_gemm_wave_split(-1)
+
+
 def test_empty_extents(ctx):
     t = ctx.alloc(64).fill(7.0)
     ctx.gated_dense_forward("silu", t, t, None, None, t, 0, 4, 4)

@@ -202,6 +202,20 @@ def test_masked_values_reach_nothing(ctx, dim, s, bad):
     assert np.isnan(gq[:, :, bad:]).all() and np.isnan(gk).all() and np.isnan(gv).all()
 
 
+@pytest.mark.parametrize("causal", [False, True])
+def test_new_tokens_of_sequences_of_all_lengths(ctx, causal):
+    """One or two new tokens a sequence, caches from nothing to long, padding that holds anything."""
+    q_lens, kv_lens = [1, 2, 0, 2, 1, 2], [5, 0, 7, 900, 1024, 1]
+    shape = (6, 6, 2, 2, 1024, 64)
+    q, k, v, g = make(47, *shape)
+    for n in range(6):
+        q[n, :, q_lens[n]:], g[n, :, q_lens[n]:] = np.nan, np.inf
+        k[n, :, kv_lens[n]:], v[n, :, kv_lens[n]:] = np.inf, np.nan
+        hidden = max(0, q_lens[n] - kv_lens[n]) if causal else (q_lens[n] if kv_lens[n] == 0 else 0)
+        g[n, :, :hidden] = np.nan
+    both(ctx, q, k, v, g, 0.125, causal, q_lens, kv_lens, what="new tokens")
+
+
 @pytest.mark.parametrize("dim", [24, 64, 96, 128])
 def test_a_few_rows_beside_a_masked_nan(ctx, dim):
     """Four new tokens against a long cache whose last keys only the last of them see."""

@@ -12,6 +12,8 @@ namespace {
 constexpr int64_t kMhaMaxDim = 128;
 constexpr int64_t kMhaMaxRow = (int64_t)1 << 22;  // position stride: a block of 64 rows stays inside 32-bit offsets
 
+constexpr int64_t kMhaMaxBlocks = ((int64_t)1 << 24) - 1;  // 32-row blocks to split in one launch
+
 // Element strides that a call only reads, or (written) also writes.
 bool mha_strides_ok(int64_t sb, int64_t sh, int64_t ss, int64_t batch, int64_t heads, int64_t rows, int64_t dim,
                     bool written) {
@@ -32,8 +34,8 @@ int mha_args(zn_ctx *ctx, ZnMhaArgs &a, int64_t batch, int64_t q_heads, int64_t 
         !mha_strides_ok(ks[0], ks[1], ks[2], batch, kv_heads, kv_len, head_dim, backward) ||
         !mha_strides_ok(os[0], os[1], os[2], batch, q_heads, q_len, head_dim, !backward))
         return ZN_ERR_INVALID_ARG;
-    constexpr int64_t kMax = INT_MAX / 2;
-    if (batch > kMax || q_heads > kMax || q_len > kMax || kv_len > kMax || batch * q_heads > kMax || batch * kv_heads > kMax)
+    constexpr int64_t kMax = INT_MAX / 2, kMaxHeads = (int64_t)1 << 22;  // heads: a launch has fewer than 2^32 threads
+    if (batch > kMax || q_heads > kMax || q_len > kMax || kv_len > kMax || batch * q_heads > kMax || batch * kv_heads > kMaxHeads)
         return ZN_ERR_OVERFLOW;
     constexpr int64_t kMaxRows = (int64_t)65535 * kMhaTile;  // the grid's second extent
     if (kv_len + (kv_heads ? q_heads / kv_heads * (q_len + kMhaTile) : 0) > kMaxRows) return ZN_ERR_OVERFLOW;
@@ -174,7 +176,7 @@ int zn_hip_mha_forward(zn_ctx *ctx, const float *q, const float *k, const float 
     MhaImages im(ctx);
     if (kernel == kMhaForward && kv_len > 0) {
         const int64_t ki = im.add(a, k, a.ks, a.kv_lens, a.kv_heads, a.kv_len, 1.0f), vi = im.add(a, v, a.ks, a.kv_lens, a.kv_heads, a.kv_len, 1.0f);
-        if (im.groups > INT_MAX / 2) return ZN_ERR_OVERFLOW;
+        if (im.groups > kMhaMaxBlocks) return ZN_ERR_OVERFLOW;
         if ((rc = im.get(0))) return rc;
         a.k_blocks = im.s.op[0].blocks;
         a.ki = im.s.op[0].dst = im.at(ki);
@@ -219,7 +221,7 @@ int zn_hip_mha_backward(zn_ctx *ctx, const float *q, const float *k, const float
     const int64_t gi = im.add(a, grad_out, a.os, a.q_lens, a.q_heads, a.q_len, 1.0f);
     const int64_t ki = im.add(a, k, a.ks, a.kv_lens, a.kv_heads, a.kv_len, 1.0f);
     const int64_t vi = im.add(a, v, a.ks, a.kv_lens, a.kv_heads, a.kv_len, 1.0f);
-    if (im.groups > INT_MAX / 2) return ZN_ERR_OVERFLOW;
+    if (im.groups > kMhaMaxBlocks) return ZN_ERR_OVERFLOW;
     a.q_blocks = im.s.op[0].blocks;
     a.k_blocks = im.s.op[2].blocks;
     if ((rc = im.get((int64_t)a.batch * a.q_heads * a.q_blocks * 256))) return rc;
@@ -254,12 +256,14 @@ int zn_hip_mha_backward(zn_ctx *ctx, const float *q, const float *k, const float
 }
 
 // ----------------------------------------------------------- gated Dense
-static bool gated_extents_ok(int64_t batch, int64_t in_size, int64_t hidden) {
-    return batch <= INT_MAX && in_size <= INT_MAX && hidden <= INT_MAX / 2;
-}
-
-// One problem's operands stay below 2 GiB, as every GEMM's.
+// One problem's operands stay below 2 GiB, as every GEMM's: x, W and, for the backward, z.
 constexpr int64_t kGatedLimit = (int64_t)INT_MAX / 4;
+
+static bool gated_extents_ok(int64_t batch, int64_t in_size, int64_t hidden, bool backward) {
+    if (batch > INT_MAX || in_size > INT_MAX || hidden > INT_MAX / 2) return false;
+    const int64_t n = 2 * hidden;
+    return batch * in_size <= kGatedLimit && in_size * n <= kGatedLimit && (!backward || batch * n <= kGatedLimit);
+}
 
 // At most 16 rows: from this many weights on the kernel that reads them once
 // (MI355X, us with it and as a product and a pass: 4 x 1024 x 8192 9.4 and 14.6,
@@ -286,7 +290,7 @@ int zn_hip_gated_dense_forward(zn_ctx *ctx, int act, const float *x, const float
                                float *h, int64_t batch, int64_t in_size, int64_t hidden) {
     if (!ctx || act < ZN_GATE_LINEAR || act > ZN_GATE_GELU || batch < 0 || in_size < 0 || hidden < 0)
         return ZN_ERR_INVALID_ARG;
-    if (!gated_extents_ok(batch, in_size, hidden)) return ZN_ERR_OVERFLOW;
+    if (!gated_extents_ok(batch, in_size, hidden, false)) return ZN_ERR_OVERFLOW;
     if (batch == 0 || hidden == 0) return ZN_OK;
     if (!h || (in_size > 0 && (!x || !w))) return ZN_ERR_INVALID_ARG;
     int rc = select_device(ctx);
@@ -310,8 +314,9 @@ int zn_hip_gated_dense_forward(zn_ctx *ctx, int act, const float *x, const float
     p.splits = 1;
     p.batch = 1;
     p.k_chunk = (int32_t)in_size;
-    const bool fits = in_size > 0 && batch <= kGatedLimit / std::max<int64_t>(in_size, 1) && in_size <= kGatedLimit / n;
-    if (fits && batch <= 16 && in_size * n >= kFewWeights) {
+    // a forced tile, split or wave split takes the product and a pass
+    const bool free = in_size > 0 && ctx->forced_tile < 0 && ctx->forced_splits == 0 && ctx->forced_wave_split < 0 && ctx->forced_persistent < 0;
+    if (free && batch <= 16 && in_size * n >= kFewWeights) {
         const int64_t wgs = cdiv(hidden, 32);
         p.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>(cus_now(ctx) / wgs, in_size / 1024));
         Lease part(ctx);
@@ -322,7 +327,7 @@ int zn_hip_gated_dense_forward(zn_ctx *ctx, int act, const float *x, const float
         if ((rc = launch(ctx, ctx->gated_few, (unsigned)wgs, 1, 1024, &p, (unsigned)p.splits)) || p.splits == 1) return rc;
         return launch(ctx, ctx->gated_few_join, (unsigned)cdiv(hidden, 256), (unsigned)batch, 256, &p);
     }
-    if (fits && gated_pays(ctx, batch, n, in_size)) {
+    if (free && gated_pays(ctx, batch, n, in_size)) {
         const Tile tile = estimate_split(ctx, batch, n, in_size, 1, 0).tile;
         p.tiles_m = (int32_t)cdiv(batch, kTiles[tile].bm);
         p.tiles_n = (int32_t)cdiv(hidden, kTiles[tile].bn / 2);
@@ -352,7 +357,7 @@ int zn_hip_gated_dense_backward(zn_ctx *ctx, int act, const float *x, const floa
                                 int64_t batch, int64_t in_size, int64_t hidden) {
     if (!ctx || act < ZN_GATE_LINEAR || act > ZN_GATE_GELU || batch < 0 || in_size < 0 || hidden < 0)
         return ZN_ERR_INVALID_ARG;
-    if (!gated_extents_ok(batch, in_size, hidden)) return ZN_ERR_OVERFLOW;
+    if (!gated_extents_ok(batch, in_size, hidden, true)) return ZN_ERR_OVERFLOW;
     const int64_t n = 2 * hidden;
     if (batch > 0 && hidden > 0 && (!z || !grad_h || !grad_z)) return ZN_ERR_INVALID_ARG;
     if (in_size > 0 && hidden > 0 && (!grad_w || (batch > 0 && (!x || !w)))) return ZN_ERR_INVALID_ARG;
