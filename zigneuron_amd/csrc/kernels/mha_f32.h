@@ -95,18 +95,19 @@ struct MhaRowState {
 
 __device__ __forceinline__ float mha_lse(float m, float l) { return l == 0.0f ? -INFINITY : (m + __log2f(l)) * kLn2; }
 
-// Where sums go: to the tensor's row, or to this split's part of it.
-__device__ __forceinline__ float *mha_part(const ZnMhaArgs &p, int64_t row) { return p.part + (row * p.splits + blockIdx.z) * p.part_ld; }
+// Where sums go: to the tensor's row, or to the row's part z (of the walk that the workgroup takes).
+__device__ __forceinline__ float *mha_query_part(const ZnMhaArgs &p, int64_t row, int z) { return p.part + (row * p.splits + z) * p.part_ld; }
+__device__ __forceinline__ float *mha_key_part(const ZnMhaArgs &p, int64_t row, int z) { return p.kv_part + (row * p.kv_splits + z) * p.part_ld; }
 __device__ __forceinline__ int64_t mha_query_row(const ZnMhaArgs &p, int b, int h, int i) { return ((int64_t)b * p.q_heads + h) * p.q_len + i; }
-// ... key rows behind all query rows, dK's then dV's
+// ... dK's key rows, then dV's
 __device__ __forceinline__ int64_t mha_key_row(const ZnMhaArgs &p, int b, int kh, int j, bool v) {
-    return (int64_t)p.batch * p.q_heads * p.q_len + (((int64_t)(v ? p.batch : 0) + b) * p.kv_heads + kh) * p.kv_len + j;
+    return (((int64_t)(v ? p.batch : 0) + b) * p.kv_heads + kh) * p.kv_len + j;
 }
 
 // O and lse of a row from its sums, or its part: dims lane and lane + 64.
-__device__ __forceinline__ void mha_row_finish(const ZnMhaArgs &p, int b, int h, int i, int lane, float m, float l, float oa, float ob) {
+__device__ __forceinline__ void mha_row_finish(const ZnMhaArgs &p, int b, int h, int i, int z, int lane, float m, float l, float oa, float ob) {
     if (p.splits > 1) {
-        float *part = mha_part(p, mha_query_row(p, b, h, i));
+        float *part = mha_query_part(p, mha_query_row(p, b, h, i), z);
         MhaRow::store(part, p.dim, lane, oa, ob);
         if (lane == 0) {
             part[p.part_ld - 4] = m;
@@ -120,10 +121,10 @@ __device__ __forceinline__ void mha_row_finish(const ZnMhaArgs &p, int b, int h,
 }
 
 // A row's walk over keys [from, to), those of them that it sees.
-__device__ __forceinline__ void mha_row_forward(const ZnMhaArgs &p, int b, int h, int i, int from, int to, int lane) {
+__device__ __forceinline__ void mha_row_forward(const ZnMhaArgs &p, int b, int h, int i, int z, int from, int to, int lane) {
     MhaRowState s;
     s.walk(p, b, h, i, from, min(to, MhaSeq(p, b).seen(i)), lane);
-    mha_row_finish(p, b, h, i, lane, s.m, s.l, s.oa, s.ob);
+    mha_row_finish(p, b, h, i, z, lane, s.m, s.l, s.oa, s.ob);
 }
 
 // Where a query's lse (log2 domain) and delta lie.
@@ -132,7 +133,7 @@ __device__ __forceinline__ const float *mha_side(const ZnMhaArgs &p, int b, int 
 }
 
 // grad_q of a row over keys [from, to).
-__device__ __forceinline__ void mha_row_grad_q(const ZnMhaArgs &p, int b, int h, int i, int from, int to, int lane) {
+__device__ __forceinline__ void mha_row_grad_q(const ZnMhaArgs &p, int b, int h, int i, int z, int from, int to, int lane) {
     const MhaSeq seq(p, b);
     int n = min(to, seq.seen(i));
     const float *side = mha_side(p, b, h, i);
@@ -151,13 +152,13 @@ __device__ __forceinline__ void mha_row_grad_q(const ZnMhaArgs &p, int b, int h,
         ga += ds * kr.a;
         gb += ds * kr.b;
     }
-    if (p.splits > 1) MhaRow::store(mha_part(p, mha_query_row(p, b, h, i)), p.dim, lane, ga, gb);
+    if (p.splits > 1) MhaRow::store(mha_query_part(p, mha_query_row(p, b, h, i), z), p.dim, lane, ga, gb);
     else MhaRow::store(p.grad_q + qat, p.dim, lane, ga * p.scale, gb * p.scale);
 }
 
 // grad_k and grad_v of a row over the query blocks [from, to) of its tile's walk: nb blocks from b0 of each query head of the
 // group, the heads in order, the queries ascending.
-__device__ __forceinline__ void mha_row_grad_kv(const ZnMhaArgs &p, int b, int kh, int j, int b0, int nb, int from, int to, int lane) {
+__device__ __forceinline__ void mha_row_grad_kv(const ZnMhaArgs &p, int b, int kh, int j, int z, int b0, int nb, int from, int to, int lane) {
     const MhaSeq seq(p, b);
     const bool in = j < seq.kl;
     const int64_t kat = b * p.ks[0] + kh * p.ks[1] + j * p.ks[2];
@@ -179,9 +180,9 @@ __device__ __forceinline__ void mha_row_grad_kv(const ZnMhaArgs &p, int b, int k
             kb += ds * q.b;
         }
     }
-    const bool part = p.splits > 1;
-    MhaRow::store(part ? mha_part(p, mha_key_row(p, b, kh, j, false)) : p.grad_k + kat, p.dim, lane, ka * p.scale, kb * p.scale);
-    MhaRow::store(part ? mha_part(p, mha_key_row(p, b, kh, j, true)) : p.grad_v + kat, p.dim, lane, va, vb);
+    const bool part = p.kv_splits > 1;
+    MhaRow::store(part ? mha_key_part(p, mha_key_row(p, b, kh, j, false), z) : p.grad_k + kat, p.dim, lane, ka * p.scale, kb * p.scale);
+    MhaRow::store(part ? mha_key_part(p, mha_key_row(p, b, kh, j, true), z) : p.grad_v + kat, p.dim, lane, va, vb);
 }
 
 // ------------------------------------------------------------------- tiles
@@ -204,6 +205,18 @@ __device__ __forceinline__ void mha_row_grad_kv(const ZnMhaArgs &p, int b, int k
 // staged blocks (10 bytes of traffic a value), which the tiles then bring to LDS
 // by DMA (MhaImageStage).  Where it goes past few, the thread that loads a value
 // splits it (MhaRawStage).
+//
+// What bounds the tiles is the matrix cores: six bf16 products for one fp32
+// product, at a clock that the power limit holds near 2 GHz while they are three
+// quarters busy (the split GEMM's share too).  MI355X, forward of 2 x 16 heads
+// (4 key/value) of 2048 x 128, causal: 168 us with the split, 205 TFLOP/s of
+// fp32 products; both gradients of 2 x 32 heads (8) of 4096 x 128, causal, 4.4 ms,
+// 158 TFLOP/s; of 8 x 16 heads of 1024 x 64, 560 us, 153 TFLOP/s.
+//
+// Sums stand at 2^48 times their value, so that nothing of a split is lost: one
+// beyond 2^80 or so, an infinity or a NaN (visible, or masked for some rows
+// of a block only, where it meets a probability of 0) makes a sum that is not
+// finite, and the wave then takes its rows one at a time.
 template <int DP>
 struct MhaBlock {
     static constexpr int BR = 32, SL = DP / 32, DB = DP / 16;
@@ -519,8 +532,8 @@ struct MhaQueryTile {
     static constexpr int kBytes = 2 * Frags::kStage;
     static_assert(IMAGE || !BACK, "the backward's tensors are all split before");
 
-    // Tile y: causal rows see more the later they come, so the last tiles of each head come first.
-    __device__ static __forceinline__ void run(const ZnMhaArgs &p, int y, char *lds) {
+    // Tile y, part z of its walk: causal rows see more the later they come, so the last tiles of each head come first.
+    __device__ static __forceinline__ void run(const ZnMhaArgs &p, int y, int z, char *lds) {
         const int tid = threadIdx.x, lane = tid & (kWave - 1);
         const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
         const int li = lane & 15, lh = lane >> 4;
@@ -585,9 +598,9 @@ struct MhaQueryTile {
         }
 
         const Frags fr(lds, lane);
-        // this split's share of the blocks
+        // the part's share of the blocks
         const int all_blocks = (last + 31) / 32, share = (all_blocks + p.splits - 1) / p.splits;
-        const int blk0 = __builtin_amdgcn_readfirstlane(min((int)blockIdx.z * share, all_blocks)), nblk = __builtin_amdgcn_readfirstlane(min(blk0 + share, all_blocks));
+        const int blk0 = __builtin_amdgcn_readfirstlane(min(z * share, all_blocks)), nblk = __builtin_amdgcn_readfirstlane(min(blk0 + share, all_blocks));
         auto walk = [&](Stage sg) {
             if (blk0 < nblk) {
                 sg.fetch(0, blk0);
@@ -626,8 +639,8 @@ struct MhaQueryTile {
             for (int x = 0; x < 16 * FQ; ++x) {
                 const MhaQuery r(p, kh, w0 + x);
                 if (!r.in) break;
-                if constexpr (BACK) mha_row_grad_q(p, b, r.h, r.i, 32 * blk0, 32 * nblk, lane);
-                else mha_row_forward(p, b, r.h, r.i, 32 * blk0, 32 * nblk, lane);
+                if constexpr (BACK) mha_row_grad_q(p, b, r.h, r.i, z, 32 * blk0, 32 * nblk, lane);
+                else mha_row_forward(p, b, r.h, r.i, z, 32 * blk0, 32 * nblk, lane);
             }
             return;
         }
@@ -641,7 +654,7 @@ struct MhaQueryTile {
             }
             if (!r.in) continue;
             if (p.splits > 1) {
-                float *part = mha_part(p, mha_query_row(p, b, r.h, r.i));
+                float *part = mha_query_part(p, mha_query_row(p, b, r.h, r.i), z);
 #pragma unroll
                 for (int d = 0; d < DB; ++d) mha_store4(part, Frags::dim_of(d, lh), p.dim, o[f][d]);
                 if (!BACK && lh == 0) {
@@ -766,7 +779,7 @@ struct MhaKeyTile {
     static constexpr int kSide = 2 * Frags::kStage;  // lse and delta of two stages' rows: [stage][lse, delta][32]
     static constexpr int kBytes = kSide + 2 * 64 * 4;
 
-    __device__ static __forceinline__ void run(const ZnMhaArgs &p, int y, char *lds) {
+    __device__ static __forceinline__ void run(const ZnMhaArgs &p, int y, int z, char *lds) {
         const int tid = threadIdx.x, lane = tid & (kWave - 1);
         const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
         const int li = lane & 15, lh = lane >> 4;
@@ -801,9 +814,9 @@ struct MhaKeyTile {
         }
         // query blocks of a head that see any of the tile's keys
         const int b0 = j0 < kl ? max(0, j0 - edge) / 32 : 0, nb = j0 < kl ? max(0, (ql + 31) / 32 - b0) : 0;
-        // this split's share of the blocks of all the group's heads
-        const int share = (nb * p.group + p.splits - 1) / p.splits;
-        const int from = __builtin_amdgcn_readfirstlane(min((int)blockIdx.z * share, nb * p.group));
+        // the part's share of the blocks of all the group's heads
+        const int share = (nb * p.group + p.kv_splits - 1) / p.kv_splits;
+        const int from = __builtin_amdgcn_readfirstlane(min(z * share, nb * p.group));
         const int total = __builtin_amdgcn_readfirstlane(min(from + share, nb * p.group));
         const float *side = reinterpret_cast<const float *>(lds + kSide);
         const int64_t head0 = ((int64_t)b * p.q_heads + kh * p.group) * p.q_blocks;  // the group's first query block
@@ -851,16 +864,16 @@ struct MhaKeyTile {
                     dv[f][d][r] *= kSplitUnscale;
                 }
         if (__builtin_amdgcn_ballot_w64(bad)) {
-            for (int j = w0; j < min(w0 + FK * 16, p.kv_len); ++j) mha_row_grad_kv(p, b, kh, j, b0, nb, from, total, lane);
+            for (int j = w0; j < min(w0 + FK * 16, p.kv_len); ++j) mha_row_grad_kv(p, b, kh, j, z, b0, nb, from, total, lane);
             return;
         }
 #pragma unroll
         for (int f = 0; f < FK; ++f) {
             const int j = w0 + 16 * f + li;
             if (j >= p.kv_len) continue;
-            const bool part = p.splits > 1;
-            float *rk = part ? mha_part(p, mha_key_row(p, b, kh, j, false)) : p.grad_k + kat + j * p.ks[2];
-            float *rv = part ? mha_part(p, mha_key_row(p, b, kh, j, true)) : p.grad_v + kat + j * p.ks[2];
+            const bool part = p.kv_splits > 1;
+            float *rk = part ? mha_key_part(p, mha_key_row(p, b, kh, j, false), z) : p.grad_k + kat + j * p.ks[2];
+            float *rv = part ? mha_key_part(p, mha_key_row(p, b, kh, j, true), z) : p.grad_v + kat + j * p.ks[2];
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
                 mha_store4(rk, Frags::dim_of(d, lh), p.dim, dk[f][d]);
@@ -968,7 +981,9 @@ struct MhaKeyTile {
 // through LDS: each of the NW waves of each workgroup and split walks its own
 // keys, 16 at a time, loaded one step ahead straight into the fragments (K:
 // lane li a key, 4 dims of each 16 per quarter; V: lane li DB neighbouring
-// dims of one key per quarter).  The waves' sums are joined in LDS.
+// dims of one key per quarter).  The waves' sums are joined in LDS.  MI355X, 8
+// tokens of 16 heads (4) against 2048 x 64: 9.6 us for 33.5 MB (3.5 TB/s; a
+// wave has four steps), and 4 us for the join of the splits.
 template <int DP, int NW>
 struct MhaFew {
     static constexpr int G = DP / 16;  // groups of 16 dims; also the 16-dim blocks of O^T, block c the dims G li + c
@@ -1126,7 +1141,7 @@ struct MhaFew {
                 if (lane < p.dim) oa += f * t[lane];
                 if (lane + 64 < p.dim) ob += f * t[lane + 64];
             }
-            mha_row_finish(p, b, w.h, w.i, lane, mx, sl, oa, ob);
+            mha_row_finish(p, b, w.h, w.i, blockIdx.z, lane, mx, sl, oa, ob);
         }
     }
 };
@@ -1134,7 +1149,8 @@ struct MhaFew {
 // Tensors to their images: a workgroup to a block of 32 rows, a unit of 8
 // values to a thread and step.  Rows past a sequence's length are zeros, and on
 // the query side rows that see nothing (lse -inf); blocks past it are not read
-// and not written.  10 bytes of traffic a value, and out's 4 for delta.
+// and not written.  10 bytes of traffic a value, and out's 4 for delta (MI355X, the
+// four tensors of 8 x 16 heads of 1024 x 64: 66 us, 5.6 TB/s).
 template <int DP>
 __device__ __forceinline__ void mha_split(const ZnMhaSplitArgs &a) {
     typedef MhaBlock<DP> B;
@@ -1191,27 +1207,27 @@ __device__ __forceinline__ void mha_split(const ZnMhaSplitArgs &a) {
 
 }  // namespace
 
-// Rows of partial sums: the splits in order, a wave to a row, lane l its dims l
+// Rows of partial sums: the parts in order, a wave to a row, lane l its dims l
 // and l + 64, eight splits' loads in flight.
 extern "C" __global__ __launch_bounds__(256) void zn_mha_join(ZnMhaJoinArgs a) {
     const ZnMhaJoinOp &p = a.op[blockIdx.y];
     const int lane = threadIdx.x & (kWave - 1);
     const int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
     if (row >= p.rows) return;
-    const float *src = p.part + row * a.splits * a.part_ld;
+    const float *src = p.part + row * p.splits * a.part_ld;
     float mx = -INFINITY;
     if (a.forward) {
-        for (int z = lane; z < a.splits; z += kWave) mx = fmaxf(mx, src[(int64_t)z * a.part_ld + a.part_ld - 4]);
+        for (int z = lane; z < p.splits; z += kWave) mx = fmaxf(mx, src[(int64_t)z * a.part_ld + a.part_ld - 4]);
 #pragma unroll
         for (int s = 32; s > 0; s >>= 1) mx = fmaxf(mx, __shfl_xor(mx, s));
     }
     const float ref = mx == -INFINITY ? 0.0f : mx;
     float sl = 0.0f, oa = 0.0f, ob = 0.0f;
-    for (int z0 = 0; z0 < a.splits; z0 += 8) {
+    for (int z0 = 0; z0 < p.splits; z0 += 8) {
         float x[8], y[8], m[8], l[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
-            const bool in = z0 + u < a.splits;
+            const bool in = z0 + u < p.splits;
             const float *t = src + (int64_t)(in ? z0 + u : 0) * a.part_ld;
             x[u] = in && lane < a.dim ? t[lane] : 0.0f;
             y[u] = in && lane + 64 < a.dim ? t[lane + 64] : 0.0f;
@@ -1237,28 +1253,35 @@ extern "C" __global__ __launch_bounds__(256) void zn_mha_join(ZnMhaJoinArgs a) {
     }
 }
 
-// Grid: x = sequence and key/value head (its tiles share an XCD's L2), y = tiles, z = splits.
+// Grid: x = sequence and key/value head (its tiles share an XCD's L2), y = the parts of each tile, the longest walks first (the
+// gradients': tiles of keys before those of queries).  zn_mha_few_*: z = the parts.
 #define ZN_MHA_KERNEL(NAME, NW, BYTES, ...)                                           \
     extern "C" __global__ __launch_bounds__(NW * 64, 2) void NAME(ZnMhaArgs p) {      \
         __shared__ __attribute__((aligned(1024))) char lds[BYTES];                    \
         __VA_ARGS__;                                                                  \
     }
-#define ZN_MHA_KERNELS(DP, NW, F)                                                                               \
-    typedef MhaQueryTile<DP, NW, F, false, true> MhaForward##DP;                                                \
-    typedef MhaQueryTile<DP, NW, F, false, false> MhaForwardRaw##DP;                                            \
-    typedef MhaQueryTile<DP, NW, F, true, true> MhaGradQ##DP;                                                   \
-    typedef MhaKeyTile<DP, NW, F> MhaGradKv##DP;                                                                \
-    typedef MhaFew<DP, 4> MhaFew##DP;                                                                           \
-    ZN_MHA_KERNEL(zn_mha_few_##DP, 4, MhaFew##DP::kBytes, MhaFew##DP::run(p, lds))                              \
-    ZN_MHA_KERNEL(zn_mha_forward_##DP, NW, MhaForward##DP::kBytes, MhaForward##DP::run(p, blockIdx.y, lds))      \
-    ZN_MHA_KERNEL(zn_mha_forward_raw_##DP, NW, MhaForwardRaw##DP::kBytes, MhaForwardRaw##DP::run(p, blockIdx.y, lds)) \
-    ZN_MHA_KERNEL(zn_mha_grad_##DP, NW, MhaGradKv##DP::kBytes,                                                  \
-                  if ((int)blockIdx.y < p.key_tiles) MhaGradKv##DP::run(p, blockIdx.y, lds);                    \
-                  else MhaGradQ##DP::run(p, blockIdx.y - p.key_tiles, lds))                                     \
+// NW waves of F blocks of 16 rows, backward BNW waves of BF.  Workgroups of 4 waves
+// share a CU by two, as far as LDS allows: up to 96 dims.  There the backward gains (both gradients of 2 x 16 heads (4) of
+// 2048 x 96, causal: 809 us with 8 waves, 694 with 4) and the forward loses (137 and 159).
+#define ZN_MHA_KERNELS(DP, NW, F, BNW, BF)                                                                         \
+    typedef MhaQueryTile<DP, NW, F, false, true> MhaForward##DP;                                                   \
+    typedef MhaQueryTile<DP, NW, F, false, false> MhaForwardRaw##DP;                                               \
+    typedef MhaQueryTile<DP, BNW, BF, true, true> MhaGradQ##DP;                                                    \
+    typedef MhaKeyTile<DP, BNW, BF> MhaGradKv##DP;                                                                 \
+    typedef MhaFew<DP, 4> MhaFew##DP;                                                                              \
+    ZN_MHA_KERNEL(zn_mha_few_##DP, 4, MhaFew##DP::kBytes, MhaFew##DP::run(p, lds))                                 \
+    ZN_MHA_KERNEL(zn_mha_forward_##DP, NW, MhaForward##DP::kBytes,                                                 \
+                  MhaForward##DP::run(p, blockIdx.y / p.splits, blockIdx.y % p.splits, lds))                       \
+    ZN_MHA_KERNEL(zn_mha_forward_raw_##DP, NW, MhaForwardRaw##DP::kBytes,                                          \
+                  MhaForwardRaw##DP::run(p, blockIdx.y / p.splits, blockIdx.y % p.splits, lds))                    \
+    ZN_MHA_KERNEL(zn_mha_grad_##DP, BNW, MhaGradKv##DP::kBytes,                                                    \
+                  const int y = (int)blockIdx.y - p.key_tiles * p.kv_splits;                                       \
+                  if (y < 0) MhaGradKv##DP::run(p, blockIdx.y / p.kv_splits, blockIdx.y % p.kv_splits, lds);       \
+                  else MhaGradQ##DP::run(p, y / p.splits, y % p.splits, lds))                                      \
     extern "C" __global__ __launch_bounds__(256) void zn_mha_split_##DP(ZnMhaSplitArgs a) { mha_split<DP>(a); }
-ZN_MHA_KERNELS(32, 4, 2)
-ZN_MHA_KERNELS(64, 4, 2)
-ZN_MHA_KERNELS(96, 8, 1)
-ZN_MHA_KERNELS(128, 8, 1)
+ZN_MHA_KERNELS(32, 4, 2, 4, 2)
+ZN_MHA_KERNELS(64, 4, 2, 4, 2)
+ZN_MHA_KERNELS(96, 8, 1, 4, 1)
+ZN_MHA_KERNELS(128, 8, 1, 8, 1)
 
 #endif

@@ -37,8 +37,8 @@ int mha_args(zn_ctx *ctx, ZnMhaArgs &a, int64_t batch, int64_t q_heads, int64_t 
     constexpr int64_t kMax = INT_MAX / 2, kMaxHeads = (int64_t)1 << 22;  // heads: a launch has fewer than 2^32 threads
     if (batch > kMax || q_heads > kMax || q_len > kMax || kv_len > kMax || batch * q_heads > kMax || batch * kv_heads > kMaxHeads)
         return ZN_ERR_OVERFLOW;
-    constexpr int64_t kMaxRows = (int64_t)65535 * kMhaTile;  // the grid's second extent
-    if (kv_len + (kv_heads ? q_heads / kv_heads * (q_len + kMhaTile) : 0) > kMaxRows) return ZN_ERR_OVERFLOW;
+    const int64_t tile = kMhaRows[kMhaGrad][(head_dim - 1) / 32], max_rows = 65533 * tile;  // tiles: the grid's second extent
+    if (kv_len + (kv_heads ? q_heads / kv_heads * (q_len + tile) : 0) > max_rows) return ZN_ERR_OVERFLOW;
     std::memset(&a, 0, sizeof(a));
     std::memcpy(a.qs, qs, sizeof(a.qs));
     std::memcpy(a.ks, ks, sizeof(a.ks));
@@ -59,39 +59,70 @@ int mha_args(zn_ctx *ctx, ZnMhaArgs &a, int64_t batch, int64_t q_heads, int64_t 
     return ZN_OK;
 }
 
-// Query tiles of a key/value head: the same number for each query head of its group.
-int64_t mha_query_tiles(const ZnMhaArgs &a) { return a.group * cdiv(cdiv((int64_t)a.group * a.q_len, kMhaTile), std::max(a.group, 1)); }
+int64_t mha_rows(MhaKernel kernel, const ZnMhaArgs &a) { return kMhaRows[kernel][(a.dim - 1) / 32]; }
 
-// Parts that tiles' walks of `blocks` blocks are cut into, at most as many as
-// fill the chip once and 64: the time of a part's blocks (forward 0.8 us and 0.012
-// a dim each, backward 1.7 times that) against the join, 4 us and `rows` rows of
-// each part written and read at 2 TB/s.  MI355X, us whole and in parts: 1 x
-// 4096 x 128 forward 232 and (9) 57, its backward 479 and (4) 160; 4 x 256 x 64
-// 23 and (8) 12; but 64 x 256 x 64 (128 tiles of 8 blocks) 24 and (2) 29.
-int mha_splits(const zn_ctx *ctx, const ZnMhaArgs &a, int64_t tiles, int64_t blocks, int64_t rows, bool backward) {
-    const int64_t slots = cus_now(ctx) * (a.dim <= 64 ? 2 : 1);  // workgroups at once
-    const int64_t most = std::min<int64_t>({64, slots / std::max<int64_t>(1, tiles), blocks});
-    const double block_us = (0.8 + 0.012 * a.dim) * (backward ? 1.7 : 1.0);
-    int best = 1;
-    double best_us = block_us * (double)blocks;
-    for (int64_t s = 2; s <= most; ++s) {
-        const double us = block_us * (double)cdiv(blocks, s) + 4.0 + 8.0 * (double)(rows * s) * a.dim / 2e6;
-        if (us < best_us) {
-            best = (int)s;
-            best_us = us;
-        }
-    }
-    return best;
+// Query tiles of a key/value head: the same number for each query head of its group.
+int64_t mha_query_tiles(MhaKernel kernel, const ZnMhaArgs &a) {
+    return a.group * cdiv(cdiv((int64_t)a.group * a.q_len, mha_rows(kernel, a)), std::max(a.group, 1));
 }
 
-int mha_tiles(zn_ctx *ctx, MhaKernel kernel, ZnMhaArgs &a, int64_t y) {
+constexpr double kPartUs = 2.0;  // the way in and out of a walk
+
+// One kind of tile of a call: how many, the blocks that one walks, the times of a
+// block, the rows that a part of its walk writes for zn_mha_join.
+struct MhaWalks {
+    int64_t tiles, blocks;
+    double block_us, alone_us;  // of a CU whose workgroups fill it, of a workgroup alone
+    int64_t rows;
+    int32_t splits;
+};
+
+// `factor`: a block's products against the forward's.  A workgroup of 4 waves has half a CU's, and alone does not fill it.
+MhaWalks mha_walks(MhaKernel kernel, const ZnMhaArgs &a, int64_t tiles, int64_t blocks, double factor, int64_t rows) {
+    const double us = (0.8 + 0.012 * a.dim) * factor * (double)mha_rows(kernel, a) / 128.0;
+    return {tiles, blocks, us, us * (kMhaThreads[kernel][(a.dim - 1) / 32] == 256 ? 1.3 : 1.0), rows, 1};
+}
+
+// The parts that each kind's walks are cut into: the least of the longest part
+// or all parts' time on the chip, whichever is more, and the join, 4 us and each
+// part's rows written and read at 2 TB/s.  A walk is long where queries of many
+// heads pass the same keys, and few tiles leave most of the chip idle; causal
+// tiles average half their walk.  MI355X, us whole (few tiles, both gradients:
+// in equal parts) and so: both gradients of 2 x 16 heads (4) of 2048 x 128,
+// causal, 1013 and 640, 4 x 28 (4) of 500 x 128 438 and 197, one of 4096 x 128
+// 142 and 107; its forward 52 and 46.  But 8 x 16 of 1024 x 128 1252 and 1236.
+void mha_splits(const zn_ctx *ctx, const ZnMhaArgs &a, MhaWalks *w, int kinds) {
+    constexpr int kParts[12] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
+    const double cus = (double)cus_now(ctx), share = a.causal ? 0.5 : 1.0;
+    const int64_t heads = (int64_t)a.batch * a.kv_heads;
+    double best = INFINITY;
+    for (int i = 0; i < (kinds > 1 ? 12 : 1); ++i)
+        for (int j = 0; j < 12; ++j) {
+            const int s[2] = {kParts[j], kParts[i]};
+            double all = 0.0, longest = 0.0, join = 0.0;
+            int64_t y = 0;
+            for (int k = 0; k < kinds; ++k) {
+                const double part = kPartUs + w[k].alone_us * (double)cdiv(w[k].blocks, s[k]);
+                all += (double)(w[k].tiles * s[k]) * kPartUs + (double)w[k].tiles * w[k].block_us * (double)w[k].blocks * share;
+                longest = std::max(longest, w[k].tiles ? part : 0.0);
+                if (s[k] > 1) join = std::max(join, 4.0) + 8.0 * (double)(w[k].rows * s[k]) * a.dim / 2e6;
+                y += w[k].tiles / heads * s[k];
+                if (s[k] > std::max<int64_t>(1, w[k].blocks)) y = INT_MAX;
+            }
+            const double us = std::max(longest, all / cus) + join;
+            if (us < best && (y <= 65535 || (s[0] == 1 && s[1] == 1))) {
+                best = us;
+                for (int k = 0; k < kinds; ++k) w[k].splits = s[k];
+            }
+        }
+}
+
+int mha_tiles(zn_ctx *ctx, MhaKernel kernel, ZnMhaArgs &a, int64_t y, int parts) {
     const int dim = (a.dim - 1) / 32;
-    return launch(ctx, ctx->mha[kernel][dim], (unsigned)(a.batch * a.kv_heads), (unsigned)y, kernel == kMhaFew ? 256 : kMhaThreads[dim], &a,
-                  (unsigned)a.splits);
+    return launch(ctx, ctx->mha[kernel][dim], (unsigned)(a.batch * a.kv_heads), (unsigned)y, kMhaThreads[kernel][dim], &a, (unsigned)parts);
 }
 
 int mha_join(zn_ctx *ctx, const ZnMhaArgs &a, ZnMhaJoinArgs &j, int ops) {
-    j.splits = a.splits;
     j.part_ld = a.part_ld;
     j.dim = a.dim;
     int64_t rows = 0;
@@ -99,13 +130,14 @@ int mha_join(zn_ctx *ctx, const ZnMhaArgs &a, ZnMhaJoinArgs &j, int ops) {
     return launch(ctx, ctx->mha_join, (unsigned)cdiv(rows, 4), (unsigned)ops, 256, &j);
 }
 
-void mha_join_op(ZnMhaJoinOp &op, const float *part, float *dst, const int64_t (&stride)[3], int64_t batch, int32_t heads, int32_t len, float factor) {
+void mha_join_op(ZnMhaJoinOp &op, const float *part, float *dst, const int64_t (&stride)[3], int64_t batch, int32_t heads, int32_t len, int32_t splits, float factor) {
     op.part = part;
     op.dst = dst;
     std::memcpy(op.stride, stride, sizeof(op.stride));
     op.rows = batch * heads * len;
     op.heads = heads;
     op.len = len;
+    op.splits = splits;
     op.factor = factor;
 }
 
@@ -163,10 +195,15 @@ int zn_hip_mha_forward(zn_ctx *ctx, const float *q, const float *k, const float 
     // At most 16 rows of a head read K and V as they are.  Each tile splits what it reads: past a few tiles, once for all of
     // them is cheaper.
     const int64_t rows = (int64_t)a.group * q_len, heads = (int64_t)a.batch * a.kv_heads;
-    const MhaKernel kernel = rows <= kMhaFewRows ? kMhaFew : rows < 3 * kMhaTile ? kMhaForwardRaw : kMhaForward;
-    a.query_tiles = kernel == kMhaFew ? 1 : (int32_t)mha_query_tiles(a);
-    a.splits = kernel == kMhaFew ? (int32_t)std::max<int64_t>(1, std::min<int64_t>({64, 2 * cus_now(ctx) / heads, kv_len / 256}))
-                                 : mha_splits(ctx, a, heads * a.query_tiles, cdiv(kv_len, 32), batch * q_heads * q_len, false);
+    const MhaKernel kernel = rows <= mha_rows(kMhaFew, a) ? kMhaFew : rows < 3 * mha_rows(kMhaForwardRaw, a) ? kMhaForwardRaw : kMhaForward;
+    a.query_tiles = kernel == kMhaFew ? 1 : (int32_t)mha_query_tiles(kernel, a);
+    if (kernel == kMhaFew) {
+        a.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({64, 2 * cus_now(ctx) / heads, kv_len / 256}));
+    } else {
+        MhaWalks w = mha_walks(kernel, a, heads * a.query_tiles, cdiv(kv_len, 32), 1.0, batch * q_heads * q_len);
+        mha_splits(ctx, a, &w, 1);
+        a.splits = w.splits;
+    }
     Lease part(ctx);
     if (a.splits > 1) {
         a.part_ld = (a.dim + 3) / 4 * 4 + 4;
@@ -183,12 +220,12 @@ int zn_hip_mha_forward(zn_ctx *ctx, const float *q, const float *k, const float 
         a.vi = im.s.op[1].dst = im.at(vi);
         if ((rc = im.run(ctx, a))) return rc;
     }
-    if ((rc = mha_tiles(ctx, kernel, a, a.query_tiles)) || a.splits == 1) return rc;
+    if ((rc = mha_tiles(ctx, kernel, a, kernel == kMhaFew ? 1 : (int64_t)a.query_tiles * a.splits, kernel == kMhaFew ? a.splits : 1)) || a.splits == 1) return rc;
     ZnMhaJoinArgs j;
     std::memset(&j, 0, sizeof(j));
     j.forward = 1;
     j.lse = lse;
-    mha_join_op(j.op[0], a.part, out, a.os, a.batch, a.q_heads, a.q_len, 1.0f);
+    mha_join_op(j.op[0], a.part, out, a.os, a.batch, a.q_heads, a.q_len, a.splits, 1.0f);
     return mha_join(ctx, a, j, 1);
 }
 
@@ -233,26 +270,32 @@ int zn_hip_mha_backward(zn_ctx *ctx, const float *q, const float *k, const float
     im.s.op[1].out = out;
     a.side = im.s.op[1].side = reinterpret_cast<float *>(im.at(im.bytes));
     if ((rc = im.run(ctx, a))) return rc;
-    a.key_tiles = (int32_t)cdiv(kv_len, kMhaTile);
-    a.query_tiles = queries ? (int32_t)mha_query_tiles(a) : 0;
-    const int64_t y = a.key_tiles + a.query_tiles;
-    const int64_t q_rows = batch * q_heads * q_len, k_rows = batch * kv_heads * kv_len;
-    a.splits = mha_splits(ctx, a, (int64_t)a.batch * a.kv_heads * y, std::max<int64_t>(a.k_blocks, (int64_t)a.group * a.q_blocks),
-                          q_rows + 2 * k_rows, true);
+    a.key_tiles = (int32_t)cdiv(kv_len, mha_rows(kMhaGrad, a));
+    a.query_tiles = queries ? (int32_t)mha_query_tiles(kMhaGrad, a) : 0;
+    const int64_t q_rows = batch * q_heads * q_len, k_rows = batch * kv_heads * kv_len, heads = (int64_t)a.batch * a.kv_heads;
+    MhaWalks w[2] = {mha_walks(kMhaGrad, a, heads * a.query_tiles, a.k_blocks, 1.35, q_rows),
+                     mha_walks(kMhaGrad, a, heads * a.key_tiles, (int64_t)a.group * a.q_blocks, 1.8, 2 * k_rows)};
+    mha_splits(ctx, a, w, 2);
+    a.splits = w[0].splits;
+    a.kv_splits = w[1].splits;
+    a.part_ld = (a.dim + 3) / 4 * 4;
     Lease part(ctx);
-    if (a.splits > 1) {
-        a.part_ld = (a.dim + 3) / 4 * 4;
-        if ((rc = part.get((size_t)(q_rows + 2 * k_rows) * a.splits * a.part_ld))) return rc;
+    const int64_t q_part = a.splits > 1 ? q_rows * a.splits * a.part_ld : 0, k_part = a.kv_splits > 1 ? k_rows * a.kv_splits * a.part_ld : 0;
+    if (q_part + k_part > 0) {
+        if ((rc = part.get((size_t)(q_part + 2 * k_part)))) return rc;
         a.part = part.ptr;
+        a.kv_part = part.ptr + q_part;
     }
-    if ((rc = mha_tiles(ctx, kMhaGrad, a, y)) || a.splits == 1) return rc;
+    if ((rc = mha_tiles(ctx, kMhaGrad, a, (int64_t)a.key_tiles * a.kv_splits + (int64_t)a.query_tiles * a.splits, 1))) return rc;
     ZnMhaJoinArgs j;
     std::memset(&j, 0, sizeof(j));
-    const int64_t per = (int64_t)a.splits * a.part_ld;
-    mha_join_op(j.op[0], a.part, grad_q, a.qs, a.batch, queries ? a.q_heads : 0, a.q_len, a.scale);
-    mha_join_op(j.op[1], a.part + q_rows * per, grad_k, a.ks, a.batch, a.kv_heads, a.kv_len, 1.0f);
-    mha_join_op(j.op[2], a.part + (q_rows + k_rows) * per, grad_v, a.ks, a.batch, a.kv_heads, a.kv_len, 1.0f);
-    return mha_join(ctx, a, j, 3);
+    int ops = 0;
+    if (q_part > 0) mha_join_op(j.op[ops++], a.part, grad_q, a.qs, a.batch, a.q_heads, a.q_len, a.splits, a.scale);
+    if (k_part > 0) {
+        mha_join_op(j.op[ops++], a.kv_part, grad_k, a.ks, a.batch, a.kv_heads, a.kv_len, a.kv_splits, 1.0f);
+        mha_join_op(j.op[ops++], a.kv_part + k_part, grad_v, a.ks, a.batch, a.kv_heads, a.kv_len, a.kv_splits, 1.0f);
+    }
+    return ops ? mha_join(ctx, a, j, ops) : ZN_OK;
 }
 
 // ----------------------------------------------------------- gated Dense

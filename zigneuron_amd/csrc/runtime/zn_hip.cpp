@@ -101,9 +101,9 @@ constexpr int kAttnSplitQueries[4] = {128, 256, 128, 128};
 // Grouped attention (kernels/mha_f32.h), in the attention code object: zn_mha_<what>_<padded head dim>.
 enum MhaKernel { kMhaFew, kMhaForward, kMhaForwardRaw, kMhaGrad, kMhaSplit, kNumMha };
 constexpr const char *kMhaName[kNumMha] = {"zn_mha_few", "zn_mha_forward", "zn_mha_forward_raw", "zn_mha_grad", "zn_mha_split"};
-constexpr unsigned kMhaThreads[4] = {256, 256, 512, 512};
-constexpr int kMhaTile = 128;  // query rows or keys of a workgroup
-constexpr int kMhaFewRows = 16;  // query rows of zn_mha_few
+// Rows (query rows; the backward's also keys) and threads of a workgroup, by dims in 32s.
+constexpr int kMhaRows[kNumMha][4] = {{16, 16, 16, 16}, {128, 128, 128, 128}, {128, 128, 128, 128}, {128, 128, 64, 128}, {32, 32, 32, 32}};
+constexpr unsigned kMhaThreads[kNumMha][4] = {{256, 256, 256, 256}, {256, 256, 512, 512}, {256, 256, 512, 512}, {256, 256, 256, 512}, {256, 256, 256, 256}};
 
 struct ScratchDevice;
 

@@ -265,13 +265,14 @@ struct ZnMhaArgs {
     const char *qi, *gi, *ki, *vi;
     const float *side;
     int32_t q_blocks, k_blocks;
-    // splits > 1: blockIdx.z takes a part of each tile's walk and writes its
-    // sums to row (row * splits + z) of part (row length part_ld: the dims, 4
-    // more for a forward's maximum and sum), which zn_mha_join adds up.  part
-    // holds the query rows, then the keys' dK rows, then their dV rows.
-    float *part;
-    int32_t splits, part_ld;
-    int32_t key_tiles, query_tiles;  // zn_mha_grad_*: blockIdx.y < key_tiles are tiles of keys, the others of queries
+    // splits > 1: a workgroup takes one part z of its query tile's walk and
+    // writes its sums to row (row * splits + z) of part (row length part_ld: the
+    // dims, 4 more for a forward's maximum and sum), which zn_mha_join adds up.
+    // The same for kv_splits, tiles of keys and kv_part, which holds the keys' dK
+    // rows, then their dV rows.
+    float *part, *kv_part;
+    int32_t splits, kv_splits, part_ld;
+    int32_t key_tiles, query_tiles;
 };
 
 // zn_mha_join: rows of `splits` partial sums each, [batch, heads, len] in
@@ -281,13 +282,13 @@ struct ZnMhaJoinOp {
     float *dst;
     int64_t stride[3];
     int64_t rows;
-    int32_t heads, len;
+    int32_t heads, len, splits;
     float factor;                 // gradients: what the sum is multiplied by
 };
 struct ZnMhaJoinArgs {
     ZnMhaJoinOp op[3];            // blockIdx.y
     float *lse;                   // forward: written where not null
-    int32_t forward, splits, part_ld, dim;
+    int32_t forward, part_ld, dim;
 };
 
 // One tensor to its image: workgroups [first, first + batch * heads * blocks).
