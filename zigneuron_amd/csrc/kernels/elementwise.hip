@@ -566,43 +566,64 @@ extern "C" __global__ __launch_bounds__(256) void zn_gate_forward(ZnGateArgs p) 
 
 // grad_z = [grad_h * up * act'(gate) | grad_h * act(gate)] and, where asked
 // for, its column sums per split of rows (grad_z may be z).  blockIdx.x: 256
-// units (_v: whole float4s, 4 units to a thread and 4 rows at once; one and one
-// otherwise), blockIdx.y: a split of rows, in ascending order.  Bound by its
-// traffic: MI355X, 4096 x 4096 units, 335 MB in 62 us, 5.4 TB/s.
-template <int W>
-__device__ __forceinline__ void gate_backward(const ZnGateArgs &p) {
-    typedef float vec __attribute__((ext_vector_type(W)));
-    constexpr int kRows = W;  // rows at once: 256 / W threads span the 256 units
-    const int lane = threadIdx.x % (256 / W), sub = threadIdx.x / (256 / W);
-    const int64_t c = (int64_t)blockIdx.x * 256 + lane * W;
+// units, 4 neighbouring ones to a thread (4-byte aligned loads and stores of 16
+// bytes: rows need not be whole float4s; at a row's end one at a time) and 4 rows
+// at once; blockIdx.y: a split of rows, in ascending order.  Bound by its traffic:
+// MI355X, 4096 x 4096 units, 335 MB in 62 us, 5.4 TB/s; 777 x 1001 units 11.8 us
+// with a unit to a thread and 16 rows a split, 7.9 so (8 rows).
+extern "C" __global__ __launch_bounds__(256) void zn_gate_backward(ZnGateArgs p) {
+    typedef float vec4u __attribute__((ext_vector_type(4), aligned(4)));
+    const int lane = threadIdx.x % 64, sub = threadIdx.x / 64;
+    const int64_t c = (int64_t)blockIdx.x * 256 + lane * 4;
     const int64_t r0 = (int64_t)blockIdx.y * p.rows_per_split, r1 = min(p.rows, r0 + p.rows_per_split);
-    float sg[W], su[W];
+    const int units = (int)max((int64_t)0, min((int64_t)4, p.n - c));
+    float sg[4] = {0.0f, 0.0f, 0.0f, 0.0f}, su[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int64_t r = r0 + sub; r < r1 && units > 0; r += 4) {
+        const int64_t at = r * 2 * p.n + c;
+        const float *zg = p.z + at, *zu = zg + p.n, *gh = p.grad_h + r * p.n + c;
+        float *dg = p.grad_z + at, *du = dg + p.n;
+        zn_f32x4 g, u, h;
+        if (units == 4) {
+            g = *reinterpret_cast<const vec4u *>(zg);
+            u = *reinterpret_cast<const vec4u *>(zu);
+            h = *reinterpret_cast<const vec4u *>(gh);
+        } else {
 #pragma unroll
-    for (int e = 0; e < W; ++e) sg[e] = su[e] = 0.0f;
-    if (c < p.n)
-        for (int64_t r = r0 + sub; r < r1; r += kRows) {
-            const int64_t at = r * 2 * p.n + c;
-            const vec g = *reinterpret_cast<const vec *>(p.z + at), u = *reinterpret_cast<const vec *>(p.z + at + p.n);
-            const vec h = *reinterpret_cast<const vec *>(p.grad_h + r * p.n + c);
-            vec dg, du;
-#pragma unroll
-            for (int e = 0; e < W; ++e) {
-                float y, d;
-                zn_gate_slope(g[e], p.act, y, d);
-                dg[e] = h[e] * u[e] * d;
-                du[e] = h[e] * y;
-                sg[e] += dg[e];
-                su[e] += du[e];
+            for (int e = 0; e < 4; ++e) {
+                const int i = min(e, units - 1);
+                g[e] = zg[i];
+                u[e] = zu[i];
+                h[e] = gh[i];
             }
-            *reinterpret_cast<vec *>(p.grad_z + at) = dg;
-            *reinterpret_cast<vec *>(p.grad_z + at + p.n) = du;
         }
-    if (!p.partial) return;
-    __shared__ float part[2][kRows][256];
+        zn_f32x4 x, y;
 #pragma unroll
-    for (int e = 0; e < W; ++e) {
-        part[0][sub][lane * W + e] = sg[e];
-        part[1][sub][lane * W + e] = su[e];
+        for (int e = 0; e < 4; ++e) {
+            float act, slope;
+            zn_gate_slope(g[e], p.act, act, slope);
+            x[e] = h[e] * u[e] * slope;
+            y[e] = h[e] * act;
+            sg[e] += x[e];
+            su[e] += y[e];
+        }
+        if (units == 4) {
+            *reinterpret_cast<vec4u *>(dg) = x;
+            *reinterpret_cast<vec4u *>(du) = y;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (e < units) {
+                    dg[e] = x[e];
+                    du[e] = y[e];
+                }
+        }
+    }
+    if (!p.partial) return;
+    __shared__ float part[2][4][256];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        part[0][sub][lane * 4 + e] = sg[e];
+        part[1][sub][lane * 4 + e] = su[e];
     }
     __syncthreads();
     const int64_t col = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -612,12 +633,10 @@ __device__ __forceinline__ void gate_backward(const ZnGateArgs &p) {
     for (int q = 0; q < 2; ++q) {
         float t = 0.0f;
 #pragma unroll
-        for (int s = 0; s < kRows; ++s) t += part[q][s][threadIdx.x];
+        for (int s = 0; s < 4; ++s) t += part[q][s][threadIdx.x];
         dst[q * p.n] = t;
     }
 }
-extern "C" __global__ __launch_bounds__(256) void zn_gate_backward(ZnGateArgs p) { gate_backward<1>(p); }
-extern "C" __global__ __launch_bounds__(256) void zn_gate_backward_v(ZnGateArgs p) { gate_backward<4>(p); }
 
 // --------------------------------------------- distillation from top logits
 // Per token: p = softmax(top / T) over the teacher's present entries, lse =

@@ -416,10 +416,9 @@ int zn_hip_gated_dense_backward(zn_ctx *ctx, int act, const float *x, const floa
     g.rows = batch;
     g.n = hidden;
     g.act = act;
-    // row splits for about 8 workgroups a CU, at least 16 rows each
-    const bool vec = hidden % 4 == 0 && aligned16(z) && aligned16(grad_h) && aligned16(grad_z);
+    // row splits for about 8 workgroups a CU, at least 8 rows each
     const int64_t cus = cus_now(ctx), groups = cdiv(hidden, 256);
-    int64_t splits = std::max<int64_t>(1, std::min<int64_t>({cdiv(batch, 16), 8 * cus / groups, 65535}));
+    int64_t splits = std::max<int64_t>(1, std::min<int64_t>({cdiv(batch, 8), 8 * cus / groups, 65535}));
     const int64_t per = cdiv(batch, splits);
     splits = cdiv(batch, per);
     g.rows_per_split = (int32_t)per;
@@ -440,7 +439,7 @@ int zn_hip_gated_dense_backward(zn_ctx *ctx, int act, const float *x, const floa
         r.act = ZN_ACT_LINEAR;
         r.vec = n % 4 == 0 && aligned16(grad_bias) && aligned16(part.ptr) ? 1 : 0;
     }
-    if ((rc = launch(ctx, ctx->elt[vec ? kGateBackwardV : kGateBackward], (unsigned)groups, (unsigned)splits, 256, &g))) return rc;
+    if ((rc = launch(ctx, ctx->elt[kGateBackward], (unsigned)groups, (unsigned)splits, 256, &g))) return rc;
     if (in_size == 0) return grad_bias ? launch_reduce(ctx, r) : ZN_OK;
     int64_t wg_nt = 0, wg_tn = 0;
     if (const int tile = grouped_tile(ctx, batch, in_size, n, grad_x != nullptr, &wg_nt, &wg_tn)) {

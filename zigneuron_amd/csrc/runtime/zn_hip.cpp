@@ -75,14 +75,14 @@ constexpr TileShape kTiles[kNumTiles] = {{256, 128, 16, 512, "x", true, true, tr
 constexpr const char *kLayoutName[3] = {"nn", "nt", "tn"};
 
 enum EltKernel { kFill, kCopy, kAddBias, kActFwd, kActBwd, kAccBias, kIm2col, kSoftmax, kCol2im, kRowSum, kDenseGrad, kRegroup, kPack, kToNhwc, kHold, kCol2imPx, kReduceSlices,
-                 kGateForward, kGateBackward, kGateBackwardV, kDistillForward, kDistillJoin, kDistillBackward, kNumElt };
+                 kGateForward, kGateBackward, kDistillForward, kDistillJoin, kDistillBackward, kNumElt };
 constexpr const char *kEltName[kNumElt] = {"zn_fill_f32",        "zn_copy_f32", "zn_add_bias",
                                            "zn_activation_forward", "zn_activation_backward",
                                            "zn_accumulate_bias", "zn_im2col",   "zn_softmax_rows",
                                            "zn_col2im",          "zn_row_sum",  "zn_dense_grad_prologue",
                                            "zn_weight_regroup", "zn_pack_rows", "zn_nchw_to_nhwc",
                                            "zn_hold_stream",     "zn_col2im_px", "zn_reduce_slices",
-                                           "zn_gate_forward",    "zn_gate_backward", "zn_gate_backward_v",
+                                           "zn_gate_forward",    "zn_gate_backward",
                                            "zn_distill_forward", "zn_distill_join", "zn_distill_backward"};
 
 constexpr const char *kGemmObject = "zn_gemm_gfx950.hsaco";
