@@ -198,7 +198,11 @@ int zn_hip_mha_forward(zn_ctx *ctx, const float *q, const float *k, const float 
     const MhaKernel kernel = rows <= mha_rows(kMhaFew, a) ? kMhaFew : rows < 3 * mha_rows(kMhaForwardRaw, a) ? kMhaForwardRaw : kMhaForward;
     a.query_tiles = kernel == kMhaFew ? 1 : (int32_t)mha_query_tiles(kernel, a);
     if (kernel == kMhaFew) {
-        a.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({64, 2 * cus_now(ctx) / heads, kv_len / 256}));
+        // parts of about 96 KB of K and V each, at most two workgroups a CU; past 8 a multiple of them, which the join reads at once
+        // (MI355X, us in parts of 256 keys and so: 4 x 8 of 700 x 64 14.2 and 11.6, 4 x 8 of 1100 x 128 28.2 and 21.7, 4 of
+        // 600 x 120 21.1 and 14.1; 8 x 4 of 2048 x 64 in 8 parts 13.7, in 11 15.7, in 16 14.8)
+        a.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({64, 2 * cus_now(ctx) / heads, (kv_len * a.dim + 4915) / 12288}));
+        if (a.splits > 8) a.splits -= a.splits % 8;
     } else {
         MhaWalks w = mha_walks(kernel, a, heads * a.query_tiles, cdiv(kv_len, 32), 1.0, batch * q_heads * q_len);
         mha_splits(ctx, a, &w, 1);
