@@ -980,13 +980,19 @@ struct MhaKeyTile {
 // for 16 keys of 64 dims: 18 TB/s of K and V), so nothing is split and nothing passes
 // through LDS: each of the NW waves of each workgroup and split walks its own
 // keys, 16 at a time, loaded one step ahead straight into the fragments (K:
-// lane li a key, 4 dims of each 16 per quarter; V: lane li DB neighbouring
+// lane li a key, 4 dims of each 16 per quarter; V: lane li G neighbouring
 // dims of one key per quarter).  The waves' sums are joined in LDS.  MI355X, 8
 // tokens of 16 heads (4) against 2048 x 64: 9.6 us for 33.5 MB (3.5 TB/s; a
 // wave has four steps), and 4 us for the join of the splits.
 template <int DP, int NW>
 struct MhaFew {
-    static constexpr int G = DP / 16;  // groups of 16 dims; also the 16-dim blocks of O^T, block c the dims G li + c
+    static constexpr int G = DP / 16;  // groups of 16 dims; also the 16-dim blocks of O^T
+    // Past 64 dims the loads above take half of each 128-byte line, and the next one waits for the line that is on its way.
+    // There a load takes whole lines: K's 32 dims of 8 keys, whose halves change lanes before their use; V's 64 dims of 4 keys.
+    // MI355X, 16 x 8 heads of 4096 x 128: 138 and 113 us (4.75 TB/s); at 64 dims whole lines of K cost 0.5 us.
+    static constexpr bool WHOLE = DP > 64;
+    // The dim of O^T's row i of block c.
+    __device__ static constexpr int dim_of(int c, int i) { return !WHOLE ? G * i + c : c < G / 4 * 4 ? 64 * (c / 4) + 4 * i + c % 4 : 16 * c + i; }
     static constexpr int kLd = DP + 4;
     static constexpr int kBytes = NW * 16 * kLd * 4;
     struct Keys {
@@ -1032,20 +1038,22 @@ struct MhaFew {
             const __amdgpu_buffer_rsrc_t rk = make_rsrc(p.k + at + (int64_t)k0 * p.ks[2], bytes);
             const __amdgpu_buffer_rsrc_t rv = make_rsrc(p.v + at + (int64_t)k0 * p.ks[2], bytes);
 #pragma unroll
-            for (int g = 0; g < G; ++g) load4(rk, (uint32_t)(li * stride) * 4u, 16 * g + 4 * lh, p.dim, x.k[g]);
+            for (int g = 0; g < G; ++g)
+                if (WHOLE) load4(rk, (uint32_t)((li % 8 + g % 2 * 8) * stride) * 4u, 32 * (g / 2) + 16 * (li / 8) + 4 * lh, p.dim, x.k[g]);
+                else load4(rk, (uint32_t)(li * stride) * 4u, 16 * g + 4 * lh, p.dim, x.k[g]);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const uint32_t off = (uint32_t)((4 * lh + e) * stride) * 4u;
 #pragma unroll
                 for (int c = 0; c + 4 <= G; c += 4) {
                     float y[4];
-                    load4(rv, off, G * li + c, p.dim, y);
+                    load4(rv, off, dim_of(c, li), p.dim, y);
 #pragma unroll
                     for (int z = 0; z < 4; ++z) x.v[e][c + z] = y[z];
                 }
 #pragma unroll
                 for (int c = G / 4 * 4; c < G; ++c) {
-                    const int d = G * li + c;
+                    const int d = dim_of(c, li);
                     x.v[e][c] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rv, d < p.dim ? off + (uint32_t)d * 4u : kOutOfRange, 0, 0));
                 }
             }
@@ -1055,7 +1063,15 @@ struct MhaFew {
         for (int c = 0; c < G; ++c) o[c] = zn_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         float m = -INFINITY, l = 0.0f;
         Keys x[2];
-        auto step = [&](int s, const Keys &y) {
+        auto step = [&](int s, Keys &y) {
+#pragma unroll
+            for (int g = 0; g < (WHOLE ? G : 0); g += 2)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int a = __builtin_bit_cast(int, y.k[g][e]), b = __builtin_bit_cast(int, y.k[g + 1][e]);
+                    y.k[g][e] = __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(a, b, 0x128, 0xf, 0xc, false));  // row_ror:8
+                    y.k[g + 1][e] = __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(b, a, 0x128, 0xf, 0x3, false));
+                }
             zn_f32x4 t[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
             for (int g = 0; g < G; ++g)
@@ -1118,7 +1134,7 @@ struct MhaFew {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
 #pragma unroll
-                for (int c = 0; c < G; ++c) mine[li * kLd + G * (4 * lh + e) + c] = o[c][e];
+                for (int c = 0; c < G; ++c) mine[li * kLd + dim_of(c, 4 * lh + e)] = o[c][e];
             if (lh == 0) {
                 mine[li * kLd + DP] = m;
                 mine[li * kLd + DP + 1] = l;
