@@ -202,6 +202,24 @@ def test_masked_values_reach_nothing(ctx, dim, s, bad):
     assert np.isnan(gq[:, :, bad:]).all() and np.isnan(gk).all() and np.isnan(gv).all()
 
 
+@pytest.mark.parametrize("shape, causal, layout", [((16, 16, 16, 500, 200, 100), True, "bhsd"), ((16, 32, 16, 400, 160, 70), False, "bshd")])
+def test_many_heads_past_64_dims(ctx, shape, causal, layout):
+    """Enough heads for the widest tiles; lengths from nothing to all, padding that holds anything."""
+    b, hq, hk, sq, sk, d = shape
+    q, k, v, _ = make(48, *shape)
+    q_lens, kv_lens = [sq - 31 * n for n in range(b)], [(17 * n) % (sk + 1) if n else sk for n in range(b)]
+    for n in range(b):
+        q[n, :, q_lens[n]:], k[n, :, kv_lens[n]:], v[n, :, kv_lens[n]:] = np.nan, np.inf, np.nan
+    announce(f"mha {shape} causal {causal} {layout}")
+    ref = Mha(q, k, v, d ** -0.5, causal, q_lens, kv_lens)
+    if causal:  # an infinity that the last query of one head alone sees, beside others of its tile that do not
+        v[0, 3, sk - 1] = np.inf
+        ref.out[0, 3, sq - 1] = np.inf
+    out, lse = run_forward(ctx, q, k, v, d ** -0.5, causal, q_lens, kv_lens, layout)
+    check(out, ref.out, ref.out_bound, "out")
+    check(lse, ref.lse, ref.lse_bound, "lse")
+
+
 @pytest.mark.parametrize("causal", [False, True])
 def test_new_tokens_of_sequences_of_all_lengths(ctx, causal):
     """One or two new tokens a sequence, caches from nothing to long, padding that holds anything."""

@@ -1299,5 +1299,14 @@ ZN_MHA_KERNELS(32, 4, 2, 4, 2)
 ZN_MHA_KERNELS(64, 4, 2, 4, 2)
 ZN_MHA_KERNELS(96, 8, 1, 4, 1)
 ZN_MHA_KERNELS(128, 8, 1, 8, 1)
+// Two blocks of rows to a wave past 64 dims too: each fragment read from LDS serves twice the products, and half as many tiles
+// are left.  MI355X, forward of 8 x 16 heads of 1024 x 128 411 us, 371 so; 2 x 16 (4) of 4096 x 96, causal, 535, 486;
+// but 2 x 16 (4) of 2048 x 128, causal, 171, 232.
+#define ZN_MHA_WIDE(DP)                                                                                             \
+    typedef MhaQueryTile<DP, 8, 2, false, true> MhaWide##DP;                                                       \
+    ZN_MHA_KERNEL(zn_mha_forward_wide_##DP, 8, MhaWide##DP::kBytes,                                                \
+                  MhaWide##DP::run(p, blockIdx.y / p.splits, blockIdx.y % p.splits, lds))
+ZN_MHA_WIDE(96)
+ZN_MHA_WIDE(128)
 
 #endif

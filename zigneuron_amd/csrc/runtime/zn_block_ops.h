@@ -91,7 +91,8 @@ MhaWalks mha_walks(MhaKernel kernel, const ZnMhaArgs &a, int64_t tiles, int64_t 
 // in equal parts) and so: both gradients of 2 x 16 heads (4) of 2048 x 128,
 // causal, 1013 and 640, 4 x 28 (4) of 500 x 128 438 and 197, one of 4096 x 128
 // 142 and 107; its forward 52 and 46.  But 8 x 16 of 1024 x 128 1252 and 1236.
-void mha_splits(const zn_ctx *ctx, const ZnMhaArgs &a, MhaWalks *w, int kinds) {
+// Returns the time so found.
+double mha_splits(const zn_ctx *ctx, const ZnMhaArgs &a, MhaWalks *w, int kinds) {
     constexpr int kParts[12] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
     const double cus = (double)cus_now(ctx), share = a.causal ? 0.5 : 1.0;
     const int64_t heads = (int64_t)a.batch * a.kv_heads;
@@ -115,6 +116,7 @@ void mha_splits(const zn_ctx *ctx, const ZnMhaArgs &a, MhaWalks *w, int kinds) {
                 for (int k = 0; k < kinds; ++k) w[k].splits = s[k];
             }
         }
+    return best;
 }
 
 int mha_tiles(zn_ctx *ctx, MhaKernel kernel, ZnMhaArgs &a, int64_t y, int parts) {
@@ -195,17 +197,26 @@ int zn_hip_mha_forward(zn_ctx *ctx, const float *q, const float *k, const float 
     // At most 16 rows of a head read K and V as they are.  Each tile splits what it reads: past a few tiles, once for all of
     // them is cheaper.
     const int64_t rows = (int64_t)a.group * q_len, heads = (int64_t)a.batch * a.kv_heads;
-    const MhaKernel kernel = rows <= mha_rows(kMhaFew, a) ? kMhaFew : rows < 3 * mha_rows(kMhaForwardRaw, a) ? kMhaForwardRaw : kMhaForward;
-    a.query_tiles = kernel == kMhaFew ? 1 : (int32_t)mha_query_tiles(kernel, a);
+    MhaKernel kernel = rows <= mha_rows(kMhaFew, a) ? kMhaFew : rows < 3 * mha_rows(kMhaForwardRaw, a) ? kMhaForwardRaw : kMhaForward;
     if (kernel == kMhaFew) {
+        a.query_tiles = 1;
         // parts of about 96 KB of K and V each, at most two workgroups a CU; past 8 a multiple of them, which the join reads at once
         // (MI355X, us in parts of 256 keys and so: 4 x 8 of 700 x 64 14.2 and 11.6, 4 x 8 of 1100 x 128 28.2 and 21.7, 4 of
         // 600 x 120 21.1 and 14.1; 8 x 4 of 2048 x 64 in 8 parts 13.7, in 11 15.7, in 16 14.8)
         a.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({64, 2 * cus_now(ctx) / heads, (kv_len * a.dim + 4915) / 12288}));
         if (a.splits > 8) a.splits -= a.splits % 8;
     } else {
-        MhaWalks w = mha_walks(kernel, a, heads * a.query_tiles, cdiv(kv_len, 32), 1.0, batch * q_heads * q_len);
-        mha_splits(ctx, a, &w, 1);
+        const int64_t q_rows = batch * q_heads * q_len, blocks = cdiv(kv_len, 32);
+        MhaWalks w = mha_walks(kernel, a, heads * mha_query_tiles(kernel, a), blocks, 1.0, q_rows);
+        const double us = mha_splits(ctx, a, &w, 1);
+        if (kernel == kMhaForward && mha_rows(kMhaForwardWide, a)) {
+            MhaWalks wide = mha_walks(kMhaForwardWide, a, heads * mha_query_tiles(kMhaForwardWide, a), blocks, 0.9, q_rows);
+            if (mha_splits(ctx, a, &wide, 1) < 0.97 * us) {
+                kernel = kMhaForwardWide;
+                w = wide;
+            }
+        }
+        a.query_tiles = (int32_t)(w.tiles / heads);
         a.splits = w.splits;
     }
     Lease part(ctx);
@@ -215,7 +226,7 @@ int zn_hip_mha_forward(zn_ctx *ctx, const float *q, const float *k, const float 
         a.part = part.ptr;
     }
     MhaImages im(ctx);
-    if (kernel == kMhaForward && kv_len > 0) {
+    if (kernel != kMhaFew && kernel != kMhaForwardRaw && kv_len > 0) {
         const int64_t ki = im.add(a, k, a.ks, a.kv_lens, a.kv_heads, a.kv_len, 1.0f), vi = im.add(a, v, a.ks, a.kv_lens, a.kv_heads, a.kv_len, 1.0f);
         if (im.groups > kMhaMaxBlocks) return ZN_ERR_OVERFLOW;
         if ((rc = im.get(0))) return rc;

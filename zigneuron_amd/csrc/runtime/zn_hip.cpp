@@ -99,11 +99,11 @@ constexpr unsigned kAttnSplitThreads[4] = {256, 512, 512, 512};
 constexpr int kAttnSplitQueries[4] = {128, 256, 128, 128};
 
 // Grouped attention (kernels/mha_f32.h), in the attention code object: zn_mha_<what>_<padded head dim>.
-enum MhaKernel { kMhaFew, kMhaForward, kMhaForwardRaw, kMhaGrad, kMhaSplit, kNumMha };
-constexpr const char *kMhaName[kNumMha] = {"zn_mha_few", "zn_mha_forward", "zn_mha_forward_raw", "zn_mha_grad", "zn_mha_split"};
-// Rows (query rows; the backward's also keys) and threads of a workgroup, by dims in 32s.
-constexpr int kMhaRows[kNumMha][4] = {{16, 16, 16, 16}, {128, 128, 128, 128}, {128, 128, 128, 128}, {128, 128, 64, 128}, {32, 32, 32, 32}};
-constexpr unsigned kMhaThreads[kNumMha][4] = {{256, 256, 256, 256}, {256, 256, 512, 512}, {256, 256, 512, 512}, {256, 256, 256, 512}, {256, 256, 256, 256}};
+enum MhaKernel { kMhaFew, kMhaForward, kMhaForwardWide, kMhaForwardRaw, kMhaGrad, kMhaSplit, kNumMha };
+constexpr const char *kMhaName[kNumMha] = {"zn_mha_few", "zn_mha_forward", "zn_mha_forward_wide", "zn_mha_forward_raw", "zn_mha_grad", "zn_mha_split"};
+// Rows (query rows; the backward's also keys) and threads of a workgroup, by dims in 32s; 0: no such kernel.
+constexpr int kMhaRows[kNumMha][4] = {{16, 16, 16, 16}, {128, 128, 128, 128}, {0, 0, 256, 256}, {128, 128, 128, 128}, {128, 128, 64, 128}, {32, 32, 32, 32}};
+constexpr unsigned kMhaThreads[kNumMha][4] = {{256, 256, 256, 256}, {256, 256, 512, 512}, {0, 0, 512, 512}, {256, 256, 512, 512}, {256, 256, 256, 512}, {256, 256, 256, 256}};
 
 struct ScratchDevice;
 
@@ -2014,6 +2014,7 @@ int zn_hip_create(int device, const char *code_object_dir, zn_ctx **out) {
         return bail(ZN_ERR_SYMBOL);
     for (int i = 0; i < kNumMha; ++i)
         for (int d = 0; d < 4; ++d) {
+            if (!kMhaRows[i][d]) continue;
             char name[64];
             std::snprintf(name, sizeof(name), "%s_%d", kMhaName[i], 32 * (d + 1));
             if (hipModuleGetFunction(&ctx->mha[i][d], ctx->attn_module, name) != hipSuccess) return bail(ZN_ERR_SYMBOL);
