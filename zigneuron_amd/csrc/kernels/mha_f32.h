@@ -1231,25 +1231,33 @@ extern "C" __global__ __launch_bounds__(256) void zn_mha_join(ZnMhaJoinArgs a) {
     const int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
     if (row >= p.rows) return;
     const float *src = p.part + row * p.splits * a.part_ld;
-    float mx = -INFINITY;
-    if (a.forward) {
-        for (int z = lane; z < p.splits; z += kWave) mx = fmaxf(mx, src[(int64_t)z * a.part_ld + a.part_ld - 4]);
-#pragma unroll
-        for (int s = 32; s > 0; s >>= 1) mx = fmaxf(mx, __shfl_xor(mx, s));
-    }
-    const float ref = mx == -INFINITY ? 0.0f : mx;
-    float sl = 0.0f, oa = 0.0f, ob = 0.0f;
+    float mx = -INFINITY, sl = 0.0f, oa = 0.0f, ob = 0.0f;
     for (int z0 = 0; z0 < p.splits; z0 += 8) {
         float x[8], y[8], m[8], l[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
-            const bool in = z0 + u < p.splits;
-            const float *t = src + (int64_t)(in ? z0 + u : 0) * a.part_ld;
-            x[u] = in && lane < a.dim ? t[lane] : 0.0f;
-            y[u] = in && lane + 64 < a.dim ? t[lane + 64] : 0.0f;
-            m[u] = in && a.forward ? t[a.part_ld - 4] : -INFINITY;
-            l[u] = in && a.forward ? t[a.part_ld - 3] : 0.0f;
+            const float *t = src + (int64_t)min(z0 + u, p.splits - 1) * a.part_ld;  // any row of parts: no load waits for a condition
+            x[u] = t[min(lane, a.dim - 1)];
+            y[u] = t[min(lane + 64, a.dim - 1)];
+            m[u] = t[a.part_ld - 4];
+            l[u] = t[a.part_ld - 3];
         }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const bool in = z0 + u < p.splits;
+            x[u] = in ? x[u] : 0.0f;
+            y[u] = in ? y[u] : 0.0f;
+            m[u] = in && a.forward ? m[u] : -INFINITY;
+            l[u] = in ? l[u] : 0.0f;
+        }
+        float mn = mx;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) mn = fmaxf(mn, m[u]);
+        const float ref = mn == -INFINITY ? 0.0f : mn, alpha = a.forward ? __builtin_amdgcn_exp2f(mx - ref) : 1.0f;
+        mx = mn;
+        sl *= alpha;
+        oa *= alpha;
+        ob *= alpha;
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
             const float f = a.forward ? __builtin_amdgcn_exp2f(m[u] - ref) : 1.0f;
@@ -1258,8 +1266,8 @@ extern "C" __global__ __launch_bounds__(256) void zn_mha_join(ZnMhaJoinArgs a) {
             ob += f * y[u];
         }
     }
-    const int64_t bh = row / p.len;
-    float *dst = p.dst + bh / p.heads * p.stride[0] + bh % p.heads * p.stride[1] + row % p.len * p.stride[2];
+    const int bh = (int)row / p.len, b = bh / p.heads;  // a launch has fewer than 2^31 rows
+    float *dst = p.dst + b * p.stride[0] + (bh - b * p.heads) * p.stride[1] + ((int)row - bh * p.len) * p.stride[2];
     if (a.forward) {
         const float r = sl == 0.0f ? 1.0f : sl;
         MhaRow::store(dst, a.dim, lane, oa / r, ob / r);
