@@ -983,7 +983,8 @@ struct MhaKeyTile {
 // lane li a key, 4 dims of each 16 per quarter; V: lane li G neighbouring
 // dims of one key per quarter).  The waves' sums are joined in LDS.  MI355X, 8
 // tokens of 16 heads (4) against 2048 x 64: 9.6 us for 33.5 MB (3.5 TB/s; a
-// wave has four steps), and 4 us for the join of the splits.
+// wave has four steps), 12.5 us with the join of the parts.  Four steps in flight
+// cost occupancy (12.9 us; 32 x 32 heads of 2048 x 64 207 and 219).
 template <int DP, int NW>
 struct MhaFew {
     static constexpr int G = DP / 16;  // groups of 16 dims; also the 16-dim blocks of O^T
