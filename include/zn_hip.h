@@ -434,6 +434,8 @@ int zn_hip_attention_forward(zn_ctx *ctx, const float *q, const float *k, const 
  *    too).  A query that sees no key has out = 0 and lse = -inf.  Rows of
  *    padding (past a sequence's length) are written the same way: out 0, lse
  *    -inf, gradients 0.
+ *  - Scores are fp32 sums.  One below fp32's range is -inf and has probability
+ *    0; a query that sees only such keys counts as one that sees none.
  *  - lse: contiguous [batch, q_heads, q_len], natural logarithm; the backward
  *    reads it.  The forward takes null where no backward follows. */
 int zn_hip_mha_forward(zn_ctx *ctx, const float *q, const float *k, const float *v, float *out, float *lse,
@@ -448,7 +450,10 @@ int zn_hip_mha_forward(zn_ctx *ctx, const float *q, const float *k, const float 
  *   dS = P o (grad_out.v^T - rowsum(grad_out o out)),
  *   grad_q = scale dS.k, grad_k = scale dS^T.q,
  * the last two and grad_v summed over the query heads that share a head.  All
- * three gradients are overwritten. */
+ * three gradients are overwritten.  lse's rounding is a relative error of its
+ * row's P, 2^-24 |lse| or so; for a row whose |lse| is past 45000 (2^16 ln 2) lse
+ * is computed again from q and k, and all that the row reaches one key at a
+ * time, tens of times slower. */
 int zn_hip_mha_backward(zn_ctx *ctx, const float *q, const float *k, const float *v, const float *out,
                         const float *lse, const float *grad_out, float *grad_q, float *grad_k, float *grad_v,
                         int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t q_len, int64_t kv_len,

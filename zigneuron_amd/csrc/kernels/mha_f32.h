@@ -127,9 +127,19 @@ __device__ __forceinline__ void mha_row_forward(const ZnMhaArgs &p, int b, int h
     mha_row_finish(p, b, h, i, z, lane, s.m, s.l, s.oa, s.ob);
 }
 
-// Where a query's lse (log2 domain) and delta lie.
+// What the backward keeps of each query beside Q and dO, 32 values each a block:
+//   [0]   lse in the log2 domain, +inf where the query sees nothing, NaN where it is far
+//   [32]  delta
+//   [64], [96]  a and r of P = exp2(S - a) r: lse and 1 or, of a far query, its maximum and 1 / its sum
+// An lse's last bit is a relative error of the whole row's probabilities: from
+// 2^16 (log2 domain) on, half of it is past 2^-9, and from 2^24 on nothing is left
+// of them.  Such a query is far: the split kernel goes over its scores again, one
+// key at a time, and its NaN makes the tiles' sums NaN, so that all that it
+// reaches is computed row by row, with scores of the very same bits as its maximum.
+constexpr int kMhaSide = 128;  // values a block
+constexpr float kMhaFar = 65536.0f;
 __device__ __forceinline__ const float *mha_side(const ZnMhaArgs &p, int b, int h, int i) {
-    return p.side + (((int64_t)b * p.q_heads + h) * p.q_blocks + i / 32) * 64 + i % 32;
+    return p.side + (((int64_t)b * p.q_heads + h) * p.q_blocks + i / 32) * kMhaSide + i % 32;
 }
 
 // grad_q of a row over keys [from, to).
@@ -137,8 +147,9 @@ __device__ __forceinline__ void mha_row_grad_q(const ZnMhaArgs &p, int b, int h,
     const MhaSeq seq(p, b);
     int n = min(to, seq.seen(i));
     const float *side = mha_side(p, b, h, i);
-    const float lse2 = from < n ? side[0] : INFINITY, delta = from < n ? side[32] : 0.0f;
-    if (lse2 == INFINITY) n = from;
+    if (from < n && side[0] == INFINITY) n = from;
+    const bool some = from < n;
+    const float delta = some ? side[32] : 0.0f, a = some ? side[64] : 0.0f, r = some ? side[96] : 0.0f;
     const float *k = p.k + b * p.ks[0] + (h / p.group) * p.ks[1], *v = p.v + b * p.ks[0] + (h / p.group) * p.ks[1];
     const int64_t qat = b * p.qs[0] + h * p.qs[1] + i * p.qs[2];
     MhaRow q(p.q + qat, from < n ? p.dim : 0, lane);
@@ -148,7 +159,7 @@ __device__ __forceinline__ void mha_row_grad_q(const ZnMhaArgs &p, int b, int h,
     float ga = 0.0f, gb = 0.0f;
     for (int j = from; j < n; ++j) {
         const MhaRow kr(k + j * p.ks[2], p.dim, lane), vr(v + j * p.ks[2], p.dim, lane);
-        const float ds = __builtin_amdgcn_exp2f(q.dot(kr) - lse2) * (g.dot(vr) - delta);
+        const float ds = __builtin_amdgcn_exp2f(q.dot(kr) - a) * r * (g.dot(vr) - delta);
         ga += ds * kr.a;
         gb += ds * kr.b;
     }
@@ -172,7 +183,7 @@ __device__ __forceinline__ void mha_row_grad_kv(const ZnMhaArgs &p, int b, int k
             const MhaRow q(p.q + b * p.qs[0] + h * p.qs[1] + i * p.qs[2], p.dim, lane);
             const MhaRow d(p.grad_out + b * p.os[0] + h * p.os[1] + i * p.os[2], p.dim, lane);
             const float s = wave_sum((q.a * p.scale_log2) * kr.a + (q.b * p.scale_log2) * kr.b);
-            const float e = __builtin_amdgcn_exp2f(s - side[0]);
+            const float e = __builtin_amdgcn_exp2f(s - side[64]) * side[96];
             const float ds = e * (d.dot(vr) - side[32]);
             va += e * d.a;
             vb += e * d.b;
@@ -216,7 +227,10 @@ __device__ __forceinline__ void mha_row_grad_kv(const ZnMhaArgs &p, int b, int k
 // Sums stand at 2^48 times their value, so that nothing of a split is lost: one
 // beyond 2^80 or so, an infinity or a NaN (visible, or masked for some rows
 // of a block only, where it meets a probability of 0) makes a sum that is not
-// finite, and the wave then takes its rows one at a time.
+// finite, and the wave then takes its rows one at a time.  A score below -2^80
+// becomes -inf, which says the same as its probability of 0, unless the row sees
+// nothing above it: the forward then finds a maximum of -inf where keys were
+// visible, and in the backward the row's lse is far (mha_side).
 template <int DP>
 struct MhaBlock {
     static constexpr int BR = 32, SL = DP / 32, DB = DP / 16;
@@ -626,7 +640,7 @@ struct MhaQueryTile {
         bool bad = false;
 #pragma unroll
         for (int f = 0; f < FQ; ++f) {
-            bad |= !BACK && !(l[f] < INFINITY);
+            bad |= !BACK && (!(l[f] < INFINITY) || (m[f] == -INFINITY && blk0 < nblk && lim[f] > 32 * blk0));
 #pragma unroll
             for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -821,7 +835,7 @@ struct MhaKeyTile {
         const float *side = reinterpret_cast<const float *>(lds + kSide);
         const int64_t head0 = ((int64_t)b * p.q_heads + kh * p.group) * p.q_blocks;  // the group's first query block
         const char *const qi = p.qi + head0 * Frags::kImage, *const gi = p.gi + head0 * Frags::kImage;
-        const float *const sides = p.side + head0 * 64;
+        const float *const sides = p.side + head0 * kMhaSide;
         const int q_blocks = p.q_blocks;
         MhaImageStage<DP, NW> sg(lds, tid, qi, gi);
         auto fetch = [&](int st, int g, int blk) {
@@ -829,8 +843,8 @@ struct MhaKeyTile {
             sg.x = qi + at * Frags::kImage;
             sg.y = gi + at * Frags::kImage;
             sg.fetch(st, blk);
-            if (wave == NW - 1) {  // 256 bytes: a value to a lane
-                const __amdgpu_buffer_rsrc_t r = make_rsrc(mha_uniform(sides + (at + blk) * 64), 256);
+            if (wave == NW - 1) {  // lse and delta, 256 bytes: a value to a lane
+                const __amdgpu_buffer_rsrc_t r = make_rsrc(mha_uniform(sides + (at + blk) * kMhaSide), 256);
                 const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(zn_lds_void *)(lds + kSide + st * 256));
                 asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, 0 offen lds" : : "s"(m0), "v"(sg.lane16 / 4), "s"(r) : "memory");
             }
@@ -1163,6 +1177,23 @@ struct MhaFew {
     }
 };
 
+// Maximum and sum of a far query's row, one key at a time (op[0]: the queries, op[2]: the keys).
+__device__ __forceinline__ void mha_row_far(const ZnMhaSplitArgs &a, int b, int h, int i, int ql, int lane, float &m, float &l) {
+    const ZnMhaSplitOp &q = a.op[0], &k = a.op[2];
+    const int kl = k.lens ? min(max(k.lens[b], 0), k.len) : k.len, n = a.causal ? max(0, min(kl, i + 1 + kl - ql)) : kl;
+    MhaRow x(q.src + b * q.stride[0] + h * q.stride[1] + i * q.stride[2], a.dim, lane);
+    x.a *= q.scale;
+    x.b *= q.scale;
+    const float *row = k.src + b * k.stride[0] + h / (q.heads / k.heads) * k.stride[1];
+    m = -INFINITY;
+    l = 0.0f;
+    for (int j = 0; j < n && l == l; ++j) {  // a NaN stays
+        const float s = x.dot(MhaRow(row + j * k.stride[2], a.dim, lane)), mn = fmaxf(m, s), ref = mn == -INFINITY ? 0.0f : mn;
+        l = l * __builtin_amdgcn_exp2f(m - ref) + __builtin_amdgcn_exp2f(s - ref);
+        m = mn;
+    }
+}
+
 // Tensors to their images: a workgroup to a block of 32 rows, a unit of 8
 // values to a thread and step.  Rows past a sequence's length are zeros, and on
 // the query side rows that see nothing (lse -inf); blocks past it are not read
@@ -1214,10 +1245,26 @@ __device__ __forceinline__ void mha_split(const ZnMhaSplitArgs &a) {
             for (int d = threadIdx.x % 8; d < a.dim; d += 8) sum = __builtin_fmaf(g[d], o[d], sum);
 #pragma unroll
         for (int s = 1; s < 8; s <<= 1) sum += __shfl_xor(sum, s);
-        float *side = p.side + ((int64_t)bh * p.blocks + blk) * 64 + row;
+        float *side = p.side + ((int64_t)bh * p.blocks + blk) * kMhaSide + row;
+        const float lse2 = lse == -INFINITY ? INFINITY : lse * kLog2e;
+        const bool far = lse != -INFINITY && !(__builtin_fabsf(lse2) < kMhaFar);
         if (threadIdx.x % 8 == 0) {
-            side[0] = lse == -INFINITY ? INFINITY : lse * kLog2e;
+            side[0] = far ? __builtin_nanf("") : lse2;
             side[32] = sum;
+            if (!far) {
+                side[64] = lse2;
+                side[96] = 1.0f;
+            }
+        }
+        const int lane = threadIdx.x % kWave;
+        for (uint64_t left = __builtin_amdgcn_ballot_w64(far && threadIdx.x % 8 == 0); left; left &= left - 1) {
+            const int from = __builtin_ctzll(left), r = (int)threadIdx.x / kWave * 8 + from / 8;  // the whole wave, row by row
+            float m, l;
+            mha_row_far(a, b, h, r0 + r, n, lane, m, l);
+            if (lane == from) {
+                side[64] = m;
+                side[96] = 1.0f / l;
+            }
         }
     }
 }

@@ -169,6 +169,7 @@ struct MhaImages {
     char *at(int64_t offset) const { return reinterpret_cast<char *>(lease.ptr) + offset; }
     int run(zn_ctx *ctx, const ZnMhaArgs &a) {
         s.dim = a.dim;
+        s.causal = a.causal;
         return groups ? launch(ctx, ctx->mha[kMhaSplit][(a.dim - 1) / 32], (unsigned)groups, 1, 256, &s) : ZN_OK;
     }
 };
@@ -276,7 +277,7 @@ int zn_hip_mha_backward(zn_ctx *ctx, const float *q, const float *k, const float
     if (im.groups > kMhaMaxBlocks) return ZN_ERR_OVERFLOW;
     a.q_blocks = im.s.op[0].blocks;
     a.k_blocks = im.s.op[2].blocks;
-    if ((rc = im.get((int64_t)a.batch * a.q_heads * a.q_blocks * 256))) return rc;
+    if ((rc = im.get((int64_t)a.batch * a.q_heads * a.q_blocks * 512))) return rc;  // and the sides
     a.qi = im.s.op[0].dst = im.at(qi);
     a.gi = im.s.op[1].dst = im.at(gi);
     a.ki = im.s.op[2].dst = im.at(ki);

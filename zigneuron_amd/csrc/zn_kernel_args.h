@@ -260,8 +260,8 @@ struct ZnMhaArgs {
     float scale, scale_log2;      // scale_log2 = scale * log2(e)
     // Split images (zn_mha_split_*): per head, blocks of 32 rows as the tiles
     // stage them; qi (times scale_log2) and gi have q_blocks blocks a head, ki
-    // and vi k_blocks.  side: per query block 32 values lse * log2(e) (+inf
-    // where a row sees nothing), then 32 of delta, the sum of grad_out * out.
+    // and vi k_blocks.  side: per query block four times 32 values (mha_side),
+    // lse * log2(e) and delta, the sum of grad_out * out, first.
     const char *qi, *gi, *ki, *vi;
     const float *side;
     int32_t q_blocks, k_blocks;
@@ -299,13 +299,13 @@ struct ZnMhaSplitOp {
     const int32_t *lens;          // valid rows of each sequence, or null: all of len
     const float *lse;             // query side: a row with lse -inf is zeros (contiguous [batch, heads, len])
     const float *out;             // grad_out: the forward's out (same strides), for delta
-    float *side;                  // grad_out: lse and delta per block
+    float *side;                  // grad_out: lse, delta and more per block
     float scale;
     int32_t heads, len, blocks, first;
 };
 struct ZnMhaSplitArgs {
-    ZnMhaSplitOp op[4];
-    int32_t ops, dim;
+    ZnMhaSplitOp op[4];           // the backward's: q, grad_out, k, v
+    int32_t ops, dim, causal;
 };
 
 // Gated Dense layer in one launch: h [m x n/2] (in c, row stride ldc) from the
