@@ -458,8 +458,9 @@ __device__ __forceinline__ void mha_group(MhaSix &a, Acc x, Operand b, Load load
     __builtin_amdgcn_sched_barrier(0);
 }
 
-// Probabilities (or dS) times kSplitScale, which their exponent has, to the parts of a fragment.
-constexpr float kSplitLog2 = 24.0f;  // log2 of kSplitScale
+// Probabilities (or dS) times kSplitScale to the parts of a fragment.  The factor is a product of its own behind the
+// exponential, or another factor's: in the exponent's argument it would round the largest probabilities' near 24, to 2^-20
+// (a probability of an even row 6 to 9 half steps off in the mean, 1 to 1.5 so).
 __device__ __forceinline__ void mha_split8(const float (&x)[8], zn_bf16x8 (&f)[3]) {
     zn_u32x4 w[3];
 #pragma unroll
@@ -568,7 +569,7 @@ struct MhaQueryTile {
             if constexpr (BACK) {
                 const float *side = mha_side(p, b, r.h, r.i);
                 lse2[f] = lim[f] ? side[0] : INFINITY;
-                delta[f] = lim[f] ? side[32] : 0.0f;
+                delta[f] = lim[f] ? side[32] * kSplitScale : 0.0f;
                 const int64_t at = (((int64_t)b * p.q_heads + r.h) * p.q_blocks + r.i / 32) * Frags::kImage;
 #pragma unroll
                 for (int sl = 0; sl < SL; ++sl)
@@ -664,7 +665,7 @@ struct MhaQueryTile {
             float sum = 0.0f;
             if constexpr (!BACK) {
                 sum = l[f] + __shfl_xor(l[f], 16);
-                sum = (sum + __shfl_xor(sum, 32)) * (1.0f / kSplitScale);  // the probabilities' factor
+                sum += __shfl_xor(sum, 32);
             }
             if (!r.in) continue;
             if (p.splits > 1) {
@@ -739,8 +740,8 @@ struct MhaQueryTile {
             if constexpr (BACK) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const float pe = __builtin_amdgcn_exp2f(__builtin_fmaf(s[f][e / 4][e % 4], kSplitUnscale, kSplitLog2 - lse2[f]));
-                    const float de = __builtin_fmaf(dp[f][e / 4][e % 4], kSplitUnscale, -delta[f]);
+                    const float pe = __builtin_amdgcn_exp2f(__builtin_fmaf(s[f][e / 4][e % 4], kSplitUnscale, -lse2[f]));
+                    const float de = __builtin_fmaf(dp[f][e / 4][e % 4], kSplitUnscale * kSplitScale, -delta[f]);  // times kSplitScale
                     x[e] = pe * de;
                 }
             } else {
@@ -751,12 +752,13 @@ struct MhaQueryTile {
                 }
                 const float mn = fmaxf(m[f], max_over_rows(mb) * kSplitUnscale);
                 const float ref = mn == -INFINITY ? 0.0f : mn;  // nothing seen so far
-                const float alpha = __builtin_amdgcn_exp2f(m[f] - ref), up = kSplitLog2 - ref;
+                const float alpha = __builtin_amdgcn_exp2f(m[f] - ref);
                 float rs = 0.0f;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[f][e / 4][e % 4], kSplitUnscale, up));
+                    x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[f][e / 4][e % 4], kSplitUnscale, -ref));
                     rs += x[e];
+                    x[e] *= kSplitScale;
                 }
                 l[f] = l[f] * alpha + rs;
                 m[f] = mn;
@@ -921,12 +923,12 @@ struct MhaKeyTile {
         {
             zn_f32x4 ml[2];
 #pragma unroll
-            for (int rb = 0; rb < 2; ++rb) ml[rb] = kSplitLog2 - *reinterpret_cast<const zn_f32x4 *>(side + 16 * rb + 4 * lh);
+            for (int rb = 0; rb < 2; ++rb) ml[rb] = *reinterpret_cast<const zn_f32x4 *>(side + 16 * rb + 4 * lh);
 #pragma unroll
             for (int f = 0; f < FK; ++f)
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    s[f][e / 4][e % 4] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[f][e / 4][e % 4], kSplitUnscale, ml[e / 4][e % 4]));
+                    s[f][e / 4][e % 4] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[f][e / 4][e % 4], kSplitUnscale, -ml[e / 4][e % 4])) * kSplitScale;
         }
         if (mask) {
 #pragma unroll
