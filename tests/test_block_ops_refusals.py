@@ -98,3 +98,10 @@ def test_distill(lib, blank):
         assert call(vocab=BIG, ld=BIG, **({"gld": BIG} if call is b else {})) == OVERFLOW
         assert call(rows=0) == 0
     assert b(gld=99) == INVALID
+
+
+def test_mha_backward_of_no_queries_and_no_keys(lib, blank):
+    """Heads without queries against heads without keys: nothing to compute, whatever the other lengths are."""
+    for nothing in ({"q_heads": 0, "kv_len": 0}, {"q_len": 0, "kv_len": 0}, {"q_heads": 0, "q_len": 0, "kv_len": 0}):
+        assert mha(lib, blank, True, **nothing) == 0, nothing
+    assert mha(lib, blank, True, q_heads=0) not in (0, INVALID, OVERFLOW)  # keys: their gradients are zeroed

@@ -257,8 +257,8 @@ int zn_hip_mha_backward(zn_ctx *ctx, const float *q, const float *k, const float
     int rc = mha_args(ctx, a, batch, q_heads, kv_heads, q_len, kv_len, head_dim, scale, causal, q_lens, kv_lens,
                       {q_stride_b, q_stride_h, q_stride_s}, {kv_stride_b, kv_stride_h, kv_stride_s},
                       {out_stride_b, out_stride_h, out_stride_s}, true, &work);
-    if (rc || !work || (q_len == 0 && kv_len == 0)) return rc;
     const bool queries = q_heads > 0 && q_len > 0;
+    if (rc || !work || (!queries && kv_len == 0)) return rc;
     if (queries && (!q || !out || !lse || !grad_out || !grad_q)) return ZN_ERR_INVALID_ARG;
     if (kv_len > 0 && (!k || !v || !grad_k || !grad_v)) return ZN_ERR_INVALID_ARG;
     if ((rc = select_device(ctx))) return rc;
