@@ -105,3 +105,10 @@ def test_mha_backward_of_no_queries_and_no_keys(lib, blank):
     for nothing in ({"q_heads": 0, "kv_len": 0}, {"q_len": 0, "kv_len": 0}, {"q_heads": 0, "q_len": 0, "kv_len": 0}):
         assert mha(lib, blank, True, **nothing) == 0, nothing
     assert mha(lib, blank, True, q_heads=0) not in (0, INVALID, OVERFLOW)  # keys: their gradients are zeroed
+
+
+@pytest.mark.parametrize("back", [False, True])
+def test_mha_key_heads_without_query_heads(lib, blank, back):
+    """Their number is bounded by itself: its product with the batch must not wrap."""
+    for batch, heads in ((1 << 30, 1 << 34), (1 << 24, 1 << 40), (1, 1 << 33), (2, 1 << 62)):
+        assert mha(lib, blank, back, batch=batch, q_heads=0, kv_heads=heads) == OVERFLOW, (batch, heads)

@@ -35,7 +35,7 @@ int mha_args(zn_ctx *ctx, ZnMhaArgs &a, int64_t batch, int64_t q_heads, int64_t 
         !mha_strides_ok(os[0], os[1], os[2], batch, q_heads, q_len, head_dim, !backward))
         return ZN_ERR_INVALID_ARG;
     constexpr int64_t kMax = INT_MAX / 2, kMaxHeads = (int64_t)1 << 22;  // heads: a launch has fewer than 2^32 threads
-    if (batch > kMax || q_heads > kMax || q_len > kMax || kv_len > kMax || batch * q_heads > kMax || batch * kv_heads > kMaxHeads)
+    if (batch > kMax || q_heads > kMax || kv_heads > kMax || q_len > kMax || kv_len > kMax || batch * q_heads > kMax || batch * kv_heads > kMaxHeads)
         return ZN_ERR_OVERFLOW;
     const int64_t tile = kMhaRows[kMhaGrad][(head_dim - 1) / 32], max_rows = 65533 * tile;  // tiles: the grid's second extent
     if (kv_len + (kv_heads ? q_heads / kv_heads * (q_len + tile) : 0) > max_rows) return ZN_ERR_OVERFLOW;
