@@ -345,6 +345,9 @@ static bool gated_pays(const zn_ctx *ctx, int64_t m, int64_t n, int64_t k) {
     return one < two + 2.0 + 6.0 * (double)m * n / 4e6;
 }
 
+// A launch has fewer than 2^32 threads.
+static bool launchable(int64_t workgroups, int64_t threads) { return workgroups <= (int64_t)UINT_MAX / threads; }
+
 int zn_hip_gated_dense_forward(zn_ctx *ctx, int act, const float *x, const float *w, const float *bias, float *z,
                                float *h, int64_t batch, int64_t in_size, int64_t hidden) {
     if (!ctx || act < ZN_GATE_LINEAR || act > ZN_GATE_GELU || batch < 0 || in_size < 0 || hidden < 0)
@@ -375,8 +378,8 @@ int zn_hip_gated_dense_forward(zn_ctx *ctx, int act, const float *x, const float
     p.k_chunk = (int32_t)in_size;
     // a forced tile, split or wave split takes the product and a pass
     const bool free = in_size > 0 && ctx->forced_tile < 0 && ctx->forced_splits == 0 && ctx->forced_wave_split < 0 && ctx->forced_persistent < 0;
-    if (free && batch <= 16 && in_size * n >= kFewWeights) {
-        const int64_t wgs = cdiv(hidden, 32);
+    const int64_t wgs = cdiv(hidden, 32);
+    if (free && batch <= 16 && in_size * n >= kFewWeights && launchable(wgs, 1024)) {
         p.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>(cus_now(ctx) / wgs, in_size / 1024));
         Lease part(ctx);
         if (p.splits > 1) {
@@ -386,11 +389,11 @@ int zn_hip_gated_dense_forward(zn_ctx *ctx, int act, const float *x, const float
         if ((rc = launch(ctx, ctx->gated_few, (unsigned)wgs, 1, 1024, &p, (unsigned)p.splits)) || p.splits == 1) return rc;
         return launch(ctx, ctx->gated_few_join, (unsigned)cdiv(hidden, 256), (unsigned)batch, 256, &p);
     }
-    if (free && gated_pays(ctx, batch, n, in_size)) {
-        const Tile tile = estimate_split(ctx, batch, n, in_size, 1, 0).tile;
+    const Tile tile = estimate_split(ctx, batch, n, in_size, 1, 0).tile;
+    const int64_t tiles = cdiv(batch, kTiles[tile].bm) * cdiv(hidden, kTiles[tile].bn / 2);
+    if (free && gated_pays(ctx, batch, n, in_size) && launchable(tiles, kTiles[tile].threads)) {
         p.tiles_m = (int32_t)cdiv(batch, kTiles[tile].bm);
         p.tiles_n = (int32_t)cdiv(hidden, kTiles[tile].bn / 2);
-        const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
         p.xcd_remap = (tile == kTileSR || tile == kTileSN) && tiles % 8 == 0;  // as the plain product's
         return launch(ctx, ctx->gated[tile - kTileSW], (unsigned)tiles, 1, (unsigned)kTiles[tile].threads, &p);
     }
