@@ -465,7 +465,10 @@ int zn_hip_mha_backward(zn_ctx *ctx, const float *q, const float *k, const float
 /* Gated Dense layer: z = x.W + bias with W [in x 2 hidden] and bias [2
  * hidden] (null: none), its first `hidden` columns the gate and the others
  * the up projection; h = act(gate) * up [batch x hidden].  act is a zn_gate.
- * z [batch x 2 hidden] is what the backward reads; null where none follows. */
+ * z [batch x 2 hidden] is what the backward reads; null where none follows.
+ * Of the GEMM overrides a tile from ZN_TILE_256x256_S to ZN_TILE_128x64_S runs
+ * the layer in one launch on that tile; the others hold for the product, which
+ * the gate then follows. */
 int zn_hip_gated_dense_forward(zn_ctx *ctx, int act, const float *x, const float *w, const float *bias, float *z,
                                float *h, int64_t batch, int64_t in_size, int64_t hidden);
 /* Its backward, as zn_hip_dense_backward of the two projections:

@@ -376,8 +376,9 @@ int zn_hip_gated_dense_forward(zn_ctx *ctx, int act, const float *x, const float
     p.splits = 1;
     p.batch = 1;
     p.k_chunk = (int32_t)in_size;
-    // a forced tile, split or wave split takes the product and a pass
-    const bool free = in_size > 0 && ctx->forced_tile < 0 && ctx->forced_splits == 0 && ctx->forced_wave_split < 0 && ctx->forced_persistent < 0;
+    // a forced split tile is the one launch's; any other forced choice takes the product and a pass
+    const bool whole = in_size > 0 && ctx->forced_splits == 0 && ctx->forced_wave_split < 0 && ctx->forced_persistent < 0;
+    const bool free = whole && ctx->forced_tile < 0, named = whole && ctx->forced_tile >= kTileSW && ctx->forced_tile <= kTileSN;
     const int64_t wgs = cdiv(hidden, 32);
     if (free && batch <= 16 && in_size * n >= kFewWeights && launchable(wgs, 1024)) {
         p.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>(cus_now(ctx) / wgs, in_size / 1024));
@@ -389,9 +390,9 @@ int zn_hip_gated_dense_forward(zn_ctx *ctx, int act, const float *x, const float
         if ((rc = launch(ctx, ctx->gated_few, (unsigned)wgs, 1, 1024, &p, (unsigned)p.splits)) || p.splits == 1) return rc;
         return launch(ctx, ctx->gated_few_join, (unsigned)cdiv(hidden, 256), (unsigned)batch, 256, &p);
     }
-    const Tile tile = estimate_split(ctx, batch, n, in_size, 1, 0).tile;
+    const Tile tile = named ? (Tile)ctx->forced_tile : estimate_split(ctx, batch, n, in_size, 1, 0).tile;
     const int64_t tiles = cdiv(batch, kTiles[tile].bm) * cdiv(hidden, kTiles[tile].bn / 2);
-    if (free && gated_pays(ctx, batch, n, in_size) && launchable(tiles, kTiles[tile].threads)) {
+    if ((named || (free && gated_pays(ctx, batch, n, in_size))) && launchable(tiles, kTiles[tile].threads)) {
         p.tiles_m = (int32_t)cdiv(batch, kTiles[tile].bm);
         p.tiles_n = (int32_t)cdiv(hidden, kTiles[tile].bn / 2);
         p.xcd_remap = (tile == kTileSR || tile == kTileSN) && tiles % 8 == 0;  // as the plain product's
