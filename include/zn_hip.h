@@ -488,7 +488,8 @@ int zn_hip_gated_dense_backward(zn_ctx *ctx, int act, const float *x, const floa
  *   lse = log sum exp(logits / T),
  *   loss = T^2 sum_i p_i (log p_i - (logits[top_index_i] / T - lse)).
  * A row with no entry has loss and lse 0, and its logits are not read.  k is
- * 0..1024; an index may stand twice, its entries then add up. */
+ * 0..1024.  An index may stand twice: each entry is a term of its own in the
+ * loss, and their probabilities add up in the gradient. */
 int zn_hip_distill_forward(zn_ctx *ctx, const float *logits, int64_t ld, const void *top_index,
                            const float *top_logits, float *loss, float *lse, int64_t rows, int64_t vocab, int64_t k,
                            float temperature);
