@@ -70,7 +70,11 @@ struct MhaRow {
 
 // The rows one at a time, a wave each: the definition, key by key.  A masked
 // pair is never touched, so nothing that it holds can reach a sum.  The tiles
-// below take these rows where a value or a sum is not finite.
+// below take these rows where a value or a sum is not finite.  That is tens of
+// times slower, so a walk whose result is NaN already ends: tensors full of NaN,
+// as a diverged step has them, cost little more than others (8 heads (4) of 1500
+// x 64, causal, a forward and a backward: 9.4 ms when all was walked, 0.22 so,
+// 0.12 without NaN).
 
 // A row's walk over keys [from, to): running maximum (log2 domain), sum and O.
 struct MhaRowState {
@@ -80,7 +84,7 @@ struct MhaRowState {
         MhaRow q(p.q + b * p.qs[0] + h * p.qs[1] + i * p.qs[2], from < to ? p.dim : 0, lane);
         q.a *= p.scale_log2;
         q.b *= p.scale_log2;
-        for (int j = from; j < to; ++j) {
+        for (int j = from; j < to && l == l; ++j) {  // a NaN sum stays one, and all of O with it
             const MhaRow kr(k + j * p.ks[2], p.dim, lane), vr(v + j * p.ks[2], p.dim, lane);
             const float s = q.dot(kr);
             const float mn = fmaxf(m, s), ref = mn == -INFINITY ? 0.0f : mn;
@@ -157,6 +161,10 @@ __device__ __forceinline__ void mha_row_grad_q(const ZnMhaArgs &p, int b, int h,
     q.a *= p.scale_log2;
     q.b *= p.scale_log2;
     float ga = 0.0f, gb = 0.0f;
+    if (r != r || delta != delta) {  // NaN in every product
+        ga = gb = __builtin_nanf("");
+        n = from;
+    }
     for (int j = from; j < n; ++j) {
         const MhaRow kr(k + j * p.ks[2], p.dim, lane), vr(v + j * p.ks[2], p.dim, lane);
         const float ds = __builtin_amdgcn_exp2f(q.dot(kr) - a) * r * (g.dot(vr) - delta);
@@ -175,6 +183,14 @@ __device__ __forceinline__ void mha_row_grad_kv(const ZnMhaArgs &p, int b, int k
     const int64_t kat = b * p.ks[0] + kh * p.ks[1] + j * p.ks[2];
     const MhaRow kr(p.k + kat, in ? p.dim : 0, lane), vr(p.v + kat, in ? p.dim : 0, lane);
     float ka = 0.0f, kb = 0.0f, va = 0.0f, vb = 0.0f;
+    // a query whose sum is NaN makes NaN of every dim
+    for (int t = from; in && t < to; ++t) {
+        const int g = t / nb, i = 32 * (b0 + t - g * nb) + lane % 32;
+        const bool nan = i >= seq.first(j) && i < seq.ql && __builtin_isnan(mha_side(p, b, kh * p.group + g, min(i, p.q_len - 1))[96]);
+        if (!__builtin_amdgcn_ballot_w64(nan)) continue;
+        ka = kb = va = vb = __builtin_nanf("");
+        to = from;
+    }
     for (int t = from; in && t < to; ++t) {
         const int g = t / nb, h = kh * p.group + g, i0 = 32 * (b0 + t - g * nb);
         for (int i = max(i0, seq.first(j)); i < min(i0 + 32, seq.ql); ++i) {
