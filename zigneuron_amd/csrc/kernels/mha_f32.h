@@ -233,12 +233,14 @@ __device__ __forceinline__ void mha_row_grad_kv(const ZnMhaArgs &p, int b, int k
 // by DMA (MhaImageStage).  Where it goes past few, the thread that loads a value
 // splits it (MhaRawStage).
 //
-// What bounds the tiles is the matrix cores: six bf16 products for one fp32
-// product, at a clock that the power limit holds near 2 GHz while they are three
-// quarters busy (the split GEMM's share too).  MI355X, forward of 2 x 16 heads
-// (4 key/value) of 2048 x 128, causal: 168 us with the split, 205 TFLOP/s of
-// fp32 products; both gradients of 2 x 32 heads (8) of 4096 x 128, causal, 4.4 ms,
-// 158 TFLOP/s; of 8 x 16 heads of 1024 x 64, 560 us, 153 TFLOP/s.
+// What bounds the gradients' tiles is the matrix cores: six bf16 products for one
+// fp32 product, at a clock that the power limit holds near 2 GHz while they are
+// 68 to 73% busy (the largest split GEMM 74%).  The causal forward's are 56%
+// busy: the softmax and the split of P are 1.5 vector instructions a product, and
+// the edge's blocks are half masked.  MI355X, forward of 2 x 16 heads (4
+// key/value) of 2048 x 128, causal: 171 us with the split, 201 TFLOP/s of fp32
+// products; both gradients of 2 x 32 heads (8) of 4096 x 128, causal, 4.23 ms, 162
+// TFLOP/s; of 8 x 16 heads of 1024 x 64, 552 us, 156 TFLOP/s.
 //
 // Sums stand at 2^48 times their value, so that nothing of a split is lost: one
 // beyond 2^80 or so, an infinity or a NaN (visible, or masked for some rows

@@ -750,14 +750,14 @@ __device__ __forceinline__ void gated_finish(const ZnGatedArgs &p, int m, int un
 }  // namespace
 
 // The same for at most 16 rows, bound by reading W once: 32 units to a
-// workgroup, whose 16 waves share its part of K (blockIdx.z of p.splits: narrow
-// layers give every CU one) in steps of 16 and add their sums in LDS, in wave
-// order.  On the fp32 matrix cores, x as the operand of 16 columns: a lane loads
+// workgroup, whose 16 waves share its part of K (blockIdx.z of p.splits, parts of
+// 1024 inputs and more while a CU has no workgroup) in steps of 16 and add their
+// sums in LDS, in wave order.  On the fp32 matrix cores, x as the operand of 16 columns: a lane loads
 // 4 neighbouring columns of a row of W (lanes 0 - 7 the gate's, 8 - 15 the up
 // projection's: 128 bytes of each a row), which are its rows of four products;
 // four steps' loads are in flight.  16 rows cost 32 clocks a kilobyte of W, 18
 // TB/s on the chip.  MI355X, 4 x 1024 x 2 x 4096: 9.4 us (W at 5.1 TB/s alone
-// 6.6); 1 x 4096 x 2 x 8192 56 us (53).
+// 6.6; 128 workgroups leave half of the CUs idle); 1 x 4096 x 2 x 8192 56 us (53).
 extern "C" __global__ __launch_bounds__(1024, 1) void zn_gated_few(ZnGatedArgs p) {
     constexpr int NW = 16, kAhead = 4, kLd = 65;
     __shared__ float sums[NW][16][kLd];  // [wave][row][32 gate, 32 up]
