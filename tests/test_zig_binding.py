@@ -245,3 +245,13 @@ def test_patch_applies_to_the_reference(tmp_path):
     fwd = fwd[:fwd.index("pub fn backward(")]
     check = fwd.index("return error.InvalidOutputSize;")
     assert check < fwd.index("if (hip_options.enable_hip)") < fwd.index("try self.backend.matMul(")
+
+
+def test_the_language_model_blocks_have_methods():
+    """Each operator of a transformer block, forward and backward, is a HipBackend method that takes all that its call does."""
+    text = open(HIP_ZIG).read()
+    body = text[text.index("pub const HipBackend = struct {"):]
+    for method, call in (("mha", "mha"), ("gatedDense", "gated_dense"), ("distill", "distill")):
+        for way in ("Forward", "Backward"):
+            at = body.index(f"pub fn {method}{way}(self: *HipBackend")
+            assert f"try check(zn_hip_{call}_{way.lower()}(self.ctx, " in body[at:body.index("\n    }", at)], (method, way)

@@ -281,6 +281,33 @@ pub const HipBackend = struct {
     pub fn attentionForwardDevice(self: *HipBackend, q: [*]const f32, k: [*]const f32, v: [*]const f32, out: [*]f32, batch: i64, seq_len: i64, d_k: i64, scale: f32) HipError!void {
         try check(zn_hip_attention_forward(self.ctx, q, k, v, out, batch, seq_len, d_k, scale));
     }
+    /// Multi-head attention with shared key/value heads, causal and length
+    /// masks, on [batch, heads, positions, head_dim] tensors at (batch, head,
+    /// position) element strides; lse null where no backward follows.
+    pub fn mhaForward(self: *HipBackend, q: [*]const f32, k: [*]const f32, v: [*]const f32, out: [*]f32, lse: ?[*]f32, batch: i64, q_heads: i64, kv_heads: i64, q_len: i64, kv_len: i64, head_dim: i64, scale: f32, causal: bool, q_lens: ?[*]const i32, kv_lens: ?[*]const i32, q_strides: [3]i64, kv_strides: [3]i64, out_strides: [3]i64) HipError!void {
+        try check(zn_hip_mha_forward(self.ctx, q, k, v, out, lse, batch, q_heads, kv_heads, q_len, kv_len, head_dim, scale, @intFromBool(causal), q_lens, kv_lens, q_strides[0], q_strides[1], q_strides[2], kv_strides[0], kv_strides[1], kv_strides[2], out_strides[0], out_strides[1], out_strides[2]));
+    }
+    pub fn mhaBackward(self: *HipBackend, q: [*]const f32, k: [*]const f32, v: [*]const f32, out: [*]const f32, lse: [*]const f32, grad_out: [*]const f32, grad_q: [*]f32, grad_k: [*]f32, grad_v: [*]f32, batch: i64, q_heads: i64, kv_heads: i64, q_len: i64, kv_len: i64, head_dim: i64, scale: f32, causal: bool, q_lens: ?[*]const i32, kv_lens: ?[*]const i32, q_strides: [3]i64, kv_strides: [3]i64, out_strides: [3]i64) HipError!void {
+        try check(zn_hip_mha_backward(self.ctx, q, k, v, out, lse, grad_out, grad_q, grad_k, grad_v, batch, q_heads, kv_heads, q_len, kv_len, head_dim, scale, @intFromBool(causal), q_lens, kv_lens, q_strides[0], q_strides[1], q_strides[2], kv_strides[0], kv_strides[1], kv_strides[2], out_strides[0], out_strides[1], out_strides[2]));
+    }
+    /// h = act(gate) * up with [gate | up] = x.W + bias; z (the projections,
+    /// what the backward reads) null where none follows.
+    pub fn gatedDenseForward(self: *HipBackend, act: Gate, x: [*]const f32, w: [*]const f32, bias: ?[*]const f32, z: ?[*]f32, h: [*]f32, batch: i64, in_size: i64, hidden: i64) HipError!void {
+        try check(zn_hip_gated_dense_forward(self.ctx, @intFromEnum(act), x, w, bias, z, h, batch, in_size, hidden));
+    }
+    /// grad_z may be z; grad_bias accumulates; grad_x and grad_bias may be null.
+    pub fn gatedDenseBackward(self: *HipBackend, act: Gate, x: [*]const f32, w: [*]const f32, z: [*]const f32, grad_h: [*]const f32, grad_z: [*]f32, grad_x: ?[*]f32, grad_w: [*]f32, grad_bias: ?[*]f32, batch: i64, in_size: i64, hidden: i64) HipError!void {
+        try check(zn_hip_gated_dense_backward(self.ctx, @intFromEnum(act), x, w, z, grad_h, grad_z, grad_x, grad_w, grad_bias, batch, in_size, hidden));
+    }
+    /// Per row, the divergence of a teacher's top logits from the student's
+    /// distribution over the vocabulary, and the lse that the backward reads.
+    pub fn distillForward(self: *HipBackend, logits: [*]const f32, ld: i64, top_index: [*]const i32, top_logits: [*]const f32, loss: [*]f32, lse: [*]f32, rows: i64, vocab: i64, k: i64, temperature: f32) HipError!void {
+        try check(zn_hip_distill_forward(self.ctx, logits, ld, top_index, top_logits, loss, lse, rows, vocab, k, temperature));
+    }
+    /// grad_logits may be logits (with grad_ld = ld).
+    pub fn distillBackward(self: *HipBackend, logits: [*]const f32, ld: i64, top_index: [*]const i32, top_logits: [*]const f32, lse: [*]const f32, grad_loss: [*]const f32, grad_logits: [*]f32, grad_ld: i64, rows: i64, vocab: i64, k: i64, temperature: f32) HipError!void {
+        try check(zn_hip_distill_backward(self.ctx, logits, ld, top_index, top_logits, lse, grad_loss, grad_logits, grad_ld, rows, vocab, k, temperature));
+    }
 
     // --- HIP graphs of device-pointer calls (run the sequence once first)
 
