@@ -102,3 +102,25 @@ def test_far_scores_beside_near_ones(ctx):
     # the far key's value has the first query's gradient and no other's
     want = g[0, :, 0].astype(np.float64).sum(0)
     check(gv[0, 0, 0], want, 8 * U * np.abs(g[0, :, 0]).sum(0), "grad_v of the far key")
+
+
+@pytest.mark.parametrize("layout", ["bshd", "gaps"])
+@pytest.mark.parametrize("causal", [False, True])
+def test_far_scores_with_lengths_and_strides(ctx, causal, layout):
+    """Sequences of all lengths at other strides, padding that holds NaN."""
+    shape = (5, 4, 2, 90, 120, 64)
+    q, k, v, g = make(11, shape, 20, -1, "all")
+    q_lens, kv_lens = [0, 1, 50, 90, 90], [120, 5, 0, 77, 120]
+    for n in range(5):
+        q[n, :, q_lens[n]:], g[n, :, q_lens[n]:] = np.nan, np.inf
+        k[n, :, kv_lens[n]:], v[n, :, kv_lens[n]:] = -np.inf, np.nan
+        hidden = max(0, q_lens[n] - kv_lens[n]) if causal else (q_lens[n] if kv_lens[n] == 0 else 0)
+        g[n, :, :hidden] = np.nan
+    announce(f"mha far scores with lengths, causal {causal} {layout}")
+    ref = Levels(q, k, v, 1.0, causal, q_lens, kv_lens)
+    out, lse = run_forward(ctx, q, k, v, 1.0, causal, q_lens, kv_lens, layout)
+    check(out, ref.out, ref.out_bound, "out")
+    grads, bounds = ref.backward(g, out, ref.lse)
+    got = run_backward(ctx, q, k, v, out, lse, g, 1.0, causal, q_lens, kv_lens, layout)
+    for name, x, r, e in zip(("grad_q", "grad_k", "grad_v"), got, grads, bounds):
+        check(x, r, e, name)
