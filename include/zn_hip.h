@@ -501,6 +501,113 @@ int zn_hip_distill_backward(zn_ctx *ctx, const float *logits, int64_t ld, const 
                             const float *top_logits, const float *lse, const float *grad_loss, float *grad_logits,
                             int64_t grad_ld, int64_t rows, int64_t vocab, int64_t k, float temperature);
 
+/* ------------------- positions and the paged cache (device pointers) */
+/* No counterpart in the reference: what turns the attention above into a
+ * served one.  They follow the conventions of the blocks above. */
+
+/* Which dims of a head are a pair of rotary positions. */
+typedef enum zn_rotary {
+    ZN_ROTARY_HALF = 0,       /* dims i and i + rot_dim / 2 */
+    ZN_ROTARY_INTERLEAVED = 1 /* dims 2 i and 2 i + 1       */
+} zn_rotary;
+
+/* How zn_hip_rotary_frequencies scales for contexts `factor` times longer than
+ * the trained_len that a model was trained on. */
+typedef enum zn_rotary_scaling {
+    ZN_ROTARY_PLAIN = 0,  /* f_i = base^(-2 i / rot_dim)                              */
+    ZN_ROTARY_LINEAR = 1, /* f_i / factor                                             */
+    ZN_ROTARY_BASE = 2,   /* base times factor^(rot_dim / (rot_dim - 2)): the last pair is slowed down by factor, the first not */
+    ZN_ROTARY_TURNS = 3,  /* pairs of `high` turns and more over trained_len keep f_i, of `low` and fewer get f_i / factor,
+                             between the two a mixture linear in the turns             */
+    ZN_ROTARY_PAIRS = 4   /* the same, linear in the pair's number between those (rounded down and up) of `high` and `low` turns */
+} zn_rotary_scaling;
+
+/* The frequencies of rot_dim / 2 pairs into freq (host memory, freq_len
+ * values), computed in 64 bits.  factor is read for all but ZN_ROTARY_PLAIN,
+ * trained_len, low and high (0 < low < high) for the last two.  rot_dim is an
+ * even 2..1024 (4.. for ZN_ROTARY_BASE). */
+int zn_hip_rotary_frequencies(float *freq, size_t freq_len, int64_t rot_dim, float base, int scaling, float factor,
+                              int64_t trained_len, float low, float high);
+/* Rotary positions: the first rot_dim (even, 0..head_dim) dims of every head
+ * turned, pair i of the token at position p by the angle p freq[i],
+ *   (x1, x2) -> scale (x1 cos - x2 sin, x1 sin + x2 cos),
+ * the other dims copied (scale does not hold for them).  layout is a zn_rotary.
+ * freq: rot_dim / 2 floats on the device.  positions: int32 on the device, len
+ * of them for each sequence, position_stride elements apart (0: the same for
+ * all); null: 0, 1, .. in every sequence.  The angle is as exact for far
+ * positions as for near ones (64 bits).
+ * x and y are [batch, heads, len, head_dim] at element strides for batch, head
+ * and position, dims contiguous, head_dim 1..1024; y may be x at x's strides.
+ * Strides are >= 0, y's > 0 over extents above 1 (rows that it writes must not
+ * overlap).  Query and key heads of one projection's output are one call. */
+int zn_hip_rotary_forward(zn_ctx *ctx, const float *x, float *y, const float *freq, const void *positions, int64_t batch,
+                          int64_t heads, int64_t len, int64_t head_dim, int64_t rot_dim, int layout, float scale,
+                          int64_t position_stride, int64_t x_stride_b, int64_t x_stride_h, int64_t x_stride_s,
+                          int64_t y_stride_b, int64_t y_stride_h, int64_t y_stride_s);
+/* Its gradient: grad_y turned back (by the negative angle, times scale) to
+ * grad_x, which may be grad_y. */
+int zn_hip_rotary_backward(zn_ctx *ctx, const float *grad_y, float *grad_x, const float *freq, const void *positions,
+                           int64_t batch, int64_t heads, int64_t len, int64_t head_dim, int64_t rot_dim, int layout,
+                           float scale, int64_t position_stride, int64_t y_stride_b, int64_t y_stride_h,
+                           int64_t y_stride_s, int64_t x_stride_b, int64_t x_stride_h, int64_t x_stride_s);
+
+/* What a cache's pages hold. */
+typedef enum zn_cache {
+    ZN_CACHE_F32 = 0,
+    ZN_CACHE_BF16 = 1 /* rounded to the nearest, ties to even, where they enter */
+} zn_cache;
+
+/* A paged cache: pools of pages of page_size positions, and the pages of each
+ * of `batch` sequences.  Position j of sequence b is slot j % page_size of page
+ * page_table[b * max_pages + j / page_size].  Calls take it by its address and
+ * keep nothing of it; all that the device arrays hold may change between calls,
+ * and between replays of a captured one.  Pages may be of more than one sequence
+ * as long as none appends to them. */
+typedef struct zn_paged_cache {
+    void *k, *v;                 /* [num_pages, kv_heads, page_size, head_dim] at the strides below, dims contiguous */
+    const void *page_table;      /* int32 [batch x max_pages]; entries past a sequence's length are not read      */
+    const void *kv_lens;         /* int32 [batch]: positions that each sequence has, its new tokens among them      */
+    int64_t batch, num_pages, page_size, max_pages, kv_heads, head_dim; /* head_dim is 1..128 */
+    int64_t stride_page, stride_head, stride_position; /* in elements, >= 0; a position's >= head_dim; append: > 0 over extents above 1 */
+    int32_t type;                /* zn_cache */
+} zn_paged_cache;
+
+/* The keys and values of new tokens into their pages, keys and queries turned on
+ * the way as zn_hip_rotary_forward does (rot_dim 0: as they are; freq may then
+ * be null).  cache points to a zn_paged_cache.
+ *  - Sequence b's new tokens are rows token_starts[b] .. token_starts[b + 1] - 1
+ *    (int32 on the device, batch + 1 of them, ascending) of k, v and q, and its
+ *    last positions: row t's is kv_lens[b] - token_starts[b + 1] + t, which is
+ *    also what it is turned by, unless positions (int32 [tokens]) says otherwise.
+ *    Rows of no sequence, of the `tokens` there are, are neither read nor written.
+ *  - k and v are [tokens, kv_heads, head_dim], q and q_out [tokens, q_heads,
+ *    head_dim] at element strides for token and head, fp32; q_out may be q at
+ *    q's strides.  q null: no queries.
+ *  - Lengths are held to 0..max_pages * page_size and starts to 0..tokens.  A
+ *    token whose position is negative or whose page is outside the cache is
+ *    not stored. */
+int zn_hip_paged_append(zn_ctx *ctx, const void *cache, const void *token_starts, int64_t tokens, const float *k,
+                        const float *v, int64_t kv_stride_t, int64_t kv_stride_h, const float *q, float *q_out,
+                        int64_t q_heads, int64_t q_stride_t, int64_t q_stride_h, int64_t q_out_stride_t,
+                        int64_t q_out_stride_h, const float *freq, int64_t rot_dim, int layout, float scale,
+                        const void *positions);
+/* Attention of the new tokens (rows as in zn_hip_paged_append) over all that
+ * their sequences' pages hold: zn_hip_mha_forward's result with q_len the
+ * sequence's new tokens and kv_len its length.  causal = 1: row t sees the
+ * positions up to its own.
+ *  - max_q_len and max_kv_len: bounds of a sequence's new tokens and length (a
+ *    captured call: of every replay's).  A length above is taken for max_kv_len,
+ *    and of more new tokens the first max_q_len are written.
+ *  - q and out are [tokens, q_heads, head_dim] at element strides for token and
+ *    head; lse contiguous [tokens x q_heads], or null.  Query head h reads
+ *    key/value head h / (q_heads / kv_heads).  Rows of no sequence are not written.
+ *  - A position whose page is outside the cache is masked.  Masked pairs, rows
+ *    that see nothing and scores below fp32's range: as in zn_hip_mha_forward. */
+int zn_hip_paged_attention(zn_ctx *ctx, const void *cache, const void *token_starts, int64_t tokens, int64_t max_q_len,
+                           int64_t max_kv_len, const float *q, float *out, float *lse, int64_t q_heads, float scale,
+                           int causal, int64_t q_stride_t, int64_t q_stride_h, int64_t out_stride_t,
+                           int64_t out_stride_h);
+
 /* ------------------------------- Backend drop-ins on host slices (sync) */
 /* Each takes the reference method's slices as (pointer, length) pairs and its
  * scalar arguments unchanged, stages through the context's cached device

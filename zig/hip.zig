@@ -29,11 +29,32 @@ pub const DeviceInfo = extern struct {
     total_mem: i64,
 };
 
+/// zn_paged_cache
+pub const PagedCache = extern struct {
+    k: ?*anyopaque,
+    v: ?*anyopaque,
+    page_table: ?*const anyopaque,
+    kv_lens: ?*const anyopaque,
+    batch: i64,
+    num_pages: i64,
+    page_size: i64,
+    max_pages: i64,
+    kv_heads: i64,
+    head_dim: i64,
+    stride_page: i64,
+    stride_head: i64,
+    stride_position: i64,
+    type: i32,
+};
+
 pub const ABI_VERSION: c_int = 1;
 
 pub const Layout = enum(c_int) { nn = 0, nt = 1, tn = 2 };
 pub const Act = enum(c_int) { linear = 0, relu = 1, sigmoid = 2, tanh = 3 };
 pub const Gate = enum(c_int) { linear = 0, relu = 1, sigmoid = 2, tanh = 3, silu = 4, gelu = 5 };
+pub const Rotary = enum(c_int) { half = 0, interleaved = 1 };
+pub const RotaryScaling = enum(c_int) { plain = 0, linear = 1, base = 2, turns = 3, pairs = 4 };
+pub const Cache = enum(i32) { f32 = 0, bf16 = 1 };
 
 // ---------------------------------------------------------------- context
 pub extern fn zn_hip_abi_version() c_int;
@@ -101,6 +122,13 @@ pub extern fn zn_hip_gated_dense_forward(ctx: ?*Ctx, act: c_int, x: ?[*]const f3
 pub extern fn zn_hip_gated_dense_backward(ctx: ?*Ctx, act: c_int, x: ?[*]const f32, w: ?[*]const f32, z: ?[*]const f32, grad_h: ?[*]const f32, grad_z: ?[*]f32, grad_x: ?[*]f32, grad_w: ?[*]f32, grad_bias: ?[*]f32, batch: i64, in_size: i64, hidden: i64) c_int;
 pub extern fn zn_hip_distill_forward(ctx: ?*Ctx, logits: ?[*]const f32, ld: i64, top_index: ?*const anyopaque, top_logits: ?[*]const f32, loss: ?[*]f32, lse: ?[*]f32, rows: i64, vocab: i64, k: i64, temperature: f32) c_int;
 pub extern fn zn_hip_distill_backward(ctx: ?*Ctx, logits: ?[*]const f32, ld: i64, top_index: ?*const anyopaque, top_logits: ?[*]const f32, lse: ?[*]const f32, grad_loss: ?[*]const f32, grad_logits: ?[*]f32, grad_ld: i64, rows: i64, vocab: i64, k: i64, temperature: f32) c_int;
+
+// ------------------ positions and the paged cache (device pointers)
+pub extern fn zn_hip_rotary_frequencies(freq: ?[*]f32, freq_len: usize, rot_dim: i64, base: f32, scaling: c_int, factor: f32, trained_len: i64, low: f32, high: f32) c_int;
+pub extern fn zn_hip_rotary_forward(ctx: ?*Ctx, x: ?[*]const f32, y: ?[*]f32, freq: ?[*]const f32, positions: ?*const anyopaque, batch: i64, heads: i64, len: i64, head_dim: i64, rot_dim: i64, layout: c_int, scale: f32, position_stride: i64, x_stride_b: i64, x_stride_h: i64, x_stride_s: i64, y_stride_b: i64, y_stride_h: i64, y_stride_s: i64) c_int;
+pub extern fn zn_hip_rotary_backward(ctx: ?*Ctx, grad_y: ?[*]const f32, grad_x: ?[*]f32, freq: ?[*]const f32, positions: ?*const anyopaque, batch: i64, heads: i64, len: i64, head_dim: i64, rot_dim: i64, layout: c_int, scale: f32, position_stride: i64, y_stride_b: i64, y_stride_h: i64, y_stride_s: i64, x_stride_b: i64, x_stride_h: i64, x_stride_s: i64) c_int;
+pub extern fn zn_hip_paged_append(ctx: ?*Ctx, cache: ?*const anyopaque, token_starts: ?*const anyopaque, tokens: i64, k: ?[*]const f32, v: ?[*]const f32, kv_stride_t: i64, kv_stride_h: i64, q: ?[*]const f32, q_out: ?[*]f32, q_heads: i64, q_stride_t: i64, q_stride_h: i64, q_out_stride_t: i64, q_out_stride_h: i64, freq: ?[*]const f32, rot_dim: i64, layout: c_int, scale: f32, positions: ?*const anyopaque) c_int;
+pub extern fn zn_hip_paged_attention(ctx: ?*Ctx, cache: ?*const anyopaque, token_starts: ?*const anyopaque, tokens: i64, max_q_len: i64, max_kv_len: i64, q: ?[*]const f32, out: ?[*]f32, lse: ?[*]f32, q_heads: i64, scale: f32, causal: c_int, q_stride_t: i64, q_stride_h: i64, out_stride_t: i64, out_stride_h: i64) c_int;
 
 // ------------------------------------ Backend drop-ins on host slices
 pub extern fn zn_hip_mat_mul(ctx: ?*Ctx, a: ?[*]const f32, a_len: usize, b: ?[*]const f32, b_len: usize, c: ?[*]f32, c_len: usize, m: usize, n: usize, k: usize, accumulate: c_int) c_int;
@@ -307,6 +335,27 @@ pub const HipBackend = struct {
     /// grad_logits may be logits (with grad_ld = ld).
     pub fn distillBackward(self: *HipBackend, logits: [*]const f32, ld: i64, top_index: [*]const i32, top_logits: [*]const f32, lse: [*]const f32, grad_loss: [*]const f32, grad_logits: [*]f32, grad_ld: i64, rows: i64, vocab: i64, k: i64, temperature: f32) HipError!void {
         try check(zn_hip_distill_backward(self.ctx, logits, ld, top_index, top_logits, lse, grad_loss, grad_logits, grad_ld, rows, vocab, k, temperature));
+    }
+
+    /// The frequencies of freq.len rotary pairs (host memory), scaled for contexts factor times trained_len.
+    pub fn rotaryFrequencies(freq: []f32, base: f32, scaling: RotaryScaling, factor: f32, trained_len: i64, low: f32, high: f32) HipError!void {
+        try check(zn_hip_rotary_frequencies(freq.ptr, freq.len, @intCast(2 * freq.len), base, @intFromEnum(scaling), factor, trained_len, low, high));
+    }
+    /// Rotary positions on [batch, heads, len, head_dim] tensors at (batch, head, position) element strides; y may be x.
+    pub fn rotaryForward(self: *HipBackend, x: [*]const f32, y: [*]f32, freq: ?[*]const f32, positions: ?[*]const i32, batch: i64, heads: i64, len: i64, head_dim: i64, rot_dim: i64, layout: Rotary, scale: f32, position_stride: i64, x_strides: [3]i64, y_strides: [3]i64) HipError!void {
+        try check(zn_hip_rotary_forward(self.ctx, x, y, freq, positions, batch, heads, len, head_dim, rot_dim, @intFromEnum(layout), scale, position_stride, x_strides[0], x_strides[1], x_strides[2], y_strides[0], y_strides[1], y_strides[2]));
+    }
+    /// grad_x may be grad_y.
+    pub fn rotaryBackward(self: *HipBackend, grad_y: [*]const f32, grad_x: [*]f32, freq: ?[*]const f32, positions: ?[*]const i32, batch: i64, heads: i64, len: i64, head_dim: i64, rot_dim: i64, layout: Rotary, scale: f32, position_stride: i64, y_strides: [3]i64, x_strides: [3]i64) HipError!void {
+        try check(zn_hip_rotary_backward(self.ctx, grad_y, grad_x, freq, positions, batch, heads, len, head_dim, rot_dim, @intFromEnum(layout), scale, position_stride, y_strides[0], y_strides[1], y_strides[2], x_strides[0], x_strides[1], x_strides[2]));
+    }
+    /// Keys and values of new tokens into their pages, keys and queries (q null: none) turned on the way.
+    pub fn pagedAppend(self: *HipBackend, cache: *const PagedCache, token_starts: [*]const i32, tokens: i64, k: [*]const f32, v: [*]const f32, kv_strides: [2]i64, q: ?[*]const f32, q_out: ?[*]f32, q_heads: i64, q_strides: [2]i64, q_out_strides: [2]i64, freq: ?[*]const f32, rot_dim: i64, layout: Rotary, scale: f32, positions: ?[*]const i32) HipError!void {
+        try check(zn_hip_paged_append(self.ctx, cache, token_starts, tokens, k, v, kv_strides[0], kv_strides[1], q, q_out, q_heads, q_strides[0], q_strides[1], q_out_strides[0], q_out_strides[1], freq, rot_dim, @intFromEnum(layout), scale, positions));
+    }
+    /// Attention of the new tokens over their sequences' pages; lse may be null.
+    pub fn pagedAttention(self: *HipBackend, cache: *const PagedCache, token_starts: [*]const i32, tokens: i64, max_q_len: i64, max_kv_len: i64, q: [*]const f32, out: [*]f32, lse: ?[*]f32, q_heads: i64, scale: f32, causal: bool, q_strides: [2]i64, out_strides: [2]i64) HipError!void {
+        try check(zn_hip_paged_attention(self.ctx, cache, token_starts, tokens, max_q_len, max_kv_len, q, out, lse, q_heads, scale, @intFromBool(causal), q_strides[0], q_strides[1], out_strides[0], out_strides[1]));
     }
 
     // --- HIP graphs of device-pointer calls (run the sequence once first)

@@ -30,6 +30,9 @@ TILES = {"auto": -1, "256x128": 0, "128x128": 1, "128x64": 2, "64x64": 3, "32x32
          "256x256": 7, "256x256s": 8, "256x128s": 9, "128x128s": 10, "128x64s": 11, "128x128sc": 12,
          "conv128x128s": 13, "conv64x128s": 14}
 ACT_LINEAR, ACT_RELU, ACT_SIGMOID, ACT_TANH = 0, 1, 2, 3
+ROTARY_LAYOUTS = {"half": 0, "interleaved": 1}
+ROTARY_SCALINGS = {"plain": 0, "linear": 1, "base": 2, "turns": 3, "pairs": 4}
+CACHE_TYPES = {"f32": 0, "bf16": 1}
 GATES = {"linear": 0, "relu": 1, "sigmoid": 2, "tanh": 3, "silu": 4, "gelu": 5}
 
 
@@ -94,6 +97,13 @@ F = ctypes.c_float
 class DeviceInfo(ctypes.Structure):
     _fields_ = [("name", ctypes.c_char * 64), ("compute_units", ctypes.c_int32),
                 ("clock_khz", ctypes.c_int32), ("total_mem", ctypes.c_int64)]
+
+
+class PagedCacheDesc(ctypes.Structure):
+    """zn_paged_cache"""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "page_table", "kv_lens")] + \
+        [(n, ctypes.c_int64) for n in ("batch", "num_pages", "page_size", "max_pages", "kv_heads", "head_dim", "stride_page",
+                                       "stride_head", "stride_position")] + [("type", ctypes.c_int32)]
 
 
 # name -> (restype, argtypes); must match include/zn_hip.h exactly.
@@ -165,6 +175,11 @@ SIGNATURES = {
     "zn_hip_gated_dense_backward": (I, [P, I] + [P] * 8 + [I64] * 3),
     "zn_hip_distill_forward": (I, [P, P, I64, P, P, P, P, I64, I64, I64, F]),
     "zn_hip_distill_backward": (I, [P, P, I64, P, P, P, P, P, I64, I64, I64, I64, F]),
+    "zn_hip_rotary_frequencies": (I, [P, S, I64, F, I, F, I64, F, F]),
+    "zn_hip_rotary_forward": (I, [P] * 5 + [I64] * 5 + [I, F] + [I64] * 7),
+    "zn_hip_rotary_backward": (I, [P] * 5 + [I64] * 5 + [I, F] + [I64] * 7),
+    "zn_hip_paged_append": (I, [P, P, P, I64, P, P, I64, I64, P, P] + [I64] * 5 + [P, I64, I, F, P]),
+    "zn_hip_paged_attention": (I, [P, P, P] + [I64] * 3 + [P, P, P, I64, F, I] + [I64] * 4),
     "zn_hip_conv2d_forward_host": (I, [P, P, S, P, S, P, S, P, S] + [S] * 11),
     "zn_hip_conv2d_backward_host": (I, [P, P, S, P, S, P, S, P, S, P, S, P, S] + [S] * 12),
     "zn_hip_attention_forward_host": (I, [P, P, S, P, S, P, S, P, S, P, S, S, S, F]),

@@ -128,6 +128,44 @@ class Event:
             pass
 
 
+def _name_id(table, name, what: str) -> int:
+    if isinstance(name, int):
+        return name
+    try:
+        return table[str(name)]
+    except KeyError:
+        raise InvalidArgumentError(_lib.ZN_ERR_INVALID_ARG, what, f"{name!r} is not one of {', '.join(table)}") from None
+
+
+def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling="plain", factor: float = 1.0, trained_len: int = 0,
+                       low: float = 1.0, high: float = 32.0) -> np.ndarray:
+    """The frequencies of rot_dim / 2 rotary pairs (host array), scaled for contexts `factor` times trained_len:
+    "plain", "linear", "base", "turns" or "pairs" (zn_rotary_scaling)."""
+    freq = np.empty(max(int(rot_dim), 0) // 2, np.float32)
+    check(_lib.load().zn_hip_rotary_frequencies(_ptr(freq), freq.size, rot_dim, float(base),
+                                                _name_id(_lib.ROTARY_SCALINGS, scaling, "rotary scaling"), float(factor),
+                                                int(trained_len), float(low), float(high)), "zn_hip_rotary_frequencies")
+    return freq
+
+
+class PagedCache:
+    """Pools of key and value pages ([num_pages, kv_heads, page_size, head_dim] at (page, head, position) element
+    strides, None: contiguous) with the page table ([batch x max_pages] int32) and lengths ([batch] int32) of the
+    sequences in them, all on the device and the caller's; dtype is "f32" or "bf16"."""
+
+    def __init__(self, k, v, page_table, kv_lens, batch, num_pages, page_size, max_pages, kv_heads, head_dim, dtype="f32",
+                 strides=None):
+        if strides is None:
+            strides = (kv_heads * page_size * head_dim, page_size * head_dim, head_dim)
+        self.desc = _lib.PagedCacheDesc(_dptr(k), _dptr(v), _dptr(page_table), _dptr(kv_lens), batch, num_pages, page_size, max_pages,
+                                        kv_heads, head_dim, *strides, _name_id(_lib.CACHE_TYPES, dtype, "cache type"))
+        self.buffers = (k, v, page_table, kv_lens)  # held as long as the descriptor
+
+    @property
+    def address(self) -> int:
+        return ctypes.addressof(self.desc)
+
+
 class DeviceBuffer:
     """A caller-owned float32 buffer in HBM (zn_hip_alloc / zn_hip_free)."""
 
@@ -413,6 +451,53 @@ class Context:
         check(_lib.load().zn_hip_distill_backward(
             self.handle, _dptr(logits), ld, _dptr(top_index), _dptr(top_logits), _dptr(lse), _dptr(grad_loss),
             _dptr(grad_logits), grad_ld, rows, vocab, k, float(temperature)), "zn_hip_distill_backward")
+
+    def rotary_forward(self, x, y, freq, batch, heads, length, head_dim, rot_dim, layout="half", positions=None,
+                       position_stride=None, scale=1.0, x_strides=None, y_strides=None) -> None:
+        """Rotary positions: the first rot_dim dims of each head of x ([batch, heads, length, head_dim] at (batch, head,
+        position) element strides, None: contiguous) turned by the token's position times the pair's frequency; y may be
+        x.  positions: int32 device array, length of them a sequence, position_stride apart (None: length); None: 0, 1, .."""
+        self._rotary("forward", x, y, freq, batch, heads, length, head_dim, rot_dim, layout, positions, position_stride, scale,
+                     x_strides, y_strides)
+
+    def rotary_backward(self, grad_y, grad_x, freq, batch, heads, length, head_dim, rot_dim, layout="half", positions=None,
+                        position_stride=None, scale=1.0, y_strides=None, x_strides=None) -> None:
+        """The gradient of rotary_forward: grad_y turned back to grad_x, which may be grad_y."""
+        self._rotary("backward", grad_y, grad_x, freq, batch, heads, length, head_dim, rot_dim, layout, positions,
+                     position_stride, scale, y_strides, x_strides)
+
+    def _rotary(self, way, src, dst, freq, batch, heads, length, head_dim, rot_dim, layout, positions, position_stride, scale,
+                src_strides, dst_strides) -> None:
+        own = (heads * length * head_dim, length * head_dim, head_dim)
+        check(getattr(_lib.load(), f"zn_hip_rotary_{way}")(
+            self.handle, _dptr(src), _dptr(dst), _dptr(freq), _dptr(positions), batch, heads, length, head_dim, rot_dim,
+            _name_id(_lib.ROTARY_LAYOUTS, layout, "rotary layout"), float(scale),
+            length if position_stride is None else position_stride, *(own if src_strides is None else src_strides),
+            *(own if dst_strides is None else dst_strides)), f"zn_hip_rotary_{way}")
+
+    def paged_append(self, cache: PagedCache, token_starts, tokens, k, v, kv_strides=None, q=None, q_out=None, q_heads=0,
+                     q_strides=None, q_out_strides=None, freq=None, rot_dim=0, layout="half", scale=1.0, positions=None) -> None:
+        """The keys and values of new tokens ([tokens, kv_heads, head_dim] at (token, head) element strides, None:
+        contiguous) into their sequences' pages, keys and queries (q to q_out, which may be q) turned on the way.
+        Sequence b's are rows token_starts[b] .. token_starts[b + 1] - 1 and its last positions."""
+        d = cache.desc
+        own, q_own = (d.kv_heads * d.head_dim, d.head_dim), (q_heads * d.head_dim, d.head_dim)
+        check(_lib.load().zn_hip_paged_append(
+            self.handle, cache.address, _dptr(token_starts), tokens, _dptr(k), _dptr(v), *(own if kv_strides is None else kv_strides),
+            _dptr(q), _dptr(q_out), q_heads, *(q_own if q_strides is None else q_strides),
+            *(q_own if q_out_strides is None else q_out_strides), _dptr(freq), rot_dim,
+            _name_id(_lib.ROTARY_LAYOUTS, layout, "rotary layout"), float(scale), _dptr(positions)), "zn_hip_paged_append")
+
+    def paged_attention(self, cache: PagedCache, token_starts, tokens, max_q_len, max_kv_len, q, out, lse, q_heads, scale,
+                        causal=True, q_strides=None, out_strides=None) -> None:
+        """Attention of the sequences' new tokens (rows as in paged_append; at most max_q_len of each) over the positions
+        (at most max_kv_len) that their pages hold; q and out are [tokens, q_heads, head_dim] at (token, head) element
+        strides (None: contiguous), lse [tokens x q_heads] or None."""
+        own = (q_heads * cache.desc.head_dim, cache.desc.head_dim)
+        check(_lib.load().zn_hip_paged_attention(
+            self.handle, cache.address, _dptr(token_starts), tokens, max_q_len, max_kv_len, _dptr(q), _dptr(out), _dptr(lse), q_heads,
+            float(scale), int(causal), *(own if q_strides is None else q_strides),
+            *(own if out_strides is None else out_strides)), "zn_hip_paged_attention")
 
     def close(self) -> None:
         if self.handle:

@@ -604,3 +604,5 @@ extern "C" __global__ __launch_bounds__(256) void zn_attention_combine(ZnAttnArg
 
 // The masked, grouped form for training (zn_mha_*).
 #include "mha_f32.h"
+// Over a paged cache, for serving (zn_paged_*).
+#include "paged_f32.h"

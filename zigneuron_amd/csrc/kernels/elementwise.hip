@@ -904,3 +904,6 @@ extern "C" __global__ __launch_bounds__(256) void zn_distill_backward(ZnDistillA
         __syncthreads();  // idx and prob are the next row's from here on
     }
 }
+
+// ------------------------------------ rotary positions, the paged cache
+#include "rotary_f32.h"

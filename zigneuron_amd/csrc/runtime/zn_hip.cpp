@@ -34,6 +34,7 @@
 
 #include "../../../include/zn_hip.h"
 #include "../zn_kernel_args.h"
+#include "../zn_paged_args.h"
 
 // Scratch of zn_hip_sgemm_noalloc: the split-K partial sums of a GEMM whose
 // caller cannot allocate.  One copy per device, held until the process ends.
@@ -75,7 +76,7 @@ constexpr TileShape kTiles[kNumTiles] = {{256, 128, 16, 512, "x", true, true, tr
 constexpr const char *kLayoutName[3] = {"nn", "nt", "tn"};
 
 enum EltKernel { kFill, kCopy, kAddBias, kActFwd, kActBwd, kAccBias, kIm2col, kSoftmax, kCol2im, kRowSum, kDenseGrad, kRegroup, kPack, kToNhwc, kHold, kCol2imPx, kReduceSlices,
-                 kGateForward, kGateBackward, kDistillForward, kDistillJoin, kDistillBackward, kNumElt };
+                 kGateForward, kGateBackward, kDistillForward, kDistillJoin, kDistillBackward, kRotary, kPagedAppendF32, kPagedAppendBf16, kNumElt };
 constexpr const char *kEltName[kNumElt] = {"zn_fill_f32",        "zn_copy_f32", "zn_add_bias",
                                            "zn_activation_forward", "zn_activation_backward",
                                            "zn_accumulate_bias", "zn_im2col",   "zn_softmax_rows",
@@ -83,7 +84,8 @@ constexpr const char *kEltName[kNumElt] = {"zn_fill_f32",        "zn_copy_f32", 
                                            "zn_weight_regroup", "zn_pack_rows", "zn_nchw_to_nhwc",
                                            "zn_hold_stream",     "zn_col2im_px", "zn_reduce_slices",
                                            "zn_gate_forward",    "zn_gate_backward",
-                                           "zn_distill_forward", "zn_distill_join", "zn_distill_backward"};
+                                           "zn_distill_forward", "zn_distill_join", "zn_distill_backward",
+                                           "zn_rotary", "zn_paged_append_f32", "zn_paged_append_bf16"};
 
 constexpr const char *kGemmObject = "zn_gemm_gfx950.hsaco";
 constexpr const char *kConvObject = "zn_conv_gfx950.hsaco";
@@ -188,6 +190,7 @@ struct zn_ctx {
     hipFunction_t attn_combine = nullptr;      // merges its key ranges
     hipFunction_t mha[kNumMha][4] = {};        // grouped attention [head dim 32/64/96/128]
     hipFunction_t mha_join = nullptr;          // adds up its splits
+    hipFunction_t paged_rows[2] = {};          // attention over a paged cache [cache type]
     hipFunction_t gated[4] = {};               // gated Dense forward [sw, sx, sr, sn]
     hipFunction_t gated_few = nullptr, gated_few_join = nullptr;  // ... of at most 16 rows
     hipFunction_t gemm[3][kNumTiles][3] = {};  // [layout][tile][staging: 4-byte, 16-byte, 16-byte unaligned (r only)]
@@ -2020,6 +2023,9 @@ int zn_hip_create(int device, const char *code_object_dir, zn_ctx **out) {
             if (hipModuleGetFunction(&ctx->mha[i][d], ctx->attn_module, name) != hipSuccess) return bail(ZN_ERR_SYMBOL);
         }
     if (hipModuleGetFunction(&ctx->mha_join, ctx->attn_module, "zn_mha_join") != hipSuccess) return bail(ZN_ERR_SYMBOL);
+    for (int i = 0; i < 2; ++i)
+        if (hipModuleGetFunction(&ctx->paged_rows[i], ctx->attn_module, i ? "zn_paged_rows_bf16" : "zn_paged_rows_f32") != hipSuccess)
+            return bail(ZN_ERR_SYMBOL);
     void *counters = nullptr;
     if ((e = hipMalloc(&counters, kCounterSlots * kCounterStride * sizeof(int32_t))) != hipSuccess) {
         (void)hipGetLastError();
@@ -3337,6 +3343,7 @@ int zn_hip_attention_forward(zn_ctx *ctx, const float *q, const float *k, const 
 
 // ------------------------------------------------ language-model blocks
 #include "zn_block_ops.h"
+#include "zn_paged_ops.h"
 
 // ------------------------------------------------ host-slice drop-ins
 int zn_hip_mat_mul(zn_ctx *ctx, const float *a, size_t a_len, const float *b, size_t b_len, float *c, size_t c_len,
