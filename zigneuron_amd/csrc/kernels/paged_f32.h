@@ -49,13 +49,31 @@ __device__ __forceinline__ void paged_walk(const ZnPagedArgs &p, int b, int t, i
     }
 }
 
+// Keys that token i of a sequence sees: positions [0, seen).
+__device__ __forceinline__ int paged_seen(const ZnPagedArgs &p, const PagedSeq &s, int i) {
+    return p.causal ? max(0, min(s.kl, s.first + i + 1)) : s.kl;
+}
+
 __device__ __forceinline__ void paged_store(const ZnPagedArgs &p, int t, int h, int lane, float m, float l, float oa, float ob) {
     const float r = l == 0.0f ? 1.0f : l;
     MhaRow::store(p.out + t * p.os[0] + h * p.os[1], p.c.dim, lane, oa / r, ob / r);
     if (p.lse && lane == 0) p.lse[(int64_t)t * p.q_heads + h] = mha_lse(m, l);
 }
 
-// Rows one at a time, a wave each: grid x the tokens, y four heads.
+// A row's sums: to the tensor, or to its part.
+__device__ __forceinline__ void paged_finish(const ZnPagedArgs &p, float *part, int t, int h, int lane, float m, float l, float oa, float ob) {
+    if (!part) return paged_store(p, t, h, lane, m, l, oa, ob);
+    MhaRow::store(part, p.c.dim, lane, oa, ob);
+    if (lane == 0) {
+        part[p.part_ld - 4] = m;
+        part[p.part_ld - 3] = l;
+    }
+}
+
+// Parts of a walk over `keys` positions: one at least.
+__device__ __forceinline__ int paged_parts(int keys, int len) { return max(1, (keys + len - 1) / len); }
+
+// Rows one at a time, a wave each: grid x the tokens, y four heads.  For heads of fewer dims than a 16-byte load of bf16 has.
 template <typename T>
 __device__ __forceinline__ void paged_rows(const ZnPagedArgs &p) {
     const int lane = threadIdx.x & (kWave - 1), h = blockIdx.y * 4 + threadIdx.x / kWave, t = blockIdx.x;
@@ -66,13 +84,741 @@ __device__ __forceinline__ void paged_rows(const ZnPagedArgs &p) {
     const int i = t - seq.t0;
     if (i < 0 || i >= min(seq.ql, p.max_q)) return;
     MhaRowState w;
-    paged_walk<T>(p, b, t, h, 0, p.causal ? max(0, min(seq.kl, seq.first + i + 1)) : seq.kl, lane, w);
+    paged_walk<T>(p, b, t, h, 0, paged_seen(p, seq, i), lane, w);
     paged_store(p, t, h, lane, w.m, w.l, w.oa, w.ob);
+}
+
+// ------------------------------------------------------------- common parts
+// Loads at any address that a cache's strides lead to: 2-byte aligned.
+typedef uint32_t zn_u32x4_2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t zn_u32x2_2 __attribute__((ext_vector_type(2), aligned(2)));
+typedef uint32_t zn_u32_2 __attribute__((aligned(2)));
+typedef uint32_t zn_u32x2 __attribute__((ext_vector_type(2)));
+
+// Dims.  A load takes W dims of a row at d, a multiple of W, and never passes the row's end: where d + W > dim it takes the last W
+// dims.  Those of them before d are another load's too: there Q holds 0 (so that each dim is counted once), and O is not stored.
+__device__ __forceinline__ int paged_dim(int d, int w, int dim) { return min(d, dim - w); }
+
+constexpr float kPagedUnscale = 1.0f / 16777216.0f;  // of sums whose other operand is bf16 already: 2^24 times their value
+
+// A lane's chunk of 8 dims of every slice of 32 of a query row (null: zeros), times `scale`, split.
+template <int SL>
+__device__ __forceinline__ void paged_query(const float *row, int dim, int lh, float scale, zn_bf16x8 (&f)[SL][3]) {
+#pragma unroll
+    for (int sl = 0; sl < SL; ++sl) {
+        const int d = 32 * sl + 8 * lh, at = paged_dim(d, 8, dim);
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = row && at + e >= d ? row[at + e] * scale : 0.0f;
+        zn_u32x4 w[3];
+        split8(x, w);
+#pragma unroll
+        for (int q = 0; q < 3; ++q) f[sl][q] = __builtin_bit_cast(zn_bf16x8, w[q]);
+    }
+}
+
+// ------------------------------------------------------------- few query rows
+// At most 16 query rows of a key/value head (a token or a few, of the heads that
+// share it) against a long cache: bound by reading K and V once.  Nothing passes
+// through LDS: each of the NW waves walks its own keys, a step's loads ahead,
+// straight into fragments; the waves' sums are joined in LDS.
+//  - fp32 pages: the fp32 matrix cores, 16 keys a step (as zn_mha_few_*).
+//  - bf16 pages: the bf16 ones, 32 keys a step: K and V are operands as they lie,
+//    Q and P are split into three parts, so that three products take one of fp32.
+//    V's rows hold one key's dims, its operand one dim's keys: pairs of keys
+//    change halves of a register (half an instruction a value).
+// Rows are read in whole 128-byte lines where they have them: K's two slices of a
+// line go to lanes 8 apart, which then exchange theirs.
+template <typename T, int DP, int NW>
+struct PagedFew {
+    static constexpr bool BF = sizeof(T) == 2;
+    static constexpr int STEP = BF ? 32 : 16;        // keys
+    static constexpr int KB = STEP / 16;             // blocks of 16 keys
+    static constexpr int KW = BF ? 8 : 4;            // dims of a load of K
+    static constexpr int KS = DP / (4 * KW);         // slices: what the four quarters of a wave load together
+    static constexpr bool WHOLE = KS >= 2 && DP * sizeof(T) >= 128;  // two slices at a time
+    static constexpr int KR = WHOLE ? 2 : 1;         // rows of K that a lane reads of each 16
+    static constexpr int VR = STEP / 4;              // ... of V
+    static constexpr int G = DP / 16;                // blocks of 16 dims of O^T
+    static constexpr int VB = DP == 96 || (DP == 128 && !BF) ? 2 : 1;  // loads of a row of V: of w dims at 64 b + w li
+    static constexpr int vw(int b) { return DP == 128 ? (BF ? 8 : 4) : DP == 96 ? (b ? 2 : 4) : DP == 64 ? 4 : 2; }
+    static constexpr int kLd = DP + 4;
+    static constexpr int kBytes = NW * 16 * kLd * 4;
+    typedef uint32_t Raw __attribute__((ext_vector_type(4)));
+    struct Keys {
+        Raw k[KB][KS];
+        uint32_t v[VR][VB][4];
+    };
+
+    template <int BYTES>
+    __device__ static __forceinline__ void load(const T *at, uint32_t (&x)[4]) {
+        if constexpr (BYTES == 16) {
+            const zn_u32x4_2 y = *reinterpret_cast<const zn_u32x4_2 *>(at);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = y[e];
+        } else if constexpr (BYTES == 8) {
+            const zn_u32x2_2 y = *reinterpret_cast<const zn_u32x2_2 *>(at);
+            x[0] = y[0];
+            x[1] = y[1];
+        } else {
+            static_assert(BYTES == 4, "2 to 8 dims");
+            x[0] = *reinterpret_cast<const zn_u32_2 *>(at);
+        }
+    }
+    // a's upper eight lanes of 16 and b's lower eight change places
+    __device__ static __forceinline__ void swap(Raw &x, Raw &y) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int a = (int)x[e], b = (int)y[e];
+            x[e] = (uint32_t)__builtin_amdgcn_update_dpp(a, b, 0x128, 0xf, 0xc, false);  // row_ror:8
+            y[e] = (uint32_t)__builtin_amdgcn_update_dpp(b, a, 0x128, 0xf, 0x3, false);
+        }
+    }
+
+    __device__ static __forceinline__ void run(const ZnPagedArgs &p, char *lds) {
+        const int tid = threadIdx.x, lane = tid & (kWave - 1);
+        const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+        const int li = lane & 15, lh = lane >> 4;
+        const int b = blockIdx.x / p.c.kv_heads, kh = blockIdx.x - b * p.c.kv_heads, dim = p.c.dim;
+        const PagedSeq seq(p.c, b);
+        const int rows = min(seq.ql, p.max_q) * p.group;
+        if (rows == 0 || rows > 16) return;
+        const int any = __builtin_amdgcn_readfirstlane(paged_seen(p, seq, (rows - 1) / p.group));
+        const int parts = paged_parts(any, p.few_len), z = blockIdx.z;
+        if (z >= parts) return;
+        const int lim = li < rows ? paged_seen(p, seq, li / p.group) : 0;
+        // the wave's share of the part's keys, whole steps
+        const int from = z * p.few_len, to = min(from + p.few_len, any);
+        const int steps = (to - from + STEP - 1) / STEP, share = (steps + NW - 1) / NW;
+        const int s0 = min(wave * share, steps), s1 = min(s0 + share, steps);
+
+        const float *row = li < rows ? p.q + (seq.t0 + li / p.group) * p.qs[0] + (kh * p.group + li % p.group) * p.qs[1] : nullptr;
+        zn_bf16x8 qf[BF ? KS : 1][3];
+        float q[BF ? 1 : KS][4];
+        if constexpr (BF) {
+            paged_query<KS>(row, dim, lh, p.scale_log2, qf);
+        } else {
+#pragma unroll
+            for (int g = 0; g < KS; ++g) {
+                const int d = 16 * g + 4 * lh, at = paged_dim(d, 4, dim);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) q[g][e] = row && at + e >= d ? row[at + e] * p.scale_log2 : 0.0f;
+            }
+        }
+
+        // where a step's rows lie: pages asked for a step ahead of the rows
+        const T *const k = reinterpret_cast<const T *>(p.c.k) + kh * p.c.stride[1], *const v = reinterpret_cast<const T *>(p.c.v) + kh * p.c.stride[1];
+        const int32_t *const table = p.c.table + (int64_t)b * p.c.max_pages;
+        int kp[KB][KR], vp[VR];
+        bool hole = false;
+        auto page_of = [&](int j) { return (int)(((uint64_t)(uint32_t)j * p.c.div_mul) >> (31 + p.c.div_shift)); };
+        auto key_k = [&](int s, int rb, int r) { return min(from + STEP * s + 16 * rb + (WHOLE ? li % 8 + 8 * r : li), to - 1); };
+        auto key_v = [&](int s, int e) { return min(from + STEP * s + 16 * (e / 4) + 4 * lh + e % 4, to - 1); };
+        auto pages = [&](int s) {
+#pragma unroll
+            for (int rb = 0; rb < KB; ++rb)
+#pragma unroll
+                for (int r = 0; r < KR; ++r) kp[rb][r] = table[page_of(key_k(s, rb, r))];
+#pragma unroll
+            for (int e = 0; e < VR; ++e) vp[e] = table[page_of(key_v(s, e))];
+        };
+        auto at = [&](int page, int j) {
+            const bool in = (uint32_t)page < (uint32_t)p.c.pages;
+            hole |= !in;
+            return (in ? page : 0) * p.c.stride[0] + (j - page_of(j) * p.c.page_size) * p.c.stride[2];
+        };
+        auto load_step = [&](int s, Keys &x) {
+#pragma unroll
+            for (int rb = 0; rb < KB; ++rb) {
+                const T *r[KR];
+#pragma unroll
+                for (int i = 0; i < KR; ++i) r[i] = k + at(kp[rb][i], key_k(s, rb, i));
+#pragma unroll
+                for (int g = 0; g < KS; ++g) {
+                    // two slices of a line together, or the last one of an odd number
+                    const bool two = WHOLE && (g | 1) < KS;
+                    const T *const of = two ? r[KR == 2 ? g & 1 : 0] : KR == 2 ? (li < 8 ? r[0] : r[KR - 1]) : r[0];
+                    const int d = two ? 4 * KW * ((g & ~1) + li / 8) + KW * lh : 4 * KW * g + KW * lh;
+                    uint32_t y[4];
+                    load<16>(of + paged_dim(d, KW, dim), y);
+                    x.k[rb][g] = Raw{y[0], y[1], y[2], y[3]};
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < VR; ++e) {
+                const T *const r = v + at(vp[e], key_v(s, e));
+#pragma unroll
+                for (int c = 0; c < VB; ++c) {
+                    if (vw(c) == 8) load<8 * (int)sizeof(T) <= 16 ? 8 * (int)sizeof(T) : 16>(r + paged_dim(64 * c + 8 * li, 8, dim), x.v[e][c]);
+                    else if (vw(c) == 4) load<4 * (int)sizeof(T)>(r + paged_dim(64 * c + 4 * li, 4, dim), x.v[e][c]);
+                    else load<2 * (int)sizeof(T)>(r + paged_dim(64 * c + 2 * li, 2, dim), x.v[e][c]);
+                }
+            }
+        };
+
+        zn_f32x4 o[G];
+#pragma unroll
+        for (int c = 0; c < G; ++c) o[c] = zn_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        float m = -INFINITY, l = 0.0f;
+        auto step = [&](int s, Keys &y) {
+#pragma unroll
+            for (int rb = 0; rb < KB; ++rb)
+#pragma unroll
+                for (int g = 0; g + 1 < KS; g += 2)
+                    if (WHOLE) swap(y.k[rb][g], y.k[rb][g + 1]);
+            zn_f32x4 t[KB];
+            if constexpr (BF) {
+#pragma unroll
+                for (int rb = 0; rb < KB; ++rb) t[rb] = zn_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int part = 2; part >= 0; --part)  // the largest last
+#pragma unroll
+                    for (int g = 0; g < KS; ++g)
+#pragma unroll
+                        for (int rb = 0; rb < KB; ++rb)
+                            t[rb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(zn_bf16x8, y.k[rb][g]), qf[g][part], t[rb], 0, 0, 0);
+#pragma unroll
+                for (int rb = 0; rb < KB; ++rb) t[rb] *= kPagedUnscale;
+            } else {
+                zn_f32x4 u[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+                for (int g = 0; g < KS; ++g)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        u[e & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, (uint32_t)y.k[0][g][e]), q[g][e], u[e & 1], 0, 0, 0);
+                t[0] = u[0] + u[1];
+            }
+            float mb = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < VR; ++e) {
+                if (from + STEP * s + 16 * (e / 4) + 4 * lh + e % 4 >= min(lim, to)) t[e / 4][e % 4] = -INFINITY;
+                mb = fmaxf(mb, t[e / 4][e % 4]);
+            }
+            const float mn = fmaxf(m, max_over_rows(mb)), ref = mn == -INFINITY ? 0.0f : mn;
+            const float alpha = __builtin_amdgcn_exp2f(m - ref);
+            float rs = 0.0f, x[VR];
+#pragma unroll
+            for (int e = 0; e < VR; ++e) {
+                x[e] = __builtin_amdgcn_exp2f(t[e / 4][e % 4] - ref);
+                rs += x[e];
+            }
+            l = l * alpha + rs;
+            m = mn;
+#pragma unroll
+            for (int c = 0; c < G; ++c) o[c] *= alpha;
+            if constexpr (BF) {
+#pragma unroll
+                for (int e = 0; e < VR; ++e) x[e] *= kSplitScale;
+                zn_bf16x8 pf[3];
+                mha_split8(x, pf);
+#pragma unroll
+                for (int c = 0; c < VB; ++c)
+#pragma unroll
+                    for (int w = 0; w < vw(c) / 2; ++w) {
+                        zn_u32x4 lo, hi;  // the pair's first and second dim of 8 keys
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            lo[e] = __builtin_amdgcn_perm(y.v[2 * e + 1][c][w], y.v[2 * e][c][w], 0x05040100u);
+                            hi[e] = __builtin_amdgcn_perm(y.v[2 * e + 1][c][w], y.v[2 * e][c][w], 0x07060302u);
+                        }
+                        const int i = 4 * c + 2 * w;
+#pragma unroll
+                        for (int part = 2; part >= 0; --part) {
+                            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(zn_bf16x8, lo), pf[part], o[i], 0, 0, 0);
+                            o[i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(zn_bf16x8, hi), pf[part], o[i + 1], 0, 0, 0);
+                        }
+                    }
+            } else {
+#pragma unroll
+                for (int e = 0; e < VR; ++e)  // key 4 lh + e
+#pragma unroll
+                    for (int c = 0; c < VB; ++c)
+#pragma unroll
+                        for (int w = 0; w < vw(c); ++w)
+                            o[4 * c + w] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, y.v[e][c][w]), x[e], o[4 * c + w], 0, 0, 0);
+            }
+        };
+        Keys x[2];
+        if (s0 < s1) {
+            pages(s0);
+            load_step(s0, x[0]);
+            pages(s0 + 1);
+        }
+        for (int s = s0; s < s1; s += 2) {
+            if (s + 1 < s1) {
+                load_step(s + 1, x[1]);
+                pages(s + 2);
+            }
+            step(s, x[0]);
+            if (s + 1 < s1) {
+                if (s + 2 < s1) {
+                    load_step(s + 2, x[0]);
+                    pages(s + 3);
+                }
+                step(s + 1, x[1]);
+            }
+        }
+        l += __shfl_xor(l, 16);
+        l += __shfl_xor(l, 32);
+        // a page that is none of the cache's, a sum that is not finite (also of a value in a pair masked for some rows only), or scores
+        // that all fell below the split's range: the rows one by one
+        bool bad = hole || !(l < INFINITY) || (BF && m == -INFINITY && s0 < s1 && lim > from + STEP * s0);
+#pragma unroll
+        for (int c = 0; c < G; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                bad |= !(__builtin_fabsf(o[c][e]) < INFINITY);
+                if (BF) o[c][e] *= kPagedUnscale;
+            }
+        float *mine = reinterpret_cast<float *>(lds) + wave * 16 * kLd;  // [row][dims, maximum, sum]
+        if (__builtin_amdgcn_ballot_w64(bad)) {
+            for (int y = 0; y < rows; ++y) {
+                MhaRowState w;
+                paged_walk<T>(p, b, seq.t0 + y / p.group, kh * p.group + y % p.group, from + STEP * s0,
+                              min(min(from + STEP * s1, to), paged_seen(p, seq, y / p.group)), lane, w);
+                MhaRow::store(mine + y * kLd, dim, lane, w.oa, w.ob);
+                if (lane == 0) {
+                    mine[y * kLd + DP] = w.m;
+                    mine[y * kLd + DP + 1] = w.l;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < VB; ++c)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int d = 64 * c + vw(c) * (4 * lh + e), to_d = paged_dim(d, vw(c), dim);
+#pragma unroll
+                    for (int w = 0; w < vw(c); ++w)
+                        if (to_d + w >= d) mine[li * kLd + to_d + w] = o[4 * c + w][e];
+                }
+            if (lh == 0) {
+                mine[li * kLd + DP] = m;
+                mine[li * kLd + DP + 1] = l;
+            }
+        }
+        __syncthreads();
+        const float *sums = reinterpret_cast<const float *>(lds);
+        for (int y = wave; y < rows; y += NW) {  // a wave to a row, the waves' sums in order
+            float mx = -INFINITY, sl = 0.0f, oa = 0.0f, ob = 0.0f;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) mx = fmaxf(mx, sums[(w * 16 + y) * kLd + DP]);
+            const float ref = mx == -INFINITY ? 0.0f : mx;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) {
+                const float *t = sums + (w * 16 + y) * kLd;
+                const float f = __builtin_amdgcn_exp2f(t[DP] - ref);
+                sl += f * t[DP + 1];
+                if (lane < dim) oa += f * t[lane];
+                if (lane + 64 < dim) ob += f * t[lane + 64];
+            }
+            float *part = parts > 1 ? p.few_part + (((int64_t)blockIdx.x * 16 + y) * p.few_splits + z) * p.part_ld : nullptr;
+            paged_finish(p, part, seq.t0 + y / p.group, kh * p.group + y % p.group, lane, mx, sl, oa, ob);
+        }
+    }
+};
+
+// ------------------------------------------------------------- tiles of rows
+// NW x FQ x 16 query rows of a key/value head against its keys in blocks of 32,
+// staged in LDS, two stages: the products of MhaQueryTile's forward, with rows of
+// the heads that share the keys beside each other (row = token * group + head), so
+// that a tile's rows see nearly the same keys.
+//  - A thread stages 8 dims of a key's K and V: its page is asked for a block
+//    before the row, the row a block before its use.  fp32 rows are split there
+//    (three parts), bf16 ones are operands as they lie (one part): six products
+//    for one of fp32, or three.
+//  - The tiles of all sequences are one range: sequence b's begin at
+//    starts[b] group / rows + b, which leaves each as many as it may need.
+template <int DP, int NP>
+struct PagedFrags {
+    typedef MhaBlock<DP> B;
+    static constexpr int kTensor = NP * B::kPart, kStage = 2 * kTensor;
+    const char *lds;
+    int frag, tr[2];  // as MhaFrags'
+    __device__ __forceinline__ PagedFrags(const char *lds, int lane) : lds(lds) {
+        frag = B::slot(lane & 15, lane >> 4);
+        tr[0] = B::slot(4 * (lane >> 4) + (lane & 15) / 4, lane % 4 / 2) + lane % 2 * 8;
+        tr[1] = tr[0] ^ 32;
+    }
+    typedef zn_bf16x8 Set[2][NP];
+    __device__ __forceinline__ void dims(int st, int t, int sl, Set &a) const {
+#pragma unroll
+        for (int q = NP - 1; q >= 0; --q)  // in the order of their use
+#pragma unroll
+            for (int rb = 0; rb < 2; ++rb)
+                a[rb][q] = __builtin_bit_cast(zn_bf16x8, *reinterpret_cast<const zn_u32x4 *>(lds + st * kStage + t * kTensor + q * B::kPart +
+                                                                                            sl * (B::BR * 64) + rb * (16 * 64) + frag));
+    }
+    __device__ __forceinline__ void rows(int st, int t, int db, Set &x) const {
+        typedef short s4 __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) s4 ls4;
+#pragma unroll
+        for (int q = NP - 1; q >= 0; --q)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const char *at = lds + st * kStage + t * kTensor + q * B::kPart + ((db + c) / 2) * (B::BR * 64) + tr[(db + c) & 1];
+                const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ls4 *)at), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ls4 *)(at + 16 * 64));
+                x[c][q] = __builtin_bit_cast(zn_bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+            }
+    }
+    // The chunk of dims whose values a lane of quarter lh has in the accumulators of block db, and which half of it.
+    __device__ static __forceinline__ int chunk_of(int db, int lh) { return 32 * (db / 2) + 8 * (2 * (db & 1) + lh / 2); }
+};
+
+template <typename T, int DP, int NW, int FQ>
+struct PagedTile {
+    static constexpr bool BF = sizeof(T) == 2;
+    static constexpr int NP = BF ? 1 : 3, PRODUCTS = BF ? 3 : 6;
+    typedef PagedFrags<DP, NP> Frags;
+    typedef typename Frags::B B;
+    static constexpr int SL = B::SL, DB = B::DB, NT = NW * kWave, ROWS = NW * FQ * 16;
+    static constexpr int kUnits = B::BR * DP / 8, UPT = (kUnits + NT - 1) / NT;
+    static constexpr int kFlag = 2 * Frags::kStage, kBytes = kFlag + 16;
+    static constexpr float kUnscale = BF ? kPagedUnscale : kSplitUnscale;
+
+    struct Stage {
+        const ZnPagedCache &c;
+        char *lds;
+        const T *k, *v;
+        const int32_t *table;
+        int tid, kl, page[UPT];
+        bool hole = false;
+        zn_u32x4_2 g[UPT][2][BF ? 1 : 2];
+        __device__ __forceinline__ Stage(const ZnPagedCache &c, char *lds, int tid, int b, int kh, int kl)
+            : c(c), lds(lds), k(reinterpret_cast<const T *>(c.k) + kh * c.stride[1]), v(reinterpret_cast<const T *>(c.v) + kh * c.stride[1]),
+              table(c.table + (int64_t)b * c.max_pages), tid(tid), kl(kl) {}
+        __device__ __forceinline__ int page_of(int j) const { return (int)(((uint64_t)(uint32_t)j * c.div_mul) >> (31 + c.div_shift)); }
+        // Unit i's row of block blk (a row past the sequence's end: the last) and dims
+        __device__ __forceinline__ int row(int i) const { return (i * NT + tid) / (DP / 8); }
+        __device__ __forceinline__ int key(int i, int blk) const { return min(32 * blk + row(i), kl - 1); }
+        __device__ __forceinline__ void pages(int blk) {
+#pragma unroll
+            for (int i = 0; i < UPT; ++i)
+                if (i * NT + tid < kUnits) page[i] = table[page_of(key(i, blk))];
+        }
+        __device__ __forceinline__ void fetch(int blk) {
+#pragma unroll
+            for (int i = 0; i < UPT; ++i) {
+                if (i * NT + tid >= kUnits) continue;
+                const bool in = (uint32_t)page[i] < (uint32_t)c.pages;
+                hole |= !in;
+                const int j = key(i, blk), d = paged_dim((i * NT + tid) % (DP / 8) * 8, 8, c.dim);
+                const int64_t at = (in ? page[i] : 0) * c.stride[0] + (j - page_of(j) * c.page_size) * c.stride[2] + d;
+                const T *const from[2] = {k + at, v + at};
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int h = 0; h < (BF ? 1 : 2); ++h) g[i][t][h] = *reinterpret_cast<const zn_u32x4_2 *>(from[t] + 4 * h);
+            }
+        }
+        __device__ __forceinline__ void commit(int st) {
+#pragma unroll
+            for (int i = 0; i < UPT; ++i) {
+                const int u = i * NT + tid;
+                if (u >= kUnits) continue;
+                const int dc = u % (DP / 8);
+                char *const to = lds + st * Frags::kStage + dc / 4 * (B::BR * 64) + B::slot(u / (DP / 8), dc % 4);
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    if constexpr (BF) {
+                        *reinterpret_cast<zn_u32x4 *>(to + t * Frags::kTensor) = zn_u32x4{g[i][t][0][0], g[i][t][0][1], g[i][t][0][2], g[i][t][0][3]};
+                    } else {
+                        float x[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) x[e] = __builtin_bit_cast(float, (uint32_t)g[i][t][e / 4][e % 4]);
+                        zn_u32x4 w[3];
+                        split8(x, w);
+#pragma unroll
+                        for (int q = 0; q < 3; ++q) *reinterpret_cast<zn_u32x4 *>(to + t * Frags::kTensor + q * B::kPart) = w[q];
+                    }
+                }
+            }
+        }
+    };
+
+    // Tile blockIdx.x / kv_heads from the last on (late tiles of a sequence see more keys), part blockIdx.z of its walk.
+    __device__ static __forceinline__ void run(const ZnPagedArgs &p, char *lds) {
+        const int tid = threadIdx.x, lane = tid & (kWave - 1);
+        const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+        const int li = lane & 15, lh = lane >> 4, dim = p.c.dim;
+        const int all_tiles = gridDim.x / p.c.kv_heads, y = blockIdx.x / p.c.kv_heads, kh = blockIdx.x - y * p.c.kv_heads, slot = all_tiles - 1 - y;
+        int b = -1;
+        for (int i0 = 0; i0 < p.c.batch; i0 += 64) {
+            const int i = min(i0 + lane, p.c.batch - 1);
+            const uint64_t at = __builtin_amdgcn_ballot_w64(i0 + lane < p.c.batch && paged_clamp(p.c.starts[i], 0, p.c.tokens) * p.group / ROWS + i <= slot);
+            b += __builtin_popcountll(at);
+            if (~at) break;
+        }
+        if (b < 0) return;
+        const PagedSeq seq(p.c, b);
+        const int rows = min(seq.ql, p.max_q) * p.group, tile = slot - seq.t0 * p.group / ROWS - b;
+        if (tile < 0 || tile >= (rows + ROWS - 1) / ROWS || (p.few && rows <= 16)) return;
+        const int r0 = tile * ROWS;
+        // keys that any row of the workgroup sees, its parts, this one's blocks
+        const int last = paged_seen(p, seq, (min(r0 + ROWS, rows) - 1) / p.group);
+        const int parts = paged_parts(last, p.tile_len), z = blockIdx.z;
+        if (z >= parts) return;
+        const int blk0 = __builtin_amdgcn_readfirstlane(z * p.tile_len / 32), nblk = __builtin_amdgcn_readfirstlane((min((z + 1) * p.tile_len, last) + 31) / 32);
+
+        const int w0 = r0 + wave * FQ * 16;
+        int lim[FQ], all = INT_MAX, any = 0;
+        zn_bf16x8 qf[FQ][SL][3];
+#pragma unroll
+        for (int f = 0; f < FQ; ++f) {
+            const int r = w0 + 16 * f + li, i = r / p.group;
+            lim[f] = r < rows ? paged_seen(p, seq, i) : 0;
+            paged_query<SL>(lim[f] ? p.q + (seq.t0 + i) * p.qs[0] + (kh * p.group + r - i * p.group) * p.qs[1] : nullptr, dim, lh, p.scale_log2, qf[f]);
+            all = min(all, lim[f]);
+            any = max(any, lim[f]);
+        }
+#pragma unroll
+        for (int s = 1; s < 16; s <<= 1) {
+            all = min(all, __shfl_xor(all, s));
+            any = max(any, __shfl_xor(any, s));
+        }
+        all = __builtin_amdgcn_readfirstlane(all);
+        any = __builtin_amdgcn_readfirstlane(any);
+
+        zn_f32x4 o[FQ][DB];
+        float m[FQ], l[FQ];
+#pragma unroll
+        for (int f = 0; f < FQ; ++f) {
+            m[f] = -INFINITY;
+            l[f] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < DB; ++d) o[f][d] = zn_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        int *const flag = reinterpret_cast<int *>(lds + kFlag);
+        if (tid == 0) *flag = 0;
+        const Frags fr(lds, lane);
+        Stage sg(p.c, lds, tid, b, kh, seq.kl);
+        if (blk0 < nblk) {
+            sg.pages(blk0);
+            sg.fetch(blk0);
+            sg.pages(blk0 + 1);
+            sg.commit(0);
+        }
+        for (int blk = blk0; blk < nblk; ++blk) {
+            const int st = (blk - blk0) & 1, k0 = 32 * blk;
+            __syncthreads();  // block blk is in LDS; every wave is done with block blk - 1
+            if (blk + 1 < nblk) {
+                sg.fetch(blk + 1);
+                sg.pages(blk + 2);
+            }
+            if (k0 < any) block(fr, st, k0 + 32 > all, k0, lane, lim, qf, o, m, l);
+            if (blk + 1 < nblk) sg.commit(st ^ 1);
+        }
+        if (sg.hole) *flag = 1;
+        __syncthreads();
+        bool bad = *flag;
+#pragma unroll
+        for (int f = 0; f < FQ; ++f) {
+            bad |= !(l[f] < INFINITY) || (m[f] == -INFINITY && blk0 < nblk && lim[f] > 32 * blk0);
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    bad |= !(__builtin_fabsf(o[f][d][r]) < INFINITY);
+                    o[f][d][r] *= kUnscale;
+                }
+        }
+        auto part_of = [&](int t, int h) { return parts > 1 ? p.tile_part + (((int64_t)t * p.q_heads + h) * p.tile_splits + z) * p.part_ld : nullptr; };
+        if (__builtin_amdgcn_ballot_w64(bad)) {  // as PagedFew's
+            for (int r = w0; r < min(w0 + 16 * FQ, rows); ++r) {
+                const int i = r / p.group, t = seq.t0 + i, h = kh * p.group + r - i * p.group;
+                MhaRowState w;
+                paged_walk<T>(p, b, t, h, 32 * blk0, min(32 * nblk, paged_seen(p, seq, i)), lane, w);
+                paged_finish(p, part_of(t, h), t, h, lane, w.m, w.l, w.oa, w.ob);
+            }
+            return;
+        }
+#pragma unroll
+        for (int f = 0; f < FQ; ++f) {
+            const int r = w0 + 16 * f + li, i = r / p.group, t = seq.t0 + i, h = kh * p.group + r - i * p.group;
+            float sum = l[f] + __shfl_xor(l[f], 16);
+            sum += __shfl_xor(sum, 32);
+            if (r >= rows) continue;
+            float *const part = part_of(t, h), *const to = part ? part : p.out + t * p.os[0] + h * p.os[1];
+            const float div = part || sum == 0.0f ? 1.0f : sum;
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+                const int at = Frags::chunk_of(d, lh), half = 4 * (lh & 1);
+                const zn_f32x4 x = o[f][d] / div;
+                if (at + 8 <= dim) {
+                    *reinterpret_cast<zn_f32x4u *>(to + at + half) = x;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (dim - 8 + half + e >= at) to[dim - 8 + half + e] = x[e];
+                }
+            }
+            if (lh != 0) continue;
+            if (part) {
+                part[p.part_ld - 4] = m[f];
+                part[p.part_ld - 3] = sum;
+            } else if (p.lse) {
+                p.lse[(int64_t)t * p.q_heads + h] = mha_lse(m[f], sum);
+            }
+        }
+    }
+
+    // One block of 32 keys: S^T = K (cQ)^T, then O^T += V^T P^T.  `mask` (of the whole wave): some of its pairs are masked.
+    __device__ static __forceinline__ void block(const Frags &sg, int st, bool mask, int k0, int lane, const int (&lim)[FQ],
+                                                 const zn_bf16x8 (&qf)[FQ][SL][3], zn_f32x4 (&o)[FQ][DB], float (&m)[FQ], float (&l)[FQ]) {
+        const int lh = lane >> 4;
+        zn_f32x4 s[FQ][2];
+#pragma unroll
+        for (int f = 0; f < FQ; ++f) s[f][0] = s[f][1] = zn_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        typename Frags::Set a[2];
+        constexpr int NR = DB / 2, M = 2 * FQ * PRODUCTS;
+        // The products' parts, the largest last.
+        constexpr int PA[6] = {BF ? 0 : 2, BF ? 0 : 1, 0, 1, 0, 0}, PB[6] = {BF ? 2 : 0, 1, BF ? 0 : 2, 0, 1, 0};
+        sg.dims(st, 0, 0, a[0]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < SL; ++i) {
+            if (i + 1 < SL) sg.dims(st, 0, i + 1, a[(i + 1) & 1]);
+            else sg.rows(st, 1, 0, a[(i + 1) & 1]);
+#pragma unroll
+            for (int pr = 0; pr < PRODUCTS; ++pr)
+#pragma unroll
+                for (int rb = 0; rb < 2; ++rb)
+#pragma unroll
+                    for (int f = 0; f < FQ; ++f)
+                        s[f][rb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i & 1][rb][PA[pr]], qf[f][i][PB[pr]], s[f][rb], 0, 0, 0);
+            if (i + 1 < SL) mha_order<M, 2 * NP>();
+            else mha_order<M, 4 * NP>();
+        }
+        if (mask) {
+#pragma unroll
+            for (int f = 0; f < FQ; ++f)
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (k0 + 16 * (e / 4) + 4 * lh + e % 4 >= lim[f]) s[f][e / 4][e % 4] = -INFINITY;
+        }
+        zn_bf16x8 pf[FQ][3];
+#pragma unroll
+        for (int f = 0; f < FQ; ++f) {
+            float x[8], mb = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) mb = fmaxf(mb, s[f][e / 4][e % 4]);
+            const float mn = fmaxf(m[f], max_over_rows(mb) * kUnscale);
+            const float ref = mn == -INFINITY ? 0.0f : mn;  // nothing seen so far
+            const float alpha = __builtin_amdgcn_exp2f(m[f] - ref);
+            float rs = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[f][e / 4][e % 4], kUnscale, -ref));
+                rs += x[e];
+                x[e] *= kSplitScale;
+            }
+            l[f] = l[f] * alpha + rs;
+            m[f] = mn;
+            if (__builtin_amdgcn_ballot_w64(alpha != 1.0f)) {
+#pragma unroll
+                for (int d = 0; d < DB; ++d) o[f][d] *= alpha;
+            }
+            mha_split8(x, pf[f]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < NR; ++i) {
+            if (i + 1 < NR) sg.rows(st, 1, 2 * (i + 1), a[(SL + i + 1) & 1]);
+#pragma unroll
+            for (int pr = 0; pr < PRODUCTS; ++pr)
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int f = 0; f < FQ; ++f)
+                        o[f][2 * i + c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[(SL + i) & 1][c][PA[pr]], pf[f][PB[pr]], o[f][2 * i + c], 0, 0, 0);
+            mha_order<M, 4 * NP>();
+        }
+    }
+};
+
+// ------------------------------------------------------------------ the join
+// A row's parts in order, a wave to a row, lane l its dims l and l + 64, eight parts' loads in flight.
+__device__ __forceinline__ void paged_join(const ZnPagedArgs &p, const float *src, int parts, int t, int h, int lane) {
+    float mx = -INFINITY, sl = 0.0f, oa = 0.0f, ob = 0.0f;
+    for (int z0 = 0; z0 < parts; z0 += 8) {
+        float x[8], y[8], m[8], l[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const float *r = src + (int64_t)min(z0 + u, parts - 1) * p.part_ld;  // any of them: no load waits for a condition
+            x[u] = r[min(lane, p.c.dim - 1)];
+            y[u] = r[min(lane + 64, p.c.dim - 1)];
+            m[u] = r[p.part_ld - 4];
+            l[u] = r[p.part_ld - 3];
+        }
+        float mn = mx;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            if (z0 + u >= parts) m[u] = -INFINITY, l[u] = x[u] = y[u] = 0.0f;
+            mn = fmaxf(mn, m[u]);
+        }
+        const float ref = mn == -INFINITY ? 0.0f : mn, alpha = __builtin_amdgcn_exp2f(mx - ref);
+        mx = mn;
+        sl *= alpha;
+        oa *= alpha;
+        ob *= alpha;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const float f = __builtin_amdgcn_exp2f(m[u] - ref);
+            sl += f * l[u];
+            oa += f * x[u];
+            ob += f * y[u];
+        }
+    }
+    paged_store(p, t, h, lane, mx, sl, oa, ob);
 }
 
 }  // namespace
 
+// Grid x: the rows of every sequence and key/value head, 16 each, four to a workgroup.
+extern "C" __global__ __launch_bounds__(256) void zn_paged_join_few(ZnPagedArgs p) {
+    const int lane = threadIdx.x & (kWave - 1), x = blockIdx.x / 4, y = blockIdx.x % 4 * 4 + threadIdx.x / kWave;
+    const int b = x / p.c.kv_heads, kh = x - b * p.c.kv_heads;
+    const PagedSeq seq(p.c, b);
+    const int rows = min(seq.ql, p.max_q) * p.group;
+    if (rows > 16 || y >= rows) return;
+    const int parts = paged_parts(paged_seen(p, seq, (rows - 1) / p.group), p.few_len);
+    if (parts > 1)
+        paged_join(p, p.few_part + ((int64_t)x * 16 + y) * p.few_splits * p.part_ld, parts, seq.t0 + y / p.group, kh * p.group + y % p.group, lane);
+}
+
+// Grid x: the tokens, y: four heads each.  tile: the query rows of a tile.
+__device__ __forceinline__ void paged_join_tiles(const ZnPagedArgs &p, int tile) {
+    const int lane = threadIdx.x & (kWave - 1), t = blockIdx.x, h = blockIdx.y * 4 + threadIdx.x / kWave;
+    const int b = paged_find(p.c, t);
+    if (b < 0 || b >= p.c.batch || h >= p.q_heads) return;
+    const PagedSeq seq(p.c, b);
+    const int i = t - seq.t0, rows = min(seq.ql, p.max_q) * p.group;
+    if (i < 0 || i * p.group >= rows || (p.few && rows <= 16)) return;
+    const int r0 = (i * p.group + h % p.group) / tile * tile;
+    const int parts = paged_parts(paged_seen(p, seq, (min(r0 + tile, rows) - 1) / p.group), p.tile_len);
+    if (parts > 1) paged_join(p, p.tile_part + ((int64_t)t * p.q_heads + h) * p.tile_splits * p.part_ld, parts, t, h, lane);
+}
+extern "C" __global__ __launch_bounds__(256) void zn_paged_join_128(ZnPagedArgs p) { paged_join_tiles(p, 128); }
+extern "C" __global__ __launch_bounds__(256) void zn_paged_join_256(ZnPagedArgs p) { paged_join_tiles(p, 256); }
+
 extern "C" __global__ __launch_bounds__(256) void zn_paged_rows_f32(ZnPagedArgs p) { paged_rows<float>(p); }
 extern "C" __global__ __launch_bounds__(256) void zn_paged_rows_bf16(ZnPagedArgs p) { paged_rows<__bf16>(p); }
+
+#define ZN_PAGED_KERNEL(NAME, NW, ...)                                             \
+    extern "C" __global__ __launch_bounds__(NW * 64, 2) void NAME(ZnPagedArgs p) { \
+        typedef __VA_ARGS__ K;                                                     \
+        __shared__ __attribute__((aligned(1024))) char lds[K::kBytes];             \
+        K::run(p, lds);                                                            \
+    }
+// NW waves of F blocks of 16 rows.
+#define ZN_PAGED_KERNELS(DP, NW, F, BNW, BF)                                       \
+    ZN_PAGED_KERNEL(zn_paged_few_f32_##DP, 4, PagedFew<float, DP, 4>)              \
+    ZN_PAGED_KERNEL(zn_paged_few_bf16_##DP, 4, PagedFew<__bf16, DP, 4>)            \
+    ZN_PAGED_KERNEL(zn_paged_tile_f32_##DP, NW, PagedTile<float, DP, NW, F>)       \
+    ZN_PAGED_KERNEL(zn_paged_tile_bf16_##DP, BNW, PagedTile<__bf16, DP, BNW, BF>)
+ZN_PAGED_KERNELS(32, 4, 2, 4, 2)
+ZN_PAGED_KERNELS(64, 4, 2, 4, 2)
+ZN_PAGED_KERNELS(96, 8, 1, 4, 2)
+ZN_PAGED_KERNELS(128, 8, 1, 4, 2)
 
 #endif

@@ -168,6 +168,37 @@ int paged_args(const zn_paged_cache *c, ZnPagedCache &a, const void *starts, int
     return ZN_OK;
 }
 
+// Parts of the walks of few query rows, in multiples of 128 positions (32 for each wave): of 96 KB of K and V at least, and as long as
+// makes six workgroups a CU of sequences that are as long as the call allows.
+void paged_few_parts(const zn_ctx *ctx, ZnPagedArgs &a, int64_t heads, int type) {
+    const int64_t least = 98304 / (2 * a.c.dim * (type == ZN_CACHE_BF16 ? 2 : 4));
+    const int64_t len = std::max({least, a.c.cap * heads / (6 * cus_now(ctx)), (int64_t)a.c.cap / 256});
+    a.few_len = (int32_t)(cdiv(std::max<int64_t>(len, 1), 128) * 128);
+    a.few_splits = (int32_t)std::max<int64_t>(1, cdiv(a.c.cap, a.few_len));
+}
+
+// Parts of the walks of tiles: the least of the longest part or all parts' time on the chip, whichever is more, and the join (as
+// mha_splits).
+void paged_tile_parts(const zn_ctx *ctx, ZnPagedArgs &a, int64_t tokens, int64_t max_q, int64_t rows, int type, int per_cu) {
+    constexpr int kParts[12] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
+    const double cus = (double)cus_now(ctx), tiles = (double)(cdiv(tokens * a.group, rows) * a.c.kv_heads), blocks = (double)cdiv(a.c.cap, 32);
+    const double share = a.causal && a.c.cap > 0 ? 1.0 - 0.5 * std::min(1.0, (double)max_q / (double)a.c.cap) : 1.0;
+    const double block_us = (0.8 + 0.012 * a.c.dim) * (double)rows / 128.0 * (type == ZN_CACHE_BF16 ? 0.6 : 1.0), alone_us = block_us * (per_cu == 2 ? 1.3 : 1.0);
+    double best = INFINITY;
+    a.tile_splits = 1;
+    for (const int s : kParts) {
+        if (s > 1 && s > blocks) break;
+        const double longest = kPartUs + alone_us * std::ceil(blocks / s), all = tiles * s * kPartUs + tiles * block_us * blocks * share;
+        const double us = std::max(longest, all / cus) + (s > 1 ? 4.0 + 8.0 * (double)tokens * a.q_heads * s * a.c.dim / 2e6 : 0.0);
+        if (us < best) {
+            best = us;
+            a.tile_splits = s;
+        }
+    }
+    a.tile_len = (int32_t)(32 * std::max<int64_t>(1, cdiv(cdiv(a.c.cap, 32), a.tile_splits)));
+    a.tile_splits = (int32_t)std::max<int64_t>(1, cdiv(a.c.cap, a.tile_len));
+}
+
 // What a call with something to do reads of the descriptor.
 bool paged_pointers(const ZnPagedCache &a) { return a.kv_lens && a.starts && (a.cap == 0 || (a.k && a.v && a.table)); }
 
@@ -238,13 +269,17 @@ int zn_hip_paged_attention(zn_ctx *ctx, const void *cache, const void *token_sta
         !stride_ok(out_stride_h, q_heads, true))
         return ZN_ERR_INVALID_ARG;
     if (rc) return rc;
-    if (q_heads > 65535 || stride_far(q_stride_t, tokens) || stride_far(q_stride_h, q_heads) || stride_far(out_stride_t, tokens) ||
-        stride_far(out_stride_h, q_heads))
+    constexpr int64_t kMaxThreads = (int64_t)UINT_MAX;  // of a launch
+    if (q_heads > 65535 || tokens * q_heads > INT_MAX / 2 || stride_far(q_stride_t, tokens) || stride_far(q_stride_h, q_heads) ||
+        stride_far(out_stride_t, tokens) || stride_far(out_stride_h, q_heads) || desc->batch * desc->kv_heads > kMaxThreads / 1024)
         return ZN_ERR_OVERFLOW;
     if (tokens == 0 || desc->batch == 0 || q_heads == 0) return ZN_OK;
     if (!q || !out || !paged_pointers(a.c)) return ZN_ERR_INVALID_ARG;
+    const int dims = (int)(desc->head_dim - 1) / 32, type = desc->type, tile = kPagedRows[type][dims];
+    const int64_t group = q_heads / desc->kv_heads, tiles = tokens * group / tile + desc->batch, cap = std::min<int64_t>(a.c.cap, max_kv_len);
+    if (tiles * desc->kv_heads > kMaxThreads / 512) return ZN_ERR_OVERFLOW;
     if ((rc = select_device(ctx))) return rc;
-    a.c.cap = (int32_t)std::min<int64_t>(a.c.cap, max_kv_len);
+    a.c.cap = (int32_t)cap;
     a.q = q;
     a.out = out;
     a.lse = lse;
@@ -257,7 +292,34 @@ int zn_hip_paged_attention(zn_ctx *ctx, const void *cache, const void *token_sta
     a.causal = causal;
     a.max_q = (int32_t)std::min<int64_t>(max_q_len, tokens);
     a.scale_log2 = scale * 1.44269504088896340736f;
-    return launch(ctx, ctx->paged_rows[desc->type], (unsigned)tokens, (unsigned)cdiv(q_heads, 4), 256, &a);
+    // a 16-byte load of bf16 takes 8 dims
+    if (desc->head_dim < 8) return launch(ctx, ctx->paged_rows[type], (unsigned)tokens, (unsigned)cdiv(q_heads, 4), 256, &a);
+    // Sequences of few query rows and those of many: both kernels where both may occur (each leaves the other's alone).
+    const bool all_few = group * max_q_len <= 16, few = all_few || tokens < desc->batch * max_q_len;
+    a.few = few;
+    a.part_ld = (int32_t)(desc->head_dim + 3) / 4 * 4 + 4;
+    const int64_t few_heads = desc->batch * desc->kv_heads;
+    paged_few_parts(ctx, a, few_heads, type);
+    if (!all_few) paged_tile_parts(ctx, a, tokens, max_q_len, tile, type, kPagedThreads[type][dims] == 256 ? 2 : 1);
+    Lease few_part(ctx), tile_part(ctx);
+    if (few && a.few_splits > 1) {
+        if ((rc = few_part.get((size_t)(few_heads * 16) * a.few_splits * a.part_ld))) return rc;
+        a.few_part = few_part.ptr;
+    }
+    if (!all_few && a.tile_splits > 1) {
+        if ((rc = tile_part.get((size_t)(tokens * q_heads) * a.tile_splits * a.part_ld))) return rc;
+        a.tile_part = tile_part.ptr;
+    }
+    if (!all_few) {
+        if ((rc = launch(ctx, ctx->paged[kPagedTile][type][dims], (unsigned)(tiles * desc->kv_heads), 1, kPagedThreads[type][dims], &a,
+                         (unsigned)a.tile_splits)))
+            return rc;
+        if (a.tile_splits > 1 && (rc = launch(ctx, ctx->paged_join[tile / 128], (unsigned)tokens, (unsigned)cdiv(q_heads, 4), 256, &a))) return rc;
+    }
+    if (!few) return ZN_OK;
+    if ((rc = launch(ctx, ctx->paged[kPagedFew][type][dims], (unsigned)few_heads, 1, 256, &a, (unsigned)a.few_splits)) || a.few_splits == 1)
+        return rc;
+    return launch(ctx, ctx->paged_join[0], (unsigned)(few_heads * 4), 1, 256, &a);
 }
 
 #endif
