@@ -818,7 +818,7 @@ extern "C" __global__ __launch_bounds__(256) void zn_paged_rows_bf16(ZnPagedArgs
     ZN_PAGED_KERNEL(zn_paged_tile_bf16_##DP, BNW, PagedTile<__bf16, DP, BNW, BF>)
 ZN_PAGED_KERNELS(32, 4, 2, 4, 2)
 ZN_PAGED_KERNELS(64, 4, 2, 4, 2)
-ZN_PAGED_KERNELS(96, 8, 1, 4, 2)
-ZN_PAGED_KERNELS(128, 8, 1, 4, 2)
+ZN_PAGED_KERNELS(96, 8, 2, 4, 2)
+ZN_PAGED_KERNELS(128, 8, 2, 4, 2)
 
 #endif

@@ -113,7 +113,7 @@ constexpr const char *kPagedName[kNumPaged] = {"zn_paged_few", "zn_paged_tile"};
 constexpr const char *kPagedJoinName[3] = {"zn_paged_join_few", "zn_paged_join_128", "zn_paged_join_256"};
 constexpr const char *kCacheName[2] = {"f32", "bf16"};
 // Query rows and threads of a tile's workgroup [cache type][dims in 32s].
-constexpr int kPagedRows[2][4] = {{128, 128, 128, 128}, {128, 128, 128, 128}};
+constexpr int kPagedRows[2][4] = {{128, 128, 256, 256}, {128, 128, 128, 128}};
 constexpr unsigned kPagedThreads[2][4] = {{256, 256, 512, 512}, {256, 256, 256, 256}};
 
 struct ScratchDevice;
