@@ -129,12 +129,11 @@ class Event:
 
 
 def _name_id(table, name, what: str) -> int:
+    if name in table:
+        return table[name]
     if isinstance(name, int):
         return name
-    try:
-        return table[str(name)]
-    except KeyError:
-        raise InvalidArgumentError(_lib.ZN_ERR_INVALID_ARG, what, f"{name!r} is not one of {', '.join(table)}") from None
+    raise InvalidArgumentError(_lib.ZN_ERR_INVALID_ARG, what, f"{name!r} is not one of {', '.join(table)}")
 
 
 def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling="plain", factor: float = 1.0, trained_len: int = 0,
@@ -457,23 +456,14 @@ class Context:
         """Rotary positions: the first rot_dim dims of each head of x ([batch, heads, length, head_dim] at (batch, head,
         position) element strides, None: contiguous) turned by the token's position times the pair's frequency; y may be
         x.  positions: int32 device array, length of them a sequence, position_stride apart (None: length); None: 0, 1, .."""
-        self._rotary("forward", x, y, freq, batch, heads, length, head_dim, rot_dim, layout, positions, position_stride, scale,
-                     x_strides, y_strides)
+        _rotary(_lib.load().zn_hip_rotary_forward, self.handle, x, y, freq, batch, heads, length, head_dim, rot_dim, layout, positions,
+                position_stride, scale, x_strides, y_strides)
 
     def rotary_backward(self, grad_y, grad_x, freq, batch, heads, length, head_dim, rot_dim, layout="half", positions=None,
                         position_stride=None, scale=1.0, y_strides=None, x_strides=None) -> None:
         """The gradient of rotary_forward: grad_y turned back to grad_x, which may be grad_y."""
-        self._rotary("backward", grad_y, grad_x, freq, batch, heads, length, head_dim, rot_dim, layout, positions,
-                     position_stride, scale, y_strides, x_strides)
-
-    def _rotary(self, way, src, dst, freq, batch, heads, length, head_dim, rot_dim, layout, positions, position_stride, scale,
-                src_strides, dst_strides) -> None:
-        own = (heads * length * head_dim, length * head_dim, head_dim)
-        check(getattr(_lib.load(), f"zn_hip_rotary_{way}")(
-            self.handle, _dptr(src), _dptr(dst), _dptr(freq), _dptr(positions), batch, heads, length, head_dim, rot_dim,
-            _name_id(_lib.ROTARY_LAYOUTS, layout, "rotary layout"), float(scale),
-            length if position_stride is None else position_stride, *(own if src_strides is None else src_strides),
-            *(own if dst_strides is None else dst_strides)), f"zn_hip_rotary_{way}")
+        _rotary(_lib.load().zn_hip_rotary_backward, self.handle, grad_y, grad_x, freq, batch, heads, length, head_dim, rot_dim, layout,
+                positions, position_stride, scale, y_strides, x_strides)
 
     def paged_append(self, cache: PagedCache, token_starts, tokens, k, v, kv_strides=None, q=None, q_out=None, q_heads=0,
                      q_strides=None, q_out_strides=None, freq=None, rot_dim=0, layout="half", scale=1.0, positions=None) -> None:
@@ -526,9 +516,20 @@ def _mha_strides(q_heads, kv_heads, q_len, kv_len, head_dim, q, kv, out):
     return (*(q_own if q is None else q), *(kv_own if kv is None else kv), *(q_own if out is None else out))
 
 
+def _rotary(call, handle, src, dst, freq, batch, heads, length, head_dim, rot_dim, layout, positions, position_stride, scale,
+            src_strides, dst_strides) -> None:
+    """Either direction's call; strides not given are contiguous [batch, heads, positions, dims]."""
+    own = (heads * length * head_dim, length * head_dim, head_dim)
+    sb, sh, ss = own if src_strides is None else src_strides
+    db, dh, ds = own if dst_strides is None else dst_strides
+    check(call(handle, _dptr(src), _dptr(dst), _dptr(freq), _dptr(positions), batch, heads, length, head_dim, rot_dim,
+               _name_id(_lib.ROTARY_LAYOUTS, layout, "rotary layout"), scale, length if position_stride is None else position_stride,
+               sb, sh, ss, db, dh, ds), call.__name__)
+
+
 def _dptr(x) -> Optional[int]:
-    if x is None:
-        return None
+    if x is None or type(x) is int:
+        return x
     if isinstance(x, DeviceBuffer):
         return x.ptr
     return int(x)

@@ -101,35 +101,33 @@ __device__ __forceinline__ int paged_dim(int d, int w, int dim) { return min(d, 
 
 constexpr float kPagedUnscale = 1.0f / 16777216.0f;  // of sums whose other operand is bf16 already: 2^24 times their value
 
-// A lane's chunk of 8 dims of every slice of 32 of a query row (null: zeros), times `scale`, split.
-template <int SL>
-__device__ __forceinline__ void paged_query(const float *row, int dim, int lh, float scale, zn_bf16x8 (&f)[SL][3]) {
+// W dims (4 or 8) of a query row at d, times `scale`; zeros of a row that is not `in` (row: any one).
+template <int W>
+__device__ __forceinline__ void paged_query(const float *row, bool in, int d, int dim, float scale, float (&x)[W]) {
+    const int at = paged_dim(d, W, dim);
 #pragma unroll
-    for (int sl = 0; sl < SL; ++sl) {
-        const int d = 32 * sl + 8 * lh, at = paged_dim(d, 8, dim);
-        float x[8];
+    for (int h = 0; h < W; h += 4) {
+        const zn_f32x4 v = *reinterpret_cast<const zn_f32x4u *>(row + at + h);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = row && at + e >= d ? row[at + e] * scale : 0.0f;
-        zn_u32x4 w[3];
-        split8(x, w);
-#pragma unroll
-        for (int q = 0; q < 3; ++q) f[sl][q] = __builtin_bit_cast(zn_bf16x8, w[q]);
+        for (int e = 0; e < 4; ++e) x[h + e] = in && at + h + e >= d ? v[e] * scale : 0.0f;
     }
 }
 
 // ------------------------------------------------------------- few query rows
-// At most 16 query rows of a key/value head (a token or a few, of the heads that
-// share it) against a long cache: bound by reading K and V once.  Nothing passes
-// through LDS: each of the NW waves walks its own keys, a step's loads ahead,
-// straight into fragments; the waves' sums are joined in LDS.
+// At most 16 RB query rows of a key/value head (a token or a few, of the heads
+// that share it) against a long cache: bound by reading K and V once.  K and V do
+// not pass through LDS: each of the NW waves walks its own keys, straight into
+// fragments; Q's fragments are in LDS, and the waves' sums are joined there.
 //  - fp32 pages: the fp32 matrix cores, 16 keys a step (as zn_mha_few_*).
 //  - bf16 pages: the bf16 ones, 32 keys a step: K and V are operands as they lie,
 //    Q and P are split into three parts, so that three products take one of fp32.
 //    V's rows hold one key's dims, its operand one dim's keys: pairs of keys
 //    change halves of a register (half an instruction a value).
+// One set of registers each for K and V: the next step's K is asked for behind
+// the products with K, its V behind those with V.
 // Rows are read in whole 128-byte lines where they have them: K's two slices of a
 // line go to lanes 8 apart, which then exchange theirs.
-template <typename T, int DP, int NW>
+template <typename T, int DP, int NW, int RB, bool PAGES16>
 struct PagedFew {
     static constexpr bool BF = sizeof(T) == 2;
     static constexpr int STEP = BF ? 32 : 16;        // keys
@@ -142,13 +140,12 @@ struct PagedFew {
     static constexpr int G = DP / 16;                // blocks of 16 dims of O^T
     static constexpr int VB = DP == 96 || (DP == 128 && !BF) ? 2 : 1;  // loads of a row of V: of w dims at 64 b + w li
     static constexpr int vw(int b) { return DP == 128 ? (BF ? 8 : 4) : DP == 96 ? (b ? 2 : 4) : DP == 64 ? 4 : 2; }
+    static constexpr int ROWS = 16 * RB;
     static constexpr int kLd = DP + 4;
-    static constexpr int kBytes = NW * 16 * kLd * 4;
+    static constexpr int QP = BF ? 3 : 1;            // parts of Q; a fragment: 16 bytes a lane
+    static constexpr int kQuery = RB * KS * QP * 1024, kSums = NW * 16 * kLd * 4;
+    static constexpr int kBytes = kQuery > kSums ? kQuery : kSums;
     typedef uint32_t Raw __attribute__((ext_vector_type(4)));
-    struct Keys {
-        Raw k[KB][KS];
-        uint32_t v[VR][VB][4];
-    };
 
     template <int BYTES>
     __device__ static __forceinline__ void load(const T *at, uint32_t (&x)[4]) {
@@ -165,7 +162,7 @@ struct PagedFew {
             x[0] = *reinterpret_cast<const zn_u32_2 *>(at);
         }
     }
-    // a's upper eight lanes of 16 and b's lower eight change places
+    // x's upper eight lanes of 16 and y's lower eight change places
     __device__ static __forceinline__ void swap(Raw &x, Raw &y) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -175,6 +172,45 @@ struct PagedFew {
         }
     }
 
+    // Where a walk's rows lie.  Pages whose size is a multiple of 16 (PAGES16) hold each block of 16 keys whole: one page of the block
+    // for the wave, read by the scalar unit.  Other pages are looked up row by row.  Either a step ahead of the rows.  Keys past the
+    // walk's end are its last.
+    struct Place {
+        typedef __attribute__((address_space(4))) const int32_t Table;  // constant: for scalar loads
+        const ZnPagedCache &c;
+        const int32_t *table;
+        int from, to, li, lh;
+        bool hole = false;
+        int kp[KB][PAGES16 ? 1 : KR], vp[PAGES16 ? KB : VR];
+        __device__ __forceinline__ Place(const ZnPagedCache &c, int b, int from, int to, int lane)
+            : c(c), table(c.table + (int64_t)b * c.max_pages), from(from), to(to), li(lane & 15), lh(lane >> 4) {}
+        __device__ __forceinline__ int page_of(int j) const { return (int)(((uint64_t)(uint32_t)j * c.div_mul) >> (31 + c.div_shift)); }
+        __device__ __forceinline__ int key_k(int rb, int r) const { return 16 * rb + (WHOLE ? li % 8 + 8 * r : li); }  // of a step
+        __device__ __forceinline__ int key_v(int e) const { return 16 * (e / 4) + 4 * lh + e % 4; }
+        __device__ __forceinline__ int key(int s, int i) const { return min(from + STEP * s + i, to - 1); }
+        __device__ __forceinline__ int page_at(int j) const { return PAGES16 ? ((Table *)(uintptr_t)table)[page_of(j)] : table[page_of(j)]; }
+        __device__ __forceinline__ void ask_k(int s) {
+#pragma unroll
+            for (int rb = 0; rb < KB; ++rb)
+#pragma unroll
+                for (int r = 0; r < (PAGES16 ? 1 : KR); ++r) kp[rb][r] = page_at(key(s, PAGES16 ? 16 * rb : key_k(rb, r)));
+        }
+        __device__ __forceinline__ void ask_v(int s) {
+#pragma unroll
+            for (int e = 0; e < (PAGES16 ? KB : VR); ++e) vp[e] = page_at(key(s, PAGES16 ? 16 * e : key_v(e)));
+        }
+        // A row's elements from the head's first: key i of step s, in block rb, whose page is `page`.
+        __device__ __forceinline__ int64_t at(int s, int rb, int page, int i) {
+            const bool in = (uint32_t)page < (uint32_t)c.pages;
+            hole |= !in;
+            const int j0 = key(s, PAGES16 ? 16 * rb : i);
+            const int64_t first = (in ? page : 0) * c.stride[0] + (j0 - page_of(j0) * c.page_size) * c.stride[2];
+            return PAGES16 ? first + (int64_t)((uint64_t)(uint32_t)(key(s, i) - j0) * (uint32_t)c.stride[2]) : first;
+        }
+        __device__ __forceinline__ int64_t at_k(int s, int rb, int r) { return at(s, rb, kp[rb][PAGES16 ? 0 : r], key_k(rb, r)); }
+        __device__ __forceinline__ int64_t at_v(int s, int e) { return at(s, e / 4, vp[PAGES16 ? e / 4 : e], key_v(e)); }
+    };
+
     __device__ static __forceinline__ void run(const ZnPagedArgs &p, char *lds) {
         const int tid = threadIdx.x, lane = tid & (kWave - 1);
         const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
@@ -182,238 +218,262 @@ struct PagedFew {
         const int b = blockIdx.x / p.c.kv_heads, kh = blockIdx.x - b * p.c.kv_heads, dim = p.c.dim;
         const PagedSeq seq(p.c, b);
         const int rows = min(seq.ql, p.max_q) * p.group;
-        if (rows == 0 || rows > 16) return;
+        if (rows == 0 || rows > ROWS) return;
         const int any = __builtin_amdgcn_readfirstlane(paged_seen(p, seq, (rows - 1) / p.group));
         const int parts = paged_parts(any, p.few_len), z = blockIdx.z;
         if (z >= parts) return;
-        const int lim = li < rows ? paged_seen(p, seq, li / p.group) : 0;
         // the wave's share of the part's keys, whole steps
         const int from = z * p.few_len, to = min(from + p.few_len, any);
         const int steps = (to - from + STEP - 1) / STEP, share = (steps + NW - 1) / NW;
-        const int s0 = min(wave * share, steps), s1 = min(s0 + share, steps);
+        const int s0 = min(wave * share, steps), s1 = min(s0 + share, steps), end = min(from + STEP * s1, to);
 
-        const float *row = li < rows ? p.q + (seq.t0 + li / p.group) * p.qs[0] + (kh * p.group + li % p.group) * p.qs[1] : nullptr;
-        zn_bf16x8 qf[BF ? KS : 1][3];
-        float q[BF ? 1 : KS][4];
-        if constexpr (BF) {
-            paged_query<KS>(row, dim, lh, p.scale_log2, qf);
-        } else {
-#pragma unroll
-            for (int g = 0; g < KS; ++g) {
-                const int d = 16 * g + 4 * lh, at = paged_dim(d, 4, dim);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) q[g][e] = row && at + e >= d ? row[at + e] * p.scale_log2 : 0.0f;
-            }
-        }
-
-        // where a step's rows lie: pages asked for a step ahead of the rows
         const T *const k = reinterpret_cast<const T *>(p.c.k) + kh * p.c.stride[1], *const v = reinterpret_cast<const T *>(p.c.v) + kh * p.c.stride[1];
-        const int32_t *const table = p.c.table + (int64_t)b * p.c.max_pages;
-        int kp[KB][KR], vp[VR];
-        bool hole = false;
-        auto page_of = [&](int j) { return (int)(((uint64_t)(uint32_t)j * p.c.div_mul) >> (31 + p.c.div_shift)); };
-        auto key_k = [&](int s, int rb, int r) { return min(from + STEP * s + 16 * rb + (WHOLE ? li % 8 + 8 * r : li), to - 1); };
-        auto key_v = [&](int s, int e) { return min(from + STEP * s + 16 * (e / 4) + 4 * lh + e % 4, to - 1); };
-        auto pages = [&](int s) {
-#pragma unroll
-            for (int rb = 0; rb < KB; ++rb)
-#pragma unroll
-                for (int r = 0; r < KR; ++r) kp[rb][r] = table[page_of(key_k(s, rb, r))];
-#pragma unroll
-            for (int e = 0; e < VR; ++e) vp[e] = table[page_of(key_v(s, e))];
-        };
-        auto at = [&](int page, int j) {
-            const bool in = (uint32_t)page < (uint32_t)p.c.pages;
-            hole |= !in;
-            return (in ? page : 0) * p.c.stride[0] + (j - page_of(j) * p.c.page_size) * p.c.stride[2];
-        };
-        auto load_step = [&](int s, Keys &x) {
+        Place at(p.c, b, from, end, lane);
+        Raw x[KB][KS];
+        uint32_t y[VR][VB][4];
+        auto load_k = [&](int s) {
 #pragma unroll
             for (int rb = 0; rb < KB; ++rb) {
                 const T *r[KR];
 #pragma unroll
-                for (int i = 0; i < KR; ++i) r[i] = k + at(kp[rb][i], key_k(s, rb, i));
+                for (int i = 0; i < KR; ++i) r[i] = k + at.at_k(s, rb, i);
 #pragma unroll
                 for (int g = 0; g < KS; ++g) {
                     // two slices of a line together, or the last one of an odd number
                     const bool two = WHOLE && (g | 1) < KS;
                     const T *const of = two ? r[KR == 2 ? g & 1 : 0] : KR == 2 ? (li < 8 ? r[0] : r[KR - 1]) : r[0];
                     const int d = two ? 4 * KW * ((g & ~1) + li / 8) + KW * lh : 4 * KW * g + KW * lh;
-                    uint32_t y[4];
-                    load<16>(of + paged_dim(d, KW, dim), y);
-                    x.k[rb][g] = Raw{y[0], y[1], y[2], y[3]};
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < VR; ++e) {
-                const T *const r = v + at(vp[e], key_v(s, e));
-#pragma unroll
-                for (int c = 0; c < VB; ++c) {
-                    if (vw(c) == 8) load<8 * (int)sizeof(T) <= 16 ? 8 * (int)sizeof(T) : 16>(r + paged_dim(64 * c + 8 * li, 8, dim), x.v[e][c]);
-                    else if (vw(c) == 4) load<4 * (int)sizeof(T)>(r + paged_dim(64 * c + 4 * li, 4, dim), x.v[e][c]);
-                    else load<2 * (int)sizeof(T)>(r + paged_dim(64 * c + 2 * li, 2, dim), x.v[e][c]);
+                    uint32_t u[4];
+                    load<16>(of + paged_dim(d, KW, dim), u);
+                    x[rb][g] = Raw{u[0], u[1], u[2], u[3]};
                 }
             }
         };
-
-        zn_f32x4 o[G];
+        auto load_v = [&](int s) {
 #pragma unroll
-        for (int c = 0; c < G; ++c) o[c] = zn_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        float m = -INFINITY, l = 0.0f;
-        auto step = [&](int s, Keys &y) {
+            for (int e = 0; e < VR; ++e) {
+                const T *const r = v + at.at_v(s, e);
+#pragma unroll
+                for (int c = 0; c < VB; ++c) {
+                    if (vw(c) == 8) load<16>(r + paged_dim(64 * c + 8 * li, 8, dim), y[e][c]);
+                    else if (vw(c) == 4) load<4 * (int)sizeof(T)>(r + paged_dim(64 * c + 4 * li, 4, dim), y[e][c]);
+                    else load<2 * (int)sizeof(T)>(r + paged_dim(64 * c + 2 * li, 2, dim), y[e][c]);
+                }
+            }
+        };
+        if (s0 < s1) {
+            at.ask_k(s0);
+            at.ask_v(s0);
+            load_k(s0);
+            load_v(s0);
+            at.ask_k(s0 + 1);
+            at.ask_v(s0 + 1);
+        }
+
+        // Q's fragments: those of row block f and slice g by one wave
+        for (int i = wave; i < RB * KS; i += NW) {
+            const int f = i / KS, g = i - f * KS, r = 16 * f + li;
+            const int i0 = min(r, rows - 1) / p.group, h = min(r, rows - 1) - i0 * p.group;
+            float q[KW];
+            paged_query(p.q + (seq.t0 + i0) * p.qs[0] + (kh * p.group + h) * p.qs[1], r < rows, 4 * KW * g + KW * lh, dim, p.scale_log2, q);
+            zn_u32x4 w[3];
+            if constexpr (BF) {
+                split8(q, w);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[0][e] = __builtin_bit_cast(uint32_t, q[e]);
+            }
+#pragma unroll
+            for (int part = 0; part < QP; ++part) *reinterpret_cast<zn_u32x4 *>(lds + (i * QP + part) * 1024 + lane * 16) = w[part];
+        }
+        int lim[RB];
+#pragma unroll
+        for (int f = 0; f < RB; ++f) lim[f] = 16 * f + li < rows ? min(paged_seen(p, seq, (16 * f + li) / p.group), to) : 0;
+        __syncthreads();
+
+        zn_f32x4 o[RB][G];
+        float m[RB], l[RB];
+#pragma unroll
+        for (int f = 0; f < RB; ++f) {
+            m[f] = -INFINITY;
+            l[f] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < G; ++c) o[f][c] = zn_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        for (int s = s0; s < s1; ++s) {
 #pragma unroll
             for (int rb = 0; rb < KB; ++rb)
 #pragma unroll
                 for (int g = 0; g + 1 < KS; g += 2)
-                    if (WHOLE) swap(y.k[rb][g], y.k[rb][g + 1]);
-            zn_f32x4 t[KB];
-            if constexpr (BF) {
+                    if (WHOLE) swap(x[rb][g], x[rb][g + 1]);
+            uint32_t qat = lane * 16;  // read again in each step: kept in registers, Q would cost a wave of every SIMD
+            asm volatile("" : "+v"(qat));
+            const char *const query = lds + qat;
+            zn_f32x4 t[RB][KB];
 #pragma unroll
-                for (int rb = 0; rb < KB; ++rb) t[rb] = zn_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int f = 0; f < RB; ++f) {
+                if constexpr (BF) {
 #pragma unroll
-                for (int part = 2; part >= 0; --part)  // the largest last
+                    for (int rb = 0; rb < KB; ++rb) t[f][rb] = zn_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (int g = 0; g < KS; ++g)
+                    for (int part = 2; part >= 0; --part)  // the largest last
 #pragma unroll
-                        for (int rb = 0; rb < KB; ++rb)
-                            t[rb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(zn_bf16x8, y.k[rb][g]), qf[g][part], t[rb], 0, 0, 0);
+                        for (int g = 0; g < KS; ++g) {
+                            const zn_bf16x8 q = __builtin_bit_cast(zn_bf16x8, *reinterpret_cast<const zn_u32x4 *>(query + ((f * KS + g) * 3 + part) * 1024));
 #pragma unroll
-                for (int rb = 0; rb < KB; ++rb) t[rb] *= kPagedUnscale;
-            } else {
-                zn_f32x4 u[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+                            for (int rb = 0; rb < KB; ++rb)
+                                t[f][rb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(zn_bf16x8, x[rb][g]), q, t[f][rb], 0, 0, 0);
+                        }
 #pragma unroll
-                for (int g = 0; g < KS; ++g)
+                    for (int rb = 0; rb < KB; ++rb) t[f][rb] *= kPagedUnscale;
+                } else {
+                    zn_f32x4 u[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        u[e & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, (uint32_t)y.k[0][g][e]), q[g][e], u[e & 1], 0, 0, 0);
-                t[0] = u[0] + u[1];
+                    for (int g = 0; g < KS; ++g) {
+                        const zn_f32x4 q = *reinterpret_cast<const zn_f32x4 *>(query + (f * KS + g) * 1024);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            u[e & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, (uint32_t)x[0][g][e]), q[e], u[e & 1], 0, 0, 0);
+                    }
+                    t[f][0] = u[0] + u[1];
+                }
             }
-            float mb = -INFINITY;
-#pragma unroll
-            for (int e = 0; e < VR; ++e) {
-                if (from + STEP * s + 16 * (e / 4) + 4 * lh + e % 4 >= min(lim, to)) t[e / 4][e % 4] = -INFINITY;
-                mb = fmaxf(mb, t[e / 4][e % 4]);
-            }
-            const float mn = fmaxf(m, max_over_rows(mb)), ref = mn == -INFINITY ? 0.0f : mn;
-            const float alpha = __builtin_amdgcn_exp2f(m - ref);
-            float rs = 0.0f, x[VR];
-#pragma unroll
-            for (int e = 0; e < VR; ++e) {
-                x[e] = __builtin_amdgcn_exp2f(t[e / 4][e % 4] - ref);
-                rs += x[e];
-            }
-            l = l * alpha + rs;
-            m = mn;
-#pragma unroll
-            for (int c = 0; c < G; ++c) o[c] *= alpha;
-            if constexpr (BF) {
-#pragma unroll
-                for (int e = 0; e < VR; ++e) x[e] *= kSplitScale;
-                zn_bf16x8 pf[3];
-                mha_split8(x, pf);
+            // Behind the last step: its last key, which no load goes to memory for, and no branch splits the loop's body.  The barriers
+            // keep the loads here: left alone the compiler asks for the next step's K and V together at the end.
+            __builtin_amdgcn_sched_barrier(0);
+            load_k(s + 1);
+            at.ask_k(s + 2);
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (BF) {  // the first and the second dim of each pair, of 8 keys
 #pragma unroll
                 for (int c = 0; c < VB; ++c)
 #pragma unroll
-                    for (int w = 0; w < vw(c) / 2; ++w) {
-                        zn_u32x4 lo, hi;  // the pair's first and second dim of 8 keys
+                    for (int w = 0; w < vw(c) / 2; ++w)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            lo[e] = __builtin_amdgcn_perm(y.v[2 * e + 1][c][w], y.v[2 * e][c][w], 0x05040100u);
-                            hi[e] = __builtin_amdgcn_perm(y.v[2 * e + 1][c][w], y.v[2 * e][c][w], 0x07060302u);
+                        for (int e = 0; e < VR; e += 2) {
+                            const uint32_t a = y[e][c][w], b = y[e + 1][c][w];
+                            y[e][c][w] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+                            y[e + 1][c][w] = __builtin_amdgcn_perm(b, a, 0x07060302u);
                         }
-                        const int i = 4 * c + 2 * w;
-#pragma unroll
-                        for (int part = 2; part >= 0; --part) {
-                            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(zn_bf16x8, lo), pf[part], o[i], 0, 0, 0);
-                            o[i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(zn_bf16x8, hi), pf[part], o[i + 1], 0, 0, 0);
-                        }
-                    }
-            } else {
-#pragma unroll
-                for (int e = 0; e < VR; ++e)  // key 4 lh + e
-#pragma unroll
-                    for (int c = 0; c < VB; ++c)
-#pragma unroll
-                        for (int w = 0; w < vw(c); ++w)
-                            o[4 * c + w] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, y.v[e][c][w]), x[e], o[4 * c + w], 0, 0, 0);
             }
-        };
-        Keys x[2];
-        if (s0 < s1) {
-            pages(s0);
-            load_step(s0, x[0]);
-            pages(s0 + 1);
-        }
-        for (int s = s0; s < s1; s += 2) {
-            if (s + 1 < s1) {
-                load_step(s + 1, x[1]);
-                pages(s + 2);
-            }
-            step(s, x[0]);
-            if (s + 1 < s1) {
-                if (s + 2 < s1) {
-                    load_step(s + 2, x[0]);
-                    pages(s + 3);
+            const int k0 = from + STEP * s;
+#pragma unroll
+            for (int f = 0; f < RB; ++f) {
+                float mb = -INFINITY;
+#pragma unroll
+                for (int e = 0; e < VR; ++e) {
+                    if (k0 + 16 * (e / 4) + 4 * lh + e % 4 >= lim[f]) t[f][e / 4][e % 4] = -INFINITY;
+                    mb = fmaxf(mb, t[f][e / 4][e % 4]);
                 }
-                step(s + 1, x[1]);
+                const float mn = fmaxf(m[f], max_over_rows(mb)), ref = mn == -INFINITY ? 0.0f : mn;
+                const float alpha = __builtin_amdgcn_exp2f(m[f] - ref);
+                float rs = 0.0f, e8[VR];
+#pragma unroll
+                for (int e = 0; e < VR; ++e) {
+                    e8[e] = __builtin_amdgcn_exp2f(t[f][e / 4][e % 4] - ref);
+                    rs += e8[e];
+                }
+                l[f] = l[f] * alpha + rs;
+                m[f] = mn;
+#pragma unroll
+                for (int c = 0; c < G; ++c) o[f][c] *= alpha;
+                if constexpr (BF) {
+#pragma unroll
+                    for (int e = 0; e < VR; ++e) e8[e] *= kSplitScale;
+                    zn_bf16x8 pf[3];
+                    mha_split8(e8, pf);
+#pragma unroll
+                    for (int part = 2; part >= 0; --part)
+#pragma unroll
+                        for (int c = 0; c < VB; ++c)
+#pragma unroll
+                            for (int w = 0; w < vw(c); ++w) {
+                                const zn_u32x4 a = {y[w % 2][c][w / 2], y[2 + w % 2][c][w / 2], y[4 + w % 2][c][w / 2], y[6 + w % 2][c][w / 2]};
+                                zn_f32x4 &z = o[f][4 * c + w];
+                                z = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(zn_bf16x8, a), pf[part], z, 0, 0, 0);
+                            }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < VR; ++e)  // key 4 lh + e
+#pragma unroll
+                        for (int c = 0; c < VB; ++c)
+#pragma unroll
+                            for (int w = 0; w < vw(c); ++w)
+                                o[f][4 * c + w] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, y[e][c][w]), e8[e], o[f][4 * c + w], 0, 0, 0);
+                }
             }
+            __builtin_amdgcn_sched_barrier(0);
+            load_v(s + 1);
+            at.ask_v(s + 2);
         }
-        l += __shfl_xor(l, 16);
-        l += __shfl_xor(l, 32);
         // a page that is none of the cache's, a sum that is not finite (also of a value in a pair masked for some rows only), or scores
         // that all fell below the split's range: the rows one by one
-        bool bad = hole || !(l < INFINITY) || (BF && m == -INFINITY && s0 < s1 && lim > from + STEP * s0);
+        bool bad = at.hole;
 #pragma unroll
-        for (int c = 0; c < G; ++c)
+        for (int f = 0; f < RB; ++f) {
+            l[f] += __shfl_xor(l[f], 16);
+            l[f] += __shfl_xor(l[f], 32);
+            bad |= !(l[f] < INFINITY) || (BF && m[f] == -INFINITY && s0 < s1 && lim[f] > from + STEP * s0);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                bad |= !(__builtin_fabsf(o[c][e]) < INFINITY);
-                if (BF) o[c][e] *= kPagedUnscale;
-            }
-        float *mine = reinterpret_cast<float *>(lds) + wave * 16 * kLd;  // [row][dims, maximum, sum]
-        if (__builtin_amdgcn_ballot_w64(bad)) {
-            for (int y = 0; y < rows; ++y) {
-                MhaRowState w;
-                paged_walk<T>(p, b, seq.t0 + y / p.group, kh * p.group + y % p.group, from + STEP * s0,
-                              min(min(from + STEP * s1, to), paged_seen(p, seq, y / p.group)), lane, w);
-                MhaRow::store(mine + y * kLd, dim, lane, w.oa, w.ob);
-                if (lane == 0) {
-                    mine[y * kLd + DP] = w.m;
-                    mine[y * kLd + DP + 1] = w.l;
-                }
-            }
-        } else {
-#pragma unroll
-            for (int c = 0; c < VB; ++c)
+            for (int c = 0; c < G; ++c)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int d = 64 * c + vw(c) * (4 * lh + e), to_d = paged_dim(d, vw(c), dim);
-#pragma unroll
-                    for (int w = 0; w < vw(c); ++w)
-                        if (to_d + w >= d) mine[li * kLd + to_d + w] = o[4 * c + w][e];
+                    bad |= !(__builtin_fabsf(o[f][c][e]) < INFINITY);
+                    if (BF) o[f][c][e] *= kPagedUnscale;
                 }
-            if (lh == 0) {
-                mine[li * kLd + DP] = m;
-                mine[li * kLd + DP + 1] = l;
-            }
         }
-        __syncthreads();
-        const float *sums = reinterpret_cast<const float *>(lds);
-        for (int y = wave; y < rows; y += NW) {  // a wave to a row, the waves' sums in order
-            float mx = -INFINITY, sl = 0.0f, oa = 0.0f, ob = 0.0f;
+        const bool one_by_one = __builtin_amdgcn_ballot_w64(bad);
+        float *mine = reinterpret_cast<float *>(lds) + wave * 16 * kLd;  // [row][dims, maximum, sum]
 #pragma unroll
-            for (int w = 0; w < NW; ++w) mx = fmaxf(mx, sums[(w * 16 + y) * kLd + DP]);
-            const float ref = mx == -INFINITY ? 0.0f : mx;
+        for (int f = 0; f < RB; ++f) {
+            if (16 * f >= rows) break;
+            __syncthreads();  // Q, or the last block's sums, are read
+            if (one_by_one) {
+                for (int i = 0; i < min(16, rows - 16 * f); ++i) {
+                    const int r = 16 * f + i;
+                    MhaRowState w;
+                    paged_walk<T>(p, b, seq.t0 + r / p.group, kh * p.group + r % p.group, from + STEP * s0,
+                                  min(end, paged_seen(p, seq, r / p.group)), lane, w);
+                    MhaRow::store(mine + i * kLd, dim, lane, w.oa, w.ob);
+                    if (lane == 0) {
+                        mine[i * kLd + DP] = w.m;
+                        mine[i * kLd + DP + 1] = w.l;
+                    }
+                }
+            } else {
 #pragma unroll
-            for (int w = 0; w < NW; ++w) {
-                const float *t = sums + (w * 16 + y) * kLd;
-                const float f = __builtin_amdgcn_exp2f(t[DP] - ref);
-                sl += f * t[DP + 1];
-                if (lane < dim) oa += f * t[lane];
-                if (lane + 64 < dim) ob += f * t[lane + 64];
+                for (int c = 0; c < VB; ++c)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int d = 64 * c + vw(c) * (4 * lh + e), to_d = paged_dim(d, vw(c), dim);
+#pragma unroll
+                        for (int w = 0; w < vw(c); ++w)
+                            if (to_d + w >= d) mine[li * kLd + to_d + w] = o[f][4 * c + w][e];
+                    }
+                if (lh == 0) {
+                    mine[li * kLd + DP] = m[f];
+                    mine[li * kLd + DP + 1] = l[f];
+                }
             }
-            float *part = parts > 1 ? p.few_part + (((int64_t)blockIdx.x * 16 + y) * p.few_splits + z) * p.part_ld : nullptr;
-            paged_finish(p, part, seq.t0 + y / p.group, kh * p.group + y % p.group, lane, mx, sl, oa, ob);
+            __syncthreads();
+            const float *sums = reinterpret_cast<const float *>(lds);
+            for (int i = wave; i < min(16, rows - 16 * f); i += NW) {  // a wave to a row, the waves' sums in order
+                float mx = -INFINITY, sl = 0.0f, oa = 0.0f, ob = 0.0f;
+#pragma unroll
+                for (int w = 0; w < NW; ++w) mx = fmaxf(mx, sums[(w * 16 + i) * kLd + DP]);
+                const float ref = mx == -INFINITY ? 0.0f : mx;
+#pragma unroll
+                for (int w = 0; w < NW; ++w) {
+                    const float *t = sums + (w * 16 + i) * kLd;
+                    const float f = __builtin_amdgcn_exp2f(t[DP] - ref);
+                    sl += f * t[DP + 1];
+                    if (lane < dim) oa += f * t[lane];
+                    if (lane + 64 < dim) ob += f * t[lane + 64];
+                }
+                const int r = 16 * f + i;
+                float *part = parts > 1 ? p.few_part + (((int64_t)blockIdx.x * p.few + r) * p.few_splits + z) * p.part_ld : nullptr;
+                paged_finish(p, part, seq.t0 + r / p.group, kh * p.group + r % p.group, lane, mx, sl, oa, ob);
+            }
         }
     }
 };
@@ -552,7 +612,7 @@ struct PagedTile {
         if (b < 0) return;
         const PagedSeq seq(p.c, b);
         const int rows = min(seq.ql, p.max_q) * p.group, tile = slot - seq.t0 * p.group / ROWS - b;
-        if (tile < 0 || tile >= (rows + ROWS - 1) / ROWS || (p.few && rows <= 16)) return;
+        if (tile < 0 || tile >= (rows + ROWS - 1) / ROWS || rows <= p.few) return;
         const int r0 = tile * ROWS;
         // keys that any row of the workgroup sees, its parts, this one's blocks
         const int last = paged_seen(p, seq, (min(r0 + ROWS, rows) - 1) / p.group);
@@ -565,9 +625,18 @@ struct PagedTile {
         zn_bf16x8 qf[FQ][SL][3];
 #pragma unroll
         for (int f = 0; f < FQ; ++f) {
-            const int r = w0 + 16 * f + li, i = r / p.group;
-            lim[f] = r < rows ? paged_seen(p, seq, i) : 0;
-            paged_query<SL>(lim[f] ? p.q + (seq.t0 + i) * p.qs[0] + (kh * p.group + r - i * p.group) * p.qs[1] : nullptr, dim, lh, p.scale_log2, qf[f]);
+            const int r = min(w0 + 16 * f + li, rows - 1), i = r / p.group;
+            lim[f] = w0 + 16 * f + li < rows ? paged_seen(p, seq, i) : 0;
+            const float *const row = p.q + (seq.t0 + i) * p.qs[0] + (kh * p.group + r - i * p.group) * p.qs[1];
+#pragma unroll
+            for (int sl = 0; sl < SL; ++sl) {
+                float x[8];
+                paged_query(row, lim[f] > 0, 32 * sl + 8 * lh, dim, p.scale_log2, x);
+                zn_u32x4 w[3];
+                split8(x, w);
+#pragma unroll
+                for (int q = 0; q < 3; ++q) qf[f][sl][q] = __builtin_bit_cast(zn_bf16x8, w[q]);
+            }
             all = min(all, lim[f]);
             any = max(any, lim[f]);
         }
@@ -774,16 +843,16 @@ __device__ __forceinline__ void paged_join(const ZnPagedArgs &p, const float *sr
 
 }  // namespace
 
-// Grid x: the rows of every sequence and key/value head, 16 each, four to a workgroup.
+// Grid x: the sequences' key/value heads, y: four rows each.
 extern "C" __global__ __launch_bounds__(256) void zn_paged_join_few(ZnPagedArgs p) {
-    const int lane = threadIdx.x & (kWave - 1), x = blockIdx.x / 4, y = blockIdx.x % 4 * 4 + threadIdx.x / kWave;
+    const int lane = threadIdx.x & (kWave - 1), x = blockIdx.x, y = blockIdx.y * 4 + threadIdx.x / kWave;
     const int b = x / p.c.kv_heads, kh = x - b * p.c.kv_heads;
     const PagedSeq seq(p.c, b);
     const int rows = min(seq.ql, p.max_q) * p.group;
-    if (rows > 16 || y >= rows) return;
+    if (rows > p.few || y >= rows) return;
     const int parts = paged_parts(paged_seen(p, seq, (rows - 1) / p.group), p.few_len);
     if (parts > 1)
-        paged_join(p, p.few_part + ((int64_t)x * 16 + y) * p.few_splits * p.part_ld, parts, seq.t0 + y / p.group, kh * p.group + y % p.group, lane);
+        paged_join(p, p.few_part + ((int64_t)x * p.few + y) * p.few_splits * p.part_ld, parts, seq.t0 + y / p.group, kh * p.group + y % p.group, lane);
 }
 
 // Grid x: the tokens, y: four heads each.  tile: the query rows of a tile.
@@ -793,7 +862,7 @@ __device__ __forceinline__ void paged_join_tiles(const ZnPagedArgs &p, int tile)
     if (b < 0 || b >= p.c.batch || h >= p.q_heads) return;
     const PagedSeq seq(p.c, b);
     const int i = t - seq.t0, rows = min(seq.ql, p.max_q) * p.group;
-    if (i < 0 || i * p.group >= rows || (p.few && rows <= 16)) return;
+    if (i < 0 || i * p.group >= rows || rows <= p.few) return;
     const int r0 = (i * p.group + h % p.group) / tile * tile;
     const int parts = paged_parts(paged_seen(p, seq, (min(r0 + tile, rows) - 1) / p.group), p.tile_len);
     if (parts > 1) paged_join(p, p.tile_part + ((int64_t)t * p.q_heads + h) * p.tile_splits * p.part_ld, parts, t, h, lane);
@@ -810,10 +879,17 @@ extern "C" __global__ __launch_bounds__(256) void zn_paged_rows_bf16(ZnPagedArgs
         __shared__ __attribute__((aligned(1024))) char lds[K::kBytes];             \
         K::run(p, lds);                                                            \
     }
+// Pages whose size is a multiple of 16 (_p), any.
+#define ZN_PAGED_FEW(DP, TYPE, T, RB, N)                                                      \
+    ZN_PAGED_KERNEL(zn_paged_few##N##_##TYPE##_##DP##_p, 4, PagedFew<T, DP, 4, RB, true>)     \
+    ZN_PAGED_KERNEL(zn_paged_few##N##_##TYPE##_##DP, 4, PagedFew<T, DP, 4, RB, false>)
 // NW waves of F blocks of 16 rows.
 #define ZN_PAGED_KERNELS(DP, NW, F, BNW, BF)                                       \
-    ZN_PAGED_KERNEL(zn_paged_few_f32_##DP, 4, PagedFew<float, DP, 4>)              \
-    ZN_PAGED_KERNEL(zn_paged_few_bf16_##DP, 4, PagedFew<__bf16, DP, 4>)            \
+    ZN_PAGED_FEW(DP, f32, float, 1, )                                              \
+    ZN_PAGED_FEW(DP, f32, float, 2, 2)                                             \
+    ZN_PAGED_FEW(DP, bf16, __bf16, 1, )                                            \
+    ZN_PAGED_FEW(DP, bf16, __bf16, 2, 2)                                           \
+    ZN_PAGED_FEW(DP, bf16, __bf16, 4, 4)                                           \
     ZN_PAGED_KERNEL(zn_paged_tile_f32_##DP, NW, PagedTile<float, DP, NW, F>)       \
     ZN_PAGED_KERNEL(zn_paged_tile_bf16_##DP, BNW, PagedTile<__bf16, DP, BNW, BF>)
 ZN_PAGED_KERNELS(32, 4, 2, 4, 2)

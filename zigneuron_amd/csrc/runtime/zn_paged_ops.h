@@ -149,6 +149,7 @@ int paged_args(const zn_paged_cache *c, ZnPagedCache &a, const void *starts, int
         return ZN_ERR_OVERFLOW;
     for (int i = 0; i < 3; ++i)
         if (stride_far(stride[i], extent[i])) return ZN_ERR_OVERFLOW;
+    if (c->stride_position > INT_MAX) return ZN_ERR_OVERFLOW;
     std::memset(&a, 0, sizeof(a));
     a.k = static_cast<char *>(c->k);
     a.v = static_cast<char *>(c->v);
@@ -295,15 +296,18 @@ int zn_hip_paged_attention(zn_ctx *ctx, const void *cache, const void *token_sta
     // a 16-byte load of bf16 takes 8 dims
     if (desc->head_dim < 8) return launch(ctx, ctx->paged_rows[type], (unsigned)tokens, (unsigned)cdiv(q_heads, 4), 256, &a);
     // Sequences of few query rows and those of many: both kernels where both may occur (each leaves the other's alone).
-    const bool all_few = group * max_q_len <= 16, few = all_few || tokens < desc->batch * max_q_len;
-    a.few = few;
+    const int64_t most = type == ZN_CACHE_BF16 ? 64 : 32, rows = group * max_q_len;
+    const bool all_few = rows <= most, few = all_few || (group <= most && tokens < desc->batch * max_q_len);
+    int kernel = 0;
+    while (kernel < 2 && kPagedFewRows[kernel] < (all_few ? rows : group)) ++kernel;
+    a.few = few ? kPagedFewRows[kernel] : 0;
     a.part_ld = (int32_t)(desc->head_dim + 3) / 4 * 4 + 4;
     const int64_t few_heads = desc->batch * desc->kv_heads;
     paged_few_parts(ctx, a, few_heads, type);
     if (!all_few) paged_tile_parts(ctx, a, tokens, max_q_len, tile, type, kPagedThreads[type][dims] == 256 ? 2 : 1);
     Lease few_part(ctx), tile_part(ctx);
     if (few && a.few_splits > 1) {
-        if ((rc = few_part.get((size_t)(few_heads * 16) * a.few_splits * a.part_ld))) return rc;
+        if ((rc = few_part.get((size_t)(few_heads * a.few) * a.few_splits * a.part_ld))) return rc;
         a.few_part = few_part.ptr;
     }
     if (!all_few && a.tile_splits > 1) {
@@ -311,15 +315,15 @@ int zn_hip_paged_attention(zn_ctx *ctx, const void *cache, const void *token_sta
         a.tile_part = tile_part.ptr;
     }
     if (!all_few) {
-        if ((rc = launch(ctx, ctx->paged[kPagedTile][type][dims], (unsigned)(tiles * desc->kv_heads), 1, kPagedThreads[type][dims], &a,
+        if ((rc = launch(ctx, ctx->paged[kPagedTile][type][dims][0], (unsigned)(tiles * desc->kv_heads), 1, kPagedThreads[type][dims], &a,
                          (unsigned)a.tile_splits)))
             return rc;
         if (a.tile_splits > 1 && (rc = launch(ctx, ctx->paged_join[tile / 128], (unsigned)tokens, (unsigned)cdiv(q_heads, 4), 256, &a))) return rc;
     }
     if (!few) return ZN_OK;
-    if ((rc = launch(ctx, ctx->paged[kPagedFew][type][dims], (unsigned)few_heads, 1, 256, &a, (unsigned)a.few_splits)) || a.few_splits == 1)
+    if ((rc = launch(ctx, ctx->paged[kernel][type][dims][desc->page_size % 16 == 0], (unsigned)few_heads, 1, 256, &a, (unsigned)a.few_splits)) || a.few_splits == 1)
         return rc;
-    return launch(ctx, ctx->paged_join[0], (unsigned)(few_heads * 4), 1, 256, &a);
+    return launch(ctx, ctx->paged_join[0], (unsigned)few_heads, (unsigned)cdiv(std::min<int64_t>(a.few, rows), 4), 256, &a);
 }
 
 #endif

@@ -51,10 +51,10 @@ struct ZnPagedArgs {
     int64_t qs[2], os[2];
     int32_t q_heads, group, causal, max_q;  // max_q: rows of a sequence past it are not written
     float scale_log2;             // scale * log2(e)
-    // Sequences of at most 16 query rows of a key/value head (new tokens times group) are few, where `few` says so; the others
-    // go in tiles.  Either kind's positions are cut into parts of few_len, tile_len, at most few_splits, tile_splits of them
+    // Sequences of at most `few` query rows of a key/value head (new tokens times group) go to the kernels for few rows, the others
+    // in tiles.  Either kind's positions are cut into parts of few_len, tile_len, at most few_splits, tile_splits of them
     // (blockIdx.z), whose sums go to rows of part_ld floats: the dims, then the maximum and the sum.  few_part: part z of row y of
-    // sequence and key/value head x at (16 x + y) few_splits + z; tile_part: of token t and head h at (t q_heads + h) tile_splits + z.
+    // sequence and key/value head x at (few x + y) few_splits + z; tile_part: of token t and head h at (t q_heads + h) tile_splits + z.
     float *few_part, *tile_part;
     int32_t few, few_len, few_splits, tile_len, tile_splits, part_ld;
 };
