@@ -60,18 +60,56 @@ __device__ __forceinline__ void paged_store(const ZnPagedArgs &p, int t, int h, 
     if (p.lse && lane == 0) p.lse[(int64_t)t * p.q_heads + h] = mha_lse(m, l);
 }
 
-// A row's sums: to the tensor, or to its part.
+// A row's sums: to the tensor, or to its part (another XCD may read that in the same launch: agent-scope stores).
 __device__ __forceinline__ void paged_finish(const ZnPagedArgs &p, float *part, int t, int h, int lane, float m, float l, float oa, float ob) {
     if (!part) return paged_store(p, t, h, lane, m, l, oa, ob);
-    MhaRow::store(part, p.c.dim, lane, oa, ob);
-    if (lane == 0) {
-        part[p.part_ld - 4] = m;
-        part[p.part_ld - 3] = l;
+    auto put = [&](int i, float x) { __hip_atomic_store(part + i, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+    if (lane < p.c.dim) put(lane, oa);
+    if (lane + 64 < p.c.dim) put(lane + 64, ob);
+    if (lane < 2) put(p.part_ld - 4 + lane, lane ? l : m);
+}
+
+// A row's parts in order, a wave to a row, lane l its dims l and l + 64, sixteen parts' loads in flight.
+__device__ __forceinline__ void paged_join(const ZnPagedArgs &p, const float *src, int parts, int t, int h, int lane) {
+    constexpr int N = 16;
+    float mx = -INFINITY, sl = 0.0f, oa = 0.0f, ob = 0.0f;
+    for (int z0 = 0; z0 < parts; z0 += N) {
+        float x[N], y[N], m[N], l[N];
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+            const float *r = src + (int64_t)min(z0 + u, parts - 1) * p.part_ld;  // any of them: no load waits for a condition
+            auto get = [&](int i) { return __hip_atomic_load(r + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+            x[u] = get(min(lane, p.c.dim - 1));
+            y[u] = get(min(lane + 64, p.c.dim - 1));
+            m[u] = get(p.part_ld - 4);
+            l[u] = get(p.part_ld - 3);
+        }
+        float mn = mx;
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+            if (z0 + u >= parts) m[u] = -INFINITY, l[u] = x[u] = y[u] = 0.0f;
+            mn = fmaxf(mn, m[u]);
+        }
+        const float ref = mn == -INFINITY ? 0.0f : mn, alpha = __builtin_amdgcn_exp2f(mx - ref);
+        mx = mn;
+        sl *= alpha;
+        oa *= alpha;
+        ob *= alpha;
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+            const float f = __builtin_amdgcn_exp2f(m[u] - ref);
+            sl += f * l[u];
+            oa += f * x[u];
+            ob += f * y[u];
+        }
     }
+    paged_store(p, t, h, lane, mx, sl, oa, ob);
 }
 
 // Parts of a walk over `keys` positions: one at least.
 __device__ __forceinline__ int paged_parts(int keys, int len) { return max(1, (keys + len - 1) / len); }
+// ... of few rows: as many equal parts as the call has, in multiples of 128 (32 for each of four waves).
+__device__ __forceinline__ int paged_few_len(const ZnPagedArgs &p, int keys) { return 128 * max(1, (int)(((uint32_t)keys + 128u * p.few_splits - 1) / (128u * p.few_splits))); }
 
 // Rows one at a time, a wave each: grid x the tokens, y four heads.  For heads of fewer dims than a 16-byte load of bf16 has.
 template <typename T>
@@ -211,19 +249,20 @@ struct PagedFew {
         __device__ __forceinline__ int64_t at_v(int s, int e) { return at(s, e / 4, vp[PAGES16 ? e / 4 : e], key_v(e)); }
     };
 
-    __device__ static __forceinline__ void run(const ZnPagedArgs &p, char *lds) {
+    // Sequence and key/value head x, part z of its walk.
+    __device__ static __forceinline__ void run(const ZnPagedArgs &p, char *lds, int x_, int z) {
         const int tid = threadIdx.x, lane = tid & (kWave - 1);
         const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
         const int li = lane & 15, lh = lane >> 4;
-        const int b = blockIdx.x / p.c.kv_heads, kh = blockIdx.x - b * p.c.kv_heads, dim = p.c.dim;
+        const int b = x_ / p.c.kv_heads, kh = x_ - b * p.c.kv_heads, dim = p.c.dim;
         const PagedSeq seq(p.c, b);
         const int rows = min(seq.ql, p.max_q) * p.group;
         if (rows == 0 || rows > ROWS) return;
         const int any = __builtin_amdgcn_readfirstlane(paged_seen(p, seq, (rows - 1) / p.group));
-        const int parts = paged_parts(any, p.few_len), z = blockIdx.z;
+        const int len = paged_few_len(p, any), parts = paged_parts(any, len);
         if (z >= parts) return;
         // the wave's share of the part's keys, whole steps
-        const int from = z * p.few_len, to = min(from + p.few_len, any);
+        const int from = z * len, to = min(from + len, any);
         const int steps = (to - from + STEP - 1) / STEP, share = (steps + NW - 1) / NW;
         const int s0 = min(wave * share, steps), s1 = min(s0 + share, steps), end = min(from + STEP * s1, to);
 
@@ -471,10 +510,21 @@ struct PagedFew {
                     if (lane + 64 < dim) ob += f * t[lane + 64];
                 }
                 const int r = 16 * f + i;
-                float *part = parts > 1 ? p.few_part + (((int64_t)blockIdx.x * p.few + r) * p.few_splits + z) * p.part_ld : nullptr;
+                float *part = parts > 1 ? p.few_part + (((int64_t)x_ * p.few + r) * p.few_splits + z) * p.part_ld : nullptr;
                 paged_finish(p, part, seq.t0 + r / p.group, kh * p.group + r % p.group, lane, mx, sl, oa, ob);
             }
         }
+        if (!p.counters || parts == 1) return;
+        // the workgroup that arrives last, whichever it is, joins the parts in their order and sets the counter back
+        __shared__ int last;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the wave's rows are written
+        __syncthreads();
+        if (tid == 0) last = __hip_atomic_fetch_add(p.counters + x_ * kCounterStride, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
+        __syncthreads();
+        if (!last) return;
+        if (tid == 0) __hip_atomic_store(p.counters + x_ * kCounterStride, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        for (int r = wave; r < rows; r += NW)
+            paged_join(p, p.few_part + ((int64_t)x_ * p.few + r) * p.few_splits * p.part_ld, parts, seq.t0 + r / p.group, kh * p.group + r % p.group, lane);
     }
 };
 
@@ -487,8 +537,11 @@ struct PagedFew {
 //    before the row, the row a block before its use.  fp32 rows are split there
 //    (three parts), bf16 ones are operands as they lie (one part): six products
 //    for one of fp32, or three.
-//  - The tiles of all sequences are one range: sequence b's begin at
-//    starts[b] group / rows + b, which leaves each as many as it may need.
+//  - The parts of all sequences' tiles are one range without gaps, and few rows of
+//    other sequences follow it: where each part of each tile had a place of its own,
+//    the gaps fell on the same XCDs or shader engines each time and left them idle (4
+//    x 32 tokens of 16 (4) x 128 over 2048, in 12 parts: 52 us, 32 so).  The workgroups
+//    that the host could not know to be too many come last.
 template <int DP, int NP>
 struct PagedFrags {
     typedef MhaBlock<DP> B;
@@ -596,27 +649,47 @@ struct PagedTile {
         }
     };
 
-    // Tile blockIdx.x / kv_heads from the last on (late tiles of a sequence see more keys), part blockIdx.z of its walk.
-    __device__ static __forceinline__ void run(const ZnPagedArgs &p, char *lds) {
+    // The sequence whose tiles' parts hold number `slot`, and which of them it is; or -1 and how many there are.  Those of 64 sequences
+    // are summed at a time.
+    __device__ static __forceinline__ int find(const ZnPagedArgs &p, int slot, int &at) {
+        const int lane = threadIdx.x & (kWave - 1);
+        int before = 0;
+        for (int i0 = 0; i0 < p.c.batch; i0 += 64) {
+            int own = 0;
+            if (i0 + lane < p.c.batch) {
+                const PagedSeq s(p.c, i0 + lane);
+                const int n = min(s.ql, p.max_q), r = n * p.group;
+                if (r > p.few) own = (r + ROWS - 1) / ROWS * paged_parts(paged_seen(p, s, n - 1), p.tile_len);
+            }
+            int sum = own;
+#pragma unroll
+            for (int s = 1; s < 64; s <<= 1) {
+                const int y = __shfl_up(sum, s);
+                if (lane >= s) sum += y;
+            }
+            const int n = __builtin_popcountll(__builtin_amdgcn_ballot_w64(before + sum <= slot));
+            if (n < 64) {
+                at = __builtin_amdgcn_readfirstlane(slot - before - __shfl(sum - own, n));
+                return __builtin_amdgcn_readfirstlane(i0 + n);
+            }
+            before += __shfl(sum, 63);
+        }
+        at = __builtin_amdgcn_readfirstlane(before);
+        return -1;
+    }
+
+    // Key/value head kh, part `at` of sequence b's tiles.
+    __device__ static __forceinline__ void run(const ZnPagedArgs &p, char *lds, int kh, int b, int at) {
         const int tid = threadIdx.x, lane = tid & (kWave - 1);
         const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
         const int li = lane & 15, lh = lane >> 4, dim = p.c.dim;
-        const int all_tiles = gridDim.x / p.c.kv_heads, y = blockIdx.x / p.c.kv_heads, kh = blockIdx.x - y * p.c.kv_heads, slot = all_tiles - 1 - y;
-        int b = -1;
-        for (int i0 = 0; i0 < p.c.batch; i0 += 64) {
-            const int i = min(i0 + lane, p.c.batch - 1);
-            const uint64_t at = __builtin_amdgcn_ballot_w64(i0 + lane < p.c.batch && paged_clamp(p.c.starts[i], 0, p.c.tokens) * p.group / ROWS + i <= slot);
-            b += __builtin_popcountll(at);
-            if (~at) break;
-        }
-        if (b < 0) return;
         const PagedSeq seq(p.c, b);
-        const int rows = min(seq.ql, p.max_q) * p.group, tile = slot - seq.t0 * p.group / ROWS - b;
-        if (tile < 0 || tile >= (rows + ROWS - 1) / ROWS || rows <= p.few) return;
-        const int r0 = tile * ROWS;
+        // part z of the tile; a sequence's last tiles first, which see more keys
+        const int rows = min(seq.ql, p.max_q) * p.group, tiles = (rows + ROWS - 1) / ROWS, z = at / tiles;
+        const int r0 = __builtin_amdgcn_readfirstlane(tiles - 1 - (at - z * tiles)) * ROWS;
         // keys that any row of the workgroup sees, its parts, this one's blocks
         const int last = paged_seen(p, seq, (min(r0 + ROWS, rows) - 1) / p.group);
-        const int parts = paged_parts(last, p.tile_len), z = blockIdx.z;
+        const int parts = paged_parts(last, p.tile_len);
         if (z >= parts) return;
         const int blk0 = __builtin_amdgcn_readfirstlane(z * p.tile_len / 32), nblk = __builtin_amdgcn_readfirstlane((min((z + 1) * p.tile_len, last) + 31) / 32);
 
@@ -805,96 +878,72 @@ struct PagedTile {
     }
 };
 
-// ------------------------------------------------------------------ the join
-// A row's parts in order, a wave to a row, lane l its dims l and l + 64, eight parts' loads in flight.
-__device__ __forceinline__ void paged_join(const ZnPagedArgs &p, const float *src, int parts, int t, int h, int lane) {
-    float mx = -INFINITY, sl = 0.0f, oa = 0.0f, ob = 0.0f;
-    for (int z0 = 0; z0 < parts; z0 += 8) {
-        float x[8], y[8], m[8], l[8];
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            const float *r = src + (int64_t)min(z0 + u, parts - 1) * p.part_ld;  // any of them: no load waits for a condition
-            x[u] = r[min(lane, p.c.dim - 1)];
-            y[u] = r[min(lane + 64, p.c.dim - 1)];
-            m[u] = r[p.part_ld - 4];
-            l[u] = r[p.part_ld - 3];
-        }
-        float mn = mx;
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            if (z0 + u >= parts) m[u] = -INFINITY, l[u] = x[u] = y[u] = 0.0f;
-            mn = fmaxf(mn, m[u]);
-        }
-        const float ref = mn == -INFINITY ? 0.0f : mn, alpha = __builtin_amdgcn_exp2f(mx - ref);
-        mx = mn;
-        sl *= alpha;
-        oa *= alpha;
-        ob *= alpha;
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            const float f = __builtin_amdgcn_exp2f(m[u] - ref);
-            sl += f * l[u];
-            oa += f * x[u];
-            ob += f * y[u];
-        }
-    }
-    paged_store(p, t, h, lane, mx, sl, oa, ob);
-}
-
 }  // namespace
 
-// Grid x: the sequences' key/value heads, y: four rows each.
-extern "C" __global__ __launch_bounds__(256) void zn_paged_join_few(ZnPagedArgs p) {
-    const int lane = threadIdx.x & (kWave - 1), x = blockIdx.x, y = blockIdx.y * 4 + threadIdx.x / kWave;
-    const int b = x / p.c.kv_heads, kh = x - b * p.c.kv_heads;
-    const PagedSeq seq(p.c, b);
-    const int rows = min(seq.ql, p.max_q) * p.group;
-    if (rows > p.few || y >= rows) return;
-    const int parts = paged_parts(paged_seen(p, seq, (rows - 1) / p.group), p.few_len);
-    if (parts > 1)
-        paged_join(p, p.few_part + ((int64_t)x * p.few + y) * p.few_splits * p.part_ld, parts, seq.t0 + y / p.group, kh * p.group + y % p.group, lane);
-}
-
-// Grid x: the tokens, y: four heads each.  tile: the query rows of a tile.
-__device__ __forceinline__ void paged_join_tiles(const ZnPagedArgs &p, int tile) {
+// The join of rows that are in parts.  Grid x: the tokens, y: four heads each.
+extern "C" __global__ __launch_bounds__(256) void zn_paged_join(ZnPagedArgs p) {
     const int lane = threadIdx.x & (kWave - 1), t = blockIdx.x, h = blockIdx.y * 4 + threadIdx.x / kWave;
     const int b = paged_find(p.c, t);
     if (b < 0 || b >= p.c.batch || h >= p.q_heads) return;
     const PagedSeq seq(p.c, b);
-    const int i = t - seq.t0, rows = min(seq.ql, p.max_q) * p.group;
-    if (i < 0 || i * p.group >= rows || rows <= p.few) return;
-    const int r0 = (i * p.group + h % p.group) / tile * tile;
-    const int parts = paged_parts(paged_seen(p, seq, (min(r0 + tile, rows) - 1) / p.group), p.tile_len);
-    if (parts > 1) paged_join(p, p.tile_part + ((int64_t)t * p.q_heads + h) * p.tile_splits * p.part_ld, parts, t, h, lane);
+    const int kh = h / p.group, rows = min(seq.ql, p.max_q) * p.group, r = (t - seq.t0) * p.group + h - kh * p.group;
+    if (t < seq.t0 || r >= rows) return;
+    if (rows <= p.few) {
+        const int any = paged_seen(p, seq, (rows - 1) / p.group), parts = paged_parts(any, paged_few_len(p, any));
+        if (parts > 1) paged_join(p, p.few_part + (((int64_t)b * p.c.kv_heads + kh) * p.few + r) * p.few_splits * p.part_ld, parts, t, h, lane);
+    } else {
+        const int parts = paged_parts(paged_seen(p, seq, (min((r / p.tile + 1) * p.tile, rows) - 1) / p.group), p.tile_len);
+        if (parts > 1) paged_join(p, p.tile_part + ((int64_t)t * p.q_heads + h) * p.tile_splits * p.part_ld, parts, t, h, lane);
+    }
 }
-extern "C" __global__ __launch_bounds__(256) void zn_paged_join_128(ZnPagedArgs p) { paged_join_tiles(p, 128); }
-extern "C" __global__ __launch_bounds__(256) void zn_paged_join_256(ZnPagedArgs p) { paged_join_tiles(p, 256); }
 
 extern "C" __global__ __launch_bounds__(256) void zn_paged_rows_f32(ZnPagedArgs p) { paged_rows<float>(p); }
 extern "C" __global__ __launch_bounds__(256) void zn_paged_rows_bf16(ZnPagedArgs p) { paged_rows<__bf16>(p); }
 
-#define ZN_PAGED_KERNEL(NAME, NW, ...)                                             \
+#define ZN_PAGED_KERNEL(NAME, NW, BYTES, ...)                                      \
     extern "C" __global__ __launch_bounds__(NW * 64, 2) void NAME(ZnPagedArgs p) { \
-        typedef __VA_ARGS__ K;                                                     \
-        __shared__ __attribute__((aligned(1024))) char lds[K::kBytes];             \
-        K::run(p, lds);                                                            \
+        __shared__ __attribute__((aligned(1024))) char lds[BYTES];                 \
+        __VA_ARGS__;                                                               \
     }
-// Pages whose size is a multiple of 16 (_p), any.
-#define ZN_PAGED_FEW(DP, TYPE, T, RB, N)                                                      \
-    ZN_PAGED_KERNEL(zn_paged_few##N##_##TYPE##_##DP##_p, 4, PagedFew<T, DP, 4, RB, true>)     \
-    ZN_PAGED_KERNEL(zn_paged_few##N##_##TYPE##_##DP, 4, PagedFew<T, DP, 4, RB, false>)
-// NW waves of F blocks of 16 rows.
-#define ZN_PAGED_KERNELS(DP, NW, F, BNW, BF)                                       \
-    ZN_PAGED_FEW(DP, f32, float, 1, )                                              \
-    ZN_PAGED_FEW(DP, f32, float, 2, 2)                                             \
-    ZN_PAGED_FEW(DP, bf16, __bf16, 1, )                                            \
-    ZN_PAGED_FEW(DP, bf16, __bf16, 2, 2)                                           \
-    ZN_PAGED_FEW(DP, bf16, __bf16, 4, 4)                                           \
-    ZN_PAGED_KERNEL(zn_paged_tile_f32_##DP, NW, PagedTile<float, DP, NW, F>)       \
-    ZN_PAGED_KERNEL(zn_paged_tile_bf16_##DP, BNW, PagedTile<__bf16, DP, BNW, BF>)
-ZN_PAGED_KERNELS(32, 4, 2, 4, 2)
-ZN_PAGED_KERNELS(64, 4, 2, 4, 2)
-ZN_PAGED_KERNELS(96, 8, 2, 4, 2)
-ZN_PAGED_KERNELS(128, 8, 2, 4, 2)
+// Few rows: grid x the sequences' key/value heads, z the parts.  P: pages whose size is a multiple of 16 (_p), any.
+#define ZN_PAGED_FEW(NAME, ...)                                                                          \
+    typedef PagedFew<__VA_ARGS__> NAME##_k;                                                             \
+    ZN_PAGED_KERNEL(NAME, 4, NAME##_k::kBytes, NAME##_k::run(p, lds, blockIdx.x, blockIdx.z))
+// NW waves of F blocks of 16 rows: the tiles' parts, then the parts of few rows.
+#define ZN_PAGED_TILE(NAME, T, DP, NW, F, P)                                                             \
+    typedef PagedTile<T, DP, NW, F> NAME##_k;                                                           \
+    typedef PagedFew<T, DP, NW, 1, P> NAME##_f;                                                         \
+    ZN_PAGED_KERNEL(NAME, NW, (NAME##_k::kBytes > NAME##_f::kBytes ? NAME##_k::kBytes : NAME##_f::kBytes), \
+                    const int slot = blockIdx.x / p.c.kv_heads;                                         \
+                    int at;                                                                             \
+                    const int b = NAME##_k::find(p, slot, at);                                          \
+                    if (b >= 0) return NAME##_k::run(p, lds, blockIdx.x - slot * p.c.kv_heads, b, at);  \
+                    const int x = (int)blockIdx.x - at * p.c.kv_heads;                                  \
+                    if (p.few && x < p.few_heads * p.few_splits) NAME##_f::run(p, lds, x % p.few_heads, x / p.few_heads))
+#define ZN_PAGED_KERNELS(DP, S, P)                                        \
+    ZN_PAGED_FEW(zn_paged_few_f32_##DP##S, float, DP, 4, 1, P)            \
+    ZN_PAGED_FEW(zn_paged_few2_f32_##DP##S, float, DP, 4, 2, P)           \
+    ZN_PAGED_FEW(zn_paged_few_bf16_##DP##S, __bf16, DP, 4, 1, P)          \
+    ZN_PAGED_FEW(zn_paged_few2_bf16_##DP##S, __bf16, DP, 4, 2, P)         \
+    ZN_PAGED_FEW(zn_paged_few4_bf16_##DP##S, __bf16, DP, 4, 4, P)
+#define ZN_PAGED_TILES(DP, NW, F, WNW, WF, BNW, BF, VNW, VF, S, P)        \
+    ZN_PAGED_TILE(zn_paged_tile_f32_##DP##S, float, DP, NW, F, P)         \
+    ZN_PAGED_TILE(zn_paged_wide_f32_##DP##S, float, DP, WNW, WF, P)       \
+    ZN_PAGED_TILE(zn_paged_tile_bf16_##DP##S, __bf16, DP, BNW, BF, P)     \
+    ZN_PAGED_TILE(zn_paged_wide_bf16_##DP##S, __bf16, DP, VNW, VF, P)
+ZN_PAGED_KERNELS(32, , false)
+ZN_PAGED_KERNELS(32, _p, true)
+ZN_PAGED_KERNELS(64, , false)
+ZN_PAGED_KERNELS(64, _p, true)
+ZN_PAGED_KERNELS(96, , false)
+ZN_PAGED_KERNELS(96, _p, true)
+ZN_PAGED_KERNELS(128, , false)
+ZN_PAGED_KERNELS(128, _p, true)
+#define ZN_PAGED_TILES2(...) ZN_PAGED_TILES(__VA_ARGS__, , false) ZN_PAGED_TILES(__VA_ARGS__, _p, true)
+// dims; fp32 pages: waves and blocks of 16 rows of tiles of 128 rows, of 256; bf16 pages: the same
+ZN_PAGED_TILES2(32, 4, 2, 8, 2, 4, 2, 8, 2)
+ZN_PAGED_TILES2(64, 4, 2, 8, 2, 4, 2, 8, 2)
+ZN_PAGED_TILES2(96, 8, 1, 8, 2, 4, 2, 8, 2)
+ZN_PAGED_TILES2(128, 8, 1, 8, 2, 4, 2, 8, 2)
 
 #endif

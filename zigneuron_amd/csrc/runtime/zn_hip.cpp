@@ -108,14 +108,12 @@ constexpr int kMhaRows[kNumMha][4] = {{16, 16, 16, 16}, {128, 128, 128, 128}, {0
 constexpr unsigned kMhaThreads[kNumMha][4] = {{256, 256, 256, 256}, {256, 256, 512, 512}, {0, 0, 512, 512}, {256, 256, 512, 512}, {256, 256, 256, 512}, {256, 256, 256, 256}};
 
 // Attention over a paged cache (kernels/paged_f32.h), in the attention code object: zn_paged_<what>_<cache type>_<padded head dim>.
-enum PagedKernel { kPagedFew, kPagedFew2, kPagedFew4, kPagedTile, kNumPaged };
-constexpr const char *kPagedName[kNumPaged] = {"zn_paged_few", "zn_paged_few2", "zn_paged_few4", "zn_paged_tile"};
-constexpr int kPagedFewRows[3] = {16, 32, 64};  // query rows that the first three take
-constexpr const char *kPagedJoinName[3] = {"zn_paged_join_few", "zn_paged_join_128", "zn_paged_join_256"};
+enum PagedKernel { kPagedFew, kPagedFew2, kPagedFew4, kPagedTile, kPagedWide, kNumPaged };
+constexpr const char *kPagedName[kNumPaged] = {"zn_paged_few", "zn_paged_few2", "zn_paged_few4", "zn_paged_tile", "zn_paged_wide"};
+constexpr int kPagedRows[kNumPaged] = {16, 32, 64, 128, 256};  // query rows of a workgroup
 constexpr const char *kCacheName[2] = {"f32", "bf16"};
-// Query rows and threads of a tile's workgroup [cache type][dims in 32s].
-constexpr int kPagedRows[2][4] = {{128, 128, 256, 256}, {128, 128, 128, 128}};
-constexpr unsigned kPagedThreads[2][4] = {{256, 256, 512, 512}, {256, 256, 256, 256}};
+// Threads of a tile's workgroup [kPagedTile, kPagedWide][cache type][dims in 32s]; the others have 256.
+constexpr unsigned kPagedThreads[2][2][4] = {{{256, 256, 512, 512}, {256, 256, 256, 256}}, {{512, 512, 512, 512}, {512, 512, 512, 512}}};
 
 struct ScratchDevice;
 
@@ -202,7 +200,7 @@ struct zn_ctx {
     hipFunction_t mha_join = nullptr;          // adds up its splits
     hipFunction_t paged_rows[2] = {};          // attention over a paged cache [cache type]
     hipFunction_t paged[kNumPaged][2][4][2] = {};  // ... [kernel][cache type][head dim 32/64/96/128][any pages, multiples of 16]
-    hipFunction_t paged_join[3] = {};          // adds up its parts [few, tiles of 128 rows, of 256]
+    hipFunction_t paged_join = nullptr;        // adds up its parts
     hipFunction_t gated[4] = {};               // gated Dense forward [sw, sx, sr, sn]
     hipFunction_t gated_few = nullptr, gated_few_join = nullptr;  // ... of at most 16 rows
     hipFunction_t gemm[3][kNumTiles][3] = {};  // [layout][tile][staging: 4-byte, 16-byte, 16-byte unaligned (r only)]
@@ -2041,14 +2039,13 @@ int zn_hip_create(int device, const char *code_object_dir, zn_ctx **out) {
         if (hipModuleGetFunction(&ctx->paged_rows[type], ctx->attn_module, name) != hipSuccess) return bail(ZN_ERR_SYMBOL);
         for (int i = 0; i < kNumPaged; ++i)
             for (int d = 0; d < 4; ++d)
-                for (int pages = 0; pages < (i == kPagedTile ? 1 : 2); ++pages) {
+                for (int pages = 0; pages < 2; ++pages) {
                     if (i == kPagedFew4 && type == ZN_CACHE_F32) continue;
                     std::snprintf(name, sizeof(name), "%s_%s_%d%s", kPagedName[i], kCacheName[type], 32 * (d + 1), pages ? "_p" : "");
                     if (hipModuleGetFunction(&ctx->paged[i][type][d][pages], ctx->attn_module, name) != hipSuccess) return bail(ZN_ERR_SYMBOL);
                 }
     }
-    for (int i = 0; i < 3; ++i)
-        if (hipModuleGetFunction(&ctx->paged_join[i], ctx->attn_module, kPagedJoinName[i]) != hipSuccess) return bail(ZN_ERR_SYMBOL);
+    if (hipModuleGetFunction(&ctx->paged_join, ctx->attn_module, "zn_paged_join") != hipSuccess) return bail(ZN_ERR_SYMBOL);
     void *counters = nullptr;
     if ((e = hipMalloc(&counters, kCounterSlots * kCounterStride * sizeof(int32_t))) != hipSuccess) {
         (void)hipGetLastError();

@@ -52,11 +52,14 @@ struct ZnPagedArgs {
     int32_t q_heads, group, causal, max_q;  // max_q: rows of a sequence past it are not written
     float scale_log2;             // scale * log2(e)
     // Sequences of at most `few` query rows of a key/value head (new tokens times group) go to the kernels for few rows, the others
-    // in tiles.  Either kind's positions are cut into parts of few_len, tile_len, at most few_splits, tile_splits of them
-    // (blockIdx.z), whose sums go to rows of part_ld floats: the dims, then the maximum and the sum.  few_part: part z of row y of
-    // sequence and key/value head x at (few x + y) few_splits + z; tile_part: of token t and head h at (t q_heads + h) tile_splits + z.
+    // in tiles of `tile` rows.  Either kind's positions are cut into parts, at most few_splits (equal ones) and tile_splits (of
+    // tile_len), whose sums go to rows of part_ld floats: the dims, then the maximum and the sum.  few_part: part z of row y of sequence and
+    // key/value head x < few_heads = batch kv_heads at (few x + y) few_splits + z; tile_part: of token t and head h at (t q_heads + h) tile_splits + z.
+    // counters: an arrival counter for each x, zero between launches, where the few
+    // rows' parts are joined in their own launch; or null.
     float *few_part, *tile_part;
-    int32_t few, few_len, few_splits, tile_len, tile_splits, part_ld;
+    int32_t *counters;
+    int32_t few, few_heads, few_splits, tile, tile_len, tile_splits, part_ld;
 };
 
 #endif
