@@ -330,11 +330,9 @@ int zn_hip_paged_attention(zn_ctx *ctx, const void *cache, const void *token_sta
             kernel = kPagedWide;
             a = wide;
         }
-        if (const char *e = std::getenv("ZNK")) { kernel = e[0] == 49 ? kPagedWide : kPagedTile; paged_tile_parts(ctx, a, tokens, max_q_len, kernel, type); if (e[1]) { a.tile_splits = std::atoi(e + 2); a.tile_len = (int32_t)(32 * std::max<int64_t>(1, cdiv(cdiv(a.c.cap, 32), a.tile_splits))); } }
         wgs = (tokens * group / a.tile + desc->batch) * desc->kv_heads * a.tile_splits + (a.few ? (int64_t)a.few_heads * a.few_splits : 0);
         if (wgs > INT_MAX / 1024) return ZN_ERR_OVERFLOW;
     }
-    if (std::getenv("ZND")) std::fprintf(stderr, "kernel %d tile %d splits %d len %d few %d splits %d\n", kernel, a.tile, a.tile_splits, a.tile_len, a.few, a.few_splits);
     Lease few_part(ctx), tile_part(ctx);
     if (a.few && a.few_splits > 1) {
         if ((rc = few_part.get((size_t)a.few_heads * a.few * a.few_splits * a.part_ld))) return rc;
