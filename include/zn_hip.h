@@ -579,7 +579,7 @@ typedef struct zn_paged_cache {
  *    (int32 on the device, batch + 1 of them, ascending) of k, v and q, and its
  *    last positions: row t's is kv_lens[b] - token_starts[b + 1] + t, which is
  *    also what it is turned by, unless positions (int32 [tokens]) says otherwise.
- *    Rows of no sequence, of the `tokens` there are, are neither read nor written.
+ *    Rows of no sequence, of the `tokens` there are, are not written.
  *  - k and v are [tokens, kv_heads, head_dim], q and q_out [tokens, q_heads,
  *    head_dim] at element strides for token and head, fp32; q_out may be q at
  *    q's strides.  q null: no queries.

@@ -685,7 +685,8 @@ struct PagedTile {
         const int li = lane & 15, lh = lane >> 4, dim = p.c.dim;
         const PagedSeq seq(p.c, b);
         // part z of the tile; a sequence's last tiles first, which see more keys
-        const int rows = min(seq.ql, p.max_q) * p.group, tiles = (rows + ROWS - 1) / ROWS, z = at / tiles;
+        const int rows = min(seq.ql, p.max_q) * p.group, tiles = max(1, (rows + ROWS - 1) / ROWS), z = at / tiles;
+        if (rows == 0 || at < 0) return;  // starts that do not ascend
         const int r0 = __builtin_amdgcn_readfirstlane(tiles - 1 - (at - z * tiles)) * ROWS;
         // keys that any row of the workgroup sees, its parts, this one's blocks
         const int last = paged_seen(p, seq, (min(r0 + ROWS, rows) - 1) / p.group);

@@ -9,14 +9,21 @@ namespace {
 
 constexpr int64_t kRotaryMaxDim = 1024;  // at most 128 threads to a head
 
-// Threads of a workgroup to tokens, heads and shares of a head: as many heads of a token at a time as fit, tokens where room is left.
+// Threads of a workgroup to tokens, heads and shares of a head.  Where a token's heads lie together (together): as many heads of a token
+// at a time as fit, tokens where room is left; where a head's tokens do: neighbouring tokens, one head after the other.
 struct RotaryGrid {
     int32_t units, slots, tokens;
     unsigned gx, gy;
-    RotaryGrid(const zn_ctx *ctx, int64_t units_, int64_t heads, int64_t all) {
+    RotaryGrid(const zn_ctx *ctx, int64_t units_, int64_t heads, int64_t all, bool together) {
         units = (int32_t)units_;
-        slots = (int32_t)std::min<int64_t>(heads, 256 / units);
-        tokens = (int32_t)std::max<int64_t>(1, 256 / (slots * units));
+        slots = together ? (int32_t)std::min<int64_t>(heads, 256 / units) : 1;
+        // Where that leaves many threads without work: the most heads that do not (6654 tokens of 20 heads of 10 shares: 200 threads of
+        // 256, or 5 heads of 5 tokens four times; 24 and 18.6 us).
+        auto busy = [&](int64_t s) { return (double)heads / (double)cdiv(heads, s) * (double)(256 / (s * units)) * (double)units / 256.0; };
+        const int64_t fit = slots;
+        for (int64_t s = fit; s > 0 && busy(fit) < 0.85; --s)
+            if (busy(s) > busy(slots)) slots = (int32_t)s;
+        tokens = (int32_t)std::max<int64_t>(1, std::min<int64_t>(all, 256 / (slots * units)));
         gx = (unsigned)cdiv(all, tokens);
         // few tokens: heads beside each other instead of one after the other
         gy = (unsigned)std::max<int64_t>(1, std::min<int64_t>(cdiv(heads, slots), 4 * cus_now(ctx) / gx));
@@ -57,7 +64,7 @@ int rotary(zn_ctx *ctx, const float *x, float *y, const float *freq, const void 
     std::memset(&a, 0, sizeof(a));
     const int64_t units = rotary_units(dim, rot, !same);
     if (units == 0) return ZN_OK;
-    const RotaryGrid g(ctx, units, heads, batch * len);
+    const RotaryGrid g(ctx, units, heads, batch * len, xs[1] <= xs[2] || len == 1);
     a.x = x;
     a.y = y;
     a.freq = freq;
@@ -173,11 +180,13 @@ int paged_args(const zn_paged_cache *c, ZnPagedCache &a, const void *starts, int
 // of K and V at most (sequences differ in length), 128 positions at least (paged_few_len).  MI355X, us in parts of 256, 512, 1024, 2048
 // and 4096 positions: 64 x 8 heads of up to 8192 x 128 bf16 311, 285, 275, 279, 291; 16 x 4 of up to 4096 x 128 bf16, five tokens, 41,
 // 31, 32, 47, 73; 16 x 8 of 4096 x 128 fp32 112, 108, 108, 107, 126; 8 of 65536 x 128 bf16 64, 54, 49, 47, 52; 8 x 4 of 2048 x 64
-// fp32 12, 16, 24, 37.  Beside tiles one of their larger workgroups a CU.  Past 4096 heads there is enough to do without.
+// fp32 12, 16, 24, 37.  Beside tiles one of their larger workgroups a CU; never
+// more than 32 a CU, which bounds the parts' memory.  Past 4096 heads there is enough to do without.
 void paged_few_parts(const zn_ctx *ctx, ZnPagedArgs &a, int type, int per_cu) {
     const int64_t most = 524288 / (2 * a.c.dim * (type == ZN_CACHE_BF16 ? 2 : 4));
-    const int64_t len = std::max<int64_t>(128, std::min<int64_t>(most, (int64_t)a.c.cap * a.few_heads / (per_cu * cus_now(ctx))));
-    a.few_splits = a.few_heads > kCounterSlots ? 1 : (int32_t)std::max<int64_t>(1, cdiv(a.c.cap, len));
+    const int64_t all = (int64_t)a.c.cap * a.few_heads, cus = cus_now(ctx);
+    const int64_t len = std::max({(int64_t)128, std::min(most, all / (per_cu * cus)), all / (32 * cus)});
+    a.few_splits = a.few_heads > kCounterSlots ? 1 : (int32_t)std::max<int64_t>(1, std::min<int64_t>(65535, cdiv(a.c.cap, len)));
 }
 
 // Parts of the walks of tiles: the least of the times of two batches added up, one whose sequences are all as long as the call allows, one
@@ -245,7 +254,7 @@ int zn_hip_paged_append(zn_ctx *ctx, const void *cache, const void *token_starts
     if (tokens == 0 || desc->batch == 0 || heads == 0) return ZN_OK;
     if (!paged_pointers(a.c) || (desc->kv_heads > 0 && (!k || !v)) || (q_heads > 0 && !q_out)) return ZN_ERR_INVALID_ARG;
     if ((rc = select_device(ctx))) return rc;
-    const RotaryGrid g(ctx, rotary_units(desc->head_dim, rot_dim, true), heads, tokens);
+    const RotaryGrid g(ctx, rotary_units(desc->head_dim, rot_dim, true), heads, tokens, true);
     a.k = k;
     a.v = v;
     a.q = q;
@@ -318,7 +327,7 @@ int zn_hip_paged_attention(zn_ctx *ctx, const void *cache, const void *token_sta
     int64_t wgs = 0;
     if (all_few) {
         while (kPagedRows[kernel] < rows) ++kernel;
-        a.few = kPagedRows[kernel];
+        a.few = (int32_t)rows;
     } else if (group <= kPagedRows[kPagedFew] && tokens < desc->batch * max_q_len) {
         a.few = kPagedRows[kPagedFew];
     }
