@@ -113,10 +113,10 @@ class Pool:
             at += n
         self.k, self.v = (np.full((self.pages, kv_heads, page, dim), np.nan, np.float32) for _ in range(2))
         for b, n in enumerate(lens):
-            for j in range(n):
-                for t in (self.k, self.v):
-                    x = rng.standard_normal((kv_heads, dim)).astype(np.float32)
-                    t[self.table[b, j // page], :, j % page] = from_bf16(to_bf16(x)) if dtype == "bf16" else x
+            j = np.arange(n)
+            for t in (self.k, self.v):
+                x = rng.standard_normal((n, kv_heads, dim)).astype(np.float32)
+                t[self.table[b, j // page], :, j % page] = from_bf16(to_bf16(x)) if dtype == "bf16" else x
         self.order = order
 
     def strides(self):
