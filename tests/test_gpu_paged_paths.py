@@ -230,3 +230,17 @@ def test_zero_scale_and_broadcast(ctx):
     ref = Mha(np.broadcast_to(q, (1, 1, 2, 32)), k, v, 0.2, True)
     for h in range(8):
         check(got[:, h][None, None], ref.out, ref.out_bound, f"head {h}")
+
+
+def test_no_new_tokens(ctx):
+    """Rows of no sequence only: nothing is written."""
+    announce("no new tokens")
+    pool = Pool(8, [50, 20], 2, 16, 32)
+    x, out, lse = run_attention(ctx, pool, [0, 0], 4, pad=3)
+    assert np.all(out == 7.0) and np.all(lse == 9.0)
+    x, out, lse = run_attention(ctx, pool, [0, 0], 4, pad=3, max_q=40)
+    assert np.all(out == 7.0) and np.all(lse == 9.0)
+    x, out, lse = run_attention(ctx, pool, [2, 1], 4, max_kv=0)  # nothing to see
+    assert np.all(out == 0) and np.all(lse == -np.inf)
+    x, out, lse = run_attention(ctx, pool, [20, 20], 4, max_kv=0)
+    assert np.all(out == 0) and np.all(lse == -np.inf)

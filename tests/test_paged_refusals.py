@@ -111,7 +111,7 @@ def test_append(lib, blank):
 def test_attention(lib, blank):
     assert attention(lib, None) == INVALID and attention(lib, blank, 0) == INVALID
     assert attention(lib, blank) not in (0, INVALID, OVERFLOW)
-    for good in ({"causal": 0}, {"lse": P}, {"qt": 0}, {"qh": 0}, {"max_q": 0}, {"max_kv": 0}, {"scale": -1.0}):
+    for good in ({"causal": 0}, {"lse": P}, {"qt": 0}, {"qh": 0}, {"max_kv": 0}, {"scale": -1.0}):
         assert attention(lib, blank, **good) not in (0, INVALID, OVERFLOW), good
     assert attention(lib, blank, desc(strides=(0, 0, 16))) not in (0, INVALID, OVERFLOW)  # read only: broadcast
     assert attention(lib, blank, desc(k=None, v=None, page_table=None, num_pages=0)) not in (0, INVALID, OVERFLOW)  # no pages: all masked
@@ -125,6 +125,7 @@ def test_attention(lib, blank):
         assert attention(lib, blank, **big) == OVERFLOW, big
     assert attention(lib, blank, desc(max_pages=1 << 20, page_size=1 << 20)) == OVERFLOW
     assert attention(lib, blank, tokens=0) == 0
+    assert attention(lib, blank, max_q=0) == 0  # no sequence has a new token
     assert attention(lib, blank, desc(batch=0)) == 0
     assert attention(lib, blank, desc(kv_heads=0), q_heads=0) == 0
 

@@ -296,7 +296,7 @@ int zn_hip_paged_attention(zn_ctx *ctx, const void *cache, const void *token_sta
     if (q_heads > 65535 || tokens * q_heads > INT_MAX / 2 || stride_far(q_stride_t, tokens) || stride_far(q_stride_h, q_heads) ||
         stride_far(out_stride_t, tokens) || stride_far(out_stride_h, q_heads) || desc->batch * desc->kv_heads > (int64_t)1 << 22)
         return ZN_ERR_OVERFLOW;
-    if (tokens == 0 || desc->batch == 0 || q_heads == 0) return ZN_OK;
+    if (tokens == 0 || desc->batch == 0 || q_heads == 0 || max_q_len == 0) return ZN_OK;
     if (!q || !out || !paged_pointers(a.c)) return ZN_ERR_INVALID_ARG;
     const int dims = (int)(desc->head_dim - 1) / 32, type = desc->type;
     const int64_t group = q_heads / desc->kv_heads, cap = std::min<int64_t>(a.c.cap, max_kv_len);
