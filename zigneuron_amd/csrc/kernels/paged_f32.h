@@ -651,13 +651,13 @@ struct PagedTile {
 
     // The sequence whose tiles' parts hold number `slot`, and which of them it is; or -1 and how many there are.  Those of 64 sequences
     // are summed at a time.
-    __device__ static __forceinline__ int find(const ZnPagedArgs &p, int slot, int &at) {
+    __device__ static __forceinline__ int find(const ZnPagedArgs &p, int slot, int &at, PagedSeq &seq) {
         const int lane = threadIdx.x & (kWave - 1);
         int before = 0;
         for (int i0 = 0; i0 < p.c.batch; i0 += 64) {
             int own = 0;
+            const PagedSeq s(p.c, min(i0 + lane, p.c.batch - 1));
             if (i0 + lane < p.c.batch) {
-                const PagedSeq s(p.c, i0 + lane);
                 const int n = min(s.ql, p.max_q), r = n * p.group;
                 if (r > p.few) own = (r + ROWS - 1) / ROWS * paged_parts(paged_seen(p, s, n - 1), p.tile_len);
             }
@@ -669,8 +669,12 @@ struct PagedTile {
             }
             const int n = __builtin_popcountll(__builtin_amdgcn_ballot_w64(before + sum <= slot));
             if (n < 64) {
-                at = __builtin_amdgcn_readfirstlane(slot - before - __shfl(sum - own, n));
-                return __builtin_amdgcn_readfirstlane(i0 + n);
+                at = __builtin_amdgcn_readlane(slot - before - sum + own, n);
+                seq.t0 = __builtin_amdgcn_readlane(s.t0, n);
+                seq.ql = __builtin_amdgcn_readlane(s.ql, n);
+                seq.kl = __builtin_amdgcn_readlane(s.kl, n);
+                seq.first = seq.kl - seq.ql;
+                return i0 + n;
             }
             before += __shfl(sum, 63);
         }
@@ -679,11 +683,10 @@ struct PagedTile {
     }
 
     // Key/value head kh, part `at` of sequence b's tiles.
-    __device__ static __forceinline__ void run(const ZnPagedArgs &p, char *lds, int kh, int b, int at) {
+    __device__ static __forceinline__ void run(const ZnPagedArgs &p, char *lds, int kh, int b, int at, const PagedSeq &seq) {
         const int tid = threadIdx.x, lane = tid & (kWave - 1);
         const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
         const int li = lane & 15, lh = lane >> 4, dim = p.c.dim;
-        const PagedSeq seq(p.c, b);
         // part z of the tile; a sequence's last tiles first, which see more keys
         const int rows = min(seq.ql, p.max_q) * p.group, tiles = max(1, (rows + ROWS - 1) / ROWS), z = at / tiles;
         if (rows == 0 || at < 0) return;  // starts that do not ascend
@@ -694,26 +697,40 @@ struct PagedTile {
         if (z >= parts) return;
         const int blk0 = __builtin_amdgcn_readfirstlane(z * p.tile_len / 32), nblk = __builtin_amdgcn_readfirstlane((min((z + 1) * p.tile_len, last) + 31) / 32);
 
+        // the first block's pages, then Q, then its rows: each on its way while the one before is waited for
+        int *const flag = reinterpret_cast<int *>(lds + kFlag);
+        if (tid == 0) *flag = 0;
+        Stage sg(p.c, lds, tid, b, kh, seq.kl);
+        if (blk0 < nblk) sg.pages(blk0);
+        __builtin_amdgcn_sched_barrier(0);
         const int w0 = r0 + wave * FQ * 16;
         int lim[FQ], all = INT_MAX, any = 0;
-        zn_bf16x8 qf[FQ][SL][3];
+        float q[FQ][SL][8];
 #pragma unroll
         for (int f = 0; f < FQ; ++f) {
             const int r = min(w0 + 16 * f + li, rows - 1), i = r / p.group;
             lim[f] = w0 + 16 * f + li < rows ? paged_seen(p, seq, i) : 0;
             const float *const row = p.q + (seq.t0 + i) * p.qs[0] + (kh * p.group + r - i * p.group) * p.qs[1];
 #pragma unroll
-            for (int sl = 0; sl < SL; ++sl) {
-                float x[8];
-                paged_query(row, lim[f] > 0, 32 * sl + 8 * lh, dim, p.scale_log2, x);
-                zn_u32x4 w[3];
-                split8(x, w);
-#pragma unroll
-                for (int q = 0; q < 3; ++q) qf[f][sl][q] = __builtin_bit_cast(zn_bf16x8, w[q]);
-            }
+            for (int sl = 0; sl < SL; ++sl) paged_query(row, lim[f] > 0, 32 * sl + 8 * lh, dim, p.scale_log2, q[f][sl]);
             all = min(all, lim[f]);
             any = max(any, lim[f]);
         }
+        if (blk0 < nblk) {
+            sg.fetch(blk0);
+            sg.pages(blk0 + 1);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        zn_bf16x8 qf[FQ][SL][3];
+#pragma unroll
+        for (int f = 0; f < FQ; ++f)
+#pragma unroll
+            for (int sl = 0; sl < SL; ++sl) {
+                zn_u32x4 w[3];
+                split8(q[f][sl], w);
+#pragma unroll
+                for (int part = 0; part < 3; ++part) qf[f][sl][part] = __builtin_bit_cast(zn_bf16x8, w[part]);
+            }
 #pragma unroll
         for (int s = 1; s < 16; s <<= 1) {
             all = min(all, __shfl_xor(all, s));
@@ -731,16 +748,8 @@ struct PagedTile {
 #pragma unroll
             for (int d = 0; d < DB; ++d) o[f][d] = zn_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
-        int *const flag = reinterpret_cast<int *>(lds + kFlag);
-        if (tid == 0) *flag = 0;
         const Frags fr(lds, lane);
-        Stage sg(p.c, lds, tid, b, kh, seq.kl);
-        if (blk0 < nblk) {
-            sg.pages(blk0);
-            sg.fetch(blk0);
-            sg.pages(blk0 + 1);
-            sg.commit(0);
-        }
+        if (blk0 < nblk) sg.commit(0);
         for (int blk = blk0; blk < nblk; ++blk) {
             const int st = (blk - blk0) & 1, k0 = 32 * blk;
             __syncthreads();  // block blk is in LDS; every wave is done with block blk - 1
@@ -917,13 +926,15 @@ extern "C" __global__ __launch_bounds__(256) void zn_paged_rows_bf16(ZnPagedArgs
     ZN_PAGED_KERNEL(NAME, NW, (NAME##_k::kBytes > NAME##_f::kBytes ? NAME##_k::kBytes : NAME##_f::kBytes), \
                     const int slot = blockIdx.x / p.c.kv_heads;                                         \
                     int at;                                                                             \
-                    const int b = NAME##_k::find(p, slot, at);                                          \
-                    if (b >= 0) return NAME##_k::run(p, lds, blockIdx.x - slot * p.c.kv_heads, b, at);  \
+                    PagedSeq seq(p.c);                                                                  \
+                    const int b = NAME##_k::find(p, slot, at, seq);                                     \
+                    if (b >= 0) return NAME##_k::run(p, lds, blockIdx.x - slot * p.c.kv_heads, b, at, seq); \
                     const int x = (int)blockIdx.x - at * p.c.kv_heads;                                  \
                     if (p.few && x < p.few_heads * p.few_splits) NAME##_f::run(p, lds, x % p.few_heads, x / p.few_heads))
 #define ZN_PAGED_KERNELS(DP, S, P)                                        \
     ZN_PAGED_FEW(zn_paged_few_f32_##DP##S, float, DP, 4, 1, P)            \
     ZN_PAGED_FEW(zn_paged_few2_f32_##DP##S, float, DP, 4, 2, P)           \
+    ZN_PAGED_FEW(zn_paged_few4_f32_##DP##S, float, DP, 4, 4, P)           \
     ZN_PAGED_FEW(zn_paged_few_bf16_##DP##S, __bf16, DP, 4, 1, P)          \
     ZN_PAGED_FEW(zn_paged_few2_bf16_##DP##S, __bf16, DP, 4, 2, P)         \
     ZN_PAGED_FEW(zn_paged_few4_bf16_##DP##S, __bf16, DP, 4, 4, P)

@@ -26,6 +26,7 @@ ZN_PAGED_FN int paged_clamp(int x, int lo, int hi) { return x < lo ? lo : x > hi
 // One sequence's new tokens and length; its token i has position first + i.
 struct PagedSeq {
     int t0, ql, kl, first;
+    ZN_PAGED_FN explicit PagedSeq(const ZnPagedCache &) : t0(0), ql(0), kl(0), first(0) {}  // none
     ZN_PAGED_FN PagedSeq(const ZnPagedCache &c, int b) {
         t0 = paged_clamp(c.starts[b], 0, c.tokens);
         ql = paged_clamp(c.starts[b + 1], t0, c.tokens) - t0;

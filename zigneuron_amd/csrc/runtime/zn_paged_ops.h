@@ -322,7 +322,12 @@ int zn_hip_paged_attention(zn_ctx *ctx, const void *cache, const void *token_sta
     // Sequences of few query rows have kernels of their own; where others are in the call too, their workgroups follow the tiles'
     // in one launch.
     const int64_t rows = group * max_q_len;
-    const bool all_few = rows <= kPagedRows[type == ZN_CACHE_BF16 ? kPagedFew4 : kPagedFew2];
+// 33 to 64 rows: in tiles where there are few heads, whose walks a workgroup then reads too slowly (MI355X, us as few rows and in
+    // tiles of 128: 16 tokens of 16 x 8 heads (4) against 4096 x 128 bf16 107 and 131, of 4 x 8 against 2048 39 and 32; fp32 of 33 x 9
+    // heads (1) of 42 tokens against up to 2713 x 127 260 and 367, 16 tokens of 16 x 8 (4) against 2048 x 128 112 and 103, of 16 x 4
+    // against 4096 x 64 66 and 98).
+    const int64_t enough = type == ZN_CACHE_BF16 || desc->head_dim <= 64 ? cus_now(ctx) / 4 : cus_now(ctx);
+    const bool all_few = rows <= kPagedRows[a.few_heads >= enough ? kPagedFew4 : kPagedFew2];
     int kernel = kPagedFew;
     int64_t wgs = 0;
     if (all_few) {
