@@ -179,6 +179,9 @@ struct PagedFew {
     static constexpr int VB = DP == 96 || (DP == 128 && !BF) ? 2 : 1;  // loads of a row of V: of w dims at 64 b + w li
     static constexpr int vw(int b) { return DP == 128 ? (BF ? 8 : 4) : DP == 96 ? (b ? 2 : 4) : DP == 64 ? 4 : 2; }
     static constexpr int ROWS = 16 * RB;
+    // Blocks of rows that a sequence does not fill are left out, except with 64 rows of 128 dims in bf16, where the branches spill (33 x 9
+    // heads of 42 tokens against up to 2713 x 127 fp32: 258 us, 226 so; 64 rows of 128 dims bf16 104, 155).
+    static constexpr bool SKIP = !(BF && DP == 128);
     static constexpr int kLd = DP + 4;
     static constexpr int QP = BF ? 3 : 1;            // parts of Q; a fragment: 16 bytes a lane
     static constexpr int kQuery = RB * KS * QP * 1024, kSums = NW * 16 * kLd * 4;
@@ -351,6 +354,7 @@ struct PagedFew {
             zn_f32x4 t[RB][KB];
 #pragma unroll
             for (int f = 0; f < RB; ++f) {
+                if (SKIP && f > 1 && 16 * f >= rows) break;
                 if constexpr (BF) {
 #pragma unroll
                     for (int rb = 0; rb < KB; ++rb) t[f][rb] = zn_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -398,6 +402,7 @@ struct PagedFew {
             const int k0 = from + STEP * s;
 #pragma unroll
             for (int f = 0; f < RB; ++f) {
+                if (SKIP && f > 1 && 16 * f >= rows) break;
                 float mb = -INFINITY;
 #pragma unroll
                 for (int e = 0; e < VR; ++e) {
