@@ -158,11 +158,8 @@ class PagedCache:
             strides = (kv_heads * page_size * head_dim, page_size * head_dim, head_dim)
         self.desc = _lib.PagedCacheDesc(_dptr(k), _dptr(v), _dptr(page_table), _dptr(kv_lens), batch, num_pages, page_size, max_pages,
                                         kv_heads, head_dim, *strides, _name_id(_lib.CACHE_TYPES, dtype, "cache type"))
+        self.address = ctypes.addressof(self.desc)
         self.buffers = (k, v, page_table, kv_lens)  # held as long as the descriptor
-
-    @property
-    def address(self) -> int:
-        return ctypes.addressof(self.desc)
 
 
 class DeviceBuffer:
@@ -471,23 +468,25 @@ class Context:
         contiguous) into their sequences' pages, keys and queries (q to q_out, which may be q) turned on the way.
         Sequence b's are rows token_starts[b] .. token_starts[b + 1] - 1 and its last positions."""
         d = cache.desc
-        own, q_own = (d.kv_heads * d.head_dim, d.head_dim), (q_heads * d.head_dim, d.head_dim)
+        kt, kh = (d.kv_heads * d.head_dim, d.head_dim) if kv_strides is None else kv_strides
+        qt, qh = (q_heads * d.head_dim, d.head_dim) if q_strides is None else q_strides
+        ot, oh = (q_heads * d.head_dim, d.head_dim) if q_out_strides is None else q_out_strides
         check(_lib.load().zn_hip_paged_append(
-            self.handle, cache.address, _dptr(token_starts), tokens, _dptr(k), _dptr(v), *(own if kv_strides is None else kv_strides),
-            _dptr(q), _dptr(q_out), q_heads, *(q_own if q_strides is None else q_strides),
-            *(q_own if q_out_strides is None else q_out_strides), _dptr(freq), rot_dim,
-            _name_id(_lib.ROTARY_LAYOUTS, layout, "rotary layout"), float(scale), _dptr(positions)), "zn_hip_paged_append")
+            self.handle, cache.address, _dptr(token_starts), tokens, _dptr(k), _dptr(v), kt, kh, _dptr(q), _dptr(q_out), q_heads, qt, qh,
+            ot, oh, _dptr(freq), rot_dim, _name_id(_lib.ROTARY_LAYOUTS, layout, "rotary layout"), scale, _dptr(positions)),
+            "zn_hip_paged_append")
 
     def paged_attention(self, cache: PagedCache, token_starts, tokens, max_q_len, max_kv_len, q, out, lse, q_heads, scale,
                         causal=True, q_strides=None, out_strides=None) -> None:
         """Attention of the sequences' new tokens (rows as in paged_append; at most max_q_len of each) over the positions
         (at most max_kv_len) that their pages hold; q and out are [tokens, q_heads, head_dim] at (token, head) element
         strides (None: contiguous), lse [tokens x q_heads] or None."""
-        own = (q_heads * cache.desc.head_dim, cache.desc.head_dim)
+        d = cache.desc
+        qt, qh = (q_heads * d.head_dim, d.head_dim) if q_strides is None else q_strides
+        ot, oh = (q_heads * d.head_dim, d.head_dim) if out_strides is None else out_strides
         check(_lib.load().zn_hip_paged_attention(
             self.handle, cache.address, _dptr(token_starts), tokens, max_q_len, max_kv_len, _dptr(q), _dptr(out), _dptr(lse), q_heads,
-            float(scale), int(causal), *(own if q_strides is None else q_strides),
-            *(own if out_strides is None else out_strides)), "zn_hip_paged_attention")
+            scale, int(causal), qt, qh, ot, oh), "zn_hip_paged_attention")
 
     def close(self) -> None:
         if self.handle:
