@@ -583,7 +583,7 @@ struct PagedFrags {
     __device__ static __forceinline__ int chunk_of(int db, int lh) { return 32 * (db / 2) + 8 * (2 * (db & 1) + lh / 2); }
 };
 
-template <typename T, int DP, int NW, int FQ>
+template <typename T, int DP, int NW, int FQ, bool PAGES16>
 struct PagedTile {
     static constexpr bool BF = sizeof(T) == 2;
     static constexpr int NP = BF ? 1 : 3, PRODUCTS = BF ? 3 : 6;
@@ -599,29 +599,41 @@ struct PagedTile {
         char *lds;
         const T *k, *v;
         const int32_t *table;
-        int tid, kl, page[UPT];
+        int tid, wave, kl, page[UPT];
         bool hole = false;
         zn_u32x4_2 g[UPT][2][BF ? 1 : 2];
-        __device__ __forceinline__ Stage(const ZnPagedCache &c, char *lds, int tid, int b, int kh, int kl)
+        __device__ __forceinline__ Stage(const ZnPagedCache &c, char *lds, int tid, int wave, int b, int kh, int kl)
             : c(c), lds(lds), k(reinterpret_cast<const T *>(c.k) + kh * c.stride[1]), v(reinterpret_cast<const T *>(c.v) + kh * c.stride[1]),
-              table(c.table + (int64_t)b * c.max_pages), tid(tid), kl(kl) {}
+              table(c.table + (int64_t)b * c.max_pages), tid(tid), wave(wave), kl(kl) {}
         __device__ __forceinline__ int page_of(int j) const { return (int)(((uint64_t)(uint32_t)j * c.div_mul) >> (31 + c.div_shift)); }
-        // Unit i's row of block blk (a row past the sequence's end: the last) and dims
+        __device__ __forceinline__ bool mine(int i) const { return (i + 1) * NT <= kUnits || i * NT + tid < kUnits; }
+        // Unit i's row of a block, and the key that its page is looked up for (past the sequence's end: its last): with pages of a
+        // multiple of 16 positions the first of its 16 rows, which a wave's rows share (16 rows are a multiple of 64 units).
         __device__ __forceinline__ int row(int i) const { return (i * NT + tid) / (DP / 8); }
-        __device__ __forceinline__ int key(int i, int blk) const { return min(32 * blk + row(i), kl - 1); }
+        __device__ __forceinline__ int key(int i, int blk) const {
+            return min(32 * blk + (PAGES16 ? (i * NT + wave * kWave) / (2 * DP) * 16 : row(i)), kl - 1);
+        }
         __device__ __forceinline__ void pages(int blk) {
+            typedef __attribute__((address_space(4))) const int32_t Table;  // constant: for scalar loads
 #pragma unroll
-            for (int i = 0; i < UPT; ++i)
-                if (i * NT + tid < kUnits) page[i] = table[page_of(key(i, blk))];
+            for (int i = 0; i < UPT; ++i) {
+                if constexpr (PAGES16) page[i] = ((Table *)(uintptr_t)table)[page_of(key(i, blk))];
+                else if (mine(i)) page[i] = table[page_of(key(i, blk))];
+            }
         }
         __device__ __forceinline__ void fetch(int blk) {
 #pragma unroll
             for (int i = 0; i < UPT; ++i) {
-                if (i * NT + tid >= kUnits) continue;
+                if (!mine(i)) continue;
                 const bool in = (uint32_t)page[i] < (uint32_t)c.pages;
                 hole |= !in;
-                const int j = key(i, blk), d = paged_dim((i * NT + tid) % (DP / 8) * 8, 8, c.dim);
-                const int64_t at = (in ? page[i] : 0) * c.stride[0] + (j - page_of(j) * c.page_size) * c.stride[2] + d;
+                const int j = key(i, blk);
+                int64_t at = (in ? page[i] : 0) * c.stride[0] + (j - page_of(j) * c.page_size) * c.stride[2];
+                if constexpr (PAGES16) {
+                    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)at), hi = __builtin_amdgcn_readfirstlane((uint32_t)(at >> 32));
+                    at = (int64_t)((uint64_t)hi << 32 | lo) + (int64_t)((uint64_t)(uint32_t)min(row(i) % 16, kl - 1 - j) * (uint32_t)c.stride[2]);
+                }
+                at += paged_dim((i * NT + tid) % (DP / 8) * 8, 8, c.dim);
                 const T *const from[2] = {k + at, v + at};
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
@@ -632,9 +644,8 @@ struct PagedTile {
         __device__ __forceinline__ void commit(int st) {
 #pragma unroll
             for (int i = 0; i < UPT; ++i) {
-                const int u = i * NT + tid;
-                if (u >= kUnits) continue;
-                const int dc = u % (DP / 8);
+                if (!mine(i)) continue;
+                const int u = i * NT + tid, dc = u % (DP / 8);
                 char *const to = lds + st * Frags::kStage + dc / 4 * (B::BR * 64) + B::slot(u / (DP / 8), dc % 4);
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
@@ -705,7 +716,7 @@ struct PagedTile {
         // the first block's pages, then Q, then its rows: each on its way while the one before is waited for
         int *const flag = reinterpret_cast<int *>(lds + kFlag);
         if (tid == 0) *flag = 0;
-        Stage sg(p.c, lds, tid, b, kh, seq.kl);
+        Stage sg(p.c, lds, tid, wave, b, kh, seq.kl);
         if (blk0 < nblk) sg.pages(blk0);
         __builtin_amdgcn_sched_barrier(0);
         const int w0 = r0 + wave * FQ * 16;
@@ -859,7 +870,9 @@ struct PagedTile {
             float x[8], mb = -INFINITY;
 #pragma unroll
             for (int e = 0; e < 8; ++e) mb = fmaxf(mb, s[f][e / 4][e % 4]);
-            const float mn = fmaxf(m[f], max_over_rows(mb) * kUnscale);
+            // The reference moves where the maximum leaves it by more than 2^8: until then the probabilities are up to 2^8 times what they
+            // are relative to the maximum, which no rounding sees, and O is not multiplied (16 vector instructions for every 16 dims).
+            const float top = max_over_rows(mb) * kUnscale, mn = top > m[f] + 8.0f ? top : m[f];
             const float ref = mn == -INFINITY ? 0.0f : mn;  // nothing seen so far
             const float alpha = __builtin_amdgcn_exp2f(m[f] - ref);
             float rs = 0.0f;
@@ -926,7 +939,7 @@ extern "C" __global__ __launch_bounds__(256) void zn_paged_rows_bf16(ZnPagedArgs
     ZN_PAGED_KERNEL(NAME, 4, NAME##_k::kBytes, NAME##_k::run(p, lds, blockIdx.x, blockIdx.z))
 // NW waves of F blocks of 16 rows: the tiles' parts, then the parts of few rows.
 #define ZN_PAGED_TILE(NAME, T, DP, NW, F, P)                                                             \
-    typedef PagedTile<T, DP, NW, F> NAME##_k;                                                           \
+    typedef PagedTile<T, DP, NW, F, P> NAME##_k;                                                        \
     typedef PagedFew<T, DP, NW, 1, P> NAME##_f;                                                         \
     ZN_PAGED_KERNEL(NAME, NW, (NAME##_k::kBytes > NAME##_f::kBytes ? NAME##_k::kBytes : NAME##_f::kBytes), \
                     const int slot = blockIdx.x / p.c.kv_heads;                                         \
