@@ -223,6 +223,16 @@ def test_attention_bounds_above_the_lengths(ctx, counts, dtype):
     assert np.array_equal(out, out2) and np.all(none == 9.0)
 
 
+@pytest.mark.parametrize("most", [2 ** 31, 2 ** 62, 2 ** 63 - 1])
+@pytest.mark.parametrize("counts", [[1, 2, 1], [40, 1, 150]])
+def test_attention_bounds_above_everything(ctx, counts, most):
+    """Bounds that no sequence can have: products with them pass 64 bits."""
+    announce(f"paged attention, bounds of {most} {counts}")
+    pool = Pool(16, [200, 31, 150], 2, 16, 64)
+    x, out, lse = run_attention(ctx, pool, counts, 8, max_q=most, max_kv=most)
+    compare(pool, counts, x, out, lse)
+
+
 @pytest.mark.parametrize("counts", [[3, 1], [60, 20]])
 def test_attention_bounds_below_the_lengths(ctx, counts):
     """A longer sequence is cut to max_kv_len, more new tokens to the first max_q_len."""

@@ -246,8 +246,9 @@ int zn_hip_paged_append(zn_ctx *ctx, const void *cache, const void *token_starts
                         !stride_ok(q_out_stride_t, tokens, true) || !stride_ok(q_out_stride_h, q_heads, true)))
         return ZN_ERR_INVALID_ARG;
     if (rc) return rc;
+    if (q_heads > INT_MAX / 4) return ZN_ERR_OVERFLOW;
     const int64_t heads = q_heads + 2 * desc->kv_heads;
-    if (q_heads > INT_MAX / 4 || heads > INT_MAX / 2 || stride_far(kv_stride_t, tokens) || stride_far(kv_stride_h, desc->kv_heads) ||
+    if (heads > INT_MAX / 2 || stride_far(kv_stride_t, tokens) || stride_far(kv_stride_h, desc->kv_heads) ||
         (q_heads > 0 && (stride_far(q_stride_t, tokens) || stride_far(q_stride_h, q_heads) || stride_far(q_out_stride_t, tokens) ||
                          stride_far(q_out_stride_h, q_heads))))
         return ZN_ERR_OVERFLOW;
@@ -298,6 +299,7 @@ int zn_hip_paged_attention(zn_ctx *ctx, const void *cache, const void *token_sta
         return ZN_ERR_OVERFLOW;
     if (tokens == 0 || desc->batch == 0 || q_heads == 0 || max_q_len == 0) return ZN_OK;
     if (!q || !out || !paged_pointers(a.c)) return ZN_ERR_INVALID_ARG;
+    max_q_len = std::min(max_q_len, tokens);
     const int dims = (int)(desc->head_dim - 1) / 32, type = desc->type;
     const int64_t group = q_heads / desc->kv_heads, cap = std::min<int64_t>(a.c.cap, max_kv_len);
     if ((rc = select_device(ctx))) return rc;
@@ -312,7 +314,7 @@ int zn_hip_paged_attention(zn_ctx *ctx, const void *cache, const void *token_sta
     a.q_heads = (int32_t)q_heads;
     a.group = (int32_t)(q_heads / desc->kv_heads);
     a.causal = causal;
-    a.max_q = (int32_t)std::min<int64_t>(max_q_len, tokens);
+    a.max_q = (int32_t)max_q_len;
     a.scale_log2 = scale * 1.44269504088896340736f;
     // a 16-byte load of bf16 takes 8 dims
     if (desc->head_dim < 8) return launch(ctx, ctx->paged_rows[type], (unsigned)tokens, (unsigned)cdiv(q_heads, 4), 256, &a);
@@ -322,7 +324,7 @@ int zn_hip_paged_attention(zn_ctx *ctx, const void *cache, const void *token_sta
     // Sequences of few query rows have kernels of their own; where others are in the call too, their workgroups follow the tiles'
     // in one launch.
     const int64_t rows = group * max_q_len;
-// 33 to 64 rows: in tiles where there are few heads, whose walks a workgroup then reads too slowly (MI355X, us as few rows and in
+    // 33 to 64 rows: in tiles where there are few heads, whose walks a workgroup then reads too slowly (MI355X, us as few rows and in
     // tiles of 128: 16 tokens of 16 x 8 heads (4) against 4096 x 128 bf16 107 and 131, of 4 x 8 against 2048 39 and 32; fp32 of 33 x 9
     // heads (1) of 42 tokens against up to 2713 x 127 260 and 367, 16 tokens of 16 x 8 (4) against 2048 x 128 112 and 103, of 16 x 4
     // against 4096 x 64 66 and 98).
