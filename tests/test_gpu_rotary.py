@@ -102,6 +102,26 @@ def test_positions(ctx, stride):
 
 
 @pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_far_and_fast(ctx, layout):
+    """Positions to both ends of 32 bits and frequencies far above 1: the angle, a product of 55 bits, passes 2^43, its quarter
+    turns pass 32 bits.  The reference has it exactly (80-bit floats), so the bound has no term of the angle: 8 U as for near ones."""
+    announce(f"rotary, far and fast {layout}")
+    assert np.finfo(np.longdouble).nmant >= 63
+    rng = np.random.default_rng(10)
+    pos = np.concatenate([[0, 1, -1, 2 ** 31 - 1, -(2 ** 31), 2 ** 31 - 2, 2 ** 30 + 1], rng.integers(-(2 ** 31), 2 ** 31, 57)]).astype(np.int32)
+    freq = np.array([1, 0.99999994, 1.5707964, 3.0, 7.7, 100.3, 1e-4, 4097.123], np.float32)
+    x = rng.standard_normal((1, 2, pos.size, 16)).astype(np.float32)
+    a = pos.astype(np.longdouble)[:, None] * freq.astype(np.longdouble)
+    s, c = np.sin(a).astype(np.float64), np.cos(a).astype(np.float64)
+    one, two = (slice(0, 8), slice(8, 16)) if layout == "half" else (slice(0, 16, 2), slice(1, 16, 2))
+    p, q = x[..., one].astype(np.float64), x[..., two].astype(np.float64)
+    ref, bound = np.empty(x.shape), np.empty(x.shape)
+    ref[..., one], ref[..., two] = p * c - q * s, p * s + q * c
+    bound[..., one] = bound[..., two] = 8 * U * (np.abs(p) + np.abs(q))
+    check(run(ctx, x, 16, layout, pos, freq=freq), ref, bound, "y")
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
 def test_gradient_against_differences(ctx, layout):
     """The turn is linear: its difference quotient along h is its value at h, and <g, f(h)> = <f'(g), h>."""
     announce(f"rotary gradient {layout}")

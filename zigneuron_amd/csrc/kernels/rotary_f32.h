@@ -6,10 +6,11 @@
 // 2 i and 2 i + 1 (layout 1); the other dims are copied.  The gradient turns
 // back (-a).
 //
-// The angle: p f_i is a product of at most 55 bits, taken in 64-bit floats, and
-// so is its reduction to a quarter turn (2 / pi in two parts): a turn of a far
-// position is as exact as that of a near one, where an angle rounded to 32 bits
-// is off by 2^-24 of itself, 0.06 of a turn's radius at 10^6.  Sine and cosine of
+// The angle: p f_i is a product of at most 55 bits, taken as a 64-bit float and
+// the rest of its rounding, and reduced to a quarter turn in 64 bits (2 / pi in
+// two parts): a turn of a far position is as exact as that of a near one, where
+// an angle rounded to 32 bits is off by 2^-24 of itself, 0.06 of a turn's radius
+// at 10^6.  Sine and cosine of
 // what is left, |y| <= pi / 4, are their Taylor polynomials to y^11 and y^10 (the
 // next terms are below 2^-27 of 1).
 #ifndef ZN_ROTARY_F32_H
@@ -27,8 +28,8 @@ typedef __bf16 zn_bf16x4_any __attribute__((ext_vector_type(4), aligned(2)));
 
 __device__ __forceinline__ void rotary_sincos(int position, float freq, float &s, float &c) {
     constexpr double kHi = 0.63661977236758138, kLo = -3.9357353350364972e-17;  // 2 / pi
-    const double a = (double)position * (double)freq, t = a * kHi, q = __builtin_rint(t);
-    const float y = (float)((t - q) + __builtin_fma(a, kLo, __builtin_fma(a, kHi, -t))) * 1.57079632679489662f, z = y * y;
+    const double p = position, f = freq, a = p * f, rest = __builtin_fma(p, f, -a), t = a * kHi, q = __builtin_rint(t);
+    const float y = (float)((t - q) + __builtin_fma(rest, kHi, __builtin_fma(a, kLo, __builtin_fma(a, kHi, -t)))) * 1.57079632679489662f, z = y * y;
     float u = __builtin_fmaf(z, -1.0f / 39916800.0f, 1.0f / 362880.0f);
     u = __builtin_fmaf(z, u, -1.0f / 5040.0f);
     u = __builtin_fmaf(z, u, 1.0f / 120.0f);
@@ -39,7 +40,7 @@ __device__ __forceinline__ void rotary_sincos(int position, float freq, float &s
     w = __builtin_fmaf(z, w, 1.0f / 24.0f);
     w = __builtin_fmaf(z, w, -0.5f);
     const float cy = __builtin_fmaf(z, w, 1.0f);
-    const int n = (int)q & 3;
+    const int n = (int)__builtin_fma(__builtin_floor(q * 0.25), -4.0, q);  // of 0..3: q itself may pass 32 bits
     s = n & 1 ? cy : sy;
     c = n & 1 ? sy : cy;
     if (n & 2) s = -s;
