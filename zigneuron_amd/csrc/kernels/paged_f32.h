@@ -165,6 +165,12 @@ __device__ __forceinline__ void paged_query(const float *row, bool in, int d, in
 // the products with K, its V behind those with V.
 // Rows are read in whole 128-byte lines where they have them: K's two slices of a
 // line go to lanes 8 apart, which then exchange theirs.
+// Each walk is cut into parts (paged_few_parts) so that a few sequences fill the
+// chip.  MI355X, one new token each: 64 x 32 heads (8) against up to 8192 x 128 bf16
+// (1.48 GB) 280 us, 5.3 TB/s, a large copy's rate 4.9; 8 x 16 (4) against 2048 x 64
+// fp32 (34 MB) 12 us: four steps of a wave, each a round trip to memory, then the
+// join.  Five tokens of 16 x 16 heads (4) against up to 4096 x 128 bf16 (83 MB) 28
+// us and the join's 5.
 template <typename T, int DP, int NW, int RB, bool PAGES16>
 struct PagedFew {
     static constexpr bool BF = sizeof(T) == 2;
@@ -542,6 +548,14 @@ struct PagedFew {
 //    before the row, the row a block before its use.  fp32 rows are split there
 //    (three parts), bf16 ones are operands as they lie (one part): six products
 //    for one of fp32, or three.
+//  - Bound by the products and the vector instructions beside them (softmax, P's
+//    split, fp32 rows' split: 1.8 a product with fp32 pages, 2.6 with bf16 ones),
+//    whose times nearly add up; the matrix cores are busy half of the time.  MI355X:
+//    4 x 512 tokens of 32 heads (8) over 2730 to 8192 x 128 fp32 555 us and the
+//    join's 25 (200 TFLOP/s), one prompt of 4096 tokens over bf16 pages 348 us (395).
+//    Measured and not kept: softmax of one block of rows between the products of the
+//    other (K and V's fragments read twice; 4 to 18% slower), a wave's priority raised
+//    over its products (within 1%), three workgroups a CU.
 //  - The parts of all sequences' tiles are one range without gaps, and few rows of
 //    other sequences follow it: where each part of each tile had a place of its own,
 //    the gaps fell on the same XCDs or shader engines each time and left them idle (4

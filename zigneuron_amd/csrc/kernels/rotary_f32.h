@@ -136,6 +136,14 @@ struct RotaryTurn {
 
 }  // namespace
 
+// A thread has the same 8 dims of one token in every head it turns, and takes
+// their sines and cosines once: a few dozen 64-bit instructions a pair, beside 16
+// bytes a head read and written.  Bound by those, or by the launch.  Neighbouring
+// threads have neighbouring dims, then heads or tokens, whichever lie together.
+// MI355X, alone in a row: 2 x 40 heads of 4096 x 128 (336 MB moved) 56 us, 6.0 TB/s,
+// where the last-level cache helps (67 among other kernels; a large copy 4.9); 3 x 12
+// heads of 2777 x 76, half turned (61 MB), 13 us; 8 x 20 heads of one token of 64 3.8
+// us, two round trips to memory behind a launch of 1.6.
 extern "C" __global__ __launch_bounds__(256) void zn_rotary(ZnRotaryArgs p) {
     const int per = p.slots * p.units, tl = threadIdx.x / per, in = threadIdx.x - tl * per, slot = in / p.units;
     const int64_t token = (int64_t)blockIdx.x * p.tokens + tl;
@@ -157,7 +165,10 @@ extern "C" __global__ __launch_bounds__(256) void zn_rotary(ZnRotaryArgs p) {
 
 namespace {
 
-// Queries, keys and values of new tokens: q turned to q_out, k turned to its page, v to its page.
+// Queries, keys and values of new tokens: q turned to q_out, k turned to its page, v to its page.  One launch, as zn_rotary's but for
+// the tokens' sequences (64 starts at a time by the whole wave) and pages.  Bound by its bytes, or by the launch.  MI355X: 8192 tokens
+// of 32 + 2 x 8 heads of 128 into bf16 (369 MB moved) 73 us, 5.1 TB/s; 6654 tokens of 10 + 2 x 5 heads of 76 19 us (25 among other
+// kernels); 64 tokens of 16 + 2 x 4 heads of 64 4.2 us, the third of three dependent loads (start, page, row).
 template <typename T>
 __device__ __forceinline__ void paged_append(const ZnAppendArgs &p) {
     const ZnPagedCache &c = p.c;
