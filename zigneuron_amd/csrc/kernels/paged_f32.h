@@ -69,9 +69,9 @@ __device__ __forceinline__ void paged_finish(const ZnPagedArgs &p, float *part, 
     if (lane < 2) put(p.part_ld - 4 + lane, lane ? l : m);
 }
 
-// A row's parts in order, a wave to a row, lane l its dims l and l + 64, sixteen parts' loads in flight.
+// A row's parts in order, a wave to a row, lane l its dims l and l + 64, N parts' loads in flight.
+template <int N>
 __device__ __forceinline__ void paged_join(const ZnPagedArgs &p, const float *src, int parts, int t, int h, int lane) {
-    constexpr int N = 16;
     float mx = -INFINITY, sl = 0.0f, oa = 0.0f, ob = 0.0f;
     for (int z0 = 0; z0 < parts; z0 += N) {
         float x[N], y[N], m[N], l[N];
@@ -104,6 +104,11 @@ __device__ __forceinline__ void paged_join(const ZnPagedArgs &p, const float *sr
         }
     }
     paged_store(p, t, h, lane, mx, sl, oa, ob);
+}
+
+__device__ __forceinline__ void paged_join(const ZnPagedArgs &p, const float *src, int parts, int t, int h, int lane) {
+    if (parts <= 4) paged_join<4>(p, src, parts, t, h, lane);
+    else paged_join<16>(p, src, parts, t, h, lane);
 }
 
 // Parts of a walk over `keys` positions: one at least.
@@ -922,20 +927,25 @@ struct PagedTile {
 
 }  // namespace
 
-// The join of rows that are in parts.  Grid x: the tokens, y: four heads each.
+// The join of rows that are in parts.  Grid x: the tokens, y: groups of four heads, a wave each (one after the other where the call
+// has many tokens: a token's place is three dependent loads).
 extern "C" __global__ __launch_bounds__(256) void zn_paged_join(ZnPagedArgs p) {
-    const int lane = threadIdx.x & (kWave - 1), t = blockIdx.x, h = blockIdx.y * 4 + threadIdx.x / kWave;
+    const int lane = threadIdx.x & (kWave - 1), t = blockIdx.x;
     const int b = paged_find(p.c, t);
-    if (b < 0 || b >= p.c.batch || h >= p.q_heads) return;
+    if (b < 0 || b >= p.c.batch) return;
     const PagedSeq seq(p.c, b);
-    const int kh = h / p.group, rows = min(seq.ql, p.max_q) * p.group, r = (t - seq.t0) * p.group + h - kh * p.group;
-    if (t < seq.t0 || r >= rows) return;
-    if (rows <= p.few) {
-        const int any = paged_seen(p, seq, (rows - 1) / p.group), parts = paged_parts(any, paged_few_len(p, any));
-        if (parts > 1) paged_join(p, p.few_part + (((int64_t)b * p.c.kv_heads + kh) * p.few + r) * p.few_splits * p.part_ld, parts, t, h, lane);
-    } else {
-        const int parts = paged_parts(paged_seen(p, seq, (min((r / p.tile + 1) * p.tile, rows) - 1) / p.group), p.tile_len);
-        if (parts > 1) paged_join(p, p.tile_part + ((int64_t)t * p.q_heads + h) * p.tile_splits * p.part_ld, parts, t, h, lane);
+    const int rows = min(seq.ql, p.max_q) * p.group, i = t - seq.t0;
+    if (i < 0 || i * p.group >= rows) return;
+    const bool few = rows <= p.few;
+    const int any = few ? paged_seen(p, seq, (rows - 1) / p.group) : 0, few_parts = few ? paged_parts(any, paged_few_len(p, any)) : 0;
+    for (int h = blockIdx.y * 4 + threadIdx.x / kWave; h < p.q_heads; h += gridDim.y * 4) {
+        const int kh = h / p.group, r = i * p.group + h - kh * p.group;
+        if (few) {
+            if (few_parts > 1) paged_join(p, p.few_part + (((int64_t)b * p.c.kv_heads + kh) * p.few + r) * p.few_splits * p.part_ld, few_parts, t, h, lane);
+        } else {
+            const int parts = paged_parts(paged_seen(p, seq, (min((r / p.tile + 1) * p.tile, rows) - 1) / p.group), p.tile_len);
+            if (parts > 1) paged_join(p, p.tile_part + ((int64_t)t * p.q_heads + h) * p.tile_splits * p.part_ld, parts, t, h, lane);
+        }
     }
 }
 

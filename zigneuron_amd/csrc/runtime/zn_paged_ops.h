@@ -365,7 +365,10 @@ int zn_hip_paged_attention(zn_ctx *ctx, const void *cache, const void *token_sta
     if (all_few) rc = launch(ctx, f, (unsigned)a.few_heads, 1, 256, &a, (unsigned)a.few_splits);
     else rc = launch(ctx, f, (unsigned)wgs, 1, kPagedThreads[kernel - kPagedTile][type][dims], &a);
     if (rc || own_join || (a.few_splits <= 1 && a.tile_splits <= 1)) return rc;
-    return launch(ctx, ctx->paged_join, (unsigned)tokens, (unsigned)cdiv(q_heads, 4), 256, &a);
+    // a token's heads beside each other while there are few tokens, eight workgroups a CU (4 x 512 tokens of 32 heads, a quarter of
+    // them in parts: 25 us with eight workgroups a token, 15 with one)
+    const int64_t join_heads = std::max<int64_t>(1, std::min<int64_t>(cdiv(q_heads, 4), 8 * cus_now(ctx) / tokens));
+    return launch(ctx, ctx->paged_join, (unsigned)tokens, (unsigned)join_heads, 256, &a);
 }
 
 #endif
