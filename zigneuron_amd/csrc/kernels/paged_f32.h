@@ -201,7 +201,7 @@ __device__ __forceinline__ void paged_query(const float *row, bool in, int d, in
 // chip.  MI355X, one new token each: 64 x 32 heads (8) against up to 8192 x 128 bf16
 // (1.48 GB) 280 us, 5.3 TB/s, a large copy's rate 4.9; 8 x 16 (4) against 2048 x 64
 // fp32 (34 MB) 12 us: four steps of a wave, each a round trip to memory, then the
-// join.  Five tokens of 16 x 16 heads (4) against up to 4096 x 128 bf16 (83 MB) 28
+// join.  Five tokens of 16 x 16 heads (4) against up to 4096 x 128 bf16 (83 MB) 27
 // us and the join's 5.
 template <typename T, int DP, int NW, int RB, bool PAGES16>
 struct PagedFew {
@@ -581,13 +581,15 @@ struct PagedFew {
 //    (three parts), bf16 ones are operands as they lie (one part): six products
 //    for one of fp32, or three.
 //  - Bound by the products and the vector instructions beside them (softmax, P's
-//    split, fp32 rows' split: 1.8 a product with fp32 pages, 2.6 with bf16 ones),
+//    split, fp32 rows' split: 1.8 a product with fp32 pages, 2.2 with bf16 ones),
 //    whose times nearly add up; the matrix cores are busy half of the time.  MI355X:
-//    4 x 512 tokens of 32 heads (8) over 2730 to 8192 x 128 fp32 555 us and the
-//    join's 25 (200 TFLOP/s), one prompt of 4096 tokens over bf16 pages 348 us (395).
+//    4 x 512 tokens of 32 heads (8) over 2730 to 8192 x 128 fp32 550 us and the
+//    join's 14 (201 TFLOP/s), one prompt of 4096 tokens over bf16 pages 349 us (394).
 //    Measured and not kept: softmax of one block of rows between the products of the
 //    other (K and V's fragments read twice; 4 to 18% slower), a wave's priority raised
-//    over its products (within 1%), three workgroups a CU.
+//    over its products (within 1%), three workgroups a CU, half of the waves half a
+//    block behind the others (5% slower to 4% faster), fp32 rows' split between the
+//    products with V (0 to 9% slower).
 //  - The parts of all sequences' tiles are one range without gaps, and few rows of
 //    other sequences follow it: where each part of each tile had a place of its own,
 //    the gaps fell on the same XCDs or shader engines each time and left them idle (4

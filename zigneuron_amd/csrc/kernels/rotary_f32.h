@@ -142,7 +142,7 @@ struct RotaryTurn {
 // threads have neighbouring dims, then heads or tokens, whichever lie together.
 // MI355X, alone in a row: 2 x 40 heads of 4096 x 128 (336 MB moved) 56 us, 6.0 TB/s,
 // where the last-level cache helps (67 among other kernels; a large copy 4.9); 3 x 12
-// heads of 2777 x 76, half turned (61 MB), 13 us; 8 x 20 heads of one token of 64 3.8
+// heads of 2777 x 76, half turned (61 MB), 13 us; 8 x 20 heads of one token of 64 3.7
 // us, two round trips to memory behind a launch of 1.6.
 extern "C" __global__ __launch_bounds__(256) void zn_rotary(ZnRotaryArgs p) {
     const int per = p.slots * p.units, tl = threadIdx.x / per, in = threadIdx.x - tl * per, slot = in / p.units;
