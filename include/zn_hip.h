@@ -519,7 +519,8 @@ typedef enum zn_rotary_scaling {
     ZN_ROTARY_BASE = 2,   /* base times factor^(rot_dim / (rot_dim - 2)): the last pair is slowed down by factor, the first not */
     ZN_ROTARY_TURNS = 3,  /* pairs of `high` turns and more over trained_len keep f_i, of `low` and fewer get f_i / factor,
                              between the two a mixture linear in the turns             */
-    ZN_ROTARY_PAIRS = 4   /* the same, linear in the pair's number between those (rounded down and up) of `high` and `low` turns */
+    ZN_ROTARY_PAIRS = 4   /* the same, linear in the pair's number between those of `high` (rounded down) and `low` turns (rounded
+                             up), which are held to 0 .. rot_dim - 1: past the last pair too */
 } zn_rotary_scaling;
 
 /* The frequencies of rot_dim / 2 pairs into freq (host memory, freq_len

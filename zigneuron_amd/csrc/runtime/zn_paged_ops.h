@@ -106,7 +106,8 @@ int zn_hip_rotary_frequencies(float *freq, size_t freq_len, int64_t rot_dim, flo
     double first = 0.0, last = 0.0;
     if (scaling == ZN_ROTARY_PAIRS) {
         first = std::max(0.0, std::floor(pair_of(high)));
-        last = std::min(n / 2.0 - 1.0, std::ceil(pair_of(low)));
+        // not the last pair, n / 2 - 1: past it lies the ramp's end wherever that pair makes more than `low` turns
+        last = std::min(n - 1.0, std::ceil(pair_of(low)));
         if (!(last > first)) last = first + 0.001;
     }
     for (int64_t i = 0; i < rot_dim / 2; ++i) {
