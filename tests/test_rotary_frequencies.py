@@ -35,3 +35,15 @@ def test_pairs_at_all_lengths(rot, base, trained, factor):
     # whatever the ramp: pairs of `high` turns and more keep their speed, none of more than `low` turns loses all of it
     assert np.all(np.abs(got - f)[turns >= 32 * base ** (2 / rot)] <= 2.0 ** -23 * f[turns >= 32 * base ** (2 / rot)])
     assert np.all(got[turns > 1] > f[turns > 1] / factor * (1 + 2.0 ** -20))
+
+
+@pytest.mark.parametrize("trained,low", [(1, 1.0), (6, 1.0), (100, 16.0), (2048, 326.0), (128, 1000.0)])
+@pytest.mark.parametrize("rot", [2, 8, 64])
+def test_pairs_that_all_turn_less_than_low(rot, trained, low):
+    """Contexts so short that even the first pair makes `low` turns or fewer: all are slowed down, as "turns" does."""
+    import zigneuron_amd as zn
+    f = 10000.0 ** (-2.0 * np.arange(rot // 2) / rot)
+    assert trained / (2 * math.pi) <= low  # the first pair's frequency is 1
+    for kind in ("pairs", "turns"):
+        got = zn.rotary_frequencies(rot, 10000.0, kind, 4.0, trained, low, 4 * low).astype(np.float64)
+        assert np.all(np.abs(got - f / 4) <= 2.0 ** -23 * f), (kind, got / f)

@@ -108,14 +108,14 @@ int zn_hip_rotary_frequencies(float *freq, size_t freq_len, int64_t rot_dim, flo
         first = std::max(0.0, std::floor(pair_of(high)));
         // not the last pair, n / 2 - 1: past it lies the ramp's end wherever that pair makes more than `low` turns
         last = std::min(n - 1.0, std::ceil(pair_of(low)));
-        if (!(last > first)) last = first + 0.001;
     }
     for (int64_t i = 0; i < rot_dim / 2; ++i) {
         const double f = std::pow(b, -2.0 * (double)i / n);
         double keep = 1.0;  // the share that keeps its speed; the rest is slowed down by factor
         if (scaling == ZN_ROTARY_LINEAR) keep = 0.0;
         else if (scaling == ZN_ROTARY_TURNS) keep = ((double)trained_len * f / circle - low) / ((double)high - low);
-        else if (scaling == ZN_ROTARY_PAIRS) keep = 1.0 - ((double)i - first) / (last - first);
+        else if (scaling == ZN_ROTARY_PAIRS)  // where even the first pair turns less, last <= first
+            keep = (double)i >= last ? 0.0 : (double)i <= first ? 1.0 : 1.0 - ((double)i - first) / (last - first);
         keep = std::min(1.0, std::max(0.0, keep));
         freq[i] = (float)(scaling == ZN_ROTARY_PLAIN || scaling == ZN_ROTARY_BASE ? f : keep * f + (1.0 - keep) * f / factor);
     }
