@@ -536,7 +536,7 @@ int zn_hip_rotary_frequencies(float *freq, size_t freq_len, int64_t rot_dim, flo
  * freq: rot_dim / 2 floats on the device.  positions: int32 on the device, len
  * of them for each sequence, position_stride elements apart (0: the same for
  * all); null: 0, 1, .. in every sequence.  The angle is as exact for far
- * positions as for near ones (64 bits).
+ * positions as for near ones (64 bits, angles up to 2^80).
  * x and y are [batch, heads, len, head_dim] at element strides for batch, head
  * and position, dims contiguous, head_dim 1..1024; y may be x at x's strides.
  * Strides are >= 0, y's > 0 over extents above 1 (rows that it writes must not

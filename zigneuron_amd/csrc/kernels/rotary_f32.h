@@ -10,9 +10,9 @@
 // the rest of its rounding, and reduced to a quarter turn in 64 bits (2 / pi in
 // two parts): a turn of a far position is as exact as that of a near one, where
 // an angle rounded to 32 bits is off by 2^-24 of itself, 0.06 of a turn's radius
-// at 10^6.  Sine and cosine of
-// what is left, |y| <= pi / 4, are their Taylor polynomials to y^11 and y^10 (the
-// next terms are below 2^-27 of 1).
+// at 10^6.  The 107 bits of 2 / pi do for angles up to 2^80 (beyond, the turn is
+// by any angle).  Sine and cosine of what is left, |y| <= pi / 4, are their Taylor
+// polynomials to y^11 and y^10 (the next terms are below 2^-27 of 1).
 #ifndef ZN_ROTARY_F32_H
 #define ZN_ROTARY_F32_H
 
@@ -26,10 +26,20 @@ namespace {
 typedef float zn_f32x4_any __attribute__((ext_vector_type(4), aligned(4)));  // at any float
 typedef __bf16 zn_bf16x4_any __attribute__((ext_vector_type(4), aligned(2)));
 
+// FAR: an angle past kRotaryNear, where the roundings of a and t are quarter turns of their own.
+constexpr float kRotaryNear = 0x1p50f;
+template <bool FAR>
 __device__ __forceinline__ void rotary_sincos(int position, float freq, float &s, float &c) {
     constexpr double kHi = 0.63661977236758138, kLo = -3.9357353350364972e-17;  // 2 / pi
     const double p = position, f = freq, a = p * f, rest = __builtin_fma(p, f, -a), t = a * kHi, q = __builtin_rint(t);
-    const float y = (float)((t - q) + __builtin_fma(rest, kHi, __builtin_fma(a, kLo, __builtin_fma(a, kHi, -t)))) * 1.57079632679489662f, z = y * y;
+    double r = (t - q) + __builtin_fma(rest, kHi, __builtin_fma(a, kLo, __builtin_fma(a, kHi, -t)));
+    int n = (int)__builtin_fma(__builtin_floor(q * 0.25), -4.0, q);  // of 0..3: q itself may pass 32 bits
+    if (FAR) {
+        const double k = __builtin_rint(r);
+        r -= k;
+        n += (int)__builtin_fma(__builtin_floor(k * 0.25), -4.0, k);
+    }
+    const float y = (float)r * 1.57079632679489662f, z = y * y;
     float u = __builtin_fmaf(z, -1.0f / 39916800.0f, 1.0f / 362880.0f);
     u = __builtin_fmaf(z, u, -1.0f / 5040.0f);
     u = __builtin_fmaf(z, u, 1.0f / 120.0f);
@@ -40,11 +50,10 @@ __device__ __forceinline__ void rotary_sincos(int position, float freq, float &s
     w = __builtin_fmaf(z, w, 1.0f / 24.0f);
     w = __builtin_fmaf(z, w, -0.5f);
     const float cy = __builtin_fmaf(z, w, 1.0f);
-    const int n = (int)__builtin_fma(__builtin_floor(q * 0.25), -4.0, q);  // of 0..3: q itself may pass 32 bits
     s = n & 1 ? cy : sy;
     c = n & 1 ? sy : cy;
     if (n & 2) s = -s;
-    if (n == 1 || n == 2) c = -c;
+    if ((n + 1) & 2) c = -c;
 }
 
 // Four values or the first n of them; the rest are 0.
@@ -102,18 +111,27 @@ struct RotaryUnit {
 // The unit's sines and cosines at one position.
 struct RotaryTurn {
     float s[4], c[4];
-    __device__ __forceinline__ RotaryTurn(const RotaryUnit &u, const float *freq, int rot, int layout, int position, float scale, float sign) {
+    __device__ __forceinline__ RotaryTurn(const RotaryUnit &u, const float *freq, int rot, int position, float scale, float sign) {
+        if (fill<false>(u, freq, rot, position, scale, sign) > kRotaryNear) fill<true>(u, freq, rot, position, scale, sign);
+    }
+    // Returns the largest angle.
+    template <bool FAR>
+    __device__ __forceinline__ float fill(const RotaryUnit &u, const float *freq, int rot, int position, float scale, float sign) {
+        float most = 0.0f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             s[e] = 0.0f;
             c[e] = 1.0f;
             const int i = (u.half ? u.da : u.da / 2) + e;
             if (u.turns && i < rot / 2) {
-                rotary_sincos(position, freq[i], s[e], c[e]);
+                const float f = freq[i];
+                most = fmaxf(most, __builtin_fabsf((float)position * f));
+                rotary_sincos<FAR>(position, f, s[e], c[e]);
                 s[e] *= sign * scale;
                 c[e] *= scale;
             }
         }
+        return most;
     }
     __device__ __forceinline__ static void turn(float &x, float &y, float s, float c) {
         const float a = x, b = y;
@@ -150,7 +168,7 @@ extern "C" __global__ __launch_bounds__(256) void zn_rotary(ZnRotaryArgs p) {
     if (tl >= p.tokens || token >= (int64_t)p.batch * p.len) return;
     const int b = (int)token / p.len, i = (int)token - b * p.len;
     const RotaryUnit u(in - slot * p.units, p.dim, p.rot, p.layout);
-    const RotaryTurn t(u, p.freq, p.rot, p.layout, p.positions ? p.positions[b * p.position_stride + i] : i, p.scale, p.sign);
+    const RotaryTurn t(u, p.freq, p.rot, p.positions ? p.positions[b * p.position_stride + i] : i, p.scale, p.sign);
     const float *x = p.x + b * p.xs[0] + i * p.xs[2];
     float *y = p.y + b * p.ys[0] + i * p.ys[2];
     for (int h = blockIdx.y * p.slots + slot; h < p.heads; h += gridDim.y * p.slots) {
@@ -182,7 +200,7 @@ __device__ __forceinline__ void paged_append(const ZnAppendArgs &p) {
     const int j = seq.first + t - seq.t0;
     if (t < seq.t0 || t >= seq.t0 + seq.ql) return;
     const RotaryUnit u(in - slot * p.units, c.dim, p.rot, p.layout);
-    const RotaryTurn turn(u, p.freq, p.rot, p.layout, p.positions ? p.positions[t] : j, p.scale, 1.0f);
+    const RotaryTurn turn(u, p.freq, p.rot, p.positions ? p.positions[t] : j, p.scale, 1.0f);
     const int64_t at = j < 0 ? -1 : paged_at(c, b, 0, j);
     for (int h = blockIdx.y * p.slots + slot; h < p.q_heads + 2 * c.kv_heads; h += gridDim.y * p.slots) {
         const int kh = h - p.q_heads, vh = kh - c.kv_heads;
