@@ -35,6 +35,7 @@
 #include "../../../include/zn_hip.h"
 #include "../zn_kernel_args.h"
 #include "../zn_paged_args.h"
+#include "zn_paged_plan.h"
 
 // Scratch of zn_hip_sgemm_noalloc: the split-K partial sums of a GEMM whose
 // caller cannot allocate.  One copy per device, held until the process ends.
@@ -106,14 +107,6 @@ constexpr const char *kMhaName[kNumMha] = {"zn_mha_few", "zn_mha_forward", "zn_m
 // Rows (query rows; the backward's also keys) and threads of a workgroup, by dims in 32s; 0: no such kernel.
 constexpr int kMhaRows[kNumMha][4] = {{16, 16, 16, 16}, {128, 128, 128, 128}, {0, 0, 256, 256}, {128, 128, 128, 128}, {128, 128, 64, 128}, {32, 32, 32, 32}};
 constexpr unsigned kMhaThreads[kNumMha][4] = {{256, 256, 256, 256}, {256, 256, 512, 512}, {0, 0, 512, 512}, {256, 256, 512, 512}, {256, 256, 256, 512}, {256, 256, 256, 256}};
-
-// Attention over a paged cache (kernels/paged_f32.h), in the attention code object: zn_paged_<what>_<cache type>_<padded head dim>.
-enum PagedKernel { kPagedFew, kPagedFew2, kPagedFew4, kPagedTile, kPagedWide, kNumPaged };
-constexpr const char *kPagedName[kNumPaged] = {"zn_paged_few", "zn_paged_few2", "zn_paged_few4", "zn_paged_tile", "zn_paged_wide"};
-constexpr int kPagedRows[kNumPaged] = {16, 32, 64, 128, 256};  // query rows of a workgroup
-constexpr const char *kCacheName[2] = {"f32", "bf16"};
-// Threads of a tile's workgroup [kPagedTile, kPagedWide][cache type][dims in 32s]; the others have 256.
-constexpr unsigned kPagedThreads[2][2][4] = {{{256, 256, 512, 512}, {256, 256, 256, 256}}, {{512, 512, 512, 512}, {512, 512, 512, 512}}};
 
 struct ScratchDevice;
 

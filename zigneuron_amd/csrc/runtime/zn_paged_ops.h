@@ -177,53 +177,6 @@ int paged_args(const zn_paged_cache *c, ZnPagedCache &a, const void *starts, int
     return ZN_OK;
 }
 
-// How many parts the walk of few query rows is cut into: two workgroups a CU of sequences that are as long as the call allows, of 512 KB
-// of K and V at most (sequences differ in length), 128 positions at least (paged_few_len).  MI355X, us in parts of 256, 512, 1024, 2048
-// and 4096 positions: 64 x 8 heads of up to 8192 x 128 bf16 311, 285, 275, 279, 291; 16 x 4 of up to 4096 x 128 bf16, five tokens, 41,
-// 31, 32, 47, 73; 16 x 8 of 4096 x 128 fp32 112, 108, 108, 107, 126; 8 of 65536 x 128 bf16 64, 54, 49, 47, 52; 8 x 4 of 2048 x 64
-// fp32 12, 16, 24, 37.  Beside tiles one of their larger workgroups a CU; never
-// more than 32 a CU, which bounds the parts' memory.  Past 4096 heads there is enough to do without.
-void paged_few_parts(const zn_ctx *ctx, ZnPagedArgs &a, int type, int per_cu) {
-    const int64_t most = 524288 / (2 * a.c.dim * (type == ZN_CACHE_BF16 ? 2 : 4));
-    const int64_t all = (int64_t)a.c.cap * a.few_heads, cus = cus_now(ctx);
-    const int64_t len = std::max({(int64_t)128, std::min(most, all / (per_cu * cus)), all / (32 * cus)});
-    a.few_splits = a.few_heads > kCounterSlots ? 1 : (int32_t)std::max<int64_t>(1, std::min<int64_t>(65535, cdiv(a.c.cap, len)));
-}
-
-// Parts of the walks of tiles: the least of the times of two batches added up, one whose sequences are all as long as the call allows, one
-// where one is and the others make it three quarters of that together.  A workgroup's way in and out is 10 us; times of a block of 32
-// keys as measured (dims 64, 96, 128; us): fp32 256 rows 2.3, 3.4, 4.0, 128 rows 2.0 alone and 3.0 where two share a CU, then 2.1, 2.5;
-// bf16 (128 dims) 2.5 and 2.6.  Without the second batch 4 x 512 tokens of 32 (8) x 128 over 2730 to 8192 positions stay whole: 1015
-// us, 550 in two parts; without the first 4 x 512 of 16 (4) x 64 over 4096 take three: 234, 186 in two.  Returns the time so found.
-double paged_tile_parts(const zn_ctx *ctx, ZnPagedArgs &a, int64_t tokens, int64_t max_q, int kernel, int type) {
-    constexpr int kParts[12] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
-    constexpr double kWay = 10.0;
-    const int rows = kPagedRows[kernel];
-    const bool pairs = kPagedThreads[kernel - kPagedTile][type][(a.c.dim - 1) / 32] == 256;  // two workgroups share a CU
-    const double cus = (double)cus_now(ctx) / (a.few ? 2.0 : 1.0), slots = cus * (pairs ? 2 : 1), tiles = (double)(cdiv(tokens * a.group, rows) * a.c.kv_heads);
-    const double wide = (0.6 + 0.0264 * a.c.dim) * (type == ZN_CACHE_BF16 ? 0.65 : 1.0), tile = type == ZN_CACHE_BF16 ? 1.0 : pairs ? 1.2 : 0.64;
-    const double full = kernel == kPagedWide ? wide : wide * tile, alone = pairs ? 0.75 * full : full;
-    const double share = a.causal && a.c.cap > 0 ? 1.0 - 0.5 * std::min(1.0, (double)max_q / (double)a.c.cap) : 1.0;  // of a walk, on average
-    const int64_t blocks = cdiv(a.c.cap, 32);
-    double best = INFINITY;
-    a.tile_splits = 1;
-    for (const int s : kParts) {
-        if (s > 1 && s > blocks) break;
-        const double n = tiles * s, len = (double)cdiv(blocks, s), longest = kWay + alone * len, all = n * (kWay + full * len * share) / slots;
-        const double join = s > 1 ? 6.0 + 8.0 * (double)tokens * a.q_heads * s * a.c.dim / 2e6 : 0.0;
-        const double even = n <= cus ? longest : share < 0.9 ? std::max(longest, all) : std::ceil(n / slots) * (kWay + full * len);
-        const double us = even + join + std::max(longest, 0.75 * all) + 0.75 * join;
-        if (us < best) {
-            best = us;
-            a.tile_splits = s;
-        }
-    }
-    a.tile = rows;
-    a.tile_len = (int32_t)(32 * std::max<int64_t>(1, cdiv(blocks, a.tile_splits)));
-    a.tile_splits = (int32_t)std::max<int64_t>(1, cdiv(a.c.cap, a.tile_len));
-    return best;
-}
-
 // What a call with something to do reads of the descriptor.
 bool paged_pointers(const ZnPagedCache &a) { return a.kv_lens && a.starts && (a.cap == 0 || (a.k && a.v && a.table)); }
 
@@ -302,7 +255,7 @@ int zn_hip_paged_attention(zn_ctx *ctx, const void *cache, const void *token_sta
     if (!q || !out || !paged_pointers(a.c)) return ZN_ERR_INVALID_ARG;
     max_q_len = std::min(max_q_len, tokens);
     const int dims = (int)(desc->head_dim - 1) / 32, type = desc->type;
-    const int64_t group = q_heads / desc->kv_heads, cap = std::min<int64_t>(a.c.cap, max_kv_len);
+    const int64_t cap = std::min<int64_t>(a.c.cap, max_kv_len);
     if ((rc = select_device(ctx))) return rc;
     a.c.cap = (int32_t)cap;
     a.q = q;
@@ -321,51 +274,23 @@ int zn_hip_paged_attention(zn_ctx *ctx, const void *cache, const void *token_sta
     if (desc->head_dim < 8) return launch(ctx, ctx->paged_rows[type], (unsigned)tokens, (unsigned)cdiv(q_heads, 4), 256, &a);
     const int pages = desc->page_size % 16 == 0;
     a.part_ld = (int32_t)(desc->head_dim + 3) / 4 * 4 + 4;
-    a.few_heads = (int32_t)(desc->batch * desc->kv_heads);
-    // Sequences of few query rows have kernels of their own; where others are in the call too, their workgroups follow the tiles'
-    // in one launch.
-    const int64_t rows = group * max_q_len;
-    // 33 to 64 rows: in tiles where there are few heads, whose walks a workgroup then reads too slowly (MI355X, us as few rows and in
-    // tiles of 128: 16 tokens of 16 x 8 heads (4) against 4096 x 128 bf16 107 and 131, of 4 x 8 against 2048 39 and 32; fp32 of 33 x 9
-    // heads (1) of 42 tokens against up to 2713 x 127 260 and 367, 16 tokens of 16 x 8 (4) against 2048 x 128 112 and 103, of 16 x 4
-    // against 4096 x 64 66 and 98).
-    const int64_t enough = type == ZN_CACHE_BF16 || desc->head_dim <= 64 ? cus_now(ctx) / 4 : cus_now(ctx);
-    const bool all_few = rows <= kPagedRows[a.few_heads >= enough ? kPagedFew4 : kPagedFew2];
-    int kernel = kPagedFew;
-    int64_t wgs = 0;
-    if (all_few) {
-        while (kPagedRows[kernel] < rows) ++kernel;
-        a.few = (int32_t)rows;
-    } else if (group <= kPagedRows[kPagedFew] && tokens < desc->batch * max_q_len) {
-        a.few = kPagedRows[kPagedFew];
-    }
-    if (a.few) paged_few_parts(ctx, a, type, all_few ? 2 : 1);
-    if (!all_few) {
-        ZnPagedArgs wide = a;
-        kernel = kPagedTile;
-        if (paged_tile_parts(ctx, wide, tokens, max_q_len, kPagedWide, type) < paged_tile_parts(ctx, a, tokens, max_q_len, kPagedTile, type)) {
-            kernel = kPagedWide;
-            a = wide;
-        }
-        wgs = (tokens * group / a.tile + desc->batch) * desc->kv_heads * a.tile_splits + (a.few ? (int64_t)a.few_heads * a.few_splits : 0);
-        if (wgs > INT_MAX / 1024) return ZN_ERR_OVERFLOW;
-    }
+    const PagedPlan plan = paged_plan(a, type, cus_now(ctx));
+    if (!plan.fits()) return ZN_ERR_OVERFLOW;
     Lease few_part(ctx), tile_part(ctx);
     if (a.few && a.few_splits > 1) {
         if ((rc = few_part.get((size_t)a.few_heads * a.few * a.few_splits * a.part_ld))) return rc;
         a.few_part = few_part.ptr;
     }
-    if (!all_few && a.tile_splits > 1) {
+    if (!plan.all_few && a.tile_splits > 1) {
         if ((rc = tile_part.get((size_t)(tokens * q_heads) * a.tile_splits * a.part_ld))) return rc;
         a.tile_part = tile_part.ptr;
     }
-    // a few rows: their last workgroup joins the parts, two rows a wave at most
-    const bool own_join = all_few && rows <= 8;
-    if (own_join && a.few_splits > 1) a.counters = ctx->counters;
-    const hipFunction_t f = ctx->paged[kernel][type][dims][pages];
-    if (all_few) rc = launch(ctx, f, (unsigned)a.few_heads, 1, 256, &a, (unsigned)a.few_splits);
-    else rc = launch(ctx, f, (unsigned)wgs, 1, kPagedThreads[kernel - kPagedTile][type][dims], &a);
-    if (rc || own_join || (a.few_splits <= 1 && a.tile_splits <= 1)) return rc;
+    static_assert(kPagedSplitHeads <= kCounterSlots, "a counter for each walk in parts");
+    if (plan.own_join && a.few_splits > 1) a.counters = ctx->counters;
+    const hipFunction_t f = ctx->paged[plan.kernel][type][dims][pages];
+    if (plan.all_few) rc = launch(ctx, f, (unsigned)a.few_heads, 1, 256, &a, (unsigned)a.few_splits);
+    else rc = launch(ctx, f, (unsigned)plan.wgs, 1, plan.threads, &a);
+    if (rc || plan.own_join || (a.few_splits <= 1 && a.tile_splits <= 1)) return rc;
     // a token's heads beside each other while there are few tokens, eight workgroups a CU (4 x 512 tokens of 32 heads, a quarter of
     // them in parts: 25 us with eight workgroups a token, 15 with one)
     const int64_t join_heads = std::max<int64_t>(1, std::min<int64_t>(cdiv(q_heads, 4), 8 * cus_now(ctx) / tokens));
