@@ -3,6 +3,7 @@ that batches of all kinds turn out to have."""
 from __future__ import annotations
 
 import os
+import re
 import shutil
 import subprocess
 import textwrap
@@ -11,7 +12,7 @@ import pytest
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
-PROGRAM = textwrap.dedent(r'''
+COMMON = textwrap.dedent(r'''
     #include <cstdio>
     #include <cstring>
     #include <random>
@@ -34,7 +35,9 @@ PROGRAM = textwrap.dedent(r'''
         a.max_q = (int32_t)(max_q < tokens ? max_q : tokens);
         return a;
     }
+''')
 
+PROGRAM = COMMON + textwrap.dedent(r'''
     int main() {
         std::mt19937_64 rng(3);
         auto pick = [&](int64_t lo, int64_t hi) { return lo + (int64_t)(rng() % (uint64_t)(hi - lo + 1)); };
@@ -88,12 +91,55 @@ PROGRAM = textwrap.dedent(r'''
 ''')
 
 
+# Prints each kernel that calls of all kinds take, once.
+TAKEN = COMMON + textwrap.dedent(r'''
+    int main() {
+        std::mt19937_64 rng(5);
+        auto log = [&](double lo, double hi) {
+            return (int64_t)std::llround(std::exp(std::log(lo) + (std::log(hi) - std::log(lo)) * (double)(rng() % 1000000) / 1e6));
+        };
+        bool seen[kNumPaged][2][4] = {};
+        for (int round = 0; round < 200000; ++round) {
+            const int64_t batch = log(1, 2000), kv = log(1, 16), group = log(1, 64), max_q = log(1, 8192), cap = log(1, 65536);
+            const int64_t tokens = std::min<int64_t>((1 << 24) - 1, rng() % 2 ? batch * max_q : max_q + (batch - 1) * log(1, (double)max_q));
+            if (tokens * kv * group > INT32_MAX / 2) continue;
+            const int dim = (int)log(8, 128), type = (int)(rng() % 2);
+            ZnPagedArgs a = call(batch, kv, group, dim, tokens, max_q, cap, (int)(rng() % 2));
+            const PagedPlan p = paged_plan(a, type, 256);
+            bool &s = seen[p.kernel][type][(dim - 1) / 32];
+            if (!s) std::printf("%s_%s_%d\n", kPagedName[p.kernel], kCacheName[type], 32 * ((dim - 1) / 32 + 1));
+            s = true;
+        }
+        return 0;
+    }
+''')
+
+
+def run(tmp_path, program, *flags):
+    src = tmp_path / "plan.cpp"
+    src.write_text(program)
+    exe = tmp_path / "plan"
+    subprocess.run(["g++", "-O1", "-std=c++17", *flags, "-I", os.path.join(ROOT, "zigneuron_amd", "csrc"), str(src), "-o", str(exe)],
+                   check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stdout + r.stderr
+    return r.stdout
+
+
+def built():
+    """The kernels of the code object."""
+    with open(os.path.join(ROOT, "zigneuron_amd", "lib", "zn_attention_gfx950.hsaco"), "rb") as f:
+        names = re.findall(rb"zn_paged_(?:few|few2|few4|tile|wide)_(?:f32|bf16)_\d+(?:_p)?(?=\.kd)", f.read())
+    return {n.decode() for n in names}
+
+
 @pytest.mark.skipif(shutil.which("g++") is None, reason="g++ not found")
 def test_workgroups_cover_the_parts_and_no_more_sequences_than_can_have_them(tmp_path):
-    src = tmp_path / "plan.cpp"
-    src.write_text(PROGRAM)
-    exe = tmp_path / "plan"
-    subprocess.run(["g++", "-O1", "-std=c++17", "-fsanitize=undefined", "-fno-sanitize-recover=all", "-I",
-                    os.path.join(ROOT, "zigneuron_amd", "csrc"), str(src), "-o", str(exe)], check=True)
-    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=120)
-    assert r.returncode == 0 and r.stdout.strip() == "OK", r.stdout + r.stderr
+    assert run(tmp_path, PROGRAM, "-fsanitize=undefined", "-fno-sanitize-recover=all").strip() == "OK"
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="g++ not found")
+def test_every_kernel_that_is_built_is_taken(tmp_path):
+    """... for pages of any size and of multiples of 16 positions alike, and none is taken that is not built."""
+    taken = run(tmp_path, TAKEN).split()
+    assert built() == {n + p for n in taken for p in ("", "_p")}

@@ -1010,11 +1010,10 @@ extern "C" __global__ __launch_bounds__(256) void zn_paged_rows_bf16(ZnPagedArgs
     ZN_PAGED_FEW(zn_paged_few_bf16_##DP##S, __bf16, DP, 4, 1, P)          \
     ZN_PAGED_FEW(zn_paged_few2_bf16_##DP##S, __bf16, DP, 4, 2, P)         \
     ZN_PAGED_FEW(zn_paged_few4_bf16_##DP##S, __bf16, DP, 4, 4, P)
-#define ZN_PAGED_TILES(DP, NW, F, WNW, WF, BNW, BF, VNW, VF, S, P)        \
+#define ZN_PAGED_TILES(DP, NW, F, S, P)                                   \
     ZN_PAGED_TILE(zn_paged_tile_f32_##DP##S, float, DP, NW, F, P)         \
-    ZN_PAGED_TILE(zn_paged_wide_f32_##DP##S, float, DP, WNW, WF, P)       \
-    ZN_PAGED_TILE(zn_paged_tile_bf16_##DP##S, __bf16, DP, BNW, BF, P)     \
-    ZN_PAGED_TILE(zn_paged_wide_bf16_##DP##S, __bf16, DP, VNW, VF, P)
+    ZN_PAGED_TILE(zn_paged_wide_f32_##DP##S, float, DP, 8, 2, P)          \
+    ZN_PAGED_TILE(zn_paged_tile_bf16_##DP##S, __bf16, DP, 4, 2, P)
 ZN_PAGED_KERNELS(32, , false)
 ZN_PAGED_KERNELS(32, _p, true)
 ZN_PAGED_KERNELS(64, , false)
@@ -1024,10 +1023,11 @@ ZN_PAGED_KERNELS(96, _p, true)
 ZN_PAGED_KERNELS(128, , false)
 ZN_PAGED_KERNELS(128, _p, true)
 #define ZN_PAGED_TILES2(...) ZN_PAGED_TILES(__VA_ARGS__, , false) ZN_PAGED_TILES(__VA_ARGS__, _p, true)
-// dims; fp32 pages: waves and blocks of 16 rows of tiles of 128 rows, of 256; bf16 pages: the same
-ZN_PAGED_TILES2(32, 4, 2, 8, 2, 4, 2, 8, 2)
-ZN_PAGED_TILES2(64, 4, 2, 8, 2, 4, 2, 8, 2)
-ZN_PAGED_TILES2(96, 8, 1, 8, 2, 4, 2, 8, 2)
-ZN_PAGED_TILES2(128, 8, 1, 8, 2, 4, 2, 8, 2)
+// dims; fp32 pages: waves and blocks of 16 rows of tiles of 128 rows.  bf16 pages have no tiles of 256: a block of 32 keys of 128 dims
+// takes 2.5 us there and 2.6 in two tiles of 128 on the same CU, which cut a call's work finer.
+ZN_PAGED_TILES2(32, 4, 2)
+ZN_PAGED_TILES2(64, 4, 2)
+ZN_PAGED_TILES2(96, 8, 1)
+ZN_PAGED_TILES2(128, 8, 1)
 
 #endif

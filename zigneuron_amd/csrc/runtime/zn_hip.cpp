@@ -2033,6 +2033,7 @@ int zn_hip_create(int device, const char *code_object_dir, zn_ctx **out) {
         for (int i = 0; i < kNumPaged; ++i)
             for (int d = 0; d < 4; ++d)
                 for (int pages = 0; pages < 2; ++pages) {
+                    if (i >= kPagedTile && kPagedThreads[i - kPagedTile][type][d] == 0) continue;
                     std::snprintf(name, sizeof(name), "%s_%s_%d%s", kPagedName[i], kCacheName[type], 32 * (d + 1), pages ? "_p" : "");
                     if (hipModuleGetFunction(&ctx->paged[i][type][d][pages], ctx->attn_module, name) != hipSuccess) return bail(ZN_ERR_SYMBOL);
                 }

@@ -18,8 +18,8 @@ enum PagedKernel { kPagedFew, kPagedFew2, kPagedFew4, kPagedTile, kPagedWide, kN
 constexpr const char *kPagedName[kNumPaged] = {"zn_paged_few", "zn_paged_few2", "zn_paged_few4", "zn_paged_tile", "zn_paged_wide"};
 constexpr int kPagedRows[kNumPaged] = {16, 32, 64, 128, 256};  // query rows of a workgroup
 constexpr const char *kCacheName[2] = {"f32", "bf16"};
-// Threads of a tile's workgroup [kPagedTile, kPagedWide][cache type][dims in 32s]; the others have 256.
-constexpr unsigned kPagedThreads[2][2][4] = {{{256, 256, 512, 512}, {256, 256, 256, 256}}, {{512, 512, 512, 512}, {512, 512, 512, 512}}};
+// Threads of a tile's workgroup [kPagedTile, kPagedWide][cache type][dims in 32s]; the others have 256.  0: there is none.
+constexpr unsigned kPagedThreads[2][2][4] = {{{256, 256, 512, 512}, {256, 256, 256, 256}}, {{512, 512, 512, 512}, {0, 0, 0, 0}}};
 constexpr int64_t kPagedSplitHeads = 4096;  // sequences' heads of few rows whose walks are cut into parts
 
 inline int64_t paged_ceil(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -107,7 +107,8 @@ inline PagedPlan paged_plan(ZnPagedArgs &a, int type, int64_t cus) {
     if (p.all_few) return p;
     ZnPagedArgs wide = a;
     p.kernel = kPagedTile;
-    if (paged_tile_parts(wide, kPagedWide, type, cus) < paged_tile_parts(a, kPagedTile, type, cus)) {
+    const double us = paged_tile_parts(a, kPagedTile, type, cus);
+    if (type == ZN_CACHE_F32 && paged_tile_parts(wide, kPagedWide, type, cus) < us) {
         p.kernel = kPagedWide;
         a = wide;
     }
