@@ -115,13 +115,27 @@ TAKEN = COMMON + textwrap.dedent(r'''
 ''')
 
 
-def run(tmp_path, program, *flags):
+# The kernel of each call that is read: batch, kv_heads, group, dim, tokens, max_q, cap, causal, type.
+NAMES = COMMON + textwrap.dedent(r'''
+    int main() {
+        long long batch, kv, group, dim, tokens, max_q, cap, causal, type;
+        while (std::scanf("%lld %lld %lld %lld %lld %lld %lld %lld %lld", &batch, &kv, &group, &dim, &tokens, &max_q, &cap, &causal, &type) == 9) {
+            ZnPagedArgs a = call(batch, kv, group, (int)dim, tokens, max_q, cap, (int)causal);
+            const PagedPlan p = paged_plan(a, (int)type, 256);
+            std::printf("%s_%s_%d\n", kPagedName[p.kernel], kCacheName[type], (int)(32 * ((dim - 1) / 32 + 1)));
+        }
+        return 0;
+    }
+''')
+
+
+def run(tmp_path, program, *flags, given=""):
     src = tmp_path / "plan.cpp"
     src.write_text(program)
     exe = tmp_path / "plan"
     subprocess.run(["g++", "-O1", "-std=c++17", *flags, "-I", os.path.join(ROOT, "zigneuron_amd", "csrc"), str(src), "-o", str(exe)],
                    check=True)
-    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=120)
+    r = subprocess.run([str(exe)], input=given, capture_output=True, text=True, timeout=120)
     assert r.returncode == 0, r.stdout + r.stderr
     return r.stdout
 
@@ -143,3 +157,18 @@ def test_every_kernel_that_is_built_is_taken(tmp_path):
     """... for pages of any size and of multiples of 16 positions alike, and none is taken that is not built."""
     taken = run(tmp_path, TAKEN).split()
     assert built() == {n + p for n in taken for p in ("", "_p")}
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="g++ not found")
+def test_the_gpu_tests_reach_every_kernel(tmp_path):
+    """tests/test_gpu_paged_kernels.py: each call is taken by the kernel that it names, and none is left out."""
+    from paged_cases import cases
+    calls, names = [], []
+    for name, lens, counts, hq, hk, page, dim, dtype in cases():
+        for causal in (0, 1):
+            calls.append((len(lens), hk, hq // hk, dim, sum(counts) + 2, max(counts), max(lens), causal, int(dtype == "bf16")))
+            names.append((name, "_p" if page % 16 == 0 else ""))
+    got = run(tmp_path, NAMES, given="\n".join(" ".join(map(str, c)) for c in calls)).split()
+    assert len(got) == len(calls)
+    assert [n for n, _ in names] == [g + p for g, (_, p) in zip(got, names)]
+    assert built() == {n for n, _ in names}
