@@ -88,3 +88,20 @@ def test_ascending_starts_between_odd_rows(ctx, new):
     ctx.paged_append(cache, ds.ptr, n, dk, dk, q=dx, q_out=q_out, q_heads=hq)
     q = q_out.download().reshape(x.shape)
     assert np.all(q[:5] == 5.0) and np.all(q[5 + 3 * new:] == 5.0) and np.array_equal(q[5:5 + 3 * new], x[5:5 + 3 * new])
+
+
+@pytest.mark.parametrize("counts,d", [([1, 1], 64), ([40, 3], 64), ([9, 0], 128), ([5, 5], 4)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_a_cache_of_no_pages(ctx, counts, d, causal):
+    """Null pools and table: nothing is stored, every position is masked; queries are turned all the same."""
+    from zigneuron_amd import PagedCache
+    announce(f"no pages {counts} {d} {causal}")
+    n, hq, hk = sum(counts), 4, 2
+    lens, starts = Ints(ctx, [50, 60]), Ints(ctx, starts_of(counts))
+    cache = PagedCache(None, None, None, lens.ptr, 2, 0, 16, 8, hk, d)
+    x = np.random.default_rng(1).standard_normal((n, hq, d)).astype(np.float32)
+    dx, do, dl = ctx.to_device(x), ctx.alloc(x.size).fill(7.0), ctx.alloc(n * hq).fill(9.0)
+    ctx.paged_attention(cache, starts.ptr, n, max(counts), 60, dx, do, dl, hq, 0.2, causal)
+    assert np.all(do.download() == 0) and np.all(dl.download() == -np.inf)
+    ctx.paged_append(cache, starts.ptr, n, dx, dx, (hq * d, d), dx, do, hq)
+    assert np.array_equal(do.download().reshape(x.shape), x)
